@@ -234,6 +234,114 @@ int wush_gemm_s4_tensor_scale(const uint8_t *xq, const uint8_t *wq, uint16_t *y,
                               int64_t M, int64_t N, int64_t K, float alpha,
                               const float *alpha_dev, hipStream_t stream);
 
+/* ------------------------------------------------------------------------
+ * 8-bit operators around the W4A4 layers.  The reference has no counterpart of
+ * anything below.
+ * ------------------------------------------------------------------------ */
+
+/* Largest K of the W8A8 entry points: 128 * 128 * 131056 < 2^31. */
+#define WUSH_W8A8_MAX_K 131056
+
+/* Per-token INT8 quantization of x (rows, K), bf16 or fp16, rows `row_stride`
+ * elements apart:
+ *   s[m] = max(amax_k |x[m][k]| / 127, 2^-126)
+ *   q[m][k] = clamp(rint(x[m][k] * (1 / s[m])), -127, 127)
+ * every step one fp32 operation.  A row with a non-finite value gets s = NaN and
+ * zero codes.  q: rows*K, s: rows fp32.  K % 16 == 0, K <= WUSH_W8A8_MAX_K, x
+ * and q 16-byte aligned, row_stride a multiple of 8. */
+int wush_quant_int8_token(const void *x, int dtype, int8_t *q, float *s, int64_t rows, int64_t K,
+                          int64_t row_stride, hipStream_t stream);
+
+/* W8A8 product: y[m][n] = (sum_k xq[m][k] wq[n][k]) * xs[m] * ws[n], the sum
+ * exact in int32, then two fp32 products and one rounding to `dtype` (bf16 or
+ * fp16).  xq (M, K), wq (N, K) int8; xs M, ws N fp32; y (M, N).  Any M, N;
+ * K % 16 == 0, K <= WUSH_W8A8_MAX_K; xq and wq 16-byte aligned.  The result's
+ * bits depend on neither the workspace nor the plan.  Bytes of workspace with which
+ * it runs its fastest plan (int32 partial sums of a split K) are asked of
+ * wush_gemm_w8a8_workspace_bytes; with fewer, K is not split. */
+size_t wush_gemm_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int wush_gemm_w8a8(const int8_t *xq, const float *xs, const int8_t *wq, const float *ws, void *y, int dtype,
+                   int64_t M, int64_t N, int64_t K, void *workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* Both in one call: y = W8A8 product of x (M, K), bf16 or fp16 as y, rows
+ * row_stride elements apart, with the same bits as wush_quant_int8_token followed by
+ * wush_gemm_w8a8.  The workspace (16-byte aligned, of at least
+ * wush_linear_w8a8_workspace_bytes) holds the codes. */
+size_t wush_linear_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int wush_linear_w8a8(const void *x, int64_t row_stride, const int8_t *wq, const float *ws, void *y, int dtype,
+                     int64_t M, int64_t N, int64_t K, void *workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* A paged key/value cache in 8 bits: `pages` pages of page_size tokens (16,
+ * 32, 64 or 128) for `heads` key/value heads of head_dim channels (64 or 128).
+ *   k        int8 (pages, heads, page_size, head_dim)
+ *   v        int8 (pages, heads, head_dim, page_size): channel by channel, the
+ *            order in which the attention's second product reads it
+ *   k_scale, v_scale  fp32 (pages, heads): a code stands for code * scale
+ * k and v 16-byte aligned. */
+typedef struct wush_kv8_cache {
+    int8_t *k, *v;
+    float *k_scale, *v_scale;
+    int64_t pages;
+    int32_t heads, page_size, head_dim;
+} wush_kv8_cache;
+
+/* The batch that the next two take, all on the device: block_table (seqs,
+ * table_stride) int32, a sequence's pages in order; seq_lens (seqs) int32, each
+ * sequence's length INCLUDING the call's new tokens, which are its last ones; cu_q
+ * (seqs + 1) int32, where each sequence's new tokens begin among the `tokens` rows, from 0
+ * up to tokens, or NULL for one new token each (tokens == seqs).  A page number out
+ * of [0, pages) stands for no page: nothing is written there, and no query sees
+ * its tokens; so do tokens behind the table's end.  Rows that cu_q gives to no sequence are left
+ * out: their output is not written. */
+
+/* Rotates q and k by position, and puts k and v into the cache, of which the
+ * new tokens' pages change.  q (tokens, q_heads, head_dim), k, v (tokens, heads,
+ * head_dim), bf16 or fp16, each with a token and a head stride: strides = {q token, q head, k token,
+ * k head, v token, v head} in elements, multiples of 8, pointers 16-byte
+ * aligned.  Row p of cos_sin (positions, rot) fp32 holds rot / 2 cosines, then rot / 2 sines;
+ * positions behind its end take its last row.  The first rot channels (a
+ * multiple of 16, at most head_dim; 0: none, and cos_sin may be NULL) turn in pairs (i, i + rot / 2), or (2 i,
+ * 2 i + 1) if `interleaved`: (a, b) -> (a c - b s, b c + a s), each product and sum
+ * rounded to fp32.  q_out (tokens, q_heads, head_dim), contiguous, rounded once;
+ * q_heads = 0: none.
+ *   A (page, head)'s scale is s' = max(s, amax of its new tokens / 127, 2^-40),
+ * s counting only where it holds older tokens; new codes are
+ * clamp(rint(x * (1 / s')), -127, 127), older ones become rint(code * (s / s')).  A non-finite
+ * value makes its (page, head)'s scale NaN until the page is begun anew, and what attends to it NaN.
+ * Running the same call again changes nothing.  No two sequences of a call may
+ * write to one page. */
+int wush_kv8_append(const void *q, const void *k, const void *v, int dtype, const int64_t strides[6],
+                    const float *cos_sin, int64_t positions, int64_t rot, int interleaved,
+                    const wush_kv8_cache *cache, const int32_t *block_table, int64_t table_stride,
+                    const int32_t *seq_lens, const int32_t *cu_q, int64_t seqs, int64_t tokens, int64_t q_heads,
+                    void *q_out, hipStream_t stream);
+
+/* Attention of the new tokens' queries over the cache (their own keys and
+ * values already in it): for the query at position p of its sequence and query head hq, key/value
+ * head hq / (q_heads / heads),
+ *   out = sum_t softmax_t(cap(scale * q . k_t)) v_t over t in [max(0, p - window + 1), p]
+ * with window 0 for all t <= p, and cap(x) = softcap * tanh(x / softcap), softcap 0 for
+ * none.  A query that sees no token gets zeros.  q (tokens, q_heads, head_dim)
+ * bf16 or fp16 with a token and a head stride (multiples of 8, 16-byte aligned);
+ * out (tokens, q_heads, head_dim) contiguous, of the same type.
+ *   max_len: a bound of seq_lens that the host knows (0: the table's room). It only
+ * decides how the work is split.  The workspace, of at least
+ * wush_kv8_attention_workspace_bytes for the same arguments (ragged: whether
+ * cu_q is given), 16-byte aligned, holds partial results. */
+size_t wush_kv8_attention_workspace_bytes(const wush_kv8_cache *cache, int64_t seqs, int64_t tokens, int ragged,
+                                          int64_t q_heads, int64_t table_stride, int64_t window, int64_t max_len);
+int wush_kv8_attention(const void *q, int dtype, int64_t q_token_stride, int64_t q_head_stride,
+                       const wush_kv8_cache *cache, const int32_t *block_table, int64_t table_stride,
+                       const int32_t *seq_lens, const int32_t *cu_q, int64_t seqs, int64_t tokens, int64_t q_heads,
+                       float scale, int64_t window, float softcap, int64_t max_len, void *out, void *workspace,
+                       size_t workspace_bytes, hipStream_t stream);
+
+/* Pages as values: k, v (n, heads, page_size, head_dim) bf16 or fp16, code *
+ * scale rounded once, of the n pages listed (device int32).  A page number out
+ * of range gives NaN. */
+int wush_kv8_read(const wush_kv8_cache *cache, const int32_t *pages, int64_t n, int dtype, void *k, void *v,
+                  hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,6 +15,15 @@ LIB_PATH = os.path.join(_PKG, "libwush_int4.so")
 
 # Every symbol include/wush_int4.h declares, with its ctypes signature.
 _P, _I64, _I, _F, _SZ = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
+
+
+class Kv8Cache(ctypes.Structure):
+    """``wush_kv8_cache``: device pointers and sizes of a paged 8-bit cache."""
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("pages", _I64),
+                ("heads", ctypes.c_int32), ("page_size", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+_KV = ctypes.POINTER(Kv8Cache)
 SIGNATURES = {
     "wush_abi_version": ([], _I),
     "wush_init": ([], _I),
@@ -35,6 +44,17 @@ SIGNATURES = {
     "wush_mfma_selftest": ([_P, _P, _P, _P], _I),
     "wush_quant_int4_tensor_scale": ([_P, _P, _I64, _F, _P, _P], _I),
     "wush_gemm_s4_tensor_scale": ([_P, _P, _P, _I64, _I64, _I64, _F, _P, _P], _I),
+    "wush_quant_int8_token": ([_P, _I, _P, _P, _I64, _I64, _I64, _P], _I),
+    "wush_gemm_w8a8_workspace_bytes": ([_I64, _I64, _I64], _SZ),
+    "wush_gemm_w8a8": ([_P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _P, _SZ, _P], _I),
+    "wush_linear_w8a8_workspace_bytes": ([_I64, _I64, _I64], _SZ),
+    "wush_linear_w8a8": ([_P, _I64, _P, _P, _P, _I, _I64, _I64, _I64, _P, _SZ, _P], _I),
+    "wush_kv8_append": ([_P, _P, _P, _I, ctypes.POINTER(_I64), _P, _I64, _I64, _I, _KV, _P, _I64, _P, _P, _I64,
+                         _I64, _I64, _P, _P], _I),
+    "wush_kv8_attention_workspace_bytes": ([_KV, _I64, _I64, _I, _I64, _I64, _I64, _I64], _SZ),
+    "wush_kv8_attention": ([_P, _I, _I64, _I64, _KV, _P, _I64, _P, _P, _I64, _I64, _I64, _F, _I64, _F, _I64, _P, _P,
+                            _SZ, _P], _I),
+    "wush_kv8_read": ([_KV, _P, _I64, _I, _P, _P, _P], _I),
 }
 
 DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2

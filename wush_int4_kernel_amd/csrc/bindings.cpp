@@ -3,13 +3,16 @@
 // meaning, output dtypes/shapes and TORCH_CHECK error behaviour.  Each op
 // validates and allocates with torch on the input's device, takes torch's
 // current HIP stream, and calls the C ABI of libwush_int4.so
-// (include/wush_int4.h).  No computation happens here.
+// (include/wush_int4.h).  No computation happens here.  Behind them, the 8-bit
+// operators that the reference lacks (quant_int8_token, w8a8_*, kv8_*).
 #include <torch/extension.h>
 
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <cmath>
+#include <optional>
 #include <vector>
 
 #include "wush_int4.h"
@@ -349,6 +352,240 @@ torch::Tensor w4a4_gemm_cutlass_dev(torch::Tensor xq, torch::Tensor wq, torch::T
     return gemm_tensor_scale_impl(xq, wq, 0.0, &alpha, "w4a4_gemm_cutlass_dev");
 }
 
+// ------------------------------------------------------------- 8-bit operators
+int half_code(at::ScalarType dt, const char* name) {
+    TORCH_CHECK(dt == torch::kBFloat16 || dt == torch::kHalf, name, " must be bf16 or fp16, got ", dt);
+    return dt == torch::kBFloat16 ? WUSH_DTYPE_BF16 : WUSH_DTYPE_F16;
+}
+
+void check_gpu(const torch::Tensor& t, const char* name, const torch::Tensor& like) {
+    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(t.device() == like.device(), name, " is on ", t.device(), ", expected ", like.device());
+}
+
+void check_int8(const torch::Tensor& t, const char* name) {
+    TORCH_CHECK(t.scalar_type() == torch::kInt8 && t.is_contiguous(), name, " must be contiguous int8");
+}
+
+void check_f32(const torch::Tensor& t, const char* name) {
+    TORCH_CHECK(t.scalar_type() == torch::kFloat32 && t.is_contiguous(), name, " must be contiguous fp32");
+}
+
+bool aligned16(const torch::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0; }
+
+// x as rows of its last dimension that the kernels can read with 16-byte
+// loads: x itself where its rows lie evenly apart, else a contiguous copy.
+torch::Tensor token_rows(const torch::Tensor& x, int64_t& rows, int64_t& stride) {
+    const int64_t K = x.size(-1);
+    rows = K ? x.numel() / K : 0;
+    if (x.dim() == 2 && x.stride(1) == 1 && x.stride(0) >= K && x.stride(0) % 8 == 0 && aligned16(x)) {
+        stride = x.stride(0);
+        return x;
+    }
+    stride = K;
+    return x.is_contiguous() && aligned16(x) ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+int64_t check_w8(const torch::Tensor& x, const torch::Tensor& wq, const torch::Tensor& ws) {
+    check_gpu(wq, "wq", x);
+    check_gpu(ws, "ws", x);
+    check_int8(wq, "wq");
+    check_f32(ws, "ws");
+    TORCH_CHECK(x.dim() >= 1 && wq.dim() == 2, "x must have a last dimension and wq be 2D (N, K)");
+    const int64_t K = wq.size(1);
+    TORCH_CHECK(x.size(-1) == K, "K mismatch: x has ", x.size(-1), " columns, wq ", K);
+    TORCH_CHECK(ws.numel() == wq.size(0), "ws must hold one scale per row of wq");
+    TORCH_CHECK(K > 0 && K % 16 == 0 && K <= WUSH_W8A8_MAX_K, "K must be a multiple of 16 and at most ", WUSH_W8A8_MAX_K);
+    TORCH_CHECK(aligned16(wq), "wq must be 16-byte aligned");
+    return K;
+}
+
+torch::Tensor bytes_like(size_t n, const torch::Tensor& t) {
+    return n ? new_tensor({(int64_t)n}, torch::kUInt8, t) : torch::Tensor();
+}
+
+std::vector<torch::Tensor> quant_int8_token(torch::Tensor x) {
+    TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    const int dt = half_code(x.scalar_type(), "x");
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) % 16 == 0 && x.size(-1) <= WUSH_W8A8_MAX_K,
+                "last dim must be a multiple of 16 and at most ", WUSH_W8A8_MAX_K);
+    const at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    const int64_t K = x.size(-1);
+    int64_t rows, stride;
+    const auto xr = token_rows(x, rows, stride);
+    auto q = new_tensor(x.sizes(), torch::kInt8, x);
+    auto s = new_tensor(x.sizes().slice(0, x.dim() - 1), torch::kFloat32, x);
+    check_status(wush_quant_int8_token(xr.data_ptr(), dt, ptr<int8_t>(q), ptr<float>(s), rows, K, stride, current_stream(x)),
+                 "quant_int8_token");
+    return {q, s};
+}
+
+torch::Tensor w8a8_gemm(torch::Tensor xq, torch::Tensor xs, torch::Tensor wq, torch::Tensor ws, at::ScalarType dtype) {
+    TORCH_CHECK(xq.is_cuda(), "xq must be a CUDA tensor");
+    const int dt = half_code(dtype, "dtype");
+    const int64_t K = check_w8(xq, wq, ws);
+    check_gpu(xs, "xs", xq);
+    check_int8(xq, "xq");
+    check_f32(xs, "xs");
+    const int64_t M = xq.numel() / K, N = wq.size(0);
+    TORCH_CHECK(xs.numel() == M, "xs must hold one scale per row of xq");
+    TORCH_CHECK(aligned16(xq), "xq must be 16-byte aligned");
+    const at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(xq.device());
+    auto y = new_tensor(with_last(xq, N), dtype, xq);
+    const size_t wsb = wush_gemm_w8a8_workspace_bytes(M, N, K);
+    auto work = bytes_like(wsb, xq);
+    check_status(wush_gemm_w8a8(ptr<int8_t>(xq), ptr<float>(xs), ptr<int8_t>(wq), ptr<float>(ws), y.data_ptr(), dt, M, N, K,
+                                wsb ? work.data_ptr() : nullptr, wsb, current_stream(xq)),
+                 "w8a8_gemm");
+    return y;
+}
+
+torch::Tensor w8a8_linear(torch::Tensor x, torch::Tensor wq, torch::Tensor ws) {
+    TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    const int dt = half_code(x.scalar_type(), "x");
+    const int64_t K = check_w8(x, wq, ws), N = wq.size(0);
+    const at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    int64_t M, stride;
+    const auto xr = token_rows(x, M, stride);
+    auto y = new_tensor(with_last(x, N), x.scalar_type(), x);
+    const size_t wsb = wush_linear_w8a8_workspace_bytes(M, N, K);
+    auto work = bytes_like(wsb, x);
+    check_status(wush_linear_w8a8(xr.data_ptr(), stride, ptr<int8_t>(wq), ptr<float>(ws), y.data_ptr(), dt, M, N, K,
+                                  wsb ? work.data_ptr() : nullptr, wsb, current_stream(x)),
+                 "w8a8_linear");
+    return y;
+}
+
+wush_kv8_cache kv8_cache(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& ks, const torch::Tensor& vs,
+                         const torch::Tensor& like) {
+    check_gpu(k, "k_cache", like);
+    check_gpu(v, "v_cache", like);
+    check_gpu(ks, "k_scale", like);
+    check_gpu(vs, "v_scale", like);
+    check_int8(k, "k_cache");
+    check_int8(v, "v_cache");
+    check_f32(ks, "k_scale");
+    check_f32(vs, "v_scale");
+    TORCH_CHECK(k.dim() == 4 && v.dim() == 4, "k_cache must be (pages, heads, page_size, head_dim), v_cache (pages, heads, head_dim, page_size)");
+    const int64_t P = k.size(0), H = k.size(1), S = k.size(2), D = k.size(3);
+    TORCH_CHECK(v.size(0) == P && v.size(1) == H && v.size(2) == D && v.size(3) == S,
+                "v_cache must be (pages, heads, head_dim, page_size) of k_cache's sizes");
+    TORCH_CHECK(ks.numel() == P * H && vs.numel() == P * H, "k_scale and v_scale must be (pages, heads)");
+    TORCH_CHECK(D == 64 || D == 128, "head_dim must be 64 or 128, got ", D);
+    TORCH_CHECK(S == 16 || S == 32 || S == 64 || S == 128, "page_size must be 16, 32, 64 or 128, got ", S);
+    TORCH_CHECK(P > 0 && P <= 0x7fffffff && H > 0 && H <= 65535, "the cache must hold pages and heads");
+    TORCH_CHECK(aligned16(k) && aligned16(v), "the cache must be 16-byte aligned");
+    return {ptr<int8_t>(k), ptr<int8_t>(v), ptr<float>(ks), ptr<float>(vs), P, (int32_t)H, (int32_t)S, (int32_t)D};
+}
+
+void check_int32(const torch::Tensor& t, const char* name, const torch::Tensor& like) {
+    check_gpu(t, name, like);
+    TORCH_CHECK(t.scalar_type() == torch::kInt32 && t.is_contiguous(), name, " must be contiguous int32");
+}
+
+struct Kv8Batch {
+    int64_t seqs, tokens, table_stride;
+    const int32_t* cu;
+};
+
+Kv8Batch kv8_batch(const torch::Tensor& q, const torch::Tensor& table, const torch::Tensor& lens,
+                   const std::optional<torch::Tensor>& cu) {
+    check_int32(table, "block_table", q);
+    check_int32(lens, "seq_lens", q);
+    TORCH_CHECK(table.dim() == 2 && lens.dim() == 1 && lens.size(0) == table.size(0),
+                "block_table must be (sequences, pages) and seq_lens (sequences)");
+    Kv8Batch b{table.size(0), q.size(0), table.size(1), nullptr};
+    if (cu.has_value()) {
+        check_int32(*cu, "cu_q", q);
+        TORCH_CHECK(cu->dim() == 1 && cu->size(0) == b.seqs + 1, "cu_q must be (sequences + 1)");
+        b.cu = ptr<int32_t>(*cu);
+    } else {
+        TORCH_CHECK(b.tokens == b.seqs, "without cu_q there is one new token per sequence: got ", b.tokens, " tokens, ",
+                    b.seqs, " sequences");
+    }
+    return b;
+}
+
+// (tokens, heads, D) that the kernels can read: itself, or a contiguous copy
+torch::Tensor heads_view(const torch::Tensor& t) {
+    const bool ok = t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && aligned16(t);
+    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+torch::Tensor kv8_append(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cos_sin, torch::Tensor k_cache,
+                         torch::Tensor v_cache, torch::Tensor k_scale, torch::Tensor v_scale, torch::Tensor block_table,
+                         torch::Tensor seq_lens, std::optional<torch::Tensor> cu_q, bool interleaved) {
+    TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+    const int dt = half_code(q.scalar_type(), "q");
+    const auto c = kv8_cache(k_cache, v_cache, k_scale, v_scale, q);
+    check_gpu(k, "k", q);
+    check_gpu(v, "v", q);
+    TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k and v must be of one type");
+    TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3, "q, k and v must be (tokens, heads, head_dim)");
+    TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(1) == c.heads && k.size(2) == c.head_dim &&
+                    q.size(2) == c.head_dim,
+                "q, k and v must agree in tokens, and k and v with the cache's heads and head_dim");
+    check_gpu(cos_sin, "cos_sin", q);
+    check_f32(cos_sin, "cos_sin");
+    TORCH_CHECK(cos_sin.dim() == 2 && cos_sin.size(0) > 0 && cos_sin.size(1) % 16 == 0 && cos_sin.size(1) <= c.head_dim,
+                "cos_sin must be (positions, rotated channels): a multiple of 16, at most head_dim");
+    const auto b = kv8_batch(q, block_table, seq_lens, cu_q);
+    const at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q.device());
+    auto out = new_tensor(q.sizes(), q.scalar_type(), q);
+    if (b.tokens == 0 || b.seqs == 0) return out;
+    const auto qv = heads_view(q), kv = heads_view(k), vv = heads_view(v);
+    const int64_t strides[6] = {qv.stride(0), qv.stride(1), kv.stride(0), kv.stride(1), vv.stride(0), vv.stride(1)};
+    check_status(wush_kv8_append(qv.data_ptr(), kv.data_ptr(), vv.data_ptr(), dt, strides, ptr<float>(cos_sin),
+                                 cos_sin.size(0), cos_sin.size(1), interleaved, &c, ptr<int32_t>(block_table),
+                                 b.table_stride, ptr<int32_t>(seq_lens), b.cu, b.seqs, b.tokens, q.size(1), out.data_ptr(),
+                                 current_stream(q)),
+                 "kv8_append");
+    return out;
+}
+
+torch::Tensor kv8_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_scale,
+                            torch::Tensor v_scale, torch::Tensor block_table, torch::Tensor seq_lens,
+                            std::optional<torch::Tensor> cu_q, std::optional<double> scale, int64_t window, double softcap,
+                            int64_t max_len) {
+    TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+    const int dt = half_code(q.scalar_type(), "q");
+    const auto c = kv8_cache(k_cache, v_cache, k_scale, v_scale, q);
+    TORCH_CHECK(q.dim() == 3 && q.size(2) == c.head_dim, "q must be (tokens, heads, head_dim) of the cache's head_dim");
+    TORCH_CHECK(q.size(1) > 0 && q.size(1) % c.heads == 0, "q's heads must be a multiple of the cache's ", c.heads);
+    TORCH_CHECK(window >= 0 && max_len >= 0, "window and max_len must not be negative");
+    TORCH_CHECK(softcap >= 0.0 && std::isfinite(softcap), "softcap must be finite and not negative");
+    const auto b = kv8_batch(q, block_table, seq_lens, cu_q);
+    const at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q.device());
+    auto out = new_tensor(q.sizes(), q.scalar_type(), q);
+    if (b.tokens == 0 || b.seqs == 0) return out;
+    const auto qv = heads_view(q);
+    const size_t wsb = wush_kv8_attention_workspace_bytes(&c, b.seqs, b.tokens, b.cu != nullptr, q.size(1), b.table_stride,
+                                                          window, max_len);
+    auto work = bytes_like(wsb, q);
+    check_status(wush_kv8_attention(qv.data_ptr(), dt, qv.stride(0), qv.stride(1), &c, ptr<int32_t>(block_table),
+                                    b.table_stride, ptr<int32_t>(seq_lens), b.cu, b.seqs, b.tokens, q.size(1),
+                                    scale.has_value() ? (float)*scale : 1.0f / std::sqrt((float)c.head_dim), window,
+                                    (float)softcap, max_len, out.data_ptr(), wsb ? work.data_ptr() : nullptr, wsb,
+                                    current_stream(q)),
+                 "kv8_attention");
+    return out;
+}
+
+std::vector<torch::Tensor> kv8_read(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_scale,
+                                    torch::Tensor v_scale, torch::Tensor pages, at::ScalarType dtype) {
+    TORCH_CHECK(k_cache.is_cuda(), "k_cache must be a CUDA tensor");
+    const int dt = half_code(dtype, "dtype");
+    const auto c = kv8_cache(k_cache, v_cache, k_scale, v_scale, k_cache);
+    check_int32(pages, "pages", k_cache);
+    TORCH_CHECK(pages.dim() == 1, "pages must be one-dimensional");
+    const at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(k_cache.device());
+    const int64_t sizes[4] = {pages.size(0), c.heads, c.page_size, c.head_dim};
+    auto k = new_tensor(c10::IntArrayRef(sizes, 4), dtype, k_cache), v = new_tensor(c10::IntArrayRef(sizes, 4), dtype, k_cache);
+    check_status(wush_kv8_read(&c, ptr<int32_t>(pages), pages.size(0), dt, k.data_ptr(), v.data_ptr(), current_stream(k_cache)),
+                 "kv8_read");
+    return {k, v};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -393,5 +630,21 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("xs"), py::arg("wq"), py::arg("ws"));
     m.def("fused_transform_quant_int4_wmma", &fused_transform_quant_int4_wmma,
           "Fused WUSH transform + INT4 quantize (bit-exact)", py::arg("x"), py::arg("t"));
+    m.def("quant_int8_token", &quant_int8_token, "Per-token INT8 quantize: (codes int8, scales fp32)", py::arg("x"));
+    m.def("w8a8_gemm", &w8a8_gemm, "W8A8 matmul, scales per token and per output channel", py::arg("xq"), py::arg("xs"),
+          py::arg("wq"), py::arg("ws"), py::arg("dtype") = at::kHalf);
+    m.def("w8a8_linear", &w8a8_linear, "quant_int8_token and w8a8_gemm in one call; y of x's type", py::arg("x"),
+          py::arg("wq"), py::arg("ws"));
+    m.def("kv8_append", &kv8_append, "rotate q and k by position, put k and v into the 8-bit paged cache; returns q rotated",
+          py::arg("q"), py::arg("k"), py::arg("v"), py::arg("cos_sin"), py::arg("k_cache"), py::arg("v_cache"),
+          py::arg("k_scale"), py::arg("v_scale"), py::arg("block_table"), py::arg("seq_lens"), py::arg("cu_q") = py::none(),
+          py::arg("interleaved") = false);
+    m.def("kv8_attention", &kv8_attention, "causal attention over the 8-bit paged cache", py::arg("q"), py::arg("k_cache"),
+          py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("block_table"), py::arg("seq_lens"),
+          py::arg("cu_q") = py::none(), py::arg("scale") = py::none(), py::arg("window") = 0, py::arg("softcap") = 0.0,
+          py::arg("max_len") = 0);
+    m.def("kv8_read", &kv8_read, "pages of the 8-bit cache as values: (k, v), each (pages, heads, page_size, head_dim)",
+          py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("pages"),
+          py::arg("dtype") = at::kBFloat16);
     m.def("abi_version", &wush_abi_version, "C ABI version of libwush_int4.so");
 }
