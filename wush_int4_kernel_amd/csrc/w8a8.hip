@@ -36,19 +36,38 @@ __device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
     }
 }
 
-__device__ __forceinline__ uint32_t pack4(const float (&v)[8], int o, float inv) {
-    uint32_t w = 0;
+// Codes of eight values, and their largest magnitude.  Magnitudes are compared as
+// bits (sign cleared): a NaN's are above those of infinity, so that one
+// maximum finds both the scale and a non-finite value.
+template <int DT>
+__device__ __forceinline__ uint2 codes_of(const uint4& w, float inv) {
+    float v[8];
+    unpack8<DT>(w, v);
+    uint32_t o[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float r = __builtin_amdgcn_fmed3f(__builtin_rintf(v[o + i] * inv), -127.0f, 127.0f);
-        w |= ((uint32_t)(int)r & 0xffu) << (8 * i);
-    }
-    return w;
+    for (int i = 0; i < 8; ++i)
+        o[i >> 2] |= ((uint32_t)(int)__builtin_amdgcn_fmed3f(__builtin_rintf(v[i] * inv), -127.0f, 127.0f) & 0xffu) << (8 * (i & 3));
+    return make_uint2(o[0], o[1]);
+}
+__device__ __forceinline__ uint32_t largest8(const uint4& w) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    uint32_t mx = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mx = max(mx, max(u[j] & 0x7fffu, (u[j] >> 16) & 0x7fffu));
+    return mx;
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d));
+    return v;
+}
+template <int DT>
+__device__ __forceinline__ float token_scale(uint32_t largest) {
+    if (largest >= (DT == WUSH_DTYPE_BF16 ? 0x7f80u : 0x7c00u)) return __builtin_nanf("");
+    return fmaxf((DT == WUSH_DTYPE_BF16 ? bf16_to_f32(largest) : f16_to_f32(largest)) / 127.0f, kScaleFloor);
 }
 
-// One workgroup per row.  Largest magnitudes are compared as bits (sign
-// cleared): above those of infinity for a NaN, so one maximum finds both the
-// scale and a non-finite value.
+// One workgroup per row.
 template <int DT>
 __global__ __launch_bounds__(kQuantThreads) void quant_int8_token_kernel(const uint16_t* __restrict__ x,
                                                                          int8_t* __restrict__ q,
@@ -58,34 +77,112 @@ __global__ __launch_bounds__(kQuantThreads) void quant_int8_token_kernel(const u
     const uint4* px = reinterpret_cast<const uint4*>(x + row * stride);
     uint2* pq = reinterpret_cast<uint2*>(q + row * K);
     uint32_t mx = 0;
-    for (int i = threadIdx.x; i < K / 8; i += kQuantThreads) {
-        const uint4 w = px[i];
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) mx = max(mx, max(u[j] & 0x7fffu, (u[j] >> 16) & 0x7fffu));
-    }
+    for (int i = threadIdx.x; i < K / 8; i += kQuantThreads) mx = max(mx, largest8(px[i]));
     __shared__ uint32_t part[kQuantThreads / 64];
-#pragma unroll
-    for (int d = 32; d; d >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, d));
+    mx = wave_max(mx);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = mx;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kQuantThreads / 64; ++i) mx = max(mx, part[i]);
-    const bool bad = mx >= (DT == WUSH_DTYPE_BF16 ? 0x7f80u : 0x7c00u);
-    const float amax = DT == WUSH_DTYPE_BF16 ? bf16_to_f32(mx) : f16_to_f32(mx);
-    const float sc = bad ? __builtin_nanf("") : fmaxf(amax / 127.0f, kScaleFloor);
+    const float sc = token_scale<DT>(mx);
     if (threadIdx.x == 0) s[row] = sc;
+    const bool bad = sc != sc;
     const float inv = 1.0f / sc;
-    for (int i = threadIdx.x; i < K / 8; i += kQuantThreads) {
-        float v[8];
-        unpack8<DT>(px[i], v);
-        pq[i] = bad ? make_uint2(0, 0) : make_uint2(pack4(v, 0, inv), pack4(v, 4, inv));
-    }
+    for (int i = threadIdx.x; i < K / 8; i += kQuantThreads) pq[i] = bad ? make_uint2(0, 0) : codes_of<DT>(px[i], inv);
 }
 
 // y rows as fp16 or bf16, each rounded once from fp32
 __device__ __forceinline__ uint16_t out_bits(float f, int dt) {
     return dt == WUSH_DTYPE_F16 ? f32_to_f16_bits(f) : (uint16_t)(f != f ? 0x7fc0u : f32_to_bf16_rne(f));
+}
+
+// One or two rows of activations: the weight stream.  A wavefront takes whole
+// weight rows, 1 KiB of contiguous codes an instruction, four instructions ahead, and
+// multiplies on v_dot4_i32_i8 with the activation codes, which every workgroup holds in
+// LDS.  SRC: codes and scales given, or (a whole linear layer) made by every
+// workgroup for itself, while its first weights are on their way: that is
+// cheaper than a launch.
+enum { kCodes = -1 };                             // else the activations' dtype
+constexpr int kGemvWaves = 4, kGemvAhead = 4;
+
+template <int MM, int SRC>
+__global__ __launch_bounds__(64 * kGemvWaves) void w8a8_gemv_kernel(const void* __restrict__ xp, int64_t stride,
+                                                                    const float* __restrict__ xs,
+                                                                    const int8_t* __restrict__ wq,
+                                                                    const float* __restrict__ ws,
+                                                                    uint16_t* __restrict__ y, int dt, int N, int K) {
+    extern __shared__ __align__(16) uint8_t codes[];          // MM rows of Kp bytes, zero past K
+    __shared__ uint32_t part[MM][kGemvWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int chunks = (K + 1023) >> 10, Kp = chunks << 10;
+    const int total = (int)gridDim.x * kGemvWaves;
+    const int groups = (chunks + kGemvAhead - 1) / kGemvAhead;
+    int row = (int)blockIdx.x * kGemvWaves + wave;
+
+    // group g of row n; a lane past the row's end reads its last 16 bytes,
+    // which meet zero activations
+    v4i w[kGemvAhead];
+    auto fetch = [&](int n, int g) {
+        const int8_t* p = wq + (size_t)min(n, N - 1) * K;
+#pragma unroll
+        for (int u = 0; u < kGemvAhead; ++u)
+            w[u] = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(p + min((g * kGemvAhead + u) * 1024 + 16 * lane, K - 16)));
+    };
+    fetch(row, 0);
+
+    float sx[MM];
+#pragma unroll
+    for (int m = 0; m < MM; ++m) {
+        uint2* q = reinterpret_cast<uint2*>(codes + m * Kp);
+        if constexpr (SRC == kCodes) {
+            const uint2* x = reinterpret_cast<const uint2*>(static_cast<const int8_t*>(xp) + m * stride);
+            for (int i = tid; i < Kp / 8; i += 64 * kGemvWaves) q[i] = i < K / 8 ? x[i] : make_uint2(0, 0);
+            sx[m] = xs[m];
+        } else {
+            const uint4* x = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(xp) + m * stride);
+            uint32_t mx = 0;
+            for (int i = tid; i < K / 8; i += 64 * kGemvWaves) mx = max(mx, largest8(x[i]));
+            mx = wave_max(mx);
+            if (lane == 0) part[m][wave] = mx;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kGemvWaves; ++i) mx = max(mx, part[m][i]);
+            sx[m] = token_scale<SRC>(mx);
+            const bool bad = sx[m] != sx[m];
+            const float inv = 1.0f / sx[m];
+            for (int i = tid; i < Kp / 8; i += 64 * kGemvWaves) q[i] = i < K / 8 && !bad ? codes_of<SRC>(x[i], inv) : make_uint2(0, 0);
+        }
+    }
+    __syncthreads();
+
+    for (; row < N; row += total) {
+        int acc[MM] = {};
+        for (int g = 0; g < groups; ++g) {
+            v4i now[kGemvAhead];
+#pragma unroll
+            for (int u = 0; u < kGemvAhead; ++u) now[u] = w[u];
+            if (g + 1 < groups) fetch(row, g + 1);
+            else if (row + total < N) fetch(row + total, 0);
+#pragma unroll
+            for (int u = 0; u < kGemvAhead; ++u) {
+                const int c = g * kGemvAhead + u;
+                if (c >= chunks) break;
+#pragma unroll
+                for (int m = 0; m < MM; ++m) {
+                    const v4i x = *reinterpret_cast<const v4i*>(codes + m * Kp + c * 1024 + 16 * lane);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[m] = __builtin_amdgcn_sdot4(now[u][e], x[e], acc[m], false);
+                }
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MM; ++m) {
+            int v = acc[m];
+#pragma unroll
+            for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+            if (lane == 0) y[(size_t)m * N + row] = out_bits((float)v * sx[m] * ws[row], dt);
+        }
+    }
 }
 
 // Streaming product: 16 rows of activations (grid.y) against 16 CB weight rows
@@ -153,6 +250,59 @@ __global__ __launch_bounds__(64 * KW) void w8a8_stream_kernel(const int8_t* __re
     }
 }
 
+// ---------------------------------------------------------------- the choice
+// One or two rows whose codes fit 64 KiB of LDS take the GEMV.
+constexpr int kGemvRows = 2, kGemvLds = 64 * 1024;
+bool gemv_shape(int64_t M, int64_t K) { return M <= kGemvRows && M * ((K + 1023) / 1024 * 1024) <= kGemvLds; }
+
+struct Plan {
+    int rows, cols, splits;                       // rows 0: the streaming kernel
+};
+
+// K % 64 == 0 takes tiles: those, and the split of K, with the least estimated
+// time, in microseconds.  A workgroup's stage of 128 codes takes `stage` on a full
+// chip (fitted to 4096 x 57344 x 8192 and, for the small tiles, 16 and 64 x 57344 x
+// 8192), 0.7 of it on an empty one; the whole no less than the weights' way from HBM.  A
+// split costs a launch and its partial sums both ways.
+Plan plan_of(int64_t M, int64_t N, int64_t K, size_t room) {
+    Plan best = {0, 0, 1};
+    if (K % 64 != 0) return best;
+    static const struct { int rows, cols; double stage; } kTiles[] = {
+        {256, 256, 1.60}, {256, 128, 0.92}, {128, 128, 0.58}, {64, 128, 0.37}, {64, 64, 0.26}, {32, 128, 0.32}, {32, 64, 0.20}};
+    const int64_t stages = (K + 127) / 128;
+    double least = 1e30;
+    for (const auto& t : kTiles) {
+        if (t.rows > 32 && t.rows >= 2 * M) continue;
+        const int64_t tiles = ((M + t.rows - 1) / t.rows) * ((N + t.cols - 1) / t.cols);
+        for (int s = 1; s <= 8 && (s == 1 || stages / s >= 4); ++s) {
+            if (s > 1 && (size_t)M * N * 4 * s > room) break;
+            const double groups = (double)tiles * s, full = groups / 256 < 1 ? groups / 256 : 1;
+            const double rounds = groups <= 1024 ? (double)(int64_t)((groups + 255) / 256) : groups / 256;
+            const double work = rounds * (double)((stages + s - 1) / s) * t.stage * (0.7 + 0.3 * full);
+            const double hbm = (double)N * K / 6.3e6;
+            double us = 4.0 + 1.0 * rounds + (work > hbm ? work : hbm);
+            if (s > 1) us += 2.5 + (double)M * N * (8.0 * s + 2) / 4.5e6;
+            if (us < least) {
+                least = us;
+                best = {t.rows, t.cols, s};
+            }
+        }
+    }
+    return best;
+}
+
+template <int SRC>
+int launch_gemv(const void* x, int64_t stride, const float* xs, const int8_t* wq, const float* ws, void* y, int dtype,
+                int64_t M, int64_t N, int64_t K, hipStream_t stream) {
+    const int64_t want = (N + kGemvWaves - 1) / kGemvWaves;
+    const unsigned grid = (unsigned)(want < 2048 ? want : 2048);   // 8 workgroups a CU
+    const size_t lds = (size_t)M * ((K + 1023) / 1024 * 1024);
+    uint16_t* o = static_cast<uint16_t*>(y);
+    if (M == 1) w8a8_gemv_kernel<1, SRC><<<grid, 64 * kGemvWaves, lds, stream>>>(x, stride, xs, wq, ws, o, dtype, (int)N, (int)K);
+    else w8a8_gemv_kernel<2, SRC><<<grid, 64 * kGemvWaves, lds, stream>>>(x, stride, xs, wq, ws, o, dtype, (int)N, (int)K);
+    return (int)hipGetLastError();
+}
+
 }  // namespace
 }  // namespace wush
 
@@ -165,7 +315,7 @@ int wush_quant_int8_token(const void* x, int dtype, int8_t* q, float* s, int64_t
     if (rows == 0) return (int)hipSuccess;
     WUSH_REQUIRE(x && q && s && rows <= 0x7fffffffLL);
     WUSH_REQUIRE(((uintptr_t)x & 15u) == 0 && ((uintptr_t)q & 15u) == 0 && ((uintptr_t)s & 3u) == 0);
-    WUSH_REQUIRE(rows == 1 || (row_stride >= K && row_stride % 8 == 0));
+    WUSH_REQUIRE(rows == 1 || (row_stride >= 0 && row_stride % 8 == 0));
     const uint16_t* px = static_cast<const uint16_t*>(x);
     if (dtype == WUSH_DTYPE_BF16)
         wush::quant_int8_token_kernel<WUSH_DTYPE_BF16><<<(unsigned)rows, wush::kQuantThreads, 0, stream>>>(px, q, s, (int)K, row_stride);
@@ -174,25 +324,10 @@ int wush_quant_int8_token(const void* x, int dtype, int8_t* q, float* s, int64_t
     return (int)hipGetLastError();
 }
 
-size_t wush_gemm_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K) { return 0; }
-
-size_t wush_linear_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    if (M <= 0 || N <= 0 || K <= 0) return 0;
-    return (size_t)M * K + (((size_t)M * 4 + 15) & ~(size_t)15) + wush_gemm_w8a8_workspace_bytes(M, N, K);
-}
-
-int wush_linear_w8a8(const void* x, int64_t row_stride, const int8_t* wq, const float* ws, void* y, int dtype, int64_t M,
-                     int64_t N, int64_t K, void* workspace, size_t workspace_bytes, hipStream_t stream) {
-    WUSH_REQUIRE(M >= 0 && N >= 0 && K > 0 && K % 16 == 0 && K <= WUSH_W8A8_MAX_K && M <= 0x7fffffffLL);
-    if (M == 0 || N == 0) return (int)hipSuccess;
-    const size_t need = wush_linear_w8a8_workspace_bytes(M, N, K), scales = ((size_t)M * 4 + 15) & ~(size_t)15;
-    WUSH_REQUIRE(x && wq && ws && y && workspace && ((uintptr_t)workspace & 15u) == 0 && workspace_bytes >= need);
-    int8_t* q = static_cast<int8_t*>(workspace);
-    float* s = reinterpret_cast<float*>(q + (size_t)M * K);
-    const int st = wush_quant_int8_token(x, dtype, q, s, M, K, row_stride, stream);
-    if (st) return st;
-    return wush_gemm_w8a8(q, s, wq, ws, y, dtype, M, N, K, reinterpret_cast<uint8_t*>(s) + scales,
-                          workspace_bytes - (size_t)M * K - scales, stream);
+size_t wush_gemm_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0 || K % 16 != 0 || wush::gemv_shape(M, K)) return 0;
+    const wush::Plan p = wush::plan_of(M, N, K, SIZE_MAX);
+    return p.splits > 1 ? (size_t)p.splits * M * N * 4 : 0;
 }
 
 int wush_gemm_w8a8(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, void* y, int dtype, int64_t M,
@@ -204,10 +339,44 @@ int wush_gemm_w8a8(const int8_t* xq, const float* xs, const int8_t* wq, const fl
     WUSH_REQUIRE(xq && xs && wq && ws && y);
     WUSH_REQUIRE(((uintptr_t)xq & 15u) == 0 && ((uintptr_t)wq & 15u) == 0 && ((uintptr_t)xs & 3u) == 0 &&
                  ((uintptr_t)ws & 3u) == 0 && ((uintptr_t)y & 1u) == 0);
+    if (wush::gemv_shape(M, K)) return wush::launch_gemv<wush::kCodes>(xq, K, xs, wq, ws, y, dtype, M, N, K, stream);
+    uint16_t* o = static_cast<uint16_t*>(y);
+    const bool usable = workspace && ((uintptr_t)workspace & 15u) == 0;
+    const wush::Plan p = wush::plan_of(M, N, K, usable ? workspace_bytes : 0);
+    if (p.rows)
+        return wush::launch_gemm_w8a8(xq, xs, wq, ws, o, dtype, (int)M, (int)N, (int)K, p.rows, p.cols, p.splits,
+                                      static_cast<int*>(workspace), stream);
     const dim3 grid((unsigned)((N + 31) / 32), (unsigned)((M + 15) / 16));
     WUSH_REQUIRE(grid.y <= 65535u);
-    wush::w8a8_stream_kernel<2, 8><<<grid, 512, 0, stream>>>(xq, xs, wq, ws, static_cast<uint16_t*>(y), dtype, (int)M, (int)N, (int)K);
+    wush::w8a8_stream_kernel<2, 4><<<grid, 256, 0, stream>>>(xq, xs, wq, ws, o, dtype, (int)M, (int)N, (int)K);
     return (int)hipGetLastError();
+}
+
+size_t wush_linear_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0 || wush::gemv_shape(M, K)) return 0;
+    return (size_t)M * K + (((size_t)M * 4 + 15) & ~(size_t)15) + wush_gemm_w8a8_workspace_bytes(M, N, K);
+}
+
+int wush_linear_w8a8(const void* x, int64_t row_stride, const int8_t* wq, const float* ws, void* y, int dtype, int64_t M,
+                     int64_t N, int64_t K, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    WUSH_REQUIRE(M >= 0 && N >= 0 && K > 0 && K % 16 == 0 && K <= WUSH_W8A8_MAX_K);
+    WUSH_REQUIRE(M <= 0x7fffffffLL && N <= 0x7fffffffLL);
+    WUSH_REQUIRE(dtype == WUSH_DTYPE_BF16 || dtype == WUSH_DTYPE_F16);
+    if (M == 0 || N == 0) return (int)hipSuccess;
+    const size_t need = wush_linear_w8a8_workspace_bytes(M, N, K), scales = ((size_t)M * 4 + 15) & ~(size_t)15;
+    WUSH_REQUIRE(x && wq && ws && y && workspace_bytes >= need && (need == 0 || (workspace && ((uintptr_t)workspace & 15u) == 0)));
+    WUSH_REQUIRE((((uintptr_t)x | (uintptr_t)wq) & 15u) == 0 && ((uintptr_t)ws & 3u) == 0 && ((uintptr_t)y & 1u) == 0);
+    WUSH_REQUIRE(M == 1 || row_stride % 8 == 0);
+    if (wush::gemv_shape(M, K))
+        return dtype == WUSH_DTYPE_BF16
+                   ? wush::launch_gemv<WUSH_DTYPE_BF16>(x, row_stride, nullptr, wq, ws, y, dtype, M, N, K, stream)
+                   : wush::launch_gemv<WUSH_DTYPE_F16>(x, row_stride, nullptr, wq, ws, y, dtype, M, N, K, stream);
+    int8_t* q = static_cast<int8_t*>(workspace);
+    float* s = reinterpret_cast<float*>(q + (size_t)M * K);
+    const int st = wush_quant_int8_token(x, dtype, q, s, M, K, row_stride, stream);
+    if (st) return st;
+    return wush_gemm_w8a8(q, s, wq, ws, y, dtype, M, N, K, reinterpret_cast<uint8_t*>(s) + scales,
+                          workspace_bytes - (size_t)M * K - scales, stream);
 }
 
 }  // extern "C"
