@@ -4,8 +4,6 @@
 // See gemm_h16.hip for the numerics.
 #pragma once
 
-#include <utility>
-
 #include "wush_device.h"
 
 namespace wush {
@@ -167,16 +165,6 @@ __device__ __forceinline__ float h16_batch_scale(const uint32_t (&v)[kH16Batch],
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t u32v4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-
-// f(0), f(1), ..., f(N - 1) with compile-time arguments
-template <typename F, int... I>
-__device__ __forceinline__ void static_for_impl(F&& f, std::integer_sequence<int, I...>) {
-    (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, typename F>
-__device__ __forceinline__ void static_for(F&& f) {
-    static_for_impl(f, std::make_integer_sequence<int, N>{});
-}
 
 // c += a * b, accumulator in place.  The compiler does not know this is an
 // MFMA: the callers keep two instructions between a VALU write of an operand

@@ -1,0 +1,92 @@
+// kv8_attention.h -- what the attention kernels of the 8-bit cache share
+// (kv8_attention.hip: few query rows a sequence, and the joining of stretches;
+// kv8_chunk.hip: many).
+#pragma once
+
+#include "kv8_device.h"
+
+namespace wush {
+
+struct AttnArgs {
+    const uint16_t* q;
+    int64_t qt, qh;                               // token and head strides
+    Kv8Cache cache;
+    Kv8Batch batch;
+    int group, window;
+    int tile_rows;                                // query rows of a work item: 16, 128 or 256
+    int tile_shift;                               // log2 of it
+    int items;                                    // work items a key/value head
+    int splits, chunk;                            // stretches of the cache, tokens of one
+    float scale, cap;                             // cap 0: none
+    uint16_t* out;
+    float* part;                                  // (token, head, split): D sums, maximum, sum of weights, 2 unused
+};
+
+constexpr int kPartExtra = 4;                     // floats of a partial result behind its D sums
+
+namespace {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
+constexpr int kTile = 64;                         // tokens taken at a time
+constexpr float kLow = -3e38f;                    // running maximum before any token: below every score
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kValueFloor = 0x1p-40f;           // smallest scale of a page
+constexpr float kMostScale = 0x1p97f;             // times 2^15 * 127 * 128: scores stay finite
+
+// 8 int8 codes -> fp16, exact: code ^ 0x80 = code + 128 in the low byte of 1024.0
+__device__ __forceinline__ h8 codes8(uint32_t a, uint32_t b) {
+    a ^= 0x80808080u;
+    b ^= 0x80808080u;
+    const h2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+    const h2 r0 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u)) - bias;
+    const h2 r1 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u)) - bias;
+    const h2 r2 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) - bias;
+    const h2 r3 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) - bias;
+    return (h8){r0[0], r0[1], r1[0], r1[1], r2[0], r2[1], r3[0], r3[1]};
+}
+
+// A score in powers of two.  With a cap, x is 2 log2(e) score / cap: cap tanh(u) =
+// cap (1 - 2 / (1 + exp(2 u))), off by a few 2^-24 of the cap.
+template <bool CAP>
+__device__ __forceinline__ float capped(const AttnArgs& a, float x) {
+    if constexpr (!CAP) return x;
+    const float top = a.cap * kLog2e;
+    return __builtin_fmaf(-2.0f * top, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x)), top);
+}
+
+// Tokens that a work item's rows, beginning at row0 of their sequence, may see:
+// from base (a multiple of kTile) to end.
+struct Span {
+    int base, end;
+};
+__device__ __forceinline__ Span span_of(const AttnArgs& a, const Kv8Seq& s, int row0) {
+    const int before = s.len - s.count;           // position of the first new token
+    const int i0 = row0 / a.group, i1 = min((row0 + a.tile_rows - 1) / a.group, s.count - 1);
+    Span r;
+    r.base = a.window > 0 ? max(before + i0 - a.window + 1, 0) & ~(kTile - 1) : 0;
+    const int64_t room = a.batch.table_stride << a.cache.page_log2;
+    r.end = (int)min((int64_t)(before + i1 + 1), room);
+    return r;
+}
+
+// Work item of a head -> sequence and first row of it
+__device__ __forceinline__ int item_rows(const AttnArgs& a, int item, int& row0) {
+    const Kv8Batch& t = a.batch;
+    if (t.cu) {
+        const int b = kv8_find(t, item, a.group, a.tile_shift, 1);
+        row0 = (item - kv8_item_start(t, b, a.group, a.tile_shift, 1)) << a.tile_shift;
+        return b;
+    }
+    const int per = (a.group + a.tile_rows - 1) >> a.tile_shift;
+    row0 = (item % per) << a.tile_shift;
+    return item / per;
+}
+
+}  // namespace
+
+// kv8_chunk.hip: tiles of 128 or 256 rows
+int launch_kv8_chunk(const AttnArgs& a, int dtype, hipStream_t stream);
+
+}  // namespace wush

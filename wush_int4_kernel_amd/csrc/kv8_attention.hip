@@ -21,45 +21,13 @@
 // log2(v_scale), weights are exp2(t - running max + 12), at most 2^12, rounded once
 // to fp16 (11 bits, normal down to 2^-26 of the largest), and the sum of the
 // probabilities takes them back times 1 / v_scale, in fp32.
-#include "kv8_device.h"
+#include "kv8_attention.h"
 
 namespace wush {
 namespace {
 
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-
 constexpr int kWaves = 4;
-constexpr int kTile = 64;                         // tokens a wavefront takes at a time
-constexpr float kLow = -3e38f;                    // running maximum before any token: below every score
 constexpr float kHead = 12.0f;                    // weights reach 2^12
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kValueFloor = 0x1p-40f;           // smallest scale of a page
-constexpr float kMostScale = 0x1p97f;             // times 2^15 * 127 * 128: scores stay finite
-
-struct AttnArgs {
-    const uint16_t* q;
-    int64_t qt, qh;
-    Kv8Cache cache;
-    Kv8Batch batch;
-    int group, window, splits, chunk, items;
-    float scale, cap;                             // cap 0: none
-    uint16_t* out;
-    float* part;                                  // (token, head, split): D sums, maximum, sum of weights
-};
-
-// 8 int8 codes -> fp16, exact: code ^ 0x80 = code + 128 in the low byte of 1024.0
-__device__ __forceinline__ h8 codes8(uint32_t a, uint32_t b) {
-    a ^= 0x80808080u;
-    b ^= 0x80808080u;
-    const h2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
-    const h2 r0 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u)) - bias;
-    const h2 r1 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u)) - bias;
-    const h2 r2 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) - bias;
-    const h2 r3 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) - bias;
-    return (h8){r0[0], r0[1], r1[0], r1[1], r2[0], r2[1], r3[0], r3[1]};
-}
 
 __device__ __forceinline__ float quarters_max(float v) {
     v = fmaxf(v, __shfl_xor(v, 16));
@@ -68,21 +36,6 @@ __device__ __forceinline__ float quarters_max(float v) {
 __device__ __forceinline__ float quarters_sum(float v) {
     v += __shfl_xor(v, 16);
     return v + __shfl_xor(v, 32);
-}
-
-// Tokens that a tile of 16 rows beginning at row0 of its sequence may see:
-// from base (a multiple of kTile) to end.
-struct Span {
-    int base, end;
-};
-__device__ __forceinline__ Span span_of(const AttnArgs& a, const Kv8Seq& s, int row0) {
-    const int before = s.len - s.count;           // position of the first new token
-    const int i0 = row0 / a.group, i1 = min((row0 + 15) / a.group, s.count - 1);
-    Span r;
-    r.base = a.window > 0 ? max(before + i0 - a.window + 1, 0) & ~(kTile - 1) : 0;
-    const int64_t room = a.batch.table_stride << a.cache.page_log2;
-    r.end = (int)min((int64_t)(before + i1 + 1), room);
-    return r;
 }
 
 template <int DT, int D, bool CAP>
@@ -94,9 +47,8 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
     const int lg = a.cache.page_log2, ps = 1 << lg, G = a.group;
     const int split = blockIdx.x % a.splits;
     const int h = (int)(blockIdx.x / a.splits) % a.cache.heads, item = (int)(blockIdx.x / a.splits) / a.cache.heads;
-    const int per = (G + 15) >> 4;
-    const int b = t.cu ? kv8_find(t, item, G, 4, 1) : item / per;
-    const int row0 = 16 * (t.cu ? item - kv8_item_start(t, b, G, 4, 1) : item % per);
+    int row0;
+    const int b = item_rows(a, item, row0);
     const Kv8Seq s = kv8_seq(t, b);
     if (row0 >= s.count * G) return;
     const Span span = span_of(a, s, row0);
@@ -110,6 +62,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
     const int64_t tok = s.first + i;
     const int pos = s.len - s.count + i;
     const int low = a.window > 0 ? pos - a.window + 1 : 0;
+    const int last_low = s.len - s.count + min((row0 + 15) / G, s.count - 1) - a.window;   // tokens behind it are in every row's window
 
     h8 q[2 * NJ];
     float c;                                      // scores in powers of two, per unit of key scale
@@ -129,7 +82,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
         mx = quarters_max(mx);
         const int ex = mx > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(mx) : 0;
         const float up = __builtin_amdgcn_ldexpf(1.0f, ex > 100 ? 100 : ex);
-        c = a.scale * (CAP ? 1.0f / a.cap : kLog2e) / up;
+        c = a.scale * (CAP ? 2.0f * kLog2e / a.cap : kLog2e) / up;
         if (quarters_max(bad ? 1.0f : 0.0f) > 0.0f) c = __builtin_nanf("");
 #pragma unroll
         for (int j = 0; j < 2 * NJ; ++j)
@@ -144,60 +97,82 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
     float m = kLow, l = 0.0f;
     const int64_t tile_bytes = (int64_t)D << lg;
     const int32_t* table = t.table + (int64_t)b * t.table_stride;
+    constexpr int kStep = kWaves * kTile;
 
-    for (int t0 = begin + wave * kTile; t0 < end; t0 += kWaves * kTile) {
-        // pages of the keys this lane loads and of the tokens whose scores it holds
-        auto page_of = [&](int tk) {
-            const int id = tk < end ? table[tk >> lg] : -1;
-            return id >= 0 && id < a.cache.pages ? id : -1;
-        };
-        const int tk = t0 + 16 * (l16 >> 2), tv = t0 + 16 * kq;
-        const int idk = page_of(tk), idv = page_of(tv);
+    // The pages of the keys that this lane loads (four 16-token groups, one of
+    // them by l16) and of the 16 tokens whose scores it holds (by kq); -1: none.
+    auto page_of = [&](int tk) {
+        const int id = table[min(tk, end - 1) >> lg];
+        return tk < end && (uint32_t)id < (uint64_t)a.cache.pages ? id : -1;
+    };
+    const int ok = 16 * (l16 >> 2), ov = 16 * kq;
+    uint4 kk[4][NJ], vv[NB];
+    float ks, vs;
+    auto load_keys = [&](int t0, int idk, int idv) {
         const int8_t* pk = a.cache.k + ((int64_t)max(idk, 0) * a.cache.heads + h) * tile_bytes +
-                           ((tk & (ps - 1)) + (l16 & 3)) * D + 16 * kq;
-        const int64_t vt = (int64_t)max(idv, 0) * a.cache.heads + h;
-        const int8_t* pv = a.cache.v + vt * tile_bytes + (l16 << lg) + (tv & (ps - 1));
-        uint4 kk[4][NJ], vv[NB];
+                           (((t0 + ok) & (ps - 1)) + (l16 & 3)) * D + 16 * kq;
 #pragma unroll
         for (int n = 0; n < 4; ++n)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) kk[n][j] = *reinterpret_cast<const uint4*>(pk + 4 * n * D + 64 * j);
+            for (int j = 0; j < NJ; ++j) kk[n][j] = load_nt16(pk + 4 * n * D + 64 * j);
+        const int64_t vt = (int64_t)max(idv, 0) * a.cache.heads + h;
+        ks = a.cache.ks[vt];
+        vs = a.cache.vs[vt];
+    };
+    auto load_values = [&](int t0, int idv) {
+        const int8_t* pv = a.cache.v + ((int64_t)max(idv, 0) * a.cache.heads + h) * tile_bytes + (l16 << lg) + ((t0 + ov) & (ps - 1));
 #pragma unroll
-        for (int d = 0; d < NB; ++d) vv[d] = *reinterpret_cast<const uint4*>(pv + ((int64_t)d << (lg + 4)));
-        const float ks = a.cache.ks[vt];
-        float vs = a.cache.vs[vt];
-        if (vs < kValueFloor) vs = kValueFloor;
+        for (int d = 0; d < NB; ++d) vv[d] = load_nt16(pv + ((int64_t)d << (lg + 4)));
+    };
 
+    // One tile.  A tile's keys go out while the last tile's weights are made, its
+    // values behind the last tile's products: the registers that held those take
+    // them.  Behind the end nothing goes out.
+    auto tile = [&](int t0, int idv, bool masked, auto&& keys_ahead, auto&& values_ahead) {
         v4f sc[4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            sc[n] = zero;
+        for (int n = 0; n < 4; ++n) sc[n] = zero;
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
+        for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
                 sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(kk[n][j].x, kk[n][j].y), q[2 * j], sc[n], 0, 0, 0);
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
                 sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(kk[n][j].z, kk[n][j].w), q[2 * j + 1], sc[n], 0, 0, 0);
-            }
+            __builtin_amdgcn_sched_barrier(0);    // codes are not converted ahead: that takes twice their registers
         }
-        // the lane's 16 tokens tv .. tv + 15, of one page
+        // the lane's 16 tokens, of one page
         float cs = c * ks;
         if (fabsf(cs) > kMostScale) cs = __builtin_copysignf(kMostScale, cs);
-        const float lv = __builtin_amdgcn_logf(vs);
-        const int last = idv >= 0 ? min(pos, end - 1) : -1;
+        const float fv = vs < kValueFloor ? kValueFloor : vs;
+        const float lv = __builtin_amdgcn_logf(fv);
+        __builtin_amdgcn_sched_barrier(0);
+        keys_ahead();
+        __builtin_amdgcn_sched_barrier(0);
+        const int tv = t0 + ov, last = idv >= 0 ? min(pos, end - 1) : -1;
         float top = kLow;
 #pragma unroll
         for (int n = 0; n < 4; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                float x = sc[n][e] * cs;
-                if constexpr (CAP) x = (a.cap * kLog2e) * (1.0f - 2.0f / (1.0f + __builtin_amdgcn_exp2f(x * (2.0f * kLog2e))));
-                x += lv;
-                const int at = tv + 4 * n + e;
-                x = at <= last && at >= low ? x : -__builtin_inff();
-                sc[n][e] = x;
-                top = fmaxf(top, x);
+                sc[n][e] = capped<CAP>(a, sc[n][e] * cs) + lv;
             }
+        if (masked) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int at = tv + 4 * n + e;
+                    sc[n][e] = at <= last && at >= low ? sc[n][e] : -__builtin_inff();
+                }
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, sc[n][e]);
         const float mn = fmaxf(m, quarters_max(top));
-        const float fade = __builtin_amdgcn_exp2f(m - mn);
+        const float fade = __builtin_amdgcn_exp2f(m - mn), less = mn - kHead;
         m = mn;
         float sum = 0.0f;
         h8 p[2];
@@ -205,17 +180,40 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
         for (int n = 0; n < 4; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float w = __builtin_amdgcn_exp2f(sc[n][e] - (mn - kHead));
+                const float w = __builtin_amdgcn_exp2f(sc[n][e] - less);
                 sum += w;
                 p[n >> 1][4 * (n & 1) + e] = (_Float16)w;
             }
-        l = l * fade + (sum != 0.0f ? sum * (1.0f / vs) : 0.0f);   // a scale may be NaN where nothing is seen
+        l = l * fade + (sum != 0.0f ? sum * (1.0f / fv) : 0.0f);  // a scale may be NaN where nothing is seen
 #pragma unroll
         for (int d = 0; d < NB; ++d) {
             acc[d] *= fade;
             acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vv[d].x, vv[d].y), p[0], acc[d], 0, 0, 0);
             acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vv[d].z, vv[d].w), p[1], acc[d], 0, 0, 0);
+            if (d & 1) __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        values_ahead();
+    };
+
+    int t0 = begin + wave * kTile;
+    if (t0 < end) {
+        int idk = page_of(t0 + ok), idv = page_of(t0 + ov);
+        load_keys(t0, idk, idv);
+        load_values(t0, idv);
+        int nk = page_of(t0 + kStep + ok), nv = page_of(t0 + kStep + ov);
+        const int least = s.len - s.count + row0 / G;             // the smallest position of these rows
+        for (; t0 + kStep < end; t0 += kStep) {
+            const int nnk = page_of(t0 + 2 * kStep + ok), nnv = page_of(t0 + 2 * kStep + ov);
+            const auto keys = [&] { load_keys(t0 + kStep, nk, nv); };
+            const auto values = [&] { load_values(t0 + kStep, nv); };
+            const bool inside = t0 + kTile - 1 <= least && (a.window == 0 || t0 > last_low) && __all(idv >= 0);
+            tile(t0, idv, !inside, keys, values);
+            idv = nv;
+            nk = nnk;
+            nv = nnv;
+        }
+        tile(t0, idv, true, [] {}, [] {});
     }
 
     // join the wavefronts: a lane holds channels 16 d + 4 kq + e of row l16
@@ -253,7 +251,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
             *reinterpret_cast<uint32_t*>(a.out + row * D + d0 + e) = out16<DT>(o[e] * inv) | out16<DT>(o[e + 1] * inv) << 16;
         return;
     }
-    float* part = a.part + (row * a.splits + split) * (D + 2);
+    float* part = a.part + (row * a.splits + split) * (D + kPartExtra);
 #pragma unroll
     for (int e = 0; e < PD; ++e) part[d0 + e] = o[e];
     if (d0 == 0) {
@@ -262,34 +260,59 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
     }
 }
 
-// One wavefront per (token, query head): the stretches that hold tokens, joined.
+// One workgroup per (token, query head): the stretches that hold tokens, joined.
+// The wavefronts take every fourth stretch, four at a time so that their loads overlap.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void kv8_join_kernel(const AttnArgs a) {
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Kv8Batch& t = a.batch;
     const int heads = a.cache.heads * a.group;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= (int64_t)t.tokens * heads) return;
+    const int64_t row = blockIdx.x;
     const int tok = (int)(row / heads);
     const int b = t.cu ? kv8_find(t, tok, 1, 0, 0) : tok;
     const Kv8Seq s = kv8_seq(t, b);
     const int i = tok - s.first;
     if (i < 0 || i >= s.count) return;
-    const Span span = span_of(a, s, (i * a.group + (int)(row % a.group)) & ~15);
+    const Span span = span_of(a, s, (i * a.group + (int)(row % a.group)) & ~(a.tile_rows - 1));
     const int n = min(a.splits, max((span.end - span.base + a.chunk - 1) / a.chunk, 1));
-    const float* part = a.part + row * a.splits * (D + 2);
+    constexpr int PD = D / 64;
+    typedef float vpd __attribute__((ext_vector_type(PD)));
+    const float* part = a.part + row * a.splits * (D + kPartExtra);
     float mm = kLow;
-    for (int k = lane; k < n; k += 64) mm = fmaxf(mm, part[(int64_t)k * (D + 2) + D]);
+    for (int k = lane; k < n; k += 64) mm = fmaxf(mm, part[(int64_t)k * (D + kPartExtra) + D]);
 #pragma unroll
     for (int d = 32; d; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
-    constexpr int PD = D / 64;
-    float ll = 0.0f, o[PD] = {};
-    for (int k = 0; k < n; ++k) {
-        const float* p = part + (int64_t)k * (D + 2);
-        const float f = __builtin_amdgcn_exp2f(p[D] - mm);
-        ll += p[D + 1] * f;
+    float ll = 0.0f;
+    vpd o = 0.0f;
+    for (int k0 = wave; k0 < n; k0 += 16) {
+        vpd v[4];
+        float f[4], w[4];
 #pragma unroll
-        for (int e = 0; e < PD; ++e) o[e] += p[lane * PD + e] * f;
+        for (int u = 0; u < 4; ++u) {
+            const float* p = part + (int64_t)min(k0 + 4 * u, n - 1) * (D + kPartExtra);
+            v[u] = *reinterpret_cast<const vpd*>(p + lane * PD);
+            f[u] = p[D];
+            w[u] = p[D + 1];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float g = k0 + 4 * u < n ? __builtin_amdgcn_exp2f(f[u] - mm) : 0.0f;
+            if (k0 + 4 * u < n) {
+                ll += w[u] * g;
+                o += v[u] * g;
+            }
+        }
+    }
+    __shared__ vpd so[4][64];
+    __shared__ float sl[4];
+    so[wave][lane] = o;
+    if (lane == 0) sl[wave] = ll;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+        o += so[w][lane];
+        ll += sl[w];
     }
     const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll
@@ -297,24 +320,39 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(const AttnArgs a) {
 }
 
 struct Plan {
-    int splits, chunk;
+    int tile_rows, splits, chunk;
     int64_t items;
 };
 
-// Stretches of the cache per row tile: about 1024 workgroups, four to a CU.
+// Tile height: 16-row items (kv8_rows_kernel) below 64 rows a sequence on average,
+// where taller ones would be mostly empty; 256-row workgroups where they fill the
+// chip, else 128.  Then the stretches of the cache per item with the least estimated
+// time, in microseconds: a workgroup's pass over `step` tokens times the workgroups of
+// a CU, and where there is more than one stretch the joining.
 Plan plan_of(const Kv8Cache& c, int64_t seqs, int64_t tokens, bool ragged, int group, int64_t table_stride, int window,
              int64_t max_len) {
     Plan p;
-    p.items = ragged ? (tokens * group >> 4) + seqs : seqs * ((group + 15) / 16);
+    const int64_t rows = tokens * group;
+    p.tile_rows = rows < 64 * seqs ? 16 : (rows / 256 + seqs) * c.heads >= 256 ? 256 : 128;
+    p.items = ragged ? rows / p.tile_rows + seqs : seqs * ((group + p.tile_rows - 1) / p.tile_rows);
     int64_t range = table_stride << c.page_log2;
     if (max_len > 0 && max_len < range) range = max_len;
-    if (window > 0 && window + 128 < range) range = window + 128;
+    if (window > 0 && window + 64 + p.tile_rows / group < range) range = window + 64 + p.tile_rows / group;
     if (range < 1) range = 1;
     if (range > 1 << 30) range = 1 << 30;         // the last stretch takes what lies behind
-    const int64_t step = kWaves * kTile, most = (range + step - 1) / step;
-    int64_t splits = 1024 / (p.items * c.heads);
-    splits = splits < 1 ? 1 : splits > most ? most : splits;
-    p.chunk = (int)((most + splits - 1) / splits * step);
+    const int64_t step = p.tile_rows == 16 ? 256 : kTile, most = (range + step - 1) / step;
+    const double pass = (p.tile_rows == 16 ? 2.5 : 1.5) * c.dim / 128;
+    double least = 1e30;
+    p.splits = 1;
+    for (int64_t n = 1; n <= most && n <= 256 && (n == 1 || p.items * c.heads * n <= 1024); n += n < 16 ? 1 : n / 16) {
+        const int64_t passes = (most + n - 1) / n, groups = p.items * c.heads * n;
+        const double us = pass * (double)passes * (double)((groups + 255) / 256) + (n > 1 ? 3.0 + 0.03 * (double)n : 0.0);
+        if (us < least) {
+            least = us;
+            p.splits = (int)n;
+        }
+    }
+    p.chunk = (int)((most + p.splits - 1) / p.splits * step);
     p.splits = (int)((range + p.chunk - 1) / p.chunk);
     return p;
 }
@@ -324,13 +362,19 @@ int launch(const AttnArgs& a, hipStream_t stream) {
     const int64_t blocks = (int64_t)a.items * a.cache.heads * a.splits;
     const int64_t rows = (int64_t)a.batch.tokens * a.cache.heads * a.group;
     WUSH_REQUIRE(blocks <= 0x7fffffffLL && rows <= 0x7fffffffLL);
-    const dim3 grid((unsigned)blocks), join((unsigned)((rows + 3) / 4));
+    if (a.tile_rows > 16) {
+        const int st = launch_kv8_chunk(a, DT, stream);
+        if (st) return st;
+    }
+    const dim3 grid((unsigned)blocks), join((unsigned)rows);
     if (a.cache.dim == 64) {
-        if (a.cap > 0.0f) kv8_rows_kernel<DT, 64, true><<<grid, 64 * kWaves, 0, stream>>>(a);
+        if (a.tile_rows > 16) {}
+        else if (a.cap > 0.0f) kv8_rows_kernel<DT, 64, true><<<grid, 64 * kWaves, 0, stream>>>(a);
         else kv8_rows_kernel<DT, 64, false><<<grid, 64 * kWaves, 0, stream>>>(a);
         if (a.splits > 1) kv8_join_kernel<DT, 64><<<join, 256, 0, stream>>>(a);
     } else {
-        if (a.cap > 0.0f) kv8_rows_kernel<DT, 128, true><<<grid, 64 * kWaves, 0, stream>>>(a);
+        if (a.tile_rows > 16) {}
+        else if (a.cap > 0.0f) kv8_rows_kernel<DT, 128, true><<<grid, 64 * kWaves, 0, stream>>>(a);
         else kv8_rows_kernel<DT, 128, false><<<grid, 64 * kWaves, 0, stream>>>(a);
         if (a.splits > 1) kv8_join_kernel<DT, 128><<<join, 256, 0, stream>>>(a);
     }
@@ -348,7 +392,7 @@ size_t wush_kv8_attention_workspace_bytes(const wush_kv8_cache* cache, int64_t s
     if (wush::kv8_cache_of(cache, &c) || seqs <= 0 || tokens <= 0 || q_heads <= 0 || q_heads % c.heads) return 0;
     const int w = window <= 0 || window > 0x7fffffff ? 0 : (int)window;
     const wush::Plan p = wush::plan_of(c, seqs, tokens, ragged != 0, (int)(q_heads / c.heads), table_stride, w, max_len);
-    return p.splits > 1 ? (size_t)tokens * q_heads * p.splits * (c.dim + 2) * 4 : 0;
+    return p.splits > 1 ? (size_t)tokens * q_heads * p.splits * (c.dim + wush::kPartExtra) * 4 : 0;
 }
 
 int wush_kv8_attention(const void* q, int dtype, int64_t q_token_stride, int64_t q_head_stride,
@@ -378,6 +422,8 @@ int wush_kv8_attention(const void* q, int dtype, int64_t q_token_stride, int64_t
     a.window = window > 0x7fffffff ? 0 : (int)window;
     const wush::Plan p = wush::plan_of(a.cache, seqs, tokens, cu_q != nullptr, a.group, table_stride, a.window, max_len);
     WUSH_REQUIRE(p.items <= 0x7fffffffLL);
+    a.tile_rows = p.tile_rows;
+    a.tile_shift = __builtin_ctz(p.tile_rows);
     a.splits = p.splits;
     a.chunk = p.chunk;
     a.items = (int)p.items;

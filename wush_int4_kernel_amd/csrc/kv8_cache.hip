@@ -253,6 +253,7 @@ __global__ __launch_bounds__(kThreads) void kv8_read_kernel(const Kv8Cache c, co
 int kv8_cache_of(const wush_kv8_cache* c, Kv8Cache* out) {
     WUSH_REQUIRE(c && c->k && c->v && c->k_scale && c->v_scale);
     WUSH_REQUIRE(c->pages > 0 && c->pages <= 0x7fffffffLL && c->heads > 0 && c->heads <= 65535);
+    WUSH_REQUIRE(c->pages * c->heads <= 0x7fffffffLL);            // tiles: 2 TB and more beyond
     WUSH_REQUIRE(c->head_dim == 64 || c->head_dim == 128);
     WUSH_REQUIRE(c->page_size == 16 || c->page_size == 32 || c->page_size == 64 || c->page_size == 128);
     WUSH_REQUIRE((((uintptr_t)c->k | (uintptr_t)c->v) & 15u) == 0 &&

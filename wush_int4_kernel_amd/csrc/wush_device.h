@@ -11,6 +11,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <utility>
+
 #define WUSH_HOST_DEVICE __host__ __device__ __forceinline__
 
 namespace wush {
@@ -320,6 +322,16 @@ __device__ __forceinline__ void dma4(const void* g, uint32_t lds) {
 }
 __device__ __forceinline__ void dma16_ordered(const void* g, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(g), "s"(lds) : "m0", "memory");
+}
+
+// f(0), f(1), ..., f(N - 1) with compile-time arguments
+template <typename F, int... I>
+__device__ __forceinline__ void static_for_impl(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+    static_for_impl(f, std::make_integer_sequence<int, N>{});
 }
 
 // s_waitcnt vmcnt(n) (n < 64) with the other counters left alone, and a
