@@ -260,21 +260,32 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
     }
 }
 
-// One workgroup per (token, query head): the stretches that hold tokens, joined.
-// The wavefronts take every fourth stretch, four at a time so that their loads overlap.
+// The stretches that hold tokens of a (token, query head), joined: by one
+// wavefront, or, where there are more than kFewSplits, by a workgroup's four, which
+// take every fourth stretch.  Four stretches at a time, so that their loads overlap.
+constexpr int kFewSplits = 16;
+
 template <int DT, int D>
 __global__ __launch_bounds__(256) void kv8_join_kernel(const AttnArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Kv8Batch& t = a.batch;
     const int heads = a.cache.heads * a.group;
-    const int64_t row = blockIdx.x;
+    const bool few = a.splits <= kFewSplits;
+    const int64_t row = few ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+    const int first = few ? 0 : wave, by = few ? 1 : 4;
     const int tok = (int)(row / heads);
-    const int b = t.cu ? kv8_find(t, tok, 1, 0, 0) : tok;
-    const Kv8Seq s = kv8_seq(t, b);
-    const int i = tok - s.first;
-    if (i < 0 || i >= s.count) return;
-    const Span span = span_of(a, s, (i * a.group + (int)(row % a.group)) & ~(a.tile_rows - 1));
-    const int n = min(a.splits, max((span.end - span.base + a.chunk - 1) / a.chunk, 1));
+    bool mine = tok < t.tokens;
+    int n = 0;
+    if (mine) {
+        const int b = t.cu ? kv8_find(t, tok, 1, 0, 0) : tok;
+        const Kv8Seq s = kv8_seq(t, b);
+        const int i = tok - s.first;
+        mine = i >= 0 && i < s.count;
+        if (mine) {
+            const Span span = span_of(a, s, (i * a.group + (int)(row % a.group)) & ~(a.tile_rows - 1));
+            n = min(a.splits, max((span.end - span.base + a.chunk - 1) / a.chunk, 1));
+        }
+    }
     constexpr int PD = D / 64;
     typedef float vpd __attribute__((ext_vector_type(PD)));
     const float* part = a.part + row * a.splits * (D + kPartExtra);
@@ -284,39 +295,42 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(const AttnArgs a) {
     for (int d = 32; d; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
     float ll = 0.0f;
     vpd o = 0.0f;
-    for (int k0 = wave; k0 < n; k0 += 16) {
+    for (int k0 = first; k0 < n; k0 += 4 * by) {
         vpd v[4];
         float f[4], w[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const float* p = part + (int64_t)min(k0 + 4 * u, n - 1) * (D + kPartExtra);
+            const float* p = part + (int64_t)min(k0 + by * u, n - 1) * (D + kPartExtra);
             v[u] = *reinterpret_cast<const vpd*>(p + lane * PD);
             f[u] = p[D];
             w[u] = p[D + 1];
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const float g = k0 + 4 * u < n ? __builtin_amdgcn_exp2f(f[u] - mm) : 0.0f;
-            if (k0 + 4 * u < n) {
+        for (int u = 0; u < 4; ++u)
+            if (k0 + by * u < n) {
+                const float g = __builtin_amdgcn_exp2f(f[u] - mm);
                 ll += w[u] * g;
                 o += v[u] * g;
             }
+    }
+    if (!few) {
+        __shared__ vpd so[4][64];
+        __shared__ float sl[4];
+        so[wave][lane] = o;
+        if (lane == 0) sl[wave] = ll;
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int w = 1; w < 4; ++w) {
+            o += so[w][lane];
+            ll += sl[w];
         }
     }
-    __shared__ vpd so[4][64];
-    __shared__ float sl[4];
-    so[wave][lane] = o;
-    if (lane == 0) sl[wave] = ll;
-    __syncthreads();
-    if (wave) return;
-#pragma unroll
-    for (int w = 1; w < 4; ++w) {
-        o += so[w][lane];
-        ll += sl[w];
-    }
+    if (!mine) return;
     const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-#pragma unroll
-    for (int e = 0; e < PD; ++e) a.out[row * D + lane * PD + e] = (uint16_t)out16<DT>(o[e] * inv);
+    uint16_t* out = a.out + row * D + lane * PD;
+    if constexpr (PD == 2) *reinterpret_cast<uint32_t*>(out) = out16<DT>(o[0] * inv) | out16<DT>(o[1] * inv) << 16;
+    else *out = (uint16_t)out16<DT>(o[0] * inv);
 }
 
 struct Plan {
@@ -342,11 +356,12 @@ Plan plan_of(const Kv8Cache& c, int64_t seqs, int64_t tokens, bool ragged, int g
     if (range > 1 << 30) range = 1 << 30;         // the last stretch takes what lies behind
     const int64_t step = p.tile_rows == 16 ? 256 : kTile, most = (range + step - 1) / step;
     const double pass = (p.tile_rows == 16 ? 2.5 : 1.5) * c.dim / 128;
+    const double joined = 0.02 + (double)rows * c.heads * (c.dim + kPartExtra) * 8 / 4e6;   // a stretch's sums both ways
     double least = 1e30;
     p.splits = 1;
     for (int64_t n = 1; n <= most && n <= 256 && (n == 1 || p.items * c.heads * n <= 1024); n += n < 16 ? 1 : n / 16) {
         const int64_t passes = (most + n - 1) / n, groups = p.items * c.heads * n;
-        const double us = pass * (double)passes * (double)((groups + 255) / 256) + (n > 1 ? 3.0 + 0.03 * (double)n : 0.0);
+        const double us = pass * (double)passes * (double)((groups + 255) / 256) + (n > 1 ? 3.0 + joined * (double)n : 0.0);
         if (us < least) {
             least = us;
             p.splits = (int)n;
@@ -366,7 +381,7 @@ int launch(const AttnArgs& a, hipStream_t stream) {
         const int st = launch_kv8_chunk(a, DT, stream);
         if (st) return st;
     }
-    const dim3 grid((unsigned)blocks), join((unsigned)rows);
+    const dim3 grid((unsigned)blocks), join((unsigned)(a.splits <= kFewSplits ? (rows + 3) / 4 : rows));
     if (a.cache.dim == 64) {
         if (a.tile_rows > 16) {}
         else if (a.cap > 0.0f) kv8_rows_kernel<DT, 64, true><<<grid, 64 * kWaves, 0, stream>>>(a);

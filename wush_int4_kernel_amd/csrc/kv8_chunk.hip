@@ -9,10 +9,10 @@
 // which are, in the order that the values are put down in, its operand of the second product.
 //
 // Wavefronts alternate between a matrix phase, the second product of tile t - 1
-// and the first of tile t, and a vector phase, tile t's weights and the staging of its
-// share of the next tiles.  The workgroup's second half runs one phase behind the first,
-// with a barrier between phases: of a SIMD's two wavefronts one feeds the matrix cores while the other
-// computes (both in step, neither unit was busy more than 60%: 2.7 us a tile).
+// and the first of tile t with the staging of a share of the next tiles among them, and a vector
+// phase, tile t's weights.  The workgroup's second half runs one phase behind the first, with a
+// barrier between phases: of a SIMD's two wavefronts one feeds the matrix cores while the
+// other computes.
 //
 // The running maximum follows lazily: it moves, and the sums are rescaled, only
 // when a score passes it by 2^7; weights are exp2(t - maximum + 8), at most 2^15,
@@ -27,7 +27,9 @@ namespace {
 typedef float v16f __attribute__((ext_vector_type(16)));
 
 constexpr float kHead = 8.0f, kSlack = 7.0f;
-constexpr float kTinyScale = 0x1p-126f;
+// a row's factor times a key scale, both kept in these ranges, stays finite and
+// normal, and so does a score: 2^37 * 2^60 * 2^15 * 127 * 128 < 2^128
+constexpr float kLeastKeyScale = 0x1p-60f, kMostKeyScale = 0x1p60f, kLeastRow = 0x1p-66f, kMostRow = 0x1p37f;
 
 template <int DT, int D, int NW, bool CAP>
 __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a) {
@@ -36,7 +38,6 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
     constexpr int kOp = kTile * D * 2;            // bytes of one operand's tile
     constexpr int kCodes = kTile * D / 16, kLoads = 2 * kCodes / kThreads;   // 16-byte chunks of one tensor's tile; a thread's of both
     __shared__ __align__(16) uint8_t smem[4 * kOp > NW * 32 * D * 2 ? 4 * kOp : NW * 32 * D * 2];
-    __shared__ __align__(16) float meta[2][3][4]; // of 16 tokens each: key scale, log2 and reciprocal of the value scale
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, hf = lane >> 5;
@@ -85,7 +86,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
         const int ex = mx > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(mx) : 0;
         const float up = __builtin_amdgcn_ldexpf(1.0f, ex > 100 ? 100 : ex);
         c = fabsf(a.scale) * (CAP ? 2.0f * kLog2e / a.cap : kLog2e) / up;
-        if (bad) c = __builtin_nanf("");
+        c = bad ? __builtin_nanf("") : __builtin_amdgcn_fmed3f(c, kLeastRow, kMostRow);
         const float sup = a.scale < 0.0f ? -up : up;
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
@@ -96,13 +97,46 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
         }
     }
 
-    typedef const __attribute__((address_space(4))) int32_t* sptr;
-    const sptr table = (sptr)(uintptr_t)(t.table + (int64_t)b * t.table_stride);
-    const int32_t most = (int32_t)a.cache.pages;
-    // page of token tk, -1 for none; tk is the same in all lanes where it is called for staging
-    auto page_at = [&](int tk) {
-        const int id = table[min(tk, end - 1) >> lg];
-        return tk < end && id >= 0 && id < most ? id : -1;
+    // The stretch's pages: a wavefront holds 128 of them, two a lane, from entry e0 of
+    // the table on: tile numbers (page, this head), and the tiles' key scale and log2 and
+    // reciprocal of the value scale.  The second 64 are loaded when the first are
+    // used up, long before they are needed.  Where there is no page the log2 is
+    // -inf (weights of zero); a NaN scale leaves the reciprocal 0 (the weights are NaN already).
+    struct Pages {
+        int tile;
+        float ks, lv, rv;
+    };
+    const int32_t* table = t.table + (int64_t)b * t.table_stride;
+    const int entries = end > 0 ? (end - 1 >> lg) + 1 : 0;
+    auto entry = [&](int e) {
+        const int id = table[min(e, max(entries - 1, 0))];
+        const bool has = e < entries && id >= 0 && id < a.cache.pages;
+        Pages r;
+        r.tile = has ? id * a.cache.heads + h : 0;
+        const float ks = a.cache.ks[r.tile];
+        float vs = a.cache.vs[r.tile];
+        r.ks = !has || ks < kLeastKeyScale ? kLeastKeyScale : ks > kMostKeyScale ? kMostKeyScale : ks;
+        if (vs < kValueFloor) vs = kValueFloor;
+        r.lv = has ? __builtin_amdgcn_logf(vs) : -__builtin_inff();
+        r.rv = has && vs == vs ? 1.0f / vs : 0.0f;
+        return r;
+    };
+    int e0 = begin >> lg;
+    Pages page0 = {}, page1 = {};
+    if (begin < end) {
+        page0 = entry(e0 + lane);
+        page1 = entry(e0 + 64 + lane);
+    }
+    auto pages_from = [&](int e) {                // the entries below e are done with
+        if (e < e0 + 64) return;
+        e0 += 64;
+        page0 = page1;
+        page1 = entry(e0 + 64 + lane);
+    };
+    // of token tk, the same in all lanes (a tile's entries lie in one of the halves)
+    auto tile_at = [&](int tk) {
+        const int e = (tk >> lg) - e0;
+        return __builtin_amdgcn_readlane(e < 64 ? page0.tile : page1.tile, e & 63);
     };
     // Staging.  Chunks of 16 codes, kCodes of the keys' tile, by token (D / 16
     // each), and kCodes of the values', by channel inside a page's part of the tile (cpp
@@ -117,9 +151,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
     }
     auto of_keys = [&](int i) { return kThreads <= kCodes ? i * kThreads < kCodes : 64 * wave < kCodes; };
     const int tile_log2 = lg + __builtin_ctz(D);
-    auto tile_of = [&](const int8_t* p, int id) {
-        return p + ((uint64_t)((uint32_t)max(id, 0) * (uint32_t)a.cache.heads + (uint32_t)h) << tile_log2);
-    };
+    auto tile_of = [&](const int8_t* p, int n) { return p + ((uint64_t)(uint32_t)n << tile_log2); };
     // the thread's share of the keys of the tile at tk0 and of the values of the one at tv0
     auto load = [&](int tk0, int tv0) {
 #pragma unroll
@@ -127,55 +159,30 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
             const int n0 = (i * kThreads + 64 * wave) & (kCodes - 1);            // the wavefront's first chunk
             if (of_keys(i)) {
                 const int tk = tk0 + n0 / (D / 16);
-                raw[i] = *reinterpret_cast<const uint4*>(tile_of(a.cache.k, page_at(tk)) + (tk & (ps - 1)) * D + 16 * lane);
+                raw[i] = *reinterpret_cast<const uint4*>(tile_of(a.cache.k, tile_at(tk)) + (tk & (ps - 1)) * D + 16 * lane);
             } else {
                 const int tv = tv0 + 16 * cpp * (n0 / D >> cpl);
-                raw[i] = *reinterpret_cast<const uint4*>(tile_of(a.cache.v, page_at(tv)) + (tv & (ps - 1)) + voff[i]);
+                raw[i] = *reinterpret_cast<const uint4*>(tile_of(a.cache.v, tile_at(tv)) + (tv & (ps - 1)) + voff[i]);
             }
         }
-    };
-    float mks = 0.0f, mvs = 0.0f;
-    bool mhas = false;
-    auto load_meta = [&](int t0) {                // threads 0 to 3: scales of the tile's 16-token groups
-        if (tid >= 4) return;
-        const int tk = t0 + 16 * tid;
-        const int id = t.table[(int64_t)b * t.table_stride + (min(tk, end - 1) >> lg)];
-        mhas = tk < end && id >= 0 && id < most;
-        const int64_t at = (int64_t)(mhas ? id : 0) * a.cache.heads + h;
-        mks = a.cache.ks[at];
-        mvs = a.cache.vs[at];
     };
     // LDS: operand fragments of 1 KiB, lane l's 16 bytes in slot l, the slots' low
     // bits mixed with the fragment's number so that the stores spread over the banks
-    auto put = [&](int kbuf, int vbuf, bool with_keys, bool with_values) {
-        uint8_t* kb = smem + kbuf * kOp;
-        uint8_t* vb = smem + (2 + vbuf) * kOp;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int n = (i * kThreads + tid) & (kCodes - 1);
-            if (of_keys(i)) {
-                if (!with_keys) continue;
-                const int tk = n / (D / 16), st = n % (D / 16);
-                uint8_t* f = kb + ((tk >> 5) * NS + st) * 1024 + 16 * ((tk & 31) ^ (st & 7));
-                *reinterpret_cast<h8*>(f) = codes8(raw[i].x, raw[i].y);
-                *reinterpret_cast<h8*>(f + 512) = codes8(raw[i].z, raw[i].w);
-            } else {
-                if (!with_values) continue;
-                const int d = n >> cpl & (D - 1), ts = (n / D >> cpl) * cpp + (n & (cpp - 1));
-                uint8_t* g = vb + ((d >> 5) * 4 + ts) * 1024 + 16 * ((d & 31) ^ ((ts & 1) << 2 | (ts & 2)));
-                *reinterpret_cast<h8*>(g) = codes8(raw[i].x, raw[i].z);        // tokens 0-3, 8-11 of 16
-                *reinterpret_cast<h8*>(g + 512) = codes8(raw[i].y, raw[i].w);  // 4-7, 12-15
-            }
+    // Piece k of a thread's staging, 8 codes converted and stored: 2 kLoads pieces.
+    auto put = [&](int k, int kbuf, int vbuf) {
+        const int i = k >> 1, n = (i * kThreads + tid) & (kCodes - 1);
+        if (of_keys(i)) {
+            const int tk = n / (D / 16), st = n % (D / 16);
+            uint8_t* f = smem + kbuf * kOp + ((tk >> 5) * NS + st) * 1024 + 16 * ((tk & 31) ^ (st & 7));
+            if (k & 1) *reinterpret_cast<h8*>(f + 512) = codes8(raw[i].z, raw[i].w);
+            else *reinterpret_cast<h8*>(f) = codes8(raw[i].x, raw[i].y);
+        } else {
+            const int d = n >> cpl & (D - 1), ts = (n / D >> cpl) * cpp + (n & (cpp - 1));
+            uint8_t* g = smem + (2 + vbuf) * kOp + ((d >> 5) * 4 + ts) * 1024 + 16 * ((d & 31) ^ ((ts & 1) << 2 | (ts & 2)));
+            if (k & 1) *reinterpret_cast<h8*>(g + 512) = codes8(raw[i].y, raw[i].w);     // tokens 4-7, 12-15 of 16
+            else *reinterpret_cast<h8*>(g) = codes8(raw[i].x, raw[i].z);                 // 0-3, 8-11
         }
     };
-    auto put_meta = [&](int buf) {
-        if (tid >= 4) return;
-        const float vs = mvs < kValueFloor ? kValueFloor : mvs;
-        meta[buf][0][tid] = !mhas ? 1.0f : mks < kTinyScale ? kTinyScale : mks;
-        meta[buf][1][tid] = mhas ? __builtin_amdgcn_logf(vs) : -__builtin_inff();
-        meta[buf][2][tid] = mhas ? 1.0f / vs : 0.0f;
-    };
-
     v16f o[NB], sc[2];
     h8 p[4];
 #pragma unroll
@@ -183,16 +190,17 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
 #pragma unroll
     for (int g = 0; g < 4; ++g) p[g] = (_Float16)0.0f;
     float m = kLow, l = 0.0f;
-    // The matrix phase: the second product of a tile (PV) and the first of the next
-    // (QK), their operands read kAhead fragments ahead of the MFMAs.
-    constexpr int kAhead = 4, kFrags = 2 * NS;                    // 4 NB = 2 NS fragments each
-    auto matrix = [&](auto pv, auto qk, int vbuf, int kbuf) {
+    // The matrix phase: the second product of a tile and (QK) the first of the next,
+    // their operands read kAhead fragments ahead of the MFMAs, and the staging: keys
+    // into the buffer that kbuf is not, values into the one that vbuf is not.
+    constexpr int kAhead = 6, kFrags = 2 * NS;                    // 4 NB = 2 NS fragments each
+    auto matrix = [&](auto qk, int vbuf, int kbuf) {
         const uint8_t* vb = smem + (2 + vbuf) * kOp + 512 * hf;
         const uint8_t* kb = smem + kbuf * kOp + 512 * hf;
-        constexpr int kTotal = (pv.value ? kFrags : 0) + (qk.value ? kFrags : 0);
+        constexpr int kTotal = qk.value ? 2 * kFrags : kFrags;
         h8 f[kAhead];
         auto read = [&](auto ic) {
-            constexpr int i = pv.value ? ic.value : ic.value + kFrags;
+            constexpr int i = ic.value;
             if constexpr (i < kFrags) {
                 constexpr int g = i / NB, d = i % NB;
                 f[ic.value % kAhead] = *reinterpret_cast<const h8*>(vb + (d * 4 + g) * 1024 + 16 * (l32 ^ ((g & 1) << 2 | (g & 2))));
@@ -208,25 +216,44 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
         }
         __builtin_amdgcn_sched_barrier(0);
         static_for<kTotal>([&](auto ic) {
-            constexpr int i = pv.value ? ic.value : ic.value + kFrags;
+            constexpr int i = ic.value;
             const h8 x = f[ic.value % kAhead];
             if constexpr (i < kFrags) o[i % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p[i / NB], o[i % NB], 0, 0, 0);
             else sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q[(i - kFrags) / 2], sc[i & 1], 0, 0, 0);
             if constexpr (ic.value + kAhead < kTotal) read(std::integral_constant<int, ic.value + kAhead>{});
+            // a piece of the staging behind every few MFMAs
+            constexpr int kEvery = 2 * kFrags / (2 * kLoads + 1);
+            if constexpr (qk.value && ic.value % kEvery == kEvery - 1 && ic.value / kEvery < 2 * kLoads)
+                put(ic.value / kEvery, kbuf ^ 1, vbuf ^ 1);
             __builtin_amdgcn_sched_barrier(0);
         });
     };
     // scores of the tile at t0 -> weights.  Register 8 g + e: token 16 g + 8 (e / 4) + 4 hf + e % 4.
-    auto weights = [&](int t0, int buf) {
-        const v4f mk = *reinterpret_cast<const v4f*>(meta[buf][0]);
-        v4f lv = *reinterpret_cast<const v4f*>(meta[buf][1]);
-        const v4f rv = *reinterpret_cast<const v4f*>(meta[buf][2]);
-        float cg[4];
+    auto weights = [&](int t0) {
+        float cg[4], lv[4], rv[4];
+        {
+            const int e = (t0 >> lg) - e0;
+            const bool half = e < 64;
+            const float ks = half ? page0.ks : page1.ks, ls = half ? page0.lv : page1.lv, rs = half ? page0.rv : page1.rv;
+            auto of = [&](float v, int at) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), at)); };
+            cg[0] = c * of(ks, e & 63);
+            lv[0] = of(ls, e & 63);
+            rv[0] = of(rs, e & 63);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            cg[g] = c * mk[g];
-            if (cg[g] > kMostScale) cg[g] = kMostScale;
-            if (cg[g] < kTinyScale) cg[g] = kTinyScale;
+            for (int g = 1; g < 4; ++g) {
+                cg[g] = cg[0];
+                lv[g] = lv[0];
+                rv[g] = rv[0];
+            }
+            if (lg < 6) {                         // several pages a tile
+#pragma unroll
+                for (int g = 1; g < 4; ++g) {
+                    const int at = (e & 63) + (16 * g >> lg);
+                    cg[g] = c * of(ks, at);
+                    lv[g] = of(ls, at);
+                    rv[g] = of(rs, at);
+                }
+            }
         }
         const bool edge = t0 + kTile - 1 > pos0 || (a.window > 0 && t0 < pos1 - a.window + 1);
         if (CAP || edge) {                        // to final scores first, then the mask
@@ -246,12 +273,14 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
         float top = kLow;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            float x = sc[g >> 1][8 * (g & 1)];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) x = fmaxf(x, sc[g >> 1][8 * (g & 1) + e]);
-            top = fmaxf(top, __builtin_fmaf(x, cg[g], lv[g]));
+            const v16f& x = sc[g >> 1];
+            const int k = 8 * (g & 1);
+            const float u = fmaxf(fmaxf(x[k], x[k + 1]), x[k + 2]), v = fmaxf(fmaxf(x[k + 3], x[k + 4]), x[k + 5]);
+            const float w = fmaxf(fmaxf(u, v), fmaxf(x[k + 6], x[k + 7]));
+            top = fmaxf(top, __builtin_fmaf(w, cg[g], lv[g]));
         }
-        top = fmaxf(top, __shfl_xor(top, 32));
+        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
         if (__any(top > m + kSlack)) {
             const float mn = fmaxf(m, top), fade = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
@@ -262,7 +291,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const float base = lv[g] - (m - kHead);
-            float sum = 0.0f;
+            float sum;
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
                 typedef float v2f __attribute__((ext_vector_type(2)));
@@ -272,55 +301,39 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
                 const h2 pr = __builtin_convertvector(x, h2);
                 p[g][e] = pr[0];
                 p[g][e + 1] = pr[1];
-                sum += x[0];
+                sum = e ? sum + x[0] : x[0];
                 sum += x[1];
             }
-            l += sum != 0.0f ? sum * rv[g] : 0.0f;                // a scale may be NaN where nothing is seen
+            l = __builtin_fmaf(sum, rv[g], l);
         }
     };
 
     const int tiles = begin < end ? (end - begin + kTile - 1) / kTile : 0;
     if (tiles > 0) {
         // Phases: the first half of the workgroup runs M(0) V(0) M(1) V(1) ... M(tiles),
-        // the second the same one phase later.  M(t) reads the values of t - 1 and the keys of t.  Keys of
-        // t + 1 and values of t are staged during M(t) of either half: by the
-        // second half ahead of its own V(t), by the first in its V(t), into
-        // the buffers that M(t - 1), over for both, was the last to read.
+        // the second the same one phase later.  M(t) reads the values of t - 1 and the
+        // keys of t (M(0)'s values are zeros), and stages keys of t + 1 and values of t
+        // into the buffers whose last readers were the two M(t - 1), over by then.
         const int behind = wave >= NW / 2 ? 1 : 0;
         load(begin, begin);
-        load_meta(begin);
-        put(0, 0, true, false);
-        put_meta(0);
+#pragma unroll
+        for (int k = 0; k < 2 * kLoads; ++k)
+            if (of_keys(k >> 1)) put(k, 0, 0);
         for (int i = tid; i < kOp / 16; i += kThreads) reinterpret_cast<uint4*>(smem + 3 * kOp)[i] = make_uint4(0, 0, 0, 0);
-        __syncthreads();
-        // staging step u: keys of tile u + 1, values of tile u, scales of tile u + 1
-        auto fetch = [&](int u) {
-            if (u >= tiles) return;
-            load(begin + min(u + 1, tiles - 1) * kTile, begin + u * kTile);
-            if (!behind && u + 1 < tiles) load_meta(begin + (u + 1) * kTile);
-        };
-        auto stage = [&](int u) {
-            if (u >= tiles) return;
-            put((u + 1) & 1, u & 1, u + 1 < tiles, true);
-            if (!behind && u + 1 < tiles) put_meta((u + 1) & 1);
-        };
+        // what M(u) stages; past the last tile, the last again, into buffers that nobody reads
+        auto fetch = [&](int u) { load(begin + min(u + 1, tiles - 1) * kTile, begin + min(u, tiles - 1) * kTile); };
         fetch(0);
-        if (behind) {
-            stage(0);
-            fetch(1);
+        WUSH_LDS_BARRIER();
+        if (behind) WUSH_LDS_BARRIER();
+        for (int i = 0; i < tiles; ++i) {
+            matrix(std::true_type{}, (i + 1) & 1, i & 1);
+            fetch(i + 1);
+            WUSH_LDS_BARRIER();
+            pages_from(begin + i * kTile >> lg);
+            weights(begin + i * kTile);
             WUSH_LDS_BARRIER();
         }
-        const std::true_type yes;
-        const std::false_type no;
-        for (int i = 0; i < tiles; ++i) {         // (the first second product: zeros)
-            matrix(yes, yes, (i + 1) & 1, i & 1);
-            WUSH_LDS_BARRIER();
-            weights(begin + i * kTile, i & 1);
-            stage(i + behind);
-            fetch(i + 1 + behind);
-            WUSH_LDS_BARRIER();
-        }
-        matrix(yes, no, (tiles - 1) & 1, 0);
+        matrix(std::false_type{}, (tiles - 1) & 1, 0);
         WUSH_LDS_BARRIER();
         if (!behind) WUSH_LDS_BARRIER();
     }
