@@ -108,7 +108,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
     };
     const int32_t* table = t.table + (int64_t)b * t.table_stride;
     const int entries = end > 0 ? (end - 1 >> lg) + 1 : 0;
-    auto entry = [&](int e) {
+    auto entry = [&](int e) __attribute__((always_inline)) {
         const int id = table[min(e, max(entries - 1, 0))];
         const bool has = e < entries && id >= 0 && id < a.cache.pages;
         Pages r;
@@ -127,14 +127,14 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
         page0 = entry(e0 + lane);
         page1 = entry(e0 + 64 + lane);
     }
-    auto pages_from = [&](int e) {                // the entries below e are done with
+    auto pages_from = [&](int e) __attribute__((always_inline)) {                // the entries below e are done with
         if (e < e0 + 64) return;
         e0 += 64;
         page0 = page1;
         page1 = entry(e0 + 64 + lane);
     };
     // of token tk, the same in all lanes (a tile's entries lie in one of the halves)
-    auto tile_at = [&](int tk) {
+    auto tile_at = [&](int tk) __attribute__((always_inline)) {
         const int e = (tk >> lg) - e0;
         return __builtin_amdgcn_readlane(e < 64 ? page0.tile : page1.tile, e & 63);
     };
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
     const int tile_log2 = lg + __builtin_ctz(D);
     auto tile_of = [&](const int8_t* p, int n) { return p + ((uint64_t)(uint32_t)n << tile_log2); };
     // the thread's share of the keys of the tile at tk0 and of the values of the one at tv0
-    auto load = [&](int tk0, int tv0) {
+    auto load = [&](int tk0, int tv0) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int n0 = (i * kThreads + 64 * wave) & (kCodes - 1);            // the wavefront's first chunk
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
     // LDS: operand fragments of 1 KiB, lane l's 16 bytes in slot l, the slots' low
     // bits mixed with the fragment's number so that the stores spread over the banks
     // Piece k of a thread's staging, 8 codes converted and stored: 2 kLoads pieces.
-    auto put = [&](int k, int kbuf, int vbuf) {
+    auto put = [&](int k, int kbuf, int vbuf) __attribute__((always_inline)) {
         const int i = k >> 1, n = (i * kThreads + tid) & (kCodes - 1);
         if (of_keys(i)) {
             const int tk = n / (D / 16), st = n % (D / 16);
@@ -192,14 +192,15 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
     float m = kLow, l = 0.0f;
     // The matrix phase: the second product of a tile and (QK) the first of the next,
     // their operands read kAhead fragments ahead of the MFMAs, and the staging: keys
-    // into the buffer that kbuf is not, values into the one that vbuf is not.
+    // into the buffer that kbuf is not, values into the one that kbuf is.
     constexpr int kAhead = 6, kFrags = 2 * NS;                    // 4 NB = 2 NS fragments each
-    auto matrix = [&](auto qk, int vbuf, int kbuf) {
+    auto matrix = [&](auto qk, auto kbufc) __attribute__((always_inline)) {
+        constexpr int kbuf = kbufc.value, vbuf = kbuf ^ 1;        // known, so that addresses are
         const uint8_t* vb = smem + (2 + vbuf) * kOp + 512 * hf;
         const uint8_t* kb = smem + kbuf * kOp + 512 * hf;
         constexpr int kTotal = qk.value ? 2 * kFrags : kFrags;
         h8 f[kAhead];
-        auto read = [&](auto ic) {
+        auto read = [&](auto ic) __attribute__((always_inline)) {
             constexpr int i = ic.value;
             if constexpr (i < kFrags) {
                 constexpr int g = i / NB, d = i % NB;
@@ -229,7 +230,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
         });
     };
     // scores of the tile at t0 -> weights.  Register 8 g + e: token 16 g + 8 (e / 4) + 4 hf + e % 4.
-    auto weights = [&](int t0) {
+    auto weights = [&](int t0) __attribute__((always_inline)) {
         float cg[4], lv[4], rv[4];
         {
             const int e = (t0 >> lg) - e0;
@@ -321,19 +322,33 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
             if (of_keys(k >> 1)) put(k, 0, 0);
         for (int i = tid; i < kOp / 16; i += kThreads) reinterpret_cast<uint4*>(smem + 3 * kOp)[i] = make_uint4(0, 0, 0, 0);
         // what M(u) stages; past the last tile, the last again, into buffers that nobody reads
-        auto fetch = [&](int u) { load(begin + min(u + 1, tiles - 1) * kTile, begin + min(u, tiles - 1) * kTile); };
+        auto fetch = [&](int u) __attribute__((always_inline)) { load(begin + min(u + 1, tiles - 1) * kTile, begin + min(u, tiles - 1) * kTile); };
         fetch(0);
         WUSH_LDS_BARRIER();
         if (behind) WUSH_LDS_BARRIER();
-        for (int i = 0; i < tiles; ++i) {
-            matrix(std::true_type{}, (i + 1) & 1, i & 1);
+        const std::integral_constant<int, 0> even;
+        const std::integral_constant<int, 1> odd;
+        auto step = [&](int i, auto parity) __attribute__((always_inline)) {
+            __builtin_amdgcn_s_setprio(1);        // few instructions, all of them waited for
+            matrix(std::true_type{}, parity);
             fetch(i + 1);
+            __builtin_amdgcn_s_setprio(0);
             WUSH_LDS_BARRIER();
             pages_from(begin + i * kTile >> lg);
             weights(begin + i * kTile);
             WUSH_LDS_BARRIER();
+        };
+        int i = 0;
+        for (; i + 1 < tiles; i += 2) {
+            step(i, even);
+            step(i + 1, odd);
         }
-        matrix(std::false_type{}, (tiles - 1) & 1, 0);
+        if (i < tiles) {
+            step(i, even);
+            matrix(std::false_type{}, odd);
+        } else {
+            matrix(std::false_type{}, even);
+        }
         WUSH_LDS_BARRIER();
         if (!behind) WUSH_LDS_BARRIER();
     }
