@@ -297,7 +297,7 @@ typedef struct wush_kv8_cache {
 /* Rotates q and k by position, and puts k and v into the cache, of which the
  * new tokens' pages change.  q (tokens, q_heads, head_dim), k, v (tokens, heads,
  * head_dim), bf16 or fp16, each with a token and a head stride: strides = {q token, q head, k token,
- * k head, v token, v head} in elements, multiples of 8, pointers 16-byte
+ * k head, v token, v head} in elements, multiples of 8, all pointers 16-byte
  * aligned.  Row p of cos_sin (positions, rot) fp32 holds rot / 2 cosines, then rot / 2 sines;
  * positions behind its end take its last row.  The first rot channels (a
  * multiple of 16, at most head_dim; 0: none, and cos_sin may be NULL) turn in pairs (i, i + rot / 2), or (2 i,

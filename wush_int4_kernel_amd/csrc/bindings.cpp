@@ -529,6 +529,7 @@ torch::Tensor kv8_append(torch::Tensor q, torch::Tensor k, torch::Tensor v, torc
     check_f32(cos_sin, "cos_sin");
     TORCH_CHECK(cos_sin.dim() == 2 && cos_sin.size(0) > 0 && cos_sin.size(1) % 16 == 0 && cos_sin.size(1) <= c.head_dim,
                 "cos_sin must be (positions, rotated channels): a multiple of 16, at most head_dim");
+    TORCH_CHECK(aligned16(cos_sin), "cos_sin must be 16-byte aligned");
     const auto b = kv8_batch(q, block_table, seq_lens, cu_q);
     const at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q.device());
     auto out = new_tensor(q.sizes(), q.scalar_type(), q);

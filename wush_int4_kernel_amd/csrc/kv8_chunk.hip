@@ -315,7 +315,10 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
         // the second the same one phase later.  M(t) reads the values of t - 1 and the
         // keys of t (M(0)'s values are zeros), and stages keys of t + 1 and values of t
         // into the buffers whose last readers were the two M(t - 1), over by then.
-        const int behind = wave >= NW / 2 ? 1 : 0;
+        // (with one wavefront a SIMD all run in step, and one barrier a tile is enough:
+        // what overlaps is another workgroup)
+        constexpr bool kShift = NW == 8;
+        const bool behind = kShift && wave >= NW / 2;
         load(begin, begin);
 #pragma unroll
         for (int k = 0; k < 2 * kLoads; ++k)
@@ -336,7 +339,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
             WUSH_LDS_BARRIER();
             pages_from(begin + i * kTile >> lg);
             weights(begin + i * kTile);
-            WUSH_LDS_BARRIER();
+            if constexpr (kShift) WUSH_LDS_BARRIER();
         };
         int i = 0;
         for (; i + 1 < tiles; i += 2) {
@@ -350,7 +353,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
             matrix(std::false_type{}, even);
         }
         WUSH_LDS_BARRIER();
-        if (!behind) WUSH_LDS_BARRIER();
+        if (kShift && !behind) WUSH_LDS_BARRIER();
     }
 
     l += __shfl_xor(l, 32);
