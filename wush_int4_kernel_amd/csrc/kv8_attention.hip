@@ -10,24 +10,30 @@
 // its own running maximum, sum and output, which meet in LDS at the end; stretches of
 // one row meet in a second kernel.
 //
-// Both products run on v_mfma_f32_16x16x32_f16, with the cache as row operand.
-// Codes are exact in fp16; a row of q is shifted by a power of two so that its
-// largest value lies near 2^15 (exact for values down to 2^-29 of it).  The score tile
-// comes out with a lane holding 16 consecutive tokens of one row (keys are loaded in
-// the order that makes it so), which is the operand that the second product
-// needs: the probabilities never leave their lanes.
+// The cache is the row operand of both products.  Scores are exact integers: keys enter
+// v_mfma_i32_16x16x64_i8 as the codes that they are, against q in 16-bit fixed
+// point, two bytes (a power of two puts the row's largest value between 2^14 and 32639;
+// values above 2^-7 of it in bf16 and 2^-4 in fp16 are exact, smaller ones are off by
+// at most 2^-15 of the largest).  Converting the keys to fp16 took 160 of about 490 vector
+// instructions a tile of 64 tokens, which bind a wavefront as much as the loads do.  The score tile comes out
+// with a lane holding 16 consecutive tokens of one row (keys are loaded in the order that
+// makes it so), which is the operand that the second product, v_mfma_f32_16x16x32_f16
+// on values converted exactly, needs: the probabilities never leave their lanes.
 //
 // A token's value scale is folded into its exponent: with t = log2(e) s +
-// log2(v_scale), weights are exp2(t - running max + 12), at most 2^12, rounded once
-// to fp16 (11 bits, normal down to 2^-26 of the largest), and the sum of the
-// probabilities takes them back times 1 / v_scale, in fp32.
+// log2(v_scale), weights are exp2(t - maximum + 12), rounded once to fp16 (11 bits, normal
+// down to 2^-26 of the largest), and the sum of the probabilities takes them, unrounded,
+// times 1 / v_scale, in fp32.  The maximum follows lazily: it moves, and the sums are
+// rescaled, only when a score passes it by 2^3.
 #include "kv8_attention.h"
 
 namespace wush {
 namespace {
 
+typedef int v4i __attribute__((ext_vector_type(4)));
+
 constexpr int kWaves = 4;
-constexpr float kHead = 12.0f;                    // weights reach 2^12
+constexpr float kHead = 12.0f, kSlack = 3.0f;       // weights reach 2^15
 
 __device__ __forceinline__ float quarters_max(float v) {
     v = fmaxf(v, __shfl_xor(v, 16));
@@ -45,8 +51,11 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
     const int l16 = lane & 15, kq = lane >> 4;
     const Kv8Batch& t = a.batch;
     const int lg = a.cache.page_log2, ps = 1 << lg, G = a.group;
-    const int split = blockIdx.x % a.splits;
-    const int h = (int)(blockIdx.x / a.splits) % a.cache.heads, item = (int)(blockIdx.x / a.splits) / a.cache.heads;
+    // Stretches slowest: the first ones, which are full, start first, and full and
+    // short ones spread over the XCDs (workgroup i runs on XCD i % 8).  With stretches fastest, two
+    // a sequence, every other XCD had the full ones: 64 ragged sequences 87 us, not 73.
+    const int h = (int)blockIdx.x % a.cache.heads, rest = (int)blockIdx.x / a.cache.heads;
+    const int item = rest % a.items, split = rest / a.items;
     int row0;
     const int b = item_rows(a, item, row0);
     const Kv8Seq s = kv8_seq(t, b);
@@ -64,7 +73,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
     const int low = a.window > 0 ? pos - a.window + 1 : 0;
     const int last_low = s.len - s.count + min((row0 + 15) / G, s.count - 1) - a.window;   // tokens behind it are in every row's window
 
-    h8 q[2 * NJ];
+    v4i qh[NJ], ql[NJ];                           // q = 256 qh + ql, in units of its row
     float c;                                      // scores in powers of two, per unit of key scale
     {
         const uint16_t* p = a.q + tok * a.qt + hq * a.qh + 16 * kq;
@@ -80,14 +89,23 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
             }
         }
         mx = quarters_max(mx);
-        const int ex = mx > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(mx) : 0;
+        int ex = mx > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(mx) : 0;
+        if (__builtin_amdgcn_ldexpf(mx, ex) > 32639.0f) --ex;     // 256 * 127 + 127
         const float up = __builtin_amdgcn_ldexpf(1.0f, ex > 100 ? 100 : ex);
         c = a.scale * (CAP ? 2.0f * kLog2e / a.cap : kLog2e) / up;
         if (quarters_max(bad ? 1.0f : 0.0f) > 0.0f) c = __builtin_nanf("");
 #pragma unroll
-        for (int j = 0; j < 2 * NJ; ++j)
+        for (int j = 0; j < NJ; ++j) {
+            uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) q[j][e] = bad ? (_Float16)0.0f : (_Float16)(x[j][e] * up);
+            for (int e = 0; e < 16; ++e) {
+                const int n = bad ? 0 : (int)__builtin_rintf(x[2 * j + (e >> 3)][e & 7] * up), u = (n + 128) >> 8;
+                hi[e >> 2] |= ((uint32_t)u & 0xffu) << (8 * (e & 3));
+                lo[e >> 2] |= ((uint32_t)(n - 256 * u) & 0xffu) << (8 * (e & 3));
+            }
+            qh[j] = (v4i){(int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+            ql[j] = (v4i){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3]};
+        }
     }
 
     const v4f zero = {0, 0, 0, 0};
@@ -106,7 +124,8 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
         return tk < end && (uint32_t)id < (uint64_t)a.cache.pages ? id : -1;
     };
     const int ok = 16 * (l16 >> 2), ov = 16 * kq;
-    uint4 kk[4][NJ], vv[NB];
+    v4i kk[4][NJ];
+    uint4 vv[NB];
     float ks, vs;
     auto load_keys = [&](int t0, int idk, int idv) {
         const int8_t* pk = a.cache.k + ((int64_t)max(idk, 0) * a.cache.heads + h) * tile_bytes +
@@ -114,7 +133,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
 #pragma unroll
         for (int n = 0; n < 4; ++n)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) kk[n][j] = load_nt16(pk + 4 * n * D + 64 * j);
+            for (int j = 0; j < NJ; ++j) kk[n][j] = *reinterpret_cast<const v4i*>(pk + 4 * n * D + 64 * j);
         const int64_t vt = (int64_t)max(idv, 0) * a.cache.heads + h;
         ks = a.cache.ks[vt];
         vs = a.cache.vs[vt];
@@ -122,26 +141,23 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
     auto load_values = [&](int t0, int idv) {
         const int8_t* pv = a.cache.v + ((int64_t)max(idv, 0) * a.cache.heads + h) * tile_bytes + (l16 << lg) + ((t0 + ov) & (ps - 1));
 #pragma unroll
-        for (int d = 0; d < NB; ++d) vv[d] = load_nt16(pv + ((int64_t)d << (lg + 4)));
+        for (int d = 0; d < NB; ++d) vv[d] = *reinterpret_cast<const uint4*>(pv + ((int64_t)d << (lg + 4)));
     };
 
     // One tile.  A tile's keys go out while the last tile's weights are made, its
     // values behind the last tile's products: the registers that held those take
     // them.  Behind the end nothing goes out.
     auto tile = [&](int t0, int idv, bool masked, auto&& keys_ahead, auto&& values_ahead) {
-        v4f sc[4];
+        v4i sh[4], sl[4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) sc[n] = zero;
+        for (int n = 0; n < 4; ++n) sh[n] = sl[n] = (v4i){0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
-                sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(kk[n][j].x, kk[n][j].y), q[2 * j], sc[n], 0, 0, 0);
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-                sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(kk[n][j].z, kk[n][j].w), q[2 * j + 1], sc[n], 0, 0, 0);
-            __builtin_amdgcn_sched_barrier(0);    // codes are not converted ahead: that takes twice their registers
-        }
+            for (int n = 0; n < 4; ++n) {
+                sh[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[n][j], qh[j], sh[n], 0, 0, 0);
+                sl[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[n][j], ql[j], sl[n], 0, 0, 0);
+            }
         // the lane's 16 tokens, of one page
         float cs = c * ks;
         if (fabsf(cs) > kMostScale) cs = __builtin_copysignf(kMostScale, cs);
@@ -150,15 +166,17 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
         __builtin_amdgcn_sched_barrier(0);
         keys_ahead();
         __builtin_amdgcn_sched_barrier(0);
+        v4f sc[4];
         const int tv = t0 + ov, last = idv >= 0 ? min(pos, end - 1) : -1;
         float top = kLow;
 #pragma unroll
         for (int n = 0; n < 4; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                sc[n][e] = capped<CAP>(a, sc[n][e] * cs) + lv;
+                sc[n][e] = capped<CAP>(a, (float)(256 * sh[n][e] + sl[n][e]) * cs) + lv;
             }
         if (masked) {
+            asm volatile("" : "+v"(top));         // a branch: not computed for every tile
 #pragma unroll
             for (int n = 0; n < 4; ++n)
 #pragma unroll
@@ -171,9 +189,15 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
         for (int n = 0; n < 4; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) top = fmaxf(top, sc[n][e]);
-        const float mn = fmaxf(m, quarters_max(top));
-        const float fade = __builtin_amdgcn_exp2f(m - mn), less = mn - kHead;
-        m = mn;
+        top = quarters_max(top);
+        if (__any(top > m + kSlack)) {
+            const float mn = fmaxf(m, top), fade = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= fade;
+#pragma unroll
+            for (int d = 0; d < NB; ++d) acc[d] *= fade;
+        }
+        const float less = m - kHead;
         float sum = 0.0f;
         h8 p[2];
 #pragma unroll
@@ -184,10 +208,9 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
                 sum += w;
                 p[n >> 1][4 * (n & 1) + e] = (_Float16)w;
             }
-        l = l * fade + (sum != 0.0f ? sum * (1.0f / fv) : 0.0f);  // a scale may be NaN where nothing is seen
+        l += sum != 0.0f ? sum * __builtin_amdgcn_rcpf(fv) : 0.0f;    // a scale may be NaN where nothing is seen
 #pragma unroll
         for (int d = 0; d < NB; ++d) {
-            acc[d] *= fade;
             acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vv[d].x, vv[d].y), p[0], acc[d], 0, 0, 0);
             acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vv[d].z, vv[d].w), p[1], acc[d], 0, 0, 0);
             if (d & 1) __builtin_amdgcn_sched_barrier(0);
@@ -218,11 +241,11 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
 
     // join the wavefronts: a lane holds channels 16 d + 4 kq + e of row l16
     __shared__ float so[kWaves][16][D + 4];
-    __shared__ float sm[kWaves][16], sl[kWaves][16];
+    __shared__ float sm[kWaves][16], ssum[kWaves][16];
     l = quarters_sum(l);
     if (kq == 0) {
         sm[wave][l16] = m;
-        sl[wave][l16] = l;
+        ssum[wave][l16] = l;
     }
 #pragma unroll
     for (int d = 0; d < NB; ++d) *reinterpret_cast<v4f*>(&so[wave][l16][16 * d + 4 * kq]) = acc[d];
@@ -238,7 +261,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
         const float f = __builtin_amdgcn_exp2f(sm[w][jr] - mm);
-        ll += sl[w][jr] * f;
+        ll += ssum[w][jr] * f;
 #pragma unroll
         for (int e = 0; e < PD; ++e) o[e] += so[w][jr][d0 + e] * f;
     }
@@ -355,7 +378,7 @@ Plan plan_of(const Kv8Cache& c, int64_t seqs, int64_t tokens, bool ragged, int g
     if (range < 1) range = 1;
     if (range > 1 << 30) range = 1 << 30;         // the last stretch takes what lies behind
     const int64_t step = p.tile_rows == 16 ? 256 : kTile, most = (range + step - 1) / step;
-    const double pass = (p.tile_rows == 16 ? 2.5 : 1.5) * c.dim / 128;
+    const double pass = (p.tile_rows == 16 ? 2.1 : 1.5) * c.dim / 128;
     const double joined = 0.02 + (double)rows * c.heads * (c.dim + kPartExtra) * 8 / 4e6;   // a stretch's sums both ways
     double least = 1e30;
     p.splits = 1;
