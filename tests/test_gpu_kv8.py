@@ -236,6 +236,29 @@ def test_chunks(dev, dtype, Hq, Hkv, D, page):
     check_attention(dev, Batch(Hq + D + 1, lens, n, Hq, Hkv, D, page, dtype), max_len=300)
 
 
+@pytest.mark.parametrize("D,page,dtype,cap,window", [(128, 16, BF, 0.0, 0), (64, 64, HF, 0.0, 200), (128, 128, HF, 20.0, 0),
+                                                     (64, 32, BF, 0.0, 0)])
+def test_chunks_that_fill_the_chip(dev, D, page, dtype, cap, window):
+    # many heads: tiles of 256 rows, whose wavefronts work in two shifted halves;
+    # lengths on both sides of a tile and of the 64 pages that a lane's half holds
+    lens, n = [300, 64, 1, 65, 2100, 129], [300, 64, 1, 65, 70, 128]
+    check_attention(dev, Batch(D + page, lens, n, 64, 32, D, page, dtype), cap=cap, window=window, max_len=2100)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_chunk_behind_a_long_context_is_split(dev, dtype):
+    # few new tokens behind many: 128-row tiles, stretches of the cache joined
+    for window in (0, 1500):
+        bt = Batch(31, [6000, 150, 4097], [70, 150, 65], 8, 2, 64, 16, dtype)
+        out = check_attention(dev, bt, window=window, max_len=6000)
+        assert torch.equal(out, check_attention(dev, bt, window=window, max_len=6000, filled=False))
+
+
+def test_negative_scale(dev):
+    for n, ragged in (([1, 1], False), ([60, 70], True)):
+        check_attention(dev, Batch(32, [60, 70], n, 8, 2, 64, 16, HF), scale=-0.2, ragged=ragged)
+
+
 @pytest.mark.parametrize("window", [1, 2, 16, 100, 129, 5000])
 @pytest.mark.parametrize("ragged", [False, True])
 def test_window(dev, window, ragged):

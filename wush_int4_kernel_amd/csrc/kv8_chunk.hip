@@ -15,8 +15,8 @@
 // other computes.
 //
 // The running maximum follows lazily: it moves, and the sums are rescaled, only
-// when a score passes it by 2^7; weights are exp2(t - maximum + 8), at most 2^15,
-// rounded once to fp16 (11 bits, normal down to 2^-22 of the largest) for the product;
+// when a score passes it by 2^3; weights are exp2(t - maximum + 12), at most 2^15,
+// rounded once to fp16 (11 bits, normal down to 2^-26 of the largest) for the product;
 // their sum takes them unrounded (pages whose values are far smaller than others' have
 // weights below fp16's range, and count in it all the same).
 #include "kv8_attention.h"
@@ -26,7 +26,7 @@ namespace {
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 
-constexpr float kHead = 8.0f, kSlack = 7.0f;
+constexpr float kHead = 12.0f, kSlack = 3.0f;
 // a row's factor times a key scale, both kept in these ranges, stays finite and
 // normal, and so does a score: 2^37 * 2^60 * 2^15 * 127 * 128 < 2^128
 constexpr float kLeastKeyScale = 0x1p-60f, kMostKeyScale = 0x1p60f, kLeastRow = 0x1p-66f, kMostRow = 0x1p37f;
