@@ -19,7 +19,7 @@ namespace {
 typedef int v4i __attribute__((ext_vector_type(4)));
 
 constexpr float kScaleFloor = 0x1p-126f;
-constexpr int kQuantThreads = 256;
+constexpr int kQuantThreads = 1024;
 
 template <int DT>
 __device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
@@ -67,28 +67,47 @@ __device__ __forceinline__ float token_scale(uint32_t largest) {
     return fmaxf((DT == WUSH_DTYPE_BF16 ? bf16_to_f32(largest) : f16_to_f32(largest)) / 127.0f, kScaleFloor);
 }
 
-// One workgroup per row.
-template <int DT>
+// One workgroup per row, of as many threads as it has groups of 8 values, up to
+// kQuantThreads; a thread keeps its NU groups in registers between the two passes (NU 0: rows
+// too long for that, read twice).  Latency-bound for few rows: 203 x 8192 WUSH_Q1 us, with 256
+// threads that read the row twice 5.0; 4096 x 8192 WUSH_Q2 us.
+template <int DT, int NU>
 __global__ __launch_bounds__(kQuantThreads) void quant_int8_token_kernel(const uint16_t* __restrict__ x,
                                                                          int8_t* __restrict__ q,
                                                                          float* __restrict__ s, int K,
                                                                          int64_t stride) {
     const int64_t row = blockIdx.x;
+    const int threads = blockDim.x, units = K / 8;
     const uint4* px = reinterpret_cast<const uint4*>(x + row * stride);
     uint2* pq = reinterpret_cast<uint2*>(q + row * K);
+    uint4 v[NU ? NU : 1];
     uint32_t mx = 0;
-    for (int i = threadIdx.x; i < K / 8; i += kQuantThreads) mx = max(mx, largest8(px[i]));
+    if constexpr (NU > 0) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) v[u] = px[min((int)threadIdx.x + u * threads, units - 1)];
+#pragma unroll
+        for (int u = 0; u < NU; ++u) mx = max(mx, largest8(v[u]));
+    } else {
+        for (int i = threadIdx.x; i < units; i += threads) mx = max(mx, largest8(px[i]));
+    }
     __shared__ uint32_t part[kQuantThreads / 64];
     mx = wave_max(mx);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = mx;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kQuantThreads / 64; ++i) mx = max(mx, part[i]);
+    for (int i = 0; i < threads / 64; ++i) mx = max(mx, part[i]);
     const float sc = token_scale<DT>(mx);
     if (threadIdx.x == 0) s[row] = sc;
     const bool bad = sc != sc;
     const float inv = 1.0f / sc;
-    for (int i = threadIdx.x; i < K / 8; i += kQuantThreads) pq[i] = bad ? make_uint2(0, 0) : codes_of<DT>(px[i], inv);
+    if constexpr (NU > 0) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            const int i = threadIdx.x + u * threads;
+            if (i < units) pq[i] = bad ? make_uint2(0, 0) : codes_of<DT>(v[u], inv);
+        }
+    } else {
+        for (int i = threadIdx.x; i < units; i += threads) pq[i] = bad ? make_uint2(0, 0) : codes_of<DT>(px[i], inv);
+    }
 }
 
 // y rows as fp16 or bf16, each rounded once from fp32
@@ -291,6 +310,19 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, size_t room) {
     return best;
 }
 
+template <int DT>
+int launch_quant(const void* x, int8_t* q, float* s, int64_t rows, int64_t K, int64_t stride, hipStream_t stream) {
+    const uint16_t* p = static_cast<const uint16_t*>(x);
+    const int64_t units = K / 8;
+    const unsigned threads = units < kQuantThreads ? (unsigned)((units + 63) / 64 * 64) : kQuantThreads;
+    const dim3 grid((unsigned)rows);
+    if (units <= threads) quant_int8_token_kernel<DT, 1><<<grid, threads, 0, stream>>>(p, q, s, (int)K, stride);
+    else if (units <= 2 * threads) quant_int8_token_kernel<DT, 2><<<grid, threads, 0, stream>>>(p, q, s, (int)K, stride);
+    else if (units <= 4 * threads) quant_int8_token_kernel<DT, 4><<<grid, threads, 0, stream>>>(p, q, s, (int)K, stride);
+    else quant_int8_token_kernel<DT, 0><<<grid, threads, 0, stream>>>(p, q, s, (int)K, stride);
+    return (int)hipGetLastError();
+}
+
 template <int SRC>
 int launch_gemv(const void* x, int64_t stride, const float* xs, const int8_t* wq, const float* ws, void* y, int dtype,
                 int64_t M, int64_t N, int64_t K, hipStream_t stream) {
@@ -316,12 +348,8 @@ int wush_quant_int8_token(const void* x, int dtype, int8_t* q, float* s, int64_t
     WUSH_REQUIRE(x && q && s && rows <= 0x7fffffffLL);
     WUSH_REQUIRE(((uintptr_t)x & 15u) == 0 && ((uintptr_t)q & 15u) == 0 && ((uintptr_t)s & 3u) == 0);
     WUSH_REQUIRE(rows == 1 || (row_stride >= 0 && row_stride % 8 == 0));
-    const uint16_t* px = static_cast<const uint16_t*>(x);
-    if (dtype == WUSH_DTYPE_BF16)
-        wush::quant_int8_token_kernel<WUSH_DTYPE_BF16><<<(unsigned)rows, wush::kQuantThreads, 0, stream>>>(px, q, s, (int)K, row_stride);
-    else
-        wush::quant_int8_token_kernel<WUSH_DTYPE_F16><<<(unsigned)rows, wush::kQuantThreads, 0, stream>>>(px, q, s, (int)K, row_stride);
-    return (int)hipGetLastError();
+    return dtype == WUSH_DTYPE_BF16 ? wush::launch_quant<WUSH_DTYPE_BF16>(x, q, s, rows, K, row_stride, stream)
+                                    : wush::launch_quant<WUSH_DTYPE_F16>(x, q, s, rows, K, row_stride, stream);
 }
 
 size_t wush_gemm_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
