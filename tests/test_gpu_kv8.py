@@ -488,7 +488,7 @@ def test_refusals(dev):
         ("head_dim must be", lambda: _C.kv8_read(wide, wide.transpose(2, 3).contiguous(), ks[:4], vs[:4], i32([0], dev))),
         ("page_size must be", lambda: _C.kv8_read(odd, odd.transpose(2, 3).contiguous(), ks[:4], vs[:4], i32([0], dev))),
         ("multiple of the cache", lambda: attend(q=q[:, :3])), ("head_dim", lambda: attend(q=q[..., :32])),
-        ("negative", lambda: attend(window=-1)), ("negative", lambda: attend(max_len=-1)), ("softcap", lambda: attend(softcap=-1.0)),
+        ("negative", lambda: attend(window=-1)), ("negative", lambda: attend(max_len=-1)), ("softcap", lambda: attend(softcap=-1.0)), ("scale must be finite", lambda: attend(scale=math.inf)),
         ("softcap", lambda: attend(softcap=math.inf)), ("bf16 or fp16", lambda: attend(q=q.float())),
         ("one new token per sequence", lambda: attend(q=torch.cat((q, q)))),
         ("bf16 or fp16", lambda: _C.kv8_read(*cache, i32([0], dev), torch.float32)),

@@ -83,7 +83,7 @@ def test_kv8_arguments(capi):
                dict(heads=-1), dict(out=None), dict(out=P(8)), dict(tokens=1 << 31, cu=P(16)), dict(heads=1 << 40)]:
         assert append(c, **kw) == INVALID, kw
     for kw in [dict(q=None), dict(q=P(8)), dict(dtype=2), dict(qt=60), dict(qh=4), dict(table=None), dict(lens=None), dict(tokens=3),
-               dict(heads=3), dict(heads=0), dict(scale=float("nan")), dict(window=-1), dict(cap=-1.0), dict(cap=float("nan")),
+               dict(heads=3), dict(heads=0), dict(scale=float("nan")), dict(scale=float("inf")), dict(window=-1), dict(cap=-1.0), dict(cap=float("nan")),
                dict(cap=float("inf")), dict(max_len=-1), dict(out=None), dict(seqs=-1), dict(ts=-1), dict(tokens=1 << 31, cu=P(16))]:
         assert attend(c, **kw) == INVALID, kw
     for kw in [dict(pages=None), dict(k=None), dict(v=P(8)), dict(dtype=2), dict(n=-1), dict(n=1 << 40)]:

@@ -554,6 +554,7 @@ torch::Tensor kv8_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tenso
     TORCH_CHECK(q.dim() == 3 && q.size(2) == c.head_dim, "q must be (tokens, heads, head_dim) of the cache's head_dim");
     TORCH_CHECK(q.size(1) > 0 && q.size(1) % c.heads == 0, "q's heads must be a multiple of the cache's ", c.heads);
     TORCH_CHECK(window >= 0 && max_len >= 0, "window and max_len must not be negative");
+    TORCH_CHECK(!scale.has_value() || std::isfinite((float)*scale), "scale must be finite");
     TORCH_CHECK(softcap >= 0.0 && std::isfinite(softcap), "softcap must be finite and not negative");
     const auto b = kv8_batch(q, block_table, seq_lens, cu_q);
     const at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q.device());

@@ -25,6 +25,12 @@
 // down to 2^-26 of the largest), and the sum of the probabilities takes them, unrounded,
 // times 1 / v_scale, in fp32.  The maximum follows lazily: it moves, and the sums are
 // rescaled, only when a score passes it by 2^3.
+//
+// Bound by HBM where the cache fills the chip (one token behind 131072, 8 heads of 128:
+// 268 MB in 56 us with 5 to join, 4.8 TB/s; 64 ragged sequences up to 4096: 344 MB in 71 us, the
+// longest sequence ending last), by a wavefront's instructions and latencies otherwise (3 x 300: 6 us).  Two
+// tiles' loads in flight instead of one changed nothing; without the non-temporal hint
+// 131072 tokens took 2 us more, but 8192-token stretches 20% less, so loads have none.
 #include "kv8_attention.h"
 
 namespace wush {
@@ -286,6 +292,9 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
 // The stretches that hold tokens of a (token, query head), joined: by one
 // wavefront, or, where there are more than kFewSplits, by a workgroup's four, which
 // take every fourth stretch.  Four stretches at a time, so that their loads overlap.
+// With 32 stretches a wavefront took 5 us more than a workgroup (decode of 1 x 131072), with 16
+// up to 3, with 2 to 8 they are equal within 1; with many rows of few stretches a workgroup a row is
+// slow (five chunks of 700 tokens 133 us, not 87).
 constexpr int kFewSplits = 16;
 
 template <int DT, int D>
@@ -361,38 +370,49 @@ struct Plan {
     int64_t items;
 };
 
-// Tile height: 16-row items (kv8_rows_kernel) below 64 rows a sequence on average,
-// where taller ones would be mostly empty; 256-row workgroups where they fill the
-// chip, else 128.  Then the stretches of the cache per item with the least estimated
-// time, in microseconds: a workgroup's pass over `step` tokens times the workgroups of
-// a CU, and where there is more than one stretch the joining.
+// For each tile height, 16 (kv8_rows_kernel), 128 and 256 (kv8_chunk.hip), the
+// stretches of the cache per item with the least estimated time, in microseconds: a
+// workgroup's pass over `step` tokens times the workgroups of a CU, and where there is
+// more than one stretch the joining.  Of the three, the height with the least time (the last
+// constants are fitted to that): over 72 shapes, from 1 to 16 sequences of 1024 and 8192 with 41 to 1024 rows of new tokens,
+// 3% slower than the fastest height on average and 38% at worst; 16 rows below a fixed number
+// of rows a sequence, tall ones above, was 15% slower on average and 98% at worst.
 Plan plan_of(const Kv8Cache& c, int64_t seqs, int64_t tokens, bool ragged, int group, int64_t table_stride, int window,
              int64_t max_len) {
-    Plan p;
+    static const struct { int rows, step; double split, start, pass; } kHeights[] = {
+        {16, 256, 2.1, 0.0, 1.3}, {128, kTile, 1.5, 2.0, 1.2}, {256, kTile, 1.5, 8.0, 2.1}};
     const int64_t rows = tokens * group;
-    p.tile_rows = rows < 64 * seqs ? 16 : (rows / 256 + seqs) * c.heads >= 256 ? 256 : 128;
-    p.items = ragged ? rows / p.tile_rows + seqs : seqs * ((group + p.tile_rows - 1) / p.tile_rows);
-    int64_t range = table_stride << c.page_log2;
-    if (max_len > 0 && max_len < range) range = max_len;
-    if (window > 0 && window + 64 + p.tile_rows / group < range) range = window + 64 + p.tile_rows / group;
-    if (range < 1) range = 1;
-    if (range > 1 << 30) range = 1 << 30;         // the last stretch takes what lies behind
-    const int64_t step = p.tile_rows == 16 ? 256 : kTile, most = (range + step - 1) / step;
-    const double pass = (p.tile_rows == 16 ? 2.1 : 1.5) * c.dim / 128;
     const double joined = 0.02 + (double)rows * c.heads * (c.dim + kPartExtra) * 8 / 4e6;   // a stretch's sums both ways
+    Plan best = {16, 1, 1, 0};
     double least = 1e30;
-    p.splits = 1;
-    for (int64_t n = 1; n <= most && n <= 256 && (n == 1 || p.items * c.heads * n <= 1024); n += n < 16 ? 1 : n / 16) {
-        const int64_t passes = (most + n - 1) / n, groups = p.items * c.heads * n;
-        const double us = pass * (double)passes * (double)((groups + 255) / 256) + (n > 1 ? 3.0 + joined * (double)n : 0.0);
+    for (const auto& t : kHeights) {
+        const int64_t items = ragged ? rows / t.rows + seqs : seqs * ((group + t.rows - 1) / t.rows);
+        int64_t range = table_stride << c.page_log2;
+        if (max_len > 0 && max_len < range) range = max_len;
+        if (window > 0 && window + 64 + t.rows / group < range) range = window + 64 + t.rows / group;
+        if (range < 1) range = 1;
+        if (range > 1 << 30) range = 1 << 30;     // the last stretch takes what lies behind
+        const int64_t most = (range + t.step - 1) / t.step;
+        double fewest = 1e30;
+        int64_t splits = 1;
+        for (int64_t n = 1; n <= most && n <= 256 && (n == 1 || items * c.heads * n <= 1024); n += n < 16 ? 1 : n / 16) {
+            const double us = t.split * c.dim / 128 * (double)((most + n - 1) / n) * (double)((items * c.heads * n + 255) / 256) +
+                              (n > 1 ? 3.0 + joined * (double)n : 0.0);
+            if (us < fewest) {
+                fewest = us;
+                splits = n;
+            }
+        }
+        const double full = (double)(items * c.heads * splits) / 256;
+        const double us = t.start + t.pass * (0.3 + 0.7 * c.dim / 128) * (double)((most + splits - 1) / splits) * (full > 1 ? full : 1) +
+                          (splits > 1 ? 3.0 + joined * (double)splits : 0.0);
         if (us < least) {
             least = us;
-            p.splits = (int)n;
+            const int chunk = (int)((most + splits - 1) / splits * t.step);
+            best = {t.rows, (int)((range + chunk - 1) / chunk), chunk, items};
         }
     }
-    p.chunk = (int)((most + p.splits - 1) / p.splits * step);
-    p.splits = (int)((range + p.chunk - 1) / p.chunk);
-    return p;
+    return best;
 }
 
 template <int DT>
@@ -444,7 +464,7 @@ int wush_kv8_attention(const void* q, int dtype, int64_t q_token_stride, int64_t
     WUSH_REQUIRE(dtype == WUSH_DTYPE_BF16 || dtype == WUSH_DTYPE_F16);
     WUSH_REQUIRE(seqs >= 0 && tokens >= 0 && table_stride >= 0 && window >= 0 && max_len >= 0);
     WUSH_REQUIRE(q_heads > 0 && q_heads % a.cache.heads == 0 && q_heads <= 65535);
-    WUSH_REQUIRE(scale == scale && softcap >= 0.0f && softcap < __builtin_inff());
+    WUSH_REQUIRE(scale - scale == 0.0f && softcap >= 0.0f && softcap < __builtin_inff());
     if (seqs == 0 || tokens == 0) return (int)hipSuccess;
     WUSH_REQUIRE(q && out && (block_table || table_stride == 0) && seq_lens && (cu_q || seqs == tokens));
     WUSH_REQUIRE(seqs <= 0x3fffffffLL && tokens <= 0x3fffffffLL);

@@ -14,6 +14,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr float kPageScaleFloor = 0x1p-40f;
+// Values of at most so many new tokens in a page are stored byte by byte: 64 sequences,
+// pages of 64, 1 token 5.8 us, through LDS 6.5; 8 tokens 11.5 and 11.8; 16 tokens in pages of 16
+// 11.9 and 10.7.
+constexpr int kFewTokens = 8;
 
 // A thread's unit of a token's head: 16 channels, 8 from a and 8 from b on, so
 // that it holds both of a pair: (i, i + rot / 2) or neighbours; behind the rotated
@@ -115,9 +119,10 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float r) {
 // workgroups that rotate the queries, a thread 16 channels of q_each heads of a token,
 // whose table row it loads once.
 //
-// Measured (bf16, 32 query and 8 key/value heads of 128): 4161 new tokens in pages of 16,
-// 96 MB, WUSH_A2 us; 64 single tokens, 64 query heads, pages of 64, WUSH_A1 us, where the
-// chain of loads (length, table, scale) and the launch are what it takes.
+// Measured (bf16, 8 key/value heads of 128): 4161 new tokens, 32 query heads, pages of 16,
+// 96 MB, 20 us (4.8 TB/s); 64 single
+// tokens, 64 query heads, pages of 64, 6.3 us, where the chain of loads (length, table,
+// scale) and the launch are what it takes.
 template <int DT, int D, int W, int NP>
 __global__ __launch_bounds__(kThreads, NP > 2 ? 4 : 6) void kv8_append_kernel(const AppendArgs a) {
     constexpr int kUnits = D / 16, TP = 64 / kUnits, TW = 4 / W, kPage = W * TP * NP;
@@ -217,7 +222,7 @@ __global__ __launch_bounds__(kThreads, NP > 2 ? 4 : 6) void kv8_append_kernel(co
             *p = c;
         }
     uint8_t* st = stage[slot];
-    const bool bytes = !grown && hi - lo <= 2;
+    const bool bytes = !grown && hi - lo <= kFewTokens;
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
         const int i = (p * W + within) * TP + lane / kUnits;
@@ -228,7 +233,7 @@ __global__ __launch_bounds__(kThreads, NP > 2 ? 4 : 6) void kv8_append_kernel(co
                 *reinterpret_cast<uint2*>(codes + i * D + u.b) = cb;
             } else {
                 const uint32_t c[4] = {ca.x, ca.y, cb.x, cb.y};
-                // a token or two into a page whose scale stays: byte by byte, no reading
+                // few tokens into a page whose scale stays: byte by byte, no reading
                 // back of what lies around them
                 if (bytes) {
 #pragma unroll
@@ -270,7 +275,8 @@ __global__ __launch_bounds__(kThreads, NP > 2 ? 4 : 6) void kv8_append_kernel(co
 }
 
 // Pages as values: k, v (n, heads, page, D).  One workgroup per (page, head, keys or
-// values).  Values are turned: through LDS, then four channels by four tokens in registers.
+// values).  Values are turned: through LDS, then eight channels by four tokens in
+// registers.  64 pages of 64 tokens (25 MB): 7.4 us, of which the launch is about 3.
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads) void kv8_read_kernel(const Kv8Cache c, const int32_t* __restrict__ ids,
                                                             uint16_t* __restrict__ k, uint16_t* __restrict__ v) {

@@ -69,8 +69,8 @@ __device__ __forceinline__ float token_scale(uint32_t largest) {
 
 // One workgroup per row, of as many threads as it has groups of 8 values, up to
 // kQuantThreads; a thread keeps its NU groups in registers between the two passes (NU 0: rows
-// too long for that, read twice).  Latency-bound for few rows: 203 x 8192 WUSH_Q1 us, with 256
-// threads that read the row twice 5.0; 4096 x 8192 WUSH_Q2 us.
+// too long for that, read twice).  Latency-bound for few rows: 203 x 8192 4.2 us, with 256
+// threads that read the row twice 5.0; 4096 x 8192 (100 MB) 25 us.
 template <int DT, int NU>
 __global__ __launch_bounds__(kQuantThreads) void quant_int8_token_kernel(const uint16_t* __restrict__ x,
                                                                          int8_t* __restrict__ q,
@@ -115,83 +115,70 @@ __device__ __forceinline__ uint16_t out_bits(float f, int dt) {
     return dt == WUSH_DTYPE_F16 ? f32_to_f16_bits(f) : (uint16_t)(f != f ? 0x7fc0u : f32_to_bf16_rne(f));
 }
 
-// One or two rows of activations: the weight stream.  A wavefront takes whole
-// weight rows, 1 KiB of contiguous codes an instruction, four instructions ahead, and
-// multiplies on v_dot4_i32_i8 with the activation codes, which every workgroup holds in
-// LDS.  SRC: codes and scales given, or (a whole linear layer) made by every
-// workgroup for itself, while its first weights are on their way: that is
-// cheaper than a launch.
-enum { kCodes = -1 };                             // else the activations' dtype
-constexpr int kGemvWaves = 4, kGemvAhead = 4;
+// A whole layer for one or two short rows, M K <= kGemvCodes: a wavefront takes whole
+// weight rows, 1 KiB of contiguous codes an instruction, the next row's loads ahead of this
+// one's v_dot4_i32_i8.  Every workgroup makes the activations' codes for itself, in LDS, while
+// its first weights are on their way: cheaper than a launch (1 x 1024 x 2048 4.2 us, not 5.9, 2 x 1024 x
+// 2048 5.1, not 6.2; 1 x 24576 x 4096 18.4, not 19.4; 1 x 4096 x 4096, 7.6 with weights from HBM, the same).  For
+// longer rows it is not: 1 x 8192 x 8192 17.4 us against 15.3, 2 x 8192 x 28672 92 against 44.
+constexpr int kGemvWaves = 4, kGemvRows = 2, kGemvCodes = 4096;
 
-template <int MM, int SRC>
-__global__ __launch_bounds__(64 * kGemvWaves) void w8a8_gemv_kernel(const void* __restrict__ xp, int64_t stride,
-                                                                    const float* __restrict__ xs,
+template <int MM, int DT>
+__global__ __launch_bounds__(64 * kGemvWaves) void w8a8_gemv_kernel(const uint16_t* __restrict__ xp, int64_t stride,
                                                                     const int8_t* __restrict__ wq,
                                                                     const float* __restrict__ ws,
-                                                                    uint16_t* __restrict__ y, int dt, int N, int K) {
-    extern __shared__ __align__(16) uint8_t codes[];          // MM rows of Kp bytes, zero past K
+                                                                    uint16_t* __restrict__ y, int N, int K) {
+    constexpr int kChunks = kGemvCodes / 1024 / MM;           // of a row, at most
+    __shared__ __align__(16) uint8_t codes[MM][1024 * kChunks];   // zero past K
     __shared__ uint32_t part[MM][kGemvWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int chunks = (K + 1023) >> 10, Kp = chunks << 10;
     const int total = (int)gridDim.x * kGemvWaves;
-    const int groups = (chunks + kGemvAhead - 1) / kGemvAhead;
     int row = (int)blockIdx.x * kGemvWaves + wave;
 
-    // group g of row n; a lane past the row's end reads its last 16 bytes,
-    // which meet zero activations
-    v4i w[kGemvAhead];
-    auto fetch = [&](int n, int g) {
+    // a lane past the row's end reads its last 16 bytes, which meet zero activations
+    v4i w[kChunks];
+    auto fetch = [&](int n) {
         const int8_t* p = wq + (size_t)min(n, N - 1) * K;
 #pragma unroll
-        for (int u = 0; u < kGemvAhead; ++u)
-            w[u] = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(p + min((g * kGemvAhead + u) * 1024 + 16 * lane, K - 16)));
+        for (int u = 0; u < kChunks; ++u)
+            if (u < chunks) w[u] = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(p + min(u * 1024 + 16 * lane, K - 16)));
     };
-    fetch(row, 0);
+    fetch(row);
 
     float sx[MM];
 #pragma unroll
     for (int m = 0; m < MM; ++m) {
-        uint2* q = reinterpret_cast<uint2*>(codes + m * Kp);
-        if constexpr (SRC == kCodes) {
-            const uint2* x = reinterpret_cast<const uint2*>(static_cast<const int8_t*>(xp) + m * stride);
-            for (int i = tid; i < Kp / 8; i += 64 * kGemvWaves) q[i] = i < K / 8 ? x[i] : make_uint2(0, 0);
-            sx[m] = xs[m];
-        } else {
-            const uint4* x = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(xp) + m * stride);
-            uint32_t mx = 0;
-            for (int i = tid; i < K / 8; i += 64 * kGemvWaves) mx = max(mx, largest8(x[i]));
-            mx = wave_max(mx);
-            if (lane == 0) part[m][wave] = mx;
-            __syncthreads();
+        uint2* q = reinterpret_cast<uint2*>(codes[m]);
+        const uint4* x = reinterpret_cast<const uint4*>(xp + m * stride);
+        uint32_t mx = 0;
+        for (int i = tid; i < K / 8; i += 64 * kGemvWaves) mx = max(mx, largest8(x[i]));
+        mx = wave_max(mx);
+        if (lane == 0) part[m][wave] = mx;
+        __syncthreads();
 #pragma unroll
-            for (int i = 0; i < kGemvWaves; ++i) mx = max(mx, part[m][i]);
-            sx[m] = token_scale<SRC>(mx);
-            const bool bad = sx[m] != sx[m];
-            const float inv = 1.0f / sx[m];
-            for (int i = tid; i < Kp / 8; i += 64 * kGemvWaves) q[i] = i < K / 8 && !bad ? codes_of<SRC>(x[i], inv) : make_uint2(0, 0);
-        }
+        for (int i = 0; i < kGemvWaves; ++i) mx = max(mx, part[m][i]);
+        sx[m] = token_scale<DT>(mx);
+        const bool bad = sx[m] != sx[m];
+        const float inv = 1.0f / sx[m];
+        for (int i = tid; i < Kp / 8; i += 64 * kGemvWaves) q[i] = i < K / 8 && !bad ? codes_of<DT>(x[i], inv) : make_uint2(0, 0);
     }
     __syncthreads();
 
     for (; row < N; row += total) {
+        v4i now[kChunks];
+#pragma unroll
+        for (int u = 0; u < kChunks; ++u) now[u] = w[u];
+        if (row + total < N) fetch(row + total);
         int acc[MM] = {};
-        for (int g = 0; g < groups; ++g) {
-            v4i now[kGemvAhead];
 #pragma unroll
-            for (int u = 0; u < kGemvAhead; ++u) now[u] = w[u];
-            if (g + 1 < groups) fetch(row, g + 1);
-            else if (row + total < N) fetch(row + total, 0);
+        for (int u = 0; u < kChunks; ++u) {
+            if (u >= chunks) break;
 #pragma unroll
-            for (int u = 0; u < kGemvAhead; ++u) {
-                const int c = g * kGemvAhead + u;
-                if (c >= chunks) break;
+            for (int m = 0; m < MM; ++m) {
+                const v4i x = *reinterpret_cast<const v4i*>(codes[m] + u * 1024 + 16 * lane);
 #pragma unroll
-                for (int m = 0; m < MM; ++m) {
-                    const v4i x = *reinterpret_cast<const v4i*>(codes + m * Kp + c * 1024 + 16 * lane);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[m] = __builtin_amdgcn_sdot4(now[u][e], x[e], acc[m], false);
-                }
+                for (int e = 0; e < 4; ++e) acc[m] = __builtin_amdgcn_sdot4(now[u][e], x[e], acc[m], false);
             }
         }
 #pragma unroll
@@ -199,9 +186,62 @@ __global__ __launch_bounds__(64 * kGemvWaves) void w8a8_gemv_kernel(const void* 
             int v = acc[m];
 #pragma unroll
             for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-            if (lane == 0) y[(size_t)m * N + row] = out_bits((float)v * sx[m] * ws[row], dt);
+            if (lane == 0) y[(size_t)m * N + row] = out_bits((float)v * sx[m] * ws[row], DT);
         }
     }
+}
+
+// Up to kDotRows rows of codes: a wavefront takes R weight rows, 1 KiB of contiguous
+// codes of each at a time, against activation codes that stay in the caches.  Bound by the weights'
+// stream: 1 x 57344 x 8192 65 us, 7.2 TB/s.  The tiles of gemm_w8a8.hip, whose
+// loads take 128 bytes of a row at a time, need 98 us there, and MFMAs on operands loaded
+// straight from HBM, 64 bytes of a row at a time, 79.  For four rows the two come close (24576 x 4096
+// 23.9 us against 25.4, 8192 x 28672 48 against 44, 57344 x 8192 83 against 92); for
+// eight the tiles are faster (92 against 105).
+constexpr int kDotRows = 4;
+template <int MM, int R>
+__global__ __launch_bounds__(256) void w8a8_dot_kernel(const int8_t* __restrict__ xq, const float* __restrict__ xs,
+                                                       const int8_t* __restrict__ wq, const float* __restrict__ ws,
+                                                       uint16_t* __restrict__ y, int dt, int N, int K) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = ((int)blockIdx.x * 4 + wave) * R;
+    if (n0 >= N) return;
+    const int8_t *pw[R], *px[MM];
+#pragma unroll
+    for (int r = 0; r < R; ++r) pw[r] = wq + (size_t)min(n0 + r, N - 1) * K;
+#pragma unroll
+    for (int m = 0; m < MM; ++m) px[m] = xq + (size_t)m * K;
+    int acc[R][MM] = {};
+    auto chunk = [&](int at, bool in) {
+        v4i w[R], x[MM];
+#pragma unroll
+        for (int r = 0; r < R; ++r) w[r] = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(pw[r] + at));
+#pragma unroll
+        for (int m = 0; m < MM; ++m) {
+            x[m] = *reinterpret_cast<const v4i*>(px[m] + at);
+            if (!in) x[m] = (v4i){0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int m = 0; m < MM; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[r][m] = __builtin_amdgcn_sdot4(w[r][e], x[m][e], acc[r][m], false);
+    };
+    const int whole = K >> 10;
+#pragma unroll R > 2 ? 2 : 4
+    for (int c = 0; c < whole; ++c) chunk((c << 10) + 16 * lane, true);
+    const int at = (whole << 10) + 16 * lane;
+    if (whole << 10 < K) chunk(min(at, K - 16), at < K);      // a lane past the row's end: zero activations
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int m = 0; m < MM; ++m) {
+            int v = acc[r][m];
+#pragma unroll
+            for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+            if (lane == 0 && n0 + r < N) y[(size_t)m * N + n0 + r] = out_bits((float)v * xs[m] * ws[n0 + r], dt);
+        }
 }
 
 // Streaming product: 16 rows of activations (grid.y) against 16 CB weight rows
@@ -270,9 +310,15 @@ __global__ __launch_bounds__(64 * KW) void w8a8_stream_kernel(const int8_t* __re
 }
 
 // ---------------------------------------------------------------- the choice
-// One or two rows whose codes fit 64 KiB of LDS take the GEMV.
-constexpr int kGemvRows = 2, kGemvLds = 64 * 1024;
-bool gemv_shape(int64_t M, int64_t K) { return M <= kGemvRows && M * ((K + 1023) / 1024 * 1024) <= kGemvLds; }
+// R: more weight rows a wavefront load the activations less often, but leave fewer
+// wavefronts.  us at R = 1, 2, 4: 1 x 24576 x 4096 17.0, 17.9, 21.4, 1 x 57344 x 8192 65, 68, 73; 2 x 4096 x 4096
+// 5.9, 6.3, 8.2, 2 x 57344 x 8192 86, 74, 74; 3 x 1024 x 2048 4.2, 5.1, 6.7, 4 x 8192 x 8192 22.0, 18.4, 19.8, 4 x 57344 x 8192
+// 125, 98, 83.
+int dot_rows(int64_t M, int64_t N, int64_t K) {
+    if (M == 1) return 1;
+    if (M == 2) return N * K < 1 << 26 ? 1 : 2;
+    return N * K < 1 << 24 ? 1 : N * K < 1 << 27 ? 2 : 4;
+}
 
 struct Plan {
     int rows, cols, splits;                       // rows 0: the streaming kernel
@@ -280,14 +326,18 @@ struct Plan {
 
 // K % 64 == 0 takes tiles: those, and the split of K, with the least estimated
 // time, in microseconds.  A workgroup's stage of 128 codes takes `stage` on a full
-// chip (fitted to 4096 x 57344 x 8192 and, for the small tiles, 16 and 64 x 57344 x
-// 8192), 0.7 of it on an empty one; the whole no less than the weights' way from HBM.  A
-// split costs a launch and its partial sums both ways.
+// chip, 0.6 of it on an empty one, and no less than HBM's latency over the stages in flight;
+// the whole takes no less than the weights' way from HBM.  A split costs a launch and its
+// partial sums both ways.  The constants are fitted to 60 shapes from 5 x 8192 x 28672 to 300 rows, weights
+// from HBM: 1.6% slower than the fastest of all tiles and splits on average, 15% at worst; without the
+// latency 5.4% and 50%.  Other K take the streaming kernel, which any K % 16 == 0 suits (tiles need
+// whole steps of 64 codes).
 Plan plan_of(int64_t M, int64_t N, int64_t K, size_t room) {
     Plan best = {0, 0, 1};
     if (K % 64 != 0) return best;
-    static const struct { int rows, cols; double stage; } kTiles[] = {
-        {256, 256, 1.60}, {256, 128, 0.92}, {128, 128, 0.58}, {64, 128, 0.37}, {64, 64, 0.26}, {32, 128, 0.32}, {32, 64, 0.20}};
+    static const struct { int rows, cols, depth; double stage; } kTiles[] = {
+        {256, 256, 2, 1.60}, {256, 128, 3, 0.92}, {128, 128, 4, 0.58}, {64, 128, 3, 0.43},
+                {64, 64, 4, 0.26}, {32, 128, 3, 0.39}, {32, 64, 4, 0.20}};
     const int64_t stages = (K + 127) / 128;
     double least = 1e30;
     for (const auto& t : kTiles) {
@@ -297,10 +347,11 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, size_t room) {
             if (s > 1 && (size_t)M * N * 4 * s > room) break;
             const double groups = (double)tiles * s, full = groups / 256 < 1 ? groups / 256 : 1;
             const double rounds = groups <= 1024 ? (double)(int64_t)((groups + 255) / 256) : groups / 256;
-            const double work = rounds * (double)((stages + s - 1) / s) * t.stage * (0.7 + 0.3 * full);
-            const double hbm = (double)N * K / 6.3e6;
+            const double busy = t.stage * (0.6 + 0.4 * full), idle = 0.72 / (t.depth - 1);
+            const double work = rounds * (double)((stages + s - 1) / s) * (busy > idle ? busy : idle);
+            const double hbm = (double)N * K / 7e6;
             double us = 4.0 + 1.0 * rounds + (work > hbm ? work : hbm);
-            if (s > 1) us += 2.5 + (double)M * N * (8.0 * s + 2) / 4.5e6;
+            if (s > 1) us += 3.3 + (double)M * N * (8.0 * s + 2) / 4.5e6;
             if (us < least) {
                 least = us;
                 best = {t.rows, t.cols, s};
@@ -323,17 +374,32 @@ int launch_quant(const void* x, int8_t* q, float* s, int64_t rows, int64_t K, in
     return (int)hipGetLastError();
 }
 
-template <int SRC>
-int launch_gemv(const void* x, int64_t stride, const float* xs, const int8_t* wq, const float* ws, void* y, int dtype,
-                int64_t M, int64_t N, int64_t K, hipStream_t stream) {
+template <int DT>
+int launch_gemv(const void* x, int64_t stride, const int8_t* wq, const float* ws, void* y, int64_t M, int64_t N, int64_t K,
+                hipStream_t stream) {
     const int64_t want = (N + kGemvWaves - 1) / kGemvWaves;
     const unsigned grid = (unsigned)(want < 2048 ? want : 2048);   // 8 workgroups a CU
-    const size_t lds = (size_t)M * ((K + 1023) / 1024 * 1024);
+    const uint16_t* p = static_cast<const uint16_t*>(x);
     uint16_t* o = static_cast<uint16_t*>(y);
-    if (M == 1) w8a8_gemv_kernel<1, SRC><<<grid, 64 * kGemvWaves, lds, stream>>>(x, stride, xs, wq, ws, o, dtype, (int)N, (int)K);
-    else w8a8_gemv_kernel<2, SRC><<<grid, 64 * kGemvWaves, lds, stream>>>(x, stride, xs, wq, ws, o, dtype, (int)N, (int)K);
+    if (M == 1) w8a8_gemv_kernel<1, DT><<<grid, 64 * kGemvWaves, 0, stream>>>(p, stride, wq, ws, o, (int)N, (int)K);
+    else w8a8_gemv_kernel<2, DT><<<grid, 64 * kGemvWaves, 0, stream>>>(p, stride, wq, ws, o, (int)N, (int)K);
     return (int)hipGetLastError();
 }
+
+template <int MM>
+int launch_dot(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, uint16_t* y, int dtype, int64_t N,
+               int64_t K, hipStream_t stream) {
+    const int r = dot_rows(MM, N, K);
+    const unsigned grid = (unsigned)((N + 4 * r - 1) / (4 * r));
+    if (r == 1) w8a8_dot_kernel<MM, 1><<<grid, 256, 0, stream>>>(xq, xs, wq, ws, y, dtype, (int)N, (int)K);
+    if constexpr (MM > 1)
+        if (r == 2) w8a8_dot_kernel<MM, 2><<<grid, 256, 0, stream>>>(xq, xs, wq, ws, y, dtype, (int)N, (int)K);
+    if constexpr (MM > 2)
+        if (r == 4) w8a8_dot_kernel<MM, 4><<<grid, 256, 0, stream>>>(xq, xs, wq, ws, y, dtype, (int)N, (int)K);
+    return (int)hipGetLastError();
+}
+
+bool gemv_shape(int64_t M, int64_t K) { return M <= kGemvRows && M * K <= kGemvCodes; }
 
 }  // namespace
 }  // namespace wush
@@ -353,7 +419,7 @@ int wush_quant_int8_token(const void* x, int dtype, int8_t* q, float* s, int64_t
 }
 
 size_t wush_gemm_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    if (M <= 0 || N <= 0 || K <= 0 || K % 16 != 0 || wush::gemv_shape(M, K)) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || K % 16 != 0 || M <= wush::kDotRows) return 0;
     const wush::Plan p = wush::plan_of(M, N, K, SIZE_MAX);
     return p.splits > 1 ? (size_t)p.splits * M * N * 4 : 0;
 }
@@ -367,8 +433,13 @@ int wush_gemm_w8a8(const int8_t* xq, const float* xs, const int8_t* wq, const fl
     WUSH_REQUIRE(xq && xs && wq && ws && y);
     WUSH_REQUIRE(((uintptr_t)xq & 15u) == 0 && ((uintptr_t)wq & 15u) == 0 && ((uintptr_t)xs & 3u) == 0 &&
                  ((uintptr_t)ws & 3u) == 0 && ((uintptr_t)y & 1u) == 0);
-    if (wush::gemv_shape(M, K)) return wush::launch_gemv<wush::kCodes>(xq, K, xs, wq, ws, y, dtype, M, N, K, stream);
     uint16_t* o = static_cast<uint16_t*>(y);
+    switch (M) {
+        case 1: return wush::launch_dot<1>(xq, xs, wq, ws, o, dtype, N, K, stream);
+        case 2: return wush::launch_dot<2>(xq, xs, wq, ws, o, dtype, N, K, stream);
+        case 3: return wush::launch_dot<3>(xq, xs, wq, ws, o, dtype, N, K, stream);
+        case 4: return wush::launch_dot<4>(xq, xs, wq, ws, o, dtype, N, K, stream);
+    }
     const bool usable = workspace && ((uintptr_t)workspace & 15u) == 0;
     const wush::Plan p = wush::plan_of(M, N, K, usable ? workspace_bytes : 0);
     if (p.rows)
@@ -394,11 +465,11 @@ int wush_linear_w8a8(const void* x, int64_t row_stride, const int8_t* wq, const 
     const size_t need = wush_linear_w8a8_workspace_bytes(M, N, K), scales = ((size_t)M * 4 + 15) & ~(size_t)15;
     WUSH_REQUIRE(x && wq && ws && y && workspace_bytes >= need && (need == 0 || (workspace && ((uintptr_t)workspace & 15u) == 0)));
     WUSH_REQUIRE((((uintptr_t)x | (uintptr_t)wq) & 15u) == 0 && ((uintptr_t)ws & 3u) == 0 && ((uintptr_t)y & 1u) == 0);
-    WUSH_REQUIRE(M == 1 || row_stride % 8 == 0);
+    WUSH_REQUIRE(M == 1 || (row_stride >= 0 && row_stride % 8 == 0));
     if (wush::gemv_shape(M, K))
         return dtype == WUSH_DTYPE_BF16
-                   ? wush::launch_gemv<WUSH_DTYPE_BF16>(x, row_stride, nullptr, wq, ws, y, dtype, M, N, K, stream)
-                   : wush::launch_gemv<WUSH_DTYPE_F16>(x, row_stride, nullptr, wq, ws, y, dtype, M, N, K, stream);
+                   ? wush::launch_gemv<WUSH_DTYPE_BF16>(x, row_stride, wq, ws, y, M, N, K, stream)
+                   : wush::launch_gemv<WUSH_DTYPE_F16>(x, row_stride, wq, ws, y, M, N, K, stream);
     int8_t* q = static_cast<int8_t*>(workspace);
     float* s = reinterpret_cast<float*>(q + (size_t)M * K);
     const int st = wush_quant_int8_token(x, dtype, q, s, M, K, row_stride, stream);
