@@ -321,7 +321,7 @@ int wush_kv8_append(const void *q, const void *k, const void *v, int dtype, cons
  * head hq / (q_heads / heads),
  *   out = sum_t softmax_t(cap(scale * q . k_t)) v_t over t in [max(0, p - window + 1), p]
  * with window 0 for all t <= p, and cap(x) = softcap * tanh(x / softcap), softcap 0 for
- * none.  A query that sees no token gets zeros.  q (tokens, q_heads, head_dim)
+ * none; scale finite, of either sign.  A query that sees no token gets zeros.  q (tokens, q_heads, head_dim)
  * bf16 or fp16 with a token and a head stride (multiples of 8, 16-byte aligned);
  * out (tokens, q_heads, head_dim) contiguous, of the same type.
  *   max_len: a bound of seq_lens that the host knows (0: the table's room). It only

@@ -373,14 +373,16 @@ struct Plan {
 // For each tile height, 16 (kv8_rows_kernel), 128 and 256 (kv8_chunk.hip), the
 // stretches of the cache per item with the least estimated time, in microseconds: a
 // workgroup's pass over `step` tokens times the workgroups of a CU, and where there is
-// more than one stretch the joining.  Of the three, the height with the least time (the last
-// constants are fitted to that): over 72 shapes, from 1 to 16 sequences of 1024 and 8192 with 41 to 1024 rows of new tokens,
-// 3% slower than the fastest height on average and 38% at worst; 16 rows below a fixed number
-// of rows a sequence, tall ones above, was 15% slower on average and 98% at worst.
+// more than one stretch the joining.  Of the three, the height with the least time: a
+// start, and passes that take `alone` where a CU has one workgroup and `pass` for each where it has
+// more.  Those constants are fitted to 72 shapes, 1 and 16 sequences of 1024 and 8192 with 41 to 1024 rows of
+// new tokens: 1% slower than the fastest height on average, 19% at worst; 16 rows below
+// a fixed number of rows a sequence, tall ones above, was 15% slower on average and 98% at
+// worst (16 sequences of 8192 with 32 heads of 64 and 170 new tokens: 467 us, now 267).
 Plan plan_of(const Kv8Cache& c, int64_t seqs, int64_t tokens, bool ragged, int group, int64_t table_stride, int window,
              int64_t max_len) {
-    static const struct { int rows, step; double split, start, pass; } kHeights[] = {
-        {16, 256, 2.1, 0.0, 1.3}, {128, kTile, 1.5, 2.0, 1.2}, {256, kTile, 1.5, 8.0, 2.1}};
+    static const struct { int rows, step; double split, start, alone, pass; } kHeights[] = {
+        {16, 256, 2.1, 0.5, 2.2, 1.65}, {128, kTile, 1.5, 3.0, 1.7, 1.2}, {256, kTile, 1.5, 8.0, 2.1, 2.1}};
     const int64_t rows = tokens * group;
     const double joined = 0.02 + (double)rows * c.heads * (c.dim + kPartExtra) * 8 / 4e6;   // a stretch's sums both ways
     Plan best = {16, 1, 1, 0};
@@ -403,8 +405,8 @@ Plan plan_of(const Kv8Cache& c, int64_t seqs, int64_t tokens, bool ragged, int g
                 splits = n;
             }
         }
-        const double full = (double)(items * c.heads * splits) / 256;
-        const double us = t.start + t.pass * (0.3 + 0.7 * c.dim / 128) * (double)((most + splits - 1) / splits) * (full > 1 ? full : 1) +
+        const double shared = t.pass * (double)(items * c.heads * splits) / 256;
+        const double us = t.start + (0.15 + 0.85 * c.dim / 128) * (double)((most + splits - 1) / splits) * (shared > t.alone ? shared : t.alone) +
                           (splits > 1 ? 3.0 + joined * (double)splits : 0.0);
         if (us < least) {
             least = us;

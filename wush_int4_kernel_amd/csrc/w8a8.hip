@@ -406,6 +406,8 @@ bool gemv_shape(int64_t M, int64_t K) { return M <= kGemvRows && M * K <= kGemvC
 
 extern "C" {
 
+static constexpr int64_t kMostRows = 0x7fff0000LL;    // rounded up to tiles, still an int
+
 int wush_quant_int8_token(const void* x, int dtype, int8_t* q, float* s, int64_t rows, int64_t K, int64_t row_stride,
                           hipStream_t stream) {
     WUSH_REQUIRE(rows >= 0 && K > 0 && K % 16 == 0 && K <= WUSH_W8A8_MAX_K);
@@ -427,7 +429,7 @@ size_t wush_gemm_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
 int wush_gemm_w8a8(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, void* y, int dtype, int64_t M,
                    int64_t N, int64_t K, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     WUSH_REQUIRE(M >= 0 && N >= 0 && K > 0 && K % 16 == 0 && K <= WUSH_W8A8_MAX_K);
-    WUSH_REQUIRE(M <= 0x7fffffffLL && N <= 0x7fffffffLL);
+    WUSH_REQUIRE(M <= kMostRows && N <= kMostRows);
     WUSH_REQUIRE(dtype == WUSH_DTYPE_BF16 || dtype == WUSH_DTYPE_F16);
     if (M == 0 || N == 0) return (int)hipSuccess;
     WUSH_REQUIRE(xq && xs && wq && ws && y);
@@ -459,7 +461,7 @@ size_t wush_linear_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
 int wush_linear_w8a8(const void* x, int64_t row_stride, const int8_t* wq, const float* ws, void* y, int dtype, int64_t M,
                      int64_t N, int64_t K, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     WUSH_REQUIRE(M >= 0 && N >= 0 && K > 0 && K % 16 == 0 && K <= WUSH_W8A8_MAX_K);
-    WUSH_REQUIRE(M <= 0x7fffffffLL && N <= 0x7fffffffLL);
+    WUSH_REQUIRE(M <= kMostRows && N <= kMostRows);
     WUSH_REQUIRE(dtype == WUSH_DTYPE_BF16 || dtype == WUSH_DTYPE_F16);
     if (M == 0 || N == 0) return (int)hipSuccess;
     const size_t need = wush_linear_w8a8_workspace_bytes(M, N, K), scales = ((size_t)M * 4 + 15) & ~(size_t)15;
