@@ -8,11 +8,10 @@
 // is placed behind an MFMA; a step's operands are read during the step before.
 //
 // 4096 x 57344 x 8192: 1.48-1.52 ms, 2.5-2.6 POP/s (a library int8 product on the
-// same card 2.1-2.3); 203 x 8192 x 8192 25.5 us, 13 x 24576 x 4096 17 to 23 us (weights from the last
+// same card 2.1-2.3); 203 x 8192 x 8192 25.5 us, 13 x 24576 x 4096 17 to 22 us (weights from the last
 // cache, or from HBM).  The large tiles are bound by what feeds them: without the DMAs the largest
 // shape takes 1.19 ms, without the MFMAs 1.28 (64 KB a stage and CU, 11.7 TB/s over the
-// chip).  Issuing the DMAs earlier, in bursts, or starting workgroups at
-// staggered depths changes nothing; stages of 64 codes, five deep, are slower (1.63 ms): a DMA of half
+// chip).  Issuing the DMAs earlier or in bursts changes nothing; stages of 64 codes, five deep, are slower (1.63 ms): a DMA of half
 // lines costs what whole lines do.
 #include "gemm_h16_device.h"
 #include "w8a8.h"
@@ -79,6 +78,12 @@ void gemm_w8a8_kernel(const int8_t* __restrict__ xq, const float* __restrict__ x
     const int NS = (K + 127) >> 7;                               // stages, the last half one if K % 128 == 64
     const int first = (int)((long long)NS * split / splits), last = (int)((long long)NS * (split + 1) / splits);
     const bool half = (K & 127) != 0;
+    // The sum does not depend on its order: column c of the tiles begins at stage c (of the
+    // whole ones; a half one stays last), so that workgroups in step do not ask for
+    // addresses a multiple of K apart, which fall on few of HBM's channels.  64 x 57344 x 8192 95 us, from the
+    // same stage on 107; 64 x 24576 x 4096 26, not 30; 256 x 57344 x 8192 128, not 143; none slower.
+    const int whole = last - first - (half && last == NS ? 1 : 0);
+    const int turn = whole > 0 ? tn % whole : 0;
     const uint32_t lds0 = lds_addr(smem);
 
     // DMA k of a stage: 8 rows; lane l fetches piece (l % 8) ^ f(r) of row r = 8
@@ -98,7 +103,8 @@ void gemm_w8a8_kernel(const int8_t* __restrict__ xq, const float* __restrict__ x
     const int8_t* abase = xq + (size_t)m0 * K;
     const int8_t* bbase = wq + (size_t)n0 * K;
     auto issue = [&](int st, int buf, int k) {
-        const size_t o = (size_t)st * 128;
+        const int at = st - first >= whole ? st : st + turn - (st + turn >= first + whole ? whole : 0);
+        const size_t o = (size_t)at * 128;
         const uint32_t dst = lds0 + buf * kBuf;
         const uint32_t v = voff[k] - (half && st == NS - 1 ? back[k >= DA][(k < DA ? k : k - DA) & 1] : 0u);
         if (k < DA) dma16_uniform(abase + o, v, dst + (wave * DA + k) * 1024);
