@@ -372,8 +372,13 @@ struct Plan {
 
 // For each tile height, 16 (kv8_rows_kernel), 128 and 256 (kv8_chunk.hip), the
 // stretches of the cache per item with the least estimated time, in microseconds: a
-// workgroup's pass over `step` tokens times the workgroups of a CU, and where there is
-// more than one stretch the joining.  Of the three, the height with the least time: a
+// workgroup's pass over `step` tokens (`split` alone on its CU, `more` for each where several
+// share it: the loads of one cover the latencies of another), `ends` passes' worth for its beginning
+// and end, and where there is more than one stretch the joining.  `more` below `split`
+// halves the stretches of long caches: 8 ragged sequences up to 32768 79 us, not 91 (8 heads of
+// 128; of 64 48, not 61), 16 up to 8192 46, not 51, one of 131072 58 to 59 in both; over 104 shapes of decode and few new
+// tokens 2.4% faster on average, 28% at best, 5% slower at worst (5 of 12000, page of 16); without `ends`
+// 12 of 3000 took 18.0 us, not 15.1.  Of the three, the height with the least time: a
 // start, and passes that take `alone` where a CU has one workgroup and `pass` for each where it has
 // more.  Those constants are fitted to 72 shapes, 1 and 16 sequences of 1024 and 8192 with 41 to 1024 rows of
 // new tokens: 1% slower than the fastest height on average, 19% at worst; 16 rows below
@@ -381,8 +386,8 @@ struct Plan {
 // worst (16 sequences of 8192 with 32 heads of 64 and 170 new tokens: 467 us, now 267).
 Plan plan_of(const Kv8Cache& c, int64_t seqs, int64_t tokens, bool ragged, int group, int64_t table_stride, int window,
              int64_t max_len) {
-    static const struct { int rows, step; double split, start, alone, pass; } kHeights[] = {
-        {16, 256, 2.1, 0.5, 2.2, 1.65}, {128, kTile, 1.5, 3.0, 1.7, 1.2}, {256, kTile, 1.5, 8.0, 2.1, 2.1}};
+    static const struct { int rows, step; double split, more, ends, start, alone, pass; } kHeights[] = {
+        {16, 256, 2.1, 1.65, 1.0, 0.5, 2.2, 1.65}, {128, kTile, 1.5, 1.5, 0.0, 3.0, 1.7, 1.2}, {256, kTile, 1.5, 1.5, 0.0, 8.0, 2.1, 2.1}};
     const int64_t rows = tokens * group;
     const double joined = 0.02 + (double)rows * c.heads * (c.dim + kPartExtra) * 8 / 4e6;   // a stretch's sums both ways
     Plan best = {16, 1, 1, 0};
@@ -398,7 +403,8 @@ Plan plan_of(const Kv8Cache& c, int64_t seqs, int64_t tokens, bool ragged, int g
         double fewest = 1e30;
         int64_t splits = 1;
         for (int64_t n = 1; n <= most && n <= 256 && (n == 1 || items * c.heads * n <= 1024); n += n < 16 ? 1 : n / 16) {
-            const double us = t.split * c.dim / 128 * (double)((most + n - 1) / n) * (double)((items * c.heads * n + 255) / 256) +
+            const int64_t deep = (items * c.heads * n + 255) / 256;          // workgroups of a CU
+            const double us = (deep > 1 ? t.more * (double)deep : t.split) * c.dim / 128 * ((double)((most + n - 1) / n) + t.ends) +
                               (n > 1 ? 3.0 + joined * (double)n : 0.0);
             if (us < fewest) {
                 fewest = us;
