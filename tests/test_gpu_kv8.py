@@ -284,6 +284,17 @@ def test_long_cache_is_split(dev, Hq, Hkv, D, page):
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("B", [33, 128, 129])
+@pytest.mark.parametrize("Hq,Hkv", [(8, 8), (40, 2), (9, 9)])
+def test_many_sequences_over_a_long_cache(dev, B, Hq, Hkv):
+    # taken by length, up to 128 of them: equal lengths, empty sequences, a round of
+    # the CUs that ends inside the batch, two workgroups a head (20 query rows)
+    lens = [(1100, 0, 70, 1, 64, 70, 300, 129)[b % 8 if b % 40 else 0] if b % 8 or b % 40 == 0 else 65 for b in range(B)]
+    bt = Batch(B + Hq, lens, [1] * B, Hq, Hkv, 64, 64, BF)
+    check_attention(dev, bt, ragged=False, max_len=1100)
+    check_attention(dev, bt, ragged=False, window=1030, filled=False)
+
+
 def test_bound_of_lengths_only_splits(dev):
     # a bound below the true lengths costs speed, not tokens; a window over a long cache
     bt = Batch(6, [5000, 300], [1, 1], 8, 2, 64, 16, BF)

@@ -17,6 +17,7 @@ struct AttnArgs {
     int tile_shift;                               // log2 of it
     int items;                                    // work items a key/value head
     int splits, chunk;                            // stretches of the cache, tokens of one
+    int round;                                    // sequences whose workgroups make one round of the CUs; 0: taken as they come
     float scale, cap;                             // cap 0: none
     uint16_t* out;
     float* part;                                  // (token, head, split): D sums, maximum, sum of weights, 2 unused

@@ -27,8 +27,8 @@
 // rescaled, only when a score passes it by 2^3.
 //
 // Bound by HBM where the cache fills the chip (one token behind 131072, 8 heads of 128:
-// 268 MB in 56 us with 5 to join, 4.8 TB/s; 64 ragged sequences up to 4096: 344 MB in 71 us, the
-// longest sequence ending last), by a wavefront's instructions and latencies otherwise (3 x 300: 6 us).  Two
+// 268 MB in 56 us with 5 to join, 4.8 TB/s; 64 ragged sequences up to 4096: 344 MB in 66 us,
+// the CUs not quite evenly loaded), by a wavefront's instructions and latencies otherwise (3 x 300: 6 us).  Two
 // tiles' loads in flight instead of one changed nothing; without the non-temporal hint
 // 131072 tokens took 2 us more, but 8192-token stretches 20% less, so loads have none.
 #include "kv8_attention.h"
@@ -50,6 +50,37 @@ __device__ __forceinline__ float quarters_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
+// The sequence that is taken at place w: by length, the longest first, every second
+// round of the CUs the other way round, so that a CU's workgroups together hold about as
+// much as another's.  A thread ranks one sequence; keys differ, so ranks do.
+// 64 ragged sequences up to 4096 (8 heads of 128) 68 us, as they come 73; 48 of 4000 60, not 69; 100 of
+// 2500 with heads of 64 38, not 45; 6% slower at worst of 34 shapes (128 of 1100 with heads of 64).  With
+// caches below kLeastSorted tokens, or more sequences than kMostSorted, the ranking costs what it
+// gives or more: 64 of 300 11.5 us, as they come 11.3; 256 of 1200 94 and 87.
+constexpr int kMostSorted = 128, kLeastSorted = 1024;
+
+__device__ __forceinline__ int by_length(const AttnArgs& a, int w) {
+    const Kv8Batch& t = a.batch;
+    __shared__ __align__(16) int key[kMostSorted];
+    __shared__ int found;
+    const int tid = threadIdx.x, mine = tid < t.seqs ? min(max(t.lens[tid], 0), 0x7fffff) << 8 | tid : -1;
+    if (tid < kMostSorted) key[tid] = mine;
+    __syncthreads();
+    const int k = w / a.round, want = k & 1 ? min((k + 1) * a.round, t.seqs) - 1 - w % a.round : w;
+    if (mine >= 0) {
+        int rank = 0;
+        for (int j = 0; j < t.seqs; j += 32)      // behind them: -1, below every key
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+                const int4 o = *reinterpret_cast<const int4*>(key + j + i);
+                rank += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+            }
+        if (rank == want) found = tid;
+    }
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(found);
+}
+
 template <int DT, int D, bool CAP>
 __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a) {
     constexpr int NJ = D / 64, NB = D / 16;
@@ -63,7 +94,8 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
     const int h = (int)blockIdx.x % a.cache.heads, rest = (int)blockIdx.x / a.cache.heads;
     const int item = rest % a.items, split = rest / a.items;
     int row0;
-    const int b = item_rows(a, item, row0);
+    int b = item_rows(a, item, row0);
+    if (a.round) b = by_length(a, b);
     const Kv8Seq s = kv8_seq(t, b);
     if (row0 >= s.count * G) return;
     const Span span = span_of(a, s, row0);
@@ -493,6 +525,13 @@ int wush_kv8_attention(const void* q, int dtype, int64_t q_token_stride, int64_t
     a.splits = p.splits;
     a.chunk = p.chunk;
     a.items = (int)p.items;
+    // Sorted by length where a stretch has more workgroups than the chip CUs, and the cache is long enough.
+    int64_t range = table_stride << a.cache.page_log2;
+    if (max_len > 0 && max_len < range) range = max_len;
+    if (a.window > 0 && a.window < range) range = a.window;
+    const int64_t wide = (int64_t)a.cache.heads * ((a.group + 15) / 16);        // workgroups of a sequence
+    const bool sorted = p.tile_rows == 16 && !cu_q && seqs <= wush::kMostSorted && wide * seqs > 256 && range >= wush::kLeastSorted;
+    a.round = !sorted ? 0 : wide < 256 ? (int)(256 / wide) : 1;
     a.scale = scale;
     a.cap = softcap;
     a.out = static_cast<uint16_t*>(out);
