@@ -27,7 +27,7 @@
 // rescaled, only when a score passes it by 2^3.
 //
 // Bound by HBM where the cache fills the chip (one token behind 131072, 8 heads of 128:
-// 268 MB in 56 us with 5 to join, 4.8 TB/s; 64 ragged sequences up to 4096: 344 MB in 66 us,
+// 268 MB in 57 us with 6 to join, 4.8 TB/s; 64 ragged sequences up to 4096: 344 MB in 66 us,
 // the CUs not quite evenly loaded), by a wavefront's instructions and latencies otherwise (3 x 300: 6 us).  Two
 // tiles' loads in flight instead of one changed nothing; without the non-temporal hint
 // 131072 tokens took 2 us more, but 8192-token stretches 20% less, so loads have none.
