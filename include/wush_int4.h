@@ -285,6 +285,9 @@ typedef struct wush_kv8_cache {
     int32_t heads, page_size, head_dim;
 } wush_kv8_cache;
 
+/* Longest sequence that a cache holds: a length beyond it (or below 0) counts as 0. */
+#define WUSH_KV8_MAX_LENGTH (1 << 30)
+
 /* The batch that the next two take, all on the device: block_table (seqs,
  * table_stride) int32, a sequence's pages in order; seq_lens (seqs) int32, each
  * sequence's length INCLUDING the call's new tokens, which are its last ones; cu_q

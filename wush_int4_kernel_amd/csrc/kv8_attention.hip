@@ -430,7 +430,7 @@ Plan plan_of(const Kv8Cache& c, int64_t seqs, int64_t tokens, bool ragged, int g
         if (max_len > 0 && max_len < range) range = max_len;
         if (window > 0 && window + 64 + t.rows / group < range) range = window + 64 + t.rows / group;
         if (range < 1) range = 1;
-        if (range > 1 << 30) range = 1 << 30;     // the last stretch takes what lies behind
+        if (range > WUSH_KV8_MAX_LENGTH) range = WUSH_KV8_MAX_LENGTH;
         const int64_t most = (range + t.step - 1) / t.step;
         double fewest = 1e30;
         int64_t splits = 1;

@@ -38,7 +38,8 @@ struct Kv8Seq {
     int first, count, len;                        // first new token, new tokens, length behind them
 };
 
-// Sequence b; device values out of range count as no tokens.
+// Sequence b; device values out of range count as no tokens.  A length of at most
+// WUSH_KV8_MAX_LENGTH keeps a position, with a window or some tiles added, in 32 bits.
 __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Batch& t, int b) {
     Kv8Seq s;
     if (t.cu) {
@@ -48,7 +49,8 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Batch& t, int b) {
         s.first = b;
         s.count = 1;
     }
-    s.len = max(t.lens[b], 0);
+    s.len = t.lens[b];
+    if (s.len < 0 || s.len > WUSH_KV8_MAX_LENGTH) s.len = 0;
     return s;
 }
 
