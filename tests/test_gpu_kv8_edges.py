@@ -36,3 +36,15 @@ def test_length_beyond_the_longest(dev, ragged):
     q, k, v, cs = (t.to(dev) for t in (bt.q, bt.k, bt.v, bt.cos_sin))
     _C.kv8_append(q, k, v, cs, *gpu, table, i32([2 ** 31 - 1, -1, -2 ** 31], dev), cu_q=cu)
     assert all(torch.equal(torch.nan_to_num(a), torch.nan_to_num(b)) for a, b in zip(gpu, kept))
+
+
+WIDE = [2 ** 30 - 1, 2 ** 30, 2 ** 31 - 1, 2 ** 31, 2 ** 62]
+
+
+@pytest.mark.parametrize("window", WIDE)
+@pytest.mark.parametrize("Hq,Hkv,lens,n", [(4, 2, [0, 3, 40], [2, 6, 40]), (64, 8, [300, 130, 5], [900, 130, 9]), (8, 8, [5000, 3], [1, 1])])
+def test_window_wider_than_every_sequence(dev, window, Hq, Hkv, lens, n):
+    # also where more tokens are new than the sequence has (positions below 0)
+    bt = Batch(42, lens, n, Hq, Hkv, 64, 16, BF)
+    out = check_attention(dev, bt, window=window)
+    assert torch.equal(out, check_attention(dev, bt, filled=False))

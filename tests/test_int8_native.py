@@ -118,3 +118,10 @@ def test_torch_operators():
         _C.kv8_attention(q, k, v, s, s, i[None], i)
     with pytest.raises(RuntimeError, match="CUDA"):
         _C.kv8_read(k, v, s, s, i)
+
+
+def test_window_wider_than_every_sequence_is_planned_as_none(capi):
+    lib = capi.load()
+    need = [lib.wush_kv8_attention_workspace_bytes(ctypes.byref(cache(capi, heads=8, head_dim=128)), 1, 1, 0, 64, 8192, w, 0)
+            for w in (0, 2 ** 30 - 1, 2 ** 30, 2 ** 31 - 1, 2 ** 31, 2 ** 62)]
+    assert need[0] > 0 and need == need[:1] * 6

@@ -397,6 +397,10 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(const AttnArgs a) {
     else *out = (uint16_t)out16<DT>(o[0] * inv);
 }
 
+// A window of the longest sequence or more hides nothing; a shorter one, added to or taken
+// from a position, stays in 32 bits.
+int window_of(int64_t window) { return window >= WUSH_KV8_MAX_LENGTH ? 0 : (int)window; }
+
 struct Plan {
     int tile_rows, splits, chunk;
     int64_t items;
@@ -488,8 +492,8 @@ size_t wush_kv8_attention_workspace_bytes(const wush_kv8_cache* cache, int64_t s
                                           int64_t q_heads, int64_t table_stride, int64_t window, int64_t max_len) {
     wush::Kv8Cache c;
     if (wush::kv8_cache_of(cache, &c) || seqs <= 0 || tokens <= 0 || q_heads <= 0 || q_heads % c.heads) return 0;
-    const int w = window <= 0 || window > 0x7fffffff ? 0 : (int)window;
-    const wush::Plan p = wush::plan_of(c, seqs, tokens, ragged != 0, (int)(q_heads / c.heads), table_stride, w, max_len);
+    const wush::Plan p = wush::plan_of(c, seqs, tokens, ragged != 0, (int)(q_heads / c.heads), table_stride,
+                                       wush::window_of(window < 0 ? 0 : window), max_len);
     return p.splits > 1 ? (size_t)tokens * q_heads * p.splits * (c.dim + wush::kPartExtra) * 4 : 0;
 }
 
@@ -517,7 +521,7 @@ int wush_kv8_attention(const void* q, int dtype, int64_t q_token_stride, int64_t
     a.qh = q_head_stride;
     a.batch = {block_table, seq_lens, cu_q, table_stride, (int)seqs, (int)tokens};
     a.group = (int)(q_heads / a.cache.heads);
-    a.window = window > 0x7fffffff ? 0 : (int)window;
+    a.window = wush::window_of(window);
     const wush::Plan p = wush::plan_of(a.cache, seqs, tokens, cu_q != nullptr, a.group, table_stride, a.window, max_len);
     WUSH_REQUIRE(p.items <= 0x7fffffffLL);
     a.tile_rows = p.tile_rows;
