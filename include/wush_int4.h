@@ -263,6 +263,18 @@ size_t wush_gemm_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int wush_gemm_w8a8(const int8_t *xq, const float *xs, const int8_t *wq, const float *ws, void *y, int dtype,
                    int64_t M, int64_t N, int64_t K, void *workspace, size_t workspace_bytes, hipStream_t stream);
 
+/* Kernels of wush_gemm_w8a8, as its plan query names them. */
+enum wush_w8a8_kernel {
+    WUSH_W8A8_DOT = 0,              /* dot products of whole weight rows (M <= 4) */
+    WUSH_W8A8_TILES = 1,            /* int8 MFMA tiles through LDS (K % 64 == 0) */
+    WUSH_W8A8_STREAM = 2            /* int8 MFMA on weights straight from memory */
+};
+
+/* The plan wush_gemm_w8a8 runs with `workspace_bytes` of 16-byte aligned workspace:
+ * plan = {kernel, output rows of a workgroup, columns, K slices}.  Host only, no device is
+ * touched; for tests and tuning. */
+int wush_gemm_w8a8_plan(int64_t M, int64_t N, int64_t K, size_t workspace_bytes, int32_t plan[4]);
+
 /* Both in one call: y = W8A8 product of x (M, K), bf16 or fp16 as y, rows
  * row_stride elements apart, with the same bits as wush_quant_int8_token followed by
  * wush_gemm_w8a8.  The workspace (16-byte aligned, of at least
@@ -338,6 +350,13 @@ int wush_kv8_attention(const void *q, int dtype, int64_t q_token_stride, int64_t
                        const int32_t *seq_lens, const int32_t *cu_q, int64_t seqs, int64_t tokens, int64_t q_heads,
                        float scale, int64_t window, float softcap, int64_t max_len, void *out, void *workspace,
                        size_t workspace_bytes, hipStream_t stream);
+
+/* The plan wush_kv8_attention runs for the same arguments: plan = {query rows of a
+ * workgroup (16, 128 or 256), stretches of the cache, tokens of a stretch, sequences of a
+ * round if single tokens' sequences are taken by length, else 0}.  Host only, no device is touched;
+ * for tests and tuning. */
+int wush_kv8_attention_plan(const wush_kv8_cache *cache, int64_t seqs, int64_t tokens, int ragged, int64_t q_heads,
+                            int64_t table_stride, int64_t window, int64_t max_len, int32_t plan[4]);
 
 /* Pages as values: k, v (n, heads, page_size, head_dim) bf16 or fp16, code *
  * scale rounded once, of the n pages listed (device int32).  A page number out

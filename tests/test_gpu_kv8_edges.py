@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import _int8 as plain
-from test_gpu_kv8 import BF, HF, Batch, check_attention, i32, starts
+from test_gpu_kv8 import BF, Batch, check_attention, i32
 
 pytestmark = pytest.mark.gpu
 

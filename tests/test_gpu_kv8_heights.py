@@ -1,0 +1,197 @@
+"""Attention over the 8-bit cache in each form that the plan has for many query
+rows, tiles of 128 and 256 rows, alone and with stretches joined.  Every test asserts the
+plan that its shapes run, so that another plan cannot take it off its subject."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import _int8 as plain
+from test_gpu_kv8 import BF, HF, Batch, check_attention, i32
+
+pytestmark = pytest.mark.gpu
+
+# rows of a tile, joined, and query heads, key/value heads, head_dim, page, lengths, new
+# tokens; the last: a window narrow enough to hide tokens with which the plan is of the same kind
+SHAPES = {
+    "128-64": (128, False, 64, 4, 64, 16, [300, 64, 1, 65, 129, 40], [300, 64, 1, 65, 70, 0], 40),
+    "128-128": (128, False, 28, 4, 128, 32, [300, 64, 1, 65, 129, 40], [300, 64, 1, 65, 70, 0], None),
+    "128-64-joined": (128, True, 8, 2, 64, 64, [4100, 3500, 1, 4050], [400, 380, 1, 350], 2900),
+    "128-128-joined": (128, True, 16, 2, 128, 16, [3100, 2500, 1, 3050, 65, 2900], [130, 80, 1, 100, 64, 160], 2000),
+    "256-64": (256, False, 32, 2, 64, 32, [1420, 1300, 1, 700, 65, 1333], [1420, 1300, 1, 630, 64, 200], 1300),
+    "256-128": (256, False, 64, 1, 128, 128, [420, 300, 1, 700, 65, 333], [420, 300, 1, 630, 64, 200], 600),
+    "256-64-joined": (256, True, 16, 2, 64, 64, [3130, 3100, 3120, 3060, 65, 3090], [130, 100, 120, 90, 64, 90], None),
+    "256-128-joined": (256, True, 16, 2, 128, 16, [3130, 3100, 3120, 3060, 65, 3090], [130, 100, 120, 90, 64, 90], 2500),
+}
+
+
+def batch(shape, dtype, seed=50, **kw):
+    _, _, Hq, Hkv, D, page, lens, n, _ = SHAPES[shape]
+    return Batch(seed, lens, n, Hq, Hkv, D, page, dtype, **kw)
+
+
+def assert_plan(bt, shape, window=0):
+    from wush_int4_kernel_amd import capi
+    rows, stretches, _, _ = capi.kv8_attention_plan(bt.cache.k.shape[0], bt.Hkv, bt.page, bt.D, len(bt.lens), sum(bt.n), True,
+                                                    bt.Hq, bt.table.shape[1], window, 0)
+    assert (rows, stretches > 1) == SHAPES[shape][:2]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_rows(dev, shape, dtype):
+    bt = batch(shape, dtype)
+    assert_plan(bt, shape)
+    out = check_attention(dev, bt)
+    assert torch.equal(out, check_attention(dev, bt, filled=False))
+
+
+@pytest.mark.parametrize("shape", [s for s in SHAPES if SHAPES[s][-1]])
+def test_window(dev, shape):
+    bt, window = batch(shape, HF, 51), SHAPES[shape][-1]
+    assert_plan(bt, shape, window)
+    check_attention(dev, bt, window=window)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_softcap(dev, shape, dtype):
+    # scores on both sides of the cap, with a window where the plan stays
+    bt, window = batch(shape, dtype, 52, size=4.0), (SHAPES[shape][-1] or 0) if dtype == BF else 0
+    assert_plan(bt, shape, window)
+    check_attention(dev, bt, cap=5.0 if dtype == BF else 30.0, window=window)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_negative_scale(dev, shape):
+    bt = batch(shape, HF, 53)
+    assert_plan(bt, shape)
+    check_attention(dev, bt, scale=-0.2)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_missing_pages_are_not_seen(dev, shape):
+    # the first page, pages in the middle, and the last of sequences; one sequence without any
+    bt = batch(shape, BF, 54)
+    assert_plan(bt, shape)
+    bt.fill(bt.lens)
+    last = bt.cache.k.shape[0]
+    for b, p in ((0, 0), (0, 2), (1, len(bt.pages[1]) - 1), (3, len(bt.pages[3]) // 2)):
+        bt.pages[b][p] = bt.table[b, p] = (-1, 2 ** 30, last)[p % 3]
+    b = len(bt.pages) - 1
+    bt.pages[b] = [-1] * len(bt.pages[b])
+    bt.table[b] = -1
+    out = check_attention(dev, bt, filled=False)
+    at = sum(bt.n[:-1])
+    assert torch.equal(out[at:], torch.zeros_like(out[at:]))
+
+
+def small_weights(bt, b, q):
+    """What one sequence's outputs may lose with the bits of small weights, (n, Hq, D): a
+    weight is p * v_scale, at least 2^12 for a row's largest, rounded to fp16, below
+    2^-14 to multiples of 2^-24: off by 2^-25, times its code."""
+    pages = [p for p in bt.pages[b] if 0 <= p < bt.cache.k.shape[0]]
+    assert len(pages) * bt.page >= bt.lens[b]
+    k, v, _ = bt.cache.sequence(bt.pages[b], bt.lens[b])
+    vs = bt.cache.vs[pages].double().repeat_interleave(bt.page, 0)[:bt.lens[b]]           # (L, Hkv)
+    codes = (v / vs[..., None]).abs().sum(0)                                              # (Hkv, D)
+    pos = bt.lens[b] - bt.n[b] + torch.arange(bt.n[b])[:, None]
+    out = torch.empty(bt.n[b], bt.Hq, bt.D, dtype=torch.float64)
+    for hq in range(bt.Hq):
+        h = hq // (bt.Hq // bt.Hkv)
+        s = (q[:, hq].double() @ k[:, h].t()) * bt.D ** -0.5
+        p = s.masked_fill(torch.arange(bt.lens[b]) > pos, -math.inf).softmax(-1)
+        out[:, hq] = (p * vs[:, h]).amax(-1, keepdim=True) * codes[h] * 2.0 ** (-25 - 12)
+    return out
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_scales_of_every_size(dev, shape):
+    # pages of zeros, of tiny and of large values side by side, scores in the hundreds
+    from my_int4 import _C
+    bt = batch(shape, BF, 55)
+    assert_plan(bt, shape)
+    bt.fill(bt.lens)
+    for pages in bt.pages:
+        for i, p in enumerate(pages):
+            f = (1.0, 0.0, 2.0 ** -20, 2.0 ** 20, 2.0 ** -39)[i % 5]
+            if f:
+                bt.cache.vs[p] *= f
+            else:
+                bt.cache.v[p] = 0
+                bt.cache.vs[p] = plain.FLOOR
+            bt.cache.ks[p] *= (1.0, 40.0, 0.01)[i % 3]
+    table, lens, cu = bt.meta(dev)
+    out = _C.kv8_attention(bt.q.to(dev), *bt.cache.to(dev), table, lens, cu_q=cu).cpu().double()
+    at = 0
+    for b, n in enumerate(bt.n):
+        q = bt.q[at:at + n]
+        ref, A, E = plain.attention(q, *bt.cache.sequence(bt.pages[b], bt.lens[b]), bt.lens[b] - n, bt.D ** -0.5)
+        bound = plain.attention_bound(ref, A, E, BF) + small_weights(bt, b, q)
+        assert bool(((out[at:at + n] - ref).abs() <= bound).all()), b
+        at += n
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_non_finite_values(dev, shape):
+    # queries, and a page's scales, that are not finite: NaN for the rows that see them only
+    from my_int4 import _C
+    bt = batch(shape, BF, 56)
+    assert_plan(bt, shape)
+    bt.fill(bt.lens)
+    bt.q[7, 1, 3] = math.nan
+    bt.q[bt.n[0] + 20, 2, 9] = -math.inf
+    b = 1                                             # the page of the sequence's 20th-last token on
+    first = bt.lens[b] - 20
+    page = bt.pages[b][first // bt.page]
+    bt.cache.vs[page, 0] = math.nan
+    bt.cache.ks[page, -1] = math.nan
+    table, lens, cu = bt.meta(dev)
+    out = _C.kv8_attention(bt.q.to(dev), *bt.cache.to(dev), table, lens, cu_q=cu).float().cpu()
+    expect = torch.zeros(sum(bt.n), bt.Hq, dtype=torch.bool)
+    expect[7, 1] = expect[bt.n[0] + 20, 2] = True
+    at = sum(bt.n[:b])
+    pos = torch.arange(bt.n[b]) + bt.lens[b] - bt.n[b]
+    sees = pos >= first // bt.page * bt.page
+    G = bt.Hq // bt.Hkv
+    expect[at:at + bt.n[b], :G] |= sees[:, None]
+    expect[at:at + bt.n[b], -G:] |= sees[:, None]
+    assert torch.equal(torch.isnan(out).all(-1), expect) and torch.equal(torch.isnan(out).any(-1), expect)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_rows_that_see_nothing(dev, shape):
+    # tokens before position 0, a length of 0, tokens behind the table
+    bt = batch(shape, HF, 57)
+    assert_plan(bt, shape)
+    bt.fill(bt.lens)
+    bt.lens = [bt.n[0] // 2, 0] + bt.lens[2:]
+    bt.lens[3] += 2 * bt.page
+    out = check_attention(dev, bt, filled=False)
+    none = bt.n[0] - bt.lens[0]
+    assert torch.equal(out[:none], torch.zeros_like(out[:none])) and out[none].abs().sum() > 0
+    assert not out[bt.n[0]:bt.n[0] + bt.n[1]].any()
+
+
+def test_offsets_past_32_bits(dev):
+    # tiles of 128 and 256 rows over the last pages of a cache of more than 2^31 codes a tensor
+    from my_int4 import _C
+    from wush_int4_kernel_amd import capi
+    Hkv, D, page = 8, 128, 128
+    pages = (2 ** 31 // (Hkv * D * page)) + 300
+    k = torch.zeros(pages, Hkv, page, D, dtype=torch.int8, device=dev)
+    v = torch.zeros(pages, Hkv, D, page, dtype=torch.int8, device=dev)
+    ks, vs = (torch.full((pages, Hkv), math.nan, device=dev) for _ in range(2))
+    for rows, Hq, room in ((128, 64, 0), (256, 32, 29)):
+        bt = Batch(rows, [300], [300], Hq, Hkv, D, page, BF, spare=0)
+        bt.fill([300])
+        at = [pages - 1, 1, pages - 2]
+        for t, c in zip((k, v, ks, vs), bt.cache.tensors()):
+            t[at] = c[bt.pages[0]].to(dev)
+        assert capi.kv8_attention_plan(pages, Hkv, page, D, 1, 300, True, Hq, 3 + room)[0] == rows
+        table = i32([at + [-1] * room], dev)
+        out = _C.kv8_attention(bt.q.to(dev), k, v, ks, vs, table, i32([300], dev), cu_q=i32([0, 300], dev)).cpu().double()
+        ref, A, E = plain.attention(bt.q, *bt.cache.sequence(bt.pages[0], 300), 0, D ** -0.5)
+        assert bool(((out - ref).abs() <= plain.attention_bound(ref, A, E, BF)).all())

@@ -125,3 +125,33 @@ def test_window_wider_than_every_sequence_is_planned_as_none(capi):
     need = [lib.wush_kv8_attention_workspace_bytes(ctypes.byref(cache(capi, heads=8, head_dim=128)), 1, 1, 0, 64, 8192, w, 0)
             for w in (0, 2 ** 30 - 1, 2 ** 30, 2 ** 31 - 1, 2 ** 31, 2 ** 62)]
     assert need[0] > 0 and need == need[:1] * 6
+
+
+def test_plan_queries(capi):
+    lib = capi.load()
+    plan = (ctypes.c_int32 * 4)()
+    for args in [(0, 8, 64), (1, 0, 64), (1, 8, 40), (1, 8, 131072), (1, 8, 0)]:
+        assert lib.wush_gemm_w8a8_plan(*args, 0, plan) == INVALID, args
+    assert lib.wush_gemm_w8a8_plan(1, 8, 64, 0, None) == INVALID
+    assert capi.gemm_w8a8_plan(4, 4096, 4096)[0] == capi.W8A8_DOT
+    assert capi.gemm_w8a8_plan(5, 4096, 4112) == (capi.W8A8_STREAM, 16, 32, 1)
+    kernel, _, _, slices = capi.gemm_w8a8_plan(13, 4096, 8192)
+    assert kernel == capi.W8A8_TILES and slices > 1 and capi.gemm_w8a8_plan(13, 4096, 8192, 0)[3] == 1
+    assert lib.wush_gemm_w8a8_workspace_bytes(13, 4096, 8192) == slices * 13 * 4096 * 4
+
+    def attend(c, seqs=2, tokens=2, ragged=0, heads=4, ts=4, window=0, max_len=0, out=plan):
+        return lib.wush_kv8_attention_plan(ctypes.byref(c), seqs, tokens, ragged, heads, ts, window, max_len, out)
+
+    c = cache(capi)
+    for kw in [dict(seqs=0), dict(tokens=0), dict(heads=3), dict(heads=0), dict(ts=-1), dict(window=-1), dict(max_len=-1), dict(out=None)]:
+        assert attend(c, **kw) == INVALID, kw
+    for kw in BAD_CACHES:
+        assert attend(cache(capi, **kw)) == INVALID, kw
+    assert attend(c) == 0 and list(plan) == [16, 1, 256, 0]
+    rows, stretches, tokens, _ = capi.kv8_attention_plan(100, 8, 64, 128, 1, 1, False, 64, 2048)
+    assert rows == 16 and stretches > 1 and (stretches - 1) * tokens < 2048 * 64 <= stretches * tokens
+    need = lib.wush_kv8_attention_workspace_bytes(ctypes.byref(cache(capi, heads=8, page_size=64, head_dim=128)), 1, 1, 0, 64, 2048, 0, 0)
+    assert need == 64 * stretches * (128 + 4) * 4
+    # single tokens are taken by length where their sequences are long and fill the chip
+    assert capi.kv8_attention_plan(100, 8, 64, 128, 64, 64, False, 64, 64)[3] == 32
+    assert capi.kv8_attention_plan(100, 8, 64, 128, 64, 64, False, 64, 8)[3] == 0

@@ -46,12 +46,14 @@ SIGNATURES = {
     "wush_gemm_s4_tensor_scale": ([_P, _P, _P, _I64, _I64, _I64, _F, _P, _P], _I),
     "wush_quant_int8_token": ([_P, _I, _P, _P, _I64, _I64, _I64, _P], _I),
     "wush_gemm_w8a8_workspace_bytes": ([_I64, _I64, _I64], _SZ),
+    "wush_gemm_w8a8_plan": ([_I64, _I64, _I64, _SZ, ctypes.POINTER(ctypes.c_int32)], _I),
     "wush_gemm_w8a8": ([_P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _P, _SZ, _P], _I),
     "wush_linear_w8a8_workspace_bytes": ([_I64, _I64, _I64], _SZ),
     "wush_linear_w8a8": ([_P, _I64, _P, _P, _P, _I, _I64, _I64, _I64, _P, _SZ, _P], _I),
     "wush_kv8_append": ([_P, _P, _P, _I, ctypes.POINTER(_I64), _P, _I64, _I64, _I, _KV, _P, _I64, _P, _P, _I64,
                          _I64, _I64, _P, _P], _I),
     "wush_kv8_attention_workspace_bytes": ([_KV, _I64, _I64, _I, _I64, _I64, _I64, _I64], _SZ),
+    "wush_kv8_attention_plan": ([_KV, _I64, _I64, _I, _I64, _I64, _I64, _I64, ctypes.POINTER(ctypes.c_int32)], _I),
     "wush_kv8_attention": ([_P, _I, _I64, _I64, _KV, _P, _I64, _P, _P, _I64, _I64, _I64, _F, _I64, _F, _I64, _P, _P,
                             _SZ, _P], _I),
     "wush_kv8_read": ([_KV, _P, _I64, _I, _P, _P, _P], _I),
@@ -166,3 +168,26 @@ def quant_int4_tensor_scale(x, q, n, inv_scale, inv_scale_dev, stream) -> None:
 def gemm_s4_tensor_scale(xq, wq, y, M, N, K, alpha, alpha_dev, stream) -> None:
     _check(load().wush_gemm_s4_tensor_scale(xq, wq, y, M, N, K, alpha, alpha_dev, stream),
            "wush_gemm_s4_tensor_scale")
+
+
+# kernels of gemm_w8a8_plan
+W8A8_DOT, W8A8_TILES, W8A8_STREAM = range(3)
+
+
+def gemm_w8a8_plan(M, N, K, workspace_bytes=None) -> tuple:
+    """(kernel, rows, columns, K slices) of gemm_w8a8 with that much workspace (None: what it asks for)."""
+    if workspace_bytes is None:
+        workspace_bytes = load().wush_gemm_w8a8_workspace_bytes(M, N, K)
+    plan = (ctypes.c_int32 * 4)()
+    _check(load().wush_gemm_w8a8_plan(M, N, K, workspace_bytes, plan), "wush_gemm_w8a8_plan")
+    return tuple(plan)
+
+
+def kv8_attention_plan(pages, heads, page_size, head_dim, seqs, tokens, ragged, q_heads, table_stride, window=0,
+                       max_len=0) -> tuple:
+    """(query rows of a workgroup, stretches, tokens of one, sequences of a round) of kv8_attention."""
+    cache = Kv8Cache(k=16, v=16, k_scale=16, v_scale=16, pages=pages, heads=heads, page_size=page_size, head_dim=head_dim)
+    plan = (ctypes.c_int32 * 4)()
+    _check(load().wush_kv8_attention_plan(ctypes.byref(cache), seqs, tokens, ragged, q_heads, table_stride, window,
+                                          max_len, plan), "wush_kv8_attention_plan")
+    return tuple(plan)

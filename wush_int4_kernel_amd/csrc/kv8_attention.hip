@@ -404,6 +404,7 @@ int window_of(int64_t window) { return window >= WUSH_KV8_MAX_LENGTH ? 0 : (int)
 struct Plan {
     int tile_rows, splits, chunk;
     int64_t items;
+    int round;                                    // AttnArgs::round
 };
 
 // For each tile height, 16 (kv8_rows_kernel), 128 and 256 (kv8_chunk.hip), the
@@ -426,7 +427,7 @@ Plan plan_of(const Kv8Cache& c, int64_t seqs, int64_t tokens, bool ragged, int g
         {16, 256, 2.1, 1.65, 1.0, 0.5, 2.2, 1.65}, {128, kTile, 1.5, 1.5, 0.0, 3.0, 1.7, 1.2}, {256, kTile, 1.5, 1.5, 0.0, 8.0, 2.1, 2.1}};
     const int64_t rows = tokens * group;
     const double joined = 0.02 + (double)rows * c.heads * (c.dim + kPartExtra) * 8 / 4e6;   // a stretch's sums both ways
-    Plan best = {16, 1, 1, 0};
+    Plan best = {16, 1, 1, 0, 0};
     double least = 1e30;
     for (const auto& t : kHeights) {
         const int64_t items = ragged ? rows / t.rows + seqs : seqs * ((group + t.rows - 1) / t.rows);
@@ -453,9 +454,16 @@ Plan plan_of(const Kv8Cache& c, int64_t seqs, int64_t tokens, bool ragged, int g
         if (us < least) {
             least = us;
             const int chunk = (int)((most + splits - 1) / splits * t.step);
-            best = {t.rows, (int)((range + chunk - 1) / chunk), chunk, items};
+            best = {t.rows, (int)((range + chunk - 1) / chunk), chunk, items, 0};
         }
     }
+    // Sorted by length where a stretch has more workgroups than the chip CUs, and the cache is long enough.
+    int64_t range = table_stride << c.page_log2;
+    if (max_len > 0 && max_len < range) range = max_len;
+    if (window > 0 && window < range) range = window;
+    const int64_t wide = (int64_t)c.heads * ((group + 15) / 16);                // workgroups of a sequence
+    if (best.tile_rows == 16 && !ragged && seqs <= kMostSorted && wide * seqs > 256 && range >= kLeastSorted)
+        best.round = wide < 256 ? (int)(256 / wide) : 1;
     return best;
 }
 
@@ -488,13 +496,33 @@ int launch(const AttnArgs& a, hipStream_t stream) {
 
 extern "C" {
 
+static bool kv8_plan(const wush_kv8_cache* cache, int64_t seqs, int64_t tokens, int ragged, int64_t q_heads,
+                     int64_t table_stride, int64_t window, int64_t max_len, wush::Kv8Cache* c, wush::Plan* p) {
+    if (wush::kv8_cache_of(cache, c) || seqs <= 0 || tokens <= 0 || q_heads <= 0 || q_heads % c->heads) return false;
+    *p = wush::plan_of(*c, seqs, tokens, ragged != 0, (int)(q_heads / c->heads), table_stride,
+                       wush::window_of(window < 0 ? 0 : window), max_len);
+    return true;
+}
+
 size_t wush_kv8_attention_workspace_bytes(const wush_kv8_cache* cache, int64_t seqs, int64_t tokens, int ragged,
                                           int64_t q_heads, int64_t table_stride, int64_t window, int64_t max_len) {
     wush::Kv8Cache c;
-    if (wush::kv8_cache_of(cache, &c) || seqs <= 0 || tokens <= 0 || q_heads <= 0 || q_heads % c.heads) return 0;
-    const wush::Plan p = wush::plan_of(c, seqs, tokens, ragged != 0, (int)(q_heads / c.heads), table_stride,
-                                       wush::window_of(window < 0 ? 0 : window), max_len);
+    wush::Plan p;
+    if (!kv8_plan(cache, seqs, tokens, ragged, q_heads, table_stride, window, max_len, &c, &p)) return 0;
     return p.splits > 1 ? (size_t)tokens * q_heads * p.splits * (c.dim + wush::kPartExtra) * 4 : 0;
+}
+
+int wush_kv8_attention_plan(const wush_kv8_cache* cache, int64_t seqs, int64_t tokens, int ragged, int64_t q_heads,
+                            int64_t table_stride, int64_t window, int64_t max_len, int32_t plan[4]) {
+    wush::Kv8Cache c;
+    wush::Plan p;
+    WUSH_REQUIRE(plan && table_stride >= 0 && window >= 0 && max_len >= 0);
+    WUSH_REQUIRE(kv8_plan(cache, seqs, tokens, ragged, q_heads, table_stride, window, max_len, &c, &p));
+    plan[0] = p.tile_rows;
+    plan[1] = p.splits;
+    plan[2] = p.chunk;
+    plan[3] = p.round;
+    return (int)hipSuccess;
 }
 
 int wush_kv8_attention(const void* q, int dtype, int64_t q_token_stride, int64_t q_head_stride,
@@ -529,13 +557,7 @@ int wush_kv8_attention(const void* q, int dtype, int64_t q_token_stride, int64_t
     a.splits = p.splits;
     a.chunk = p.chunk;
     a.items = (int)p.items;
-    // Sorted by length where a stretch has more workgroups than the chip CUs, and the cache is long enough.
-    int64_t range = table_stride << a.cache.page_log2;
-    if (max_len > 0 && max_len < range) range = max_len;
-    if (a.window > 0 && a.window < range) range = a.window;
-    const int64_t wide = (int64_t)a.cache.heads * ((a.group + 15) / 16);        // workgroups of a sequence
-    const bool sorted = p.tile_rows == 16 && !cu_q && seqs <= wush::kMostSorted && wide * seqs > 256 && range >= wush::kLeastSorted;
-    a.round = !sorted ? 0 : wide < 256 ? (int)(256 / wide) : 1;
+    a.round = p.round;
     a.scale = scale;
     a.cap = softcap;
     a.out = static_cast<uint16_t*>(out);

@@ -321,10 +321,11 @@ int dot_rows(int64_t M, int64_t N, int64_t K) {
 }
 
 struct Plan {
-    int rows, cols, splits;                       // rows 0: the streaming kernel
+    int kernel, rows, cols, splits;
 };
 
-// K % 64 == 0 takes tiles: those, and the split of K, with the least estimated
+// M <= kDotRows takes the dot products.
+// Else K % 64 == 0 takes tiles: those, and the split of K, with the least estimated
 // time, in microseconds.  A workgroup's stage of 128 codes takes `stage` on a full
 // chip, 0.6 of it on an empty one, and no less than HBM's latency over the stages in flight;
 // the whole takes no less than the weights' way from HBM.  A split costs a launch and its
@@ -333,7 +334,8 @@ struct Plan {
 // latency 5.4% and 50%.  Other K take the streaming kernel, which any K % 16 == 0 suits (tiles need
 // whole steps of 64 codes).
 Plan plan_of(int64_t M, int64_t N, int64_t K, size_t room) {
-    Plan best = {0, 0, 1};
+    if (M <= kDotRows) return {WUSH_W8A8_DOT, (int)M, 4 * dot_rows(M, N, K), 1};
+    Plan best = {WUSH_W8A8_STREAM, 16, 32, 1};
     if (K % 64 != 0) return best;
     static const struct { int rows, cols, depth; double stage; } kTiles[] = {
         {256, 256, 2, 1.60}, {256, 128, 3, 0.92}, {128, 128, 4, 0.58}, {64, 128, 3, 0.43},
@@ -354,7 +356,7 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, size_t room) {
             if (s > 1) us += 3.3 + (double)M * N * (8.0 * s + 2) / 4.5e6;
             if (us < least) {
                 least = us;
-                best = {t.rows, t.cols, s};
+                best = {WUSH_W8A8_TILES, t.rows, t.cols, s};
             }
         }
     }
@@ -421,9 +423,20 @@ int wush_quant_int8_token(const void* x, int dtype, int8_t* q, float* s, int64_t
 }
 
 size_t wush_gemm_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    if (M <= 0 || N <= 0 || K <= 0 || K % 16 != 0 || M <= wush::kDotRows) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || K % 16 != 0) return 0;
     const wush::Plan p = wush::plan_of(M, N, K, SIZE_MAX);
     return p.splits > 1 ? (size_t)p.splits * M * N * 4 : 0;
+}
+
+int wush_gemm_w8a8_plan(int64_t M, int64_t N, int64_t K, size_t workspace_bytes, int32_t plan[4]) {
+    WUSH_REQUIRE(plan && M > 0 && N > 0 && K > 0 && K % 16 == 0 && K <= WUSH_W8A8_MAX_K);
+    WUSH_REQUIRE(M <= kMostRows && N <= kMostRows);
+    const wush::Plan p = wush::plan_of(M, N, K, workspace_bytes);
+    plan[0] = p.kernel;
+    plan[1] = p.rows;
+    plan[2] = p.cols;
+    plan[3] = p.splits;
+    return (int)hipSuccess;
 }
 
 int wush_gemm_w8a8(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, void* y, int dtype, int64_t M,
@@ -444,7 +457,7 @@ int wush_gemm_w8a8(const int8_t* xq, const float* xs, const int8_t* wq, const fl
     }
     const bool usable = workspace && ((uintptr_t)workspace & 15u) == 0;
     const wush::Plan p = wush::plan_of(M, N, K, usable ? workspace_bytes : 0);
-    if (p.rows)
+    if (p.kernel == WUSH_W8A8_TILES)
         return wush::launch_gemm_w8a8(xq, xs, wq, ws, o, dtype, (int)M, (int)N, (int)K, p.rows, p.cols, p.splits,
                                       static_cast<int*>(workspace), stream);
     const dim3 grid((unsigned)((N + 31) / 32), (unsigned)((M + 15) / 16));
