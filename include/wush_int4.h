@@ -306,8 +306,8 @@ typedef struct wush_kv8_cache {
  * (seqs + 1) int32, where each sequence's new tokens begin among the `tokens` rows, from 0
  * up to tokens, or NULL for one new token each (tokens == seqs).  A page number out
  * of [0, pages) stands for no page: nothing is written there, and no query sees
- * its tokens; so do tokens behind the table's end.  Rows that cu_q gives to no sequence are left
- * out: their output is not written. */
+ * its tokens; so do tokens behind the table's end.  Rows that cu_q gives to no sequence (before its
+ * first entry, from its last one on) put nothing into the cache and come out as zeros. */
 
 /* Rotates q and k by position, and puts k and v into the cache, of which the
  * new tokens' pages change.  q (tokens, q_heads, head_dim), k, v (tokens, heads,

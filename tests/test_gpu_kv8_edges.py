@@ -48,3 +48,46 @@ def test_window_wider_than_every_sequence(dev, window, Hq, Hkv, lens, n):
     bt = Batch(42, lens, n, Hq, Hkv, 64, 16, BF)
     out = check_attention(dev, bt, window=window)
     assert torch.equal(out, check_attention(dev, bt, filled=False))
+
+
+# (query heads, key/value heads, new tokens of the sequences): 16-, 128- and 256-row tiles
+@pytest.mark.parametrize("rows,Hq,Hkv,D,n", [(16, 8, 2, 64, [3, 0, 20]), (128, 64, 4, 64, [150, 65, 200]), (256, 64, 1, 128, [420, 690, 500])])
+@pytest.mark.parametrize("before,behind", [(0, 1), (0, 40), (5, 0), (37, 130)])
+def test_tokens_of_no_sequence_are_zeros(dev, rows, Hq, Hkv, D, n, before, behind):
+    # a batch with room for more tokens than its sequences have, before their first and behind their last
+    from my_int4 import _C
+    from wush_int4_kernel_amd import capi
+    lens = [k + 70 for k in n]
+    bt = Batch(43, lens, n, Hq, Hkv, D, 64, BF)
+    bt.fill([70] * 3)
+    T = before + sum(n) + behind
+    assert capi.kv8_attention_plan(bt.cache.k.shape[0], Hkv, 64, D, 3, T, True, Hq, bt.table.shape[1])[0] == rows
+    table, lens, cu = bt.meta(dev)
+    gpu, cs = bt.cache.to(dev), bt.cos_sin.to(dev)
+    whole = torch.full((T, Hq + 2 * Hkv, D), float("nan"), dtype=BF)
+    whole[before:T - behind] = bt.qkv
+    outs = []
+    for t, c in ((bt.qkv, cu), (whole, cu + before)):
+        q, k, v = t.to(dev).split([Hq, Hkv, Hkv], 1)
+        dirty = [torch.full((T * Hq * D,), float("nan"), dtype=BF, device=dev) for _ in range(4)]
+        del dirty                                     # what the outputs' memory may hold
+        qr = _C.kv8_append(q, k, v, cs, *gpu, table, lens, cu_q=c)
+        outs.append((qr, _C.kv8_attention(qr, *gpu, table, lens, cu_q=c, max_len=max(bt.lens)), [t.clone() for t in gpu]))
+    for a, b in zip(outs[0][2], outs[1][2]):          # the same cache
+        assert torch.equal(torch.nan_to_num(a.float()), torch.nan_to_num(b.float()))
+    for a, b in zip(*(o[:2] for o in outs)):
+        assert torch.equal(a, b[before:T - behind])
+        assert not b[:before].any() and not b[T - behind:].any()
+
+
+def test_no_sequence_at_all(dev):
+    from my_int4 import _C
+    bt = Batch(44, [20], [20], 4, 2, 64, 16, BF)
+    gpu, cs = bt.cache.to(dev), bt.cos_sin.to(dev)
+    q, k, v = (t.to(dev) for t in (bt.q, bt.k, bt.v))
+    kept = [t.clone() for t in gpu]
+    for table, lens, cu in ((bt.table[:0], [], [0]), (bt.table, [20], [0, 0]), (bt.table, [20], [20, 20])):
+        args = table.to(dev), i32(lens, dev)
+        assert not _C.kv8_append(q, k, v, cs, *gpu, *args, cu_q=i32(cu, dev)).any()
+        assert not _C.kv8_attention(q, *gpu, *args, cu_q=i32(cu, dev)).any()
+    assert all(torch.equal(torch.nan_to_num(a), torch.nan_to_num(b)) for a, b in zip(gpu, kept))

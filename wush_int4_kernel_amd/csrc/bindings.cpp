@@ -533,7 +533,8 @@ torch::Tensor kv8_append(torch::Tensor q, torch::Tensor k, torch::Tensor v, torc
     const auto b = kv8_batch(q, block_table, seq_lens, cu_q);
     const at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q.device());
     auto out = new_tensor(q.sizes(), q.scalar_type(), q);
-    if (b.tokens == 0 || b.seqs == 0) return out;
+    if (b.tokens == 0) return out;
+    if (b.seqs == 0) return out.zero_();           // cu_q gives no token to a sequence
     const auto qv = heads_view(q), kv = heads_view(k), vv = heads_view(v);
     const int64_t strides[6] = {qv.stride(0), qv.stride(1), kv.stride(0), kv.stride(1), vv.stride(0), vv.stride(1)};
     check_status(wush_kv8_append(qv.data_ptr(), kv.data_ptr(), vv.data_ptr(), dt, strides, ptr<float>(cos_sin),
@@ -559,7 +560,8 @@ torch::Tensor kv8_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tenso
     const auto b = kv8_batch(q, block_table, seq_lens, cu_q);
     const at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q.device());
     auto out = new_tensor(q.sizes(), q.scalar_type(), q);
-    if (b.tokens == 0 || b.seqs == 0) return out;
+    if (b.tokens == 0) return out;
+    if (b.seqs == 0) return out.zero_();           // cu_q gives no token to a sequence
     const auto qv = heads_view(q);
     const size_t wsb = wush_kv8_attention_workspace_bytes(&c, b.seqs, b.tokens, b.cu != nullptr, q.size(1), b.table_stride,
                                                           window, max_len);

@@ -72,7 +72,19 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, const Kv8Seq& s, int 
     return r;
 }
 
-// Work item of a head -> sequence and first row of it
+// Zeros for the tokens that cu gives to no sequence, before its first entry and from its last one on.
+__device__ __forceinline__ void clear_rest(const AttnArgs& a) {
+    const Kv8Batch& t = a.batch;
+    if (!t.cu) return;
+    const int first = min(max(t.cu[0], 0), t.tokens), last = min(max(t.cu[t.seqs], first), t.tokens);
+    const int64_t row = (int64_t)a.cache.heads * a.group * a.cache.dim / 8, lo = first * row, hi = last * row;   // 16-byte pieces
+    const int64_t n = lo + t.tokens * row - hi, by = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += by)
+        reinterpret_cast<uint4*>(a.out)[i < lo ? i : i - lo + hi] = make_uint4(0, 0, 0, 0);
+}
+
+// Work item of a head -> sequence and first row of it, which is below 0 for items before the
+// first sequence's
 __device__ __forceinline__ int item_rows(const AttnArgs& a, int item, int& row0) {
     const Kv8Batch& t = a.batch;
     if (t.cu) {

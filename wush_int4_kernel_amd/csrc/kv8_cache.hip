@@ -145,9 +145,11 @@ __global__ __launch_bounds__(kThreads, NP > 2 ? 4 : 6) void kv8_append_kernel(co
         const uint16_t* q = a.q + tok * a.qt + h0 * a.qh;
         uint16_t* o = a.q_out + ((int64_t)tok * a.q_heads + h0) * D;
         const int n = min(a.q_each, a.q_heads - h0);
+        const bool given = tok >= s.first && tok - s.first < s.count;            // to a sequence; else zeros
 #pragma unroll 2
         for (int h = 0; h < n; ++h) {
-            const Values x = rotate(load_unit<DT>(q + h * a.qh, u), u, turn, a.interleaved);
+            Values x = {0.0f, 0.0f};
+            if (given) x = rotate(load_unit<DT>(q + h * a.qh, u), u, turn, a.interleaved);
             store8v<DT>(o + h * D + u.a, x.a);
             store8v<DT>(o + h * D + u.b, x.b);
         }

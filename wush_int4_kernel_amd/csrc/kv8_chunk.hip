@@ -56,7 +56,8 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
     int row0;
     const int b = item_rows(a, item, row0);
     const Kv8Seq s = kv8_seq(t, b);
-    if (row0 >= s.count * G) return;
+    clear_rest(a);
+    if (row0 < 0 || row0 >= s.count * G) return;
     const Span span = span_of(a, s, row0);
     const int begin = span.base + split * a.chunk;
     const int end = split == a.splits - 1 ? span.end : min(span.end, begin + a.chunk);
