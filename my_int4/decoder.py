@@ -57,18 +57,26 @@ class KV8Cache:
 
     def grow(self, table: torch.Tensor, row: int, tokens: int, held: int = 0) -> int:
         """Gives sequence ``row`` of the (host) block table the pages for
-        ``tokens`` tokens, of which it holds ``held`` pages; returns how many it holds then."""
+        ``tokens`` tokens and returns how many it holds then.  An entry without a page is
+        -1; pages that the row has already stay in their places, whatever ``held``, a
+        number of first entries that need not be looked at, says."""
         need = -(-tokens // self.page_size)
         if need > table.shape[1]:
             raise ValueError(f"{tokens} tokens need {need} pages, the table has {table.shape[1]}")
-        if need - held > len(self.free):
-            raise MemoryError(f"{need - held} pages needed, {len(self.free)} free")
-        for p in range(held, need):
-            table[row, p] = self.free.pop()
+        entries = table[row, held:need].tolist()
+        kept = [p for p in entries if p >= 0]
+        if kept and not set(kept).isdisjoint(self.free):
+            raise ValueError(f"row {row} of the table names a page that is free: an entry without a page is -1")
+        if len(entries) - len(kept) > len(self.free):
+            raise MemoryError(f"{len(entries) - len(kept)} pages needed, {len(self.free)} free")
+        for i, p in enumerate(entries, held):
+            if p < 0:
+                table[row, i] = self.free.pop()
         return max(need, held)
 
     def release(self, table: torch.Tensor, row: int, held: int) -> None:
-        self.free.extend(table[row, :held].tolist())
+        """Takes the row's first ``held`` entries back."""
+        self.free.extend(p for p in table[row, :held].tolist() if p >= 0)
         table[row, :held] = -1
 
 
