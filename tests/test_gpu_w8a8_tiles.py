@@ -99,3 +99,16 @@ def test_outputs_of_any_alignment(dev, shape, offset):
                               torch.cuda.current_stream().cuda_stream) == 0
     same(y[offset:offset + M * N].view(M, N), expect)
     assert (y[:offset] == 7).all() and (y[offset + M * N:] == 7).all()
+
+
+def test_streaming_more_rows_than_a_grid(dev):
+    # 16 * 65535 rows are one launch
+    from my_int4 import _C
+    M, N, K = 16 * 65535 + 21, 5, 48
+    assert_plan((M, N, K), "W8A8_STREAM", 16, 32, 1)
+    xq, xs, w, ws = (t.to(dev) for t in operands(M, N, K))
+    y = _C.w8a8_gemm(xq, xs, w, ws, dtype=torch.bfloat16)
+    same(y, plain.product(xq.cpu(), xs.cpu(), w.cpu(), ws.cpu(), torch.bfloat16))
+    x = xq.to(torch.bfloat16)                         # the layer too, whose rows are quantized in one launch
+    q, s = _C.quant_int8_token(x)
+    same(_C.w8a8_linear(x, w, ws), plain.product(q.cpu(), s.cpu(), w.cpu(), ws.cpu(), torch.bfloat16))

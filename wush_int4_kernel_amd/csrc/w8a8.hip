@@ -460,10 +460,16 @@ int wush_gemm_w8a8(const int8_t* xq, const float* xs, const int8_t* wq, const fl
     if (p.kernel == WUSH_W8A8_TILES)
         return wush::launch_gemm_w8a8(xq, xs, wq, ws, o, dtype, (int)M, (int)N, (int)K, p.rows, p.cols, p.splits,
                                       static_cast<int*>(workspace), stream);
-    const dim3 grid((unsigned)((N + 31) / 32), (unsigned)((M + 15) / 16));
-    WUSH_REQUIRE(grid.y <= 65535u);
-    wush::w8a8_stream_kernel<2, 4><<<grid, 256, 0, stream>>>(xq, xs, wq, ws, o, dtype, (int)M, (int)N, (int)K);
-    return (int)hipGetLastError();
+    // a grid has 65535 rows of workgroups at most
+    constexpr int64_t kRows = 16 * 65535;
+    for (int64_t m = 0; m < M; m += kRows) {
+        const int64_t rows = M - m < kRows ? M - m : kRows;
+        const dim3 grid((unsigned)((N + 31) / 32), (unsigned)((rows + 15) / 16));
+        wush::w8a8_stream_kernel<2, 4><<<grid, 256, 0, stream>>>(xq + m * K, xs + m, wq, ws, o + m * N, dtype, (int)rows, (int)N, (int)K);
+        const int st = (int)hipGetLastError();
+        if (st) return st;
+    }
+    return (int)hipSuccess;
 }
 
 size_t wush_linear_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
