@@ -112,3 +112,17 @@ def test_streaming_more_rows_than_a_grid(dev):
     x = xq.to(torch.bfloat16)                         # the layer too, whose rows are quantized in one launch
     q, s = _C.quant_int8_token(x)
     same(_C.w8a8_linear(x, w, ws), plain.product(q.cpu(), s.cpu(), w.cpu(), ws.cpu(), torch.bfloat16))
+
+
+def test_quantizing_more_rows_than_a_launch(dev):
+    # 2^21 rows are one launch, and 2^32 threads more than one can have: 2^26 rows of one wavefront
+    from my_int4 import _C
+    rows, K, piece = 2 ** 26 + 77, 16, 2 ** 21
+    x = torch.empty(rows, K, dtype=torch.bfloat16, device=dev)
+    x.copy_(torch.arange(rows, device=dev).remainder_(1009).sub_(504)[:, None])
+    x += torch.arange(K, device=dev, dtype=torch.bfloat16)
+    q, s = _C.quant_int8_token(x)
+    for at in (0, piece - 50, 7 * piece - 50, 2 ** 25 - 50, 2 ** 26 - 50, rows - 100):
+        eq, es = plain.quant_token(x[at:at + 100].cpu())
+        same(q[at:at + 100], eq)
+        same(s[at:at + 100], es)

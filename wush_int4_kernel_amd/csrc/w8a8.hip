@@ -20,6 +20,7 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 
 constexpr float kScaleFloor = 0x1p-126f;
 constexpr int kQuantThreads = 1024;
+constexpr int64_t kQuantRows = 1 << 21;           // of a launch, at most
 
 template <int DT>
 __device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
@@ -368,12 +369,17 @@ int launch_quant(const void* x, int8_t* q, float* s, int64_t rows, int64_t K, in
     const uint16_t* p = static_cast<const uint16_t*>(x);
     const int64_t units = K / 8;
     const unsigned threads = units < kQuantThreads ? (unsigned)((units + 63) / 64 * 64) : kQuantThreads;
-    const dim3 grid((unsigned)rows);
-    if (units <= threads) quant_int8_token_kernel<DT, 1><<<grid, threads, 0, stream>>>(p, q, s, (int)K, stride);
-    else if (units <= 2 * threads) quant_int8_token_kernel<DT, 2><<<grid, threads, 0, stream>>>(p, q, s, (int)K, stride);
-    else if (units <= 4 * threads) quant_int8_token_kernel<DT, 4><<<grid, threads, 0, stream>>>(p, q, s, (int)K, stride);
-    else quant_int8_token_kernel<DT, 0><<<grid, threads, 0, stream>>>(p, q, s, (int)K, stride);
-    return (int)hipGetLastError();
+    // a launch has fewer than 2^32 threads
+    for (int64_t r = 0; r < rows; r += kQuantRows, p += kQuantRows * stride, q += kQuantRows * K, s += kQuantRows) {
+        const dim3 grid((unsigned)(rows - r < kQuantRows ? rows - r : kQuantRows));
+        if (units <= threads) quant_int8_token_kernel<DT, 1><<<grid, threads, 0, stream>>>(p, q, s, (int)K, stride);
+        else if (units <= 2 * threads) quant_int8_token_kernel<DT, 2><<<grid, threads, 0, stream>>>(p, q, s, (int)K, stride);
+        else if (units <= 4 * threads) quant_int8_token_kernel<DT, 4><<<grid, threads, 0, stream>>>(p, q, s, (int)K, stride);
+        else quant_int8_token_kernel<DT, 0><<<grid, threads, 0, stream>>>(p, q, s, (int)K, stride);
+        const int st = (int)hipGetLastError();
+        if (st) return st;
+    }
+    return (int)hipSuccess;
 }
 
 template <int DT>
