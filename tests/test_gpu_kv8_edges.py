@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import _int8 as plain
-from test_gpu_kv8 import BF, Batch, check_attention, i32
+from test_gpu_kv8 import BF, HF, Batch, check_attention, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +91,32 @@ def test_no_sequence_at_all(dev):
         assert not _C.kv8_append(q, k, v, cs, *gpu, *args, cu_q=i32(cu, dev)).any()
         assert not _C.kv8_attention(q, *gpu, *args, cu_q=i32(cu, dev)).any()
     assert all(torch.equal(torch.nan_to_num(a), torch.nan_to_num(b)) for a, b in zip(gpu, kept))
+
+
+# (rows of a tile, head_dim, query heads, key/value heads, new tokens, sequences' lengths)
+@pytest.mark.parametrize("rows,D,Hq,Hkv,n", [(16, 128, 8, 2, [1, 1]), (16, 64, 16, 1, [1, 1]), (16, 128, 8, 2, [5, 9]), (128, 64, 64, 4, [300, 130])])
+@pytest.mark.parametrize("times,keys", [(20, 1.0), (100, 1.0), (300, 1.0), (1000, 0.0), (4000, 0.0)])
+def test_queries_with_an_outlier_channel(dev, rows, D, Hq, Hkv, n, times, keys):
+    """One channel of q many times the others, with keys as elsewhere or none: the other
+    channels' part of the scores stays.  q may be off by 2^-23 of its row's largest value."""
+    from my_int4 import _C
+    from wush_int4_kernel_amd import capi
+    lens = [700, 500]
+    bt = Batch(45, lens, n, Hq, Hkv, D, 64, HF)
+    bt.fill(lens)
+    bt.cache.k[..., 5] = (bt.cache.k[..., 5] * keys).to(torch.int8)
+    bt.q = bt.q.clone()
+    bt.q[..., 5] = times * torch.sign(bt.q[..., 5])
+    ragged = n != [1, 1]
+    assert capi.kv8_attention_plan(bt.cache.k.shape[0], Hkv, 64, D, 2, sum(n), ragged, Hq, bt.table.shape[1])[0] == rows
+    table, lens, cu = bt.meta(dev, ragged)
+    out = _C.kv8_attention(bt.q.to(dev), *bt.cache.to(dev), table, lens, cu_q=cu).cpu().double()
+    at = 0
+    for b, m in enumerate(n):
+        q = bt.q[at:at + m]
+        k, v, seen = bt.cache.sequence(bt.pages[b], bt.lens[b])
+        ref, A, E = plain.attention(q, k, v, seen, bt.lens[b] - m, D ** -0.5)
+        most = k.abs().sum(-1).amax(0).repeat_interleave(Hq // Hkv)                        # (Hq,): of a token's keys, summed
+        E = E + (2.0 ** -23 * q.double().abs().amax(-1) * most * D ** -0.5)[..., None]
+        assert bool(((out[at:at + m] - ref).abs() <= plain.attention_bound(ref, A, E, HF)).all()), b
+        at += m

@@ -34,7 +34,7 @@ constexpr int kTile = 64;                         // tokens taken at a time
 constexpr float kLow = -3e38f;                    // running maximum before any token: below every score
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kValueFloor = 0x1p-40f;           // smallest scale of a page
-constexpr float kMostScale = 0x1p97f;             // times 2^15 * 127 * 128: scores stay finite
+constexpr float kMostScale = 0x1p89f;             // times 2^23 * 127 * 128: scores stay finite
 
 // 8 int8 codes -> fp16, exact: code ^ 0x80 = code + 128 in the low byte of 1024.0
 __device__ __forceinline__ h8 codes8(uint32_t a, uint32_t b) {

@@ -11,10 +11,11 @@
 // one row meet in a second kernel.
 //
 // The cache is the row operand of both products.  Scores are exact integers: keys enter
-// v_mfma_i32_16x16x64_i8 as the codes that they are, against q in 16-bit fixed
-// point, two bytes (a power of two puts the row's largest value between 2^14 and 32639;
-// values above 2^-7 of it in bf16 and 2^-4 in fp16 are exact, smaller ones are off by
-// at most 2^-15 of the largest).  Converting the keys to fp16 took 160 of about 490 vector
+// v_mfma_i32_16x16x64_i8 as the codes that they are, against q in 24-bit fixed
+// point, three bytes (a power of two puts the row's largest value between 2^22 and 8355711;
+// values above 2^-15 of it in bf16 and 2^-12 in fp16 are exact, smaller ones are off by
+// at most 2^-23 of the largest: what fp32 sums round to).  Two bytes were off by 2^-15 of
+// the largest, and a channel 300 times the others cost these 0.3%.  Converting the keys to fp16 took 160 of about 490 vector
 // instructions a tile of 64 tokens, which bind a wavefront as much as the loads do.  The score tile comes out
 // with a lane holding 16 consecutive tokens of one row (keys are loaded in the order that
 // makes it so), which is the operand that the second product, v_mfma_f32_16x16x32_f16
@@ -112,7 +113,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
     const int low = a.window > 0 ? pos - a.window + 1 : 0;
     const int last_low = s.len - s.count + min((row0 + 15) / G, s.count - 1) - a.window;   // tokens behind it are in every row's window
 
-    v4i qh[NJ], ql[NJ];                           // q = 256 qh + ql, in units of its row
+    v4i qh[NJ], qm[NJ], ql[NJ];                   // q = 65536 qh + 256 qm + ql, in units of its row
     float c;                                      // scores in powers of two, per unit of key scale
     {
         const uint16_t* p = a.q + tok * a.qt + hq * a.qh + 16 * kq;
@@ -128,21 +129,23 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
             }
         }
         mx = quarters_max(mx);
-        int ex = mx > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(mx) : 0;
-        if (__builtin_amdgcn_ldexpf(mx, ex) > 32639.0f) --ex;     // 256 * 127 + 127
-        const float up = __builtin_amdgcn_ldexpf(1.0f, ex > 100 ? 100 : ex);
-        c = a.scale * (CAP ? 2.0f * kLog2e / a.cap : kLog2e) / up;
+        int ex = mx > 0.0f ? 23 - __builtin_amdgcn_frexp_expf(mx) : 0;
+        if (__builtin_amdgcn_ldexpf(mx, ex) > 8355711.0f) --ex;   // 127 in each byte
+        c = __builtin_amdgcn_ldexpf(a.scale * (CAP ? 2.0f * kLog2e / a.cap : kLog2e), -ex);
         if (quarters_max(bad ? 1.0f : 0.0f) > 0.0f) c = __builtin_nanf("");
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+            uint32_t hi[4] = {0, 0, 0, 0}, mid[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const int n = bad ? 0 : (int)__builtin_rintf(x[2 * j + (e >> 3)][e & 7] * up), u = (n + 128) >> 8;
-                hi[e >> 2] |= ((uint32_t)u & 0xffu) << (8 * (e & 3));
+                const int n = bad ? 0 : (int)__builtin_rintf(__builtin_amdgcn_ldexpf(x[2 * j + (e >> 3)][e & 7], ex));
+                const int u = (n + 128) >> 8, w = (u + 128) >> 8;                // digits of -128 to 127
+                hi[e >> 2] |= ((uint32_t)w & 0xffu) << (8 * (e & 3));
+                mid[e >> 2] |= ((uint32_t)(u - 256 * w) & 0xffu) << (8 * (e & 3));
                 lo[e >> 2] |= ((uint32_t)(n - 256 * u) & 0xffu) << (8 * (e & 3));
             }
             qh[j] = (v4i){(int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+            qm[j] = (v4i){(int)mid[0], (int)mid[1], (int)mid[2], (int)mid[3]};
             ql[j] = (v4i){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3]};
         }
     }
@@ -187,14 +190,15 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
     // values behind the last tile's products: the registers that held those take
     // them.  Behind the end nothing goes out.
     auto tile = [&](int t0, int idv, bool masked, auto&& keys_ahead, auto&& values_ahead) {
-        v4i sh[4], sl[4];
+        v4i sh[4], sm[4], sl[4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) sh[n] = sl[n] = (v4i){0, 0, 0, 0};
+        for (int n = 0; n < 4; ++n) sh[n] = sm[n] = sl[n] = (v4i){0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
                 sh[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[n][j], qh[j], sh[n], 0, 0, 0);
+                sm[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[n][j], qm[j], sm[n], 0, 0, 0);
                 sl[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[n][j], ql[j], sl[n], 0, 0, 0);
             }
         // the lane's 16 tokens, of one page
@@ -212,7 +216,8 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
         for (int n = 0; n < 4; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                sc[n][e] = capped<CAP>(a, (float)(256 * sh[n][e] + sl[n][e]) * cs) + lv;
+                const float x = __builtin_fmaf((float)(256 * sh[n][e] + sm[n][e]), 256.0f, (float)sl[n][e]);
+                sc[n][e] = capped<CAP>(a, x * cs) + lv;
             }
         if (masked) {
             asm volatile("" : "+v"(top));         // a branch: not computed for every tile
