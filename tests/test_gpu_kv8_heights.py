@@ -27,8 +27,15 @@ SHAPES = {
 }
 
 
+# the same for few rows, which have tests of their own
+FEW = {
+    "16": (16, False, 8, 2, 64, 16, [40, 9], [40, 9], None),
+    "16-joined": (16, True, 8, 2, 128, 64, [3000, 700, 64], [5, 1, 9], None),
+}
+
+
 def batch(shape, dtype, seed=50, **kw):
-    _, _, Hq, Hkv, D, page, lens, n, _ = SHAPES[shape]
+    _, _, Hq, Hkv, D, page, lens, n, _ = {**SHAPES, **FEW}[shape]
     return Batch(seed, lens, n, Hq, Hkv, D, page, dtype, **kw)
 
 
@@ -36,7 +43,7 @@ def assert_plan(bt, shape, window=0):
     from wush_int4_kernel_amd import capi
     rows, stretches, _, _ = capi.kv8_attention_plan(bt.cache.k.shape[0], bt.Hkv, bt.page, bt.D, len(bt.lens), sum(bt.n), True,
                                                     bt.Hq, bt.table.shape[1], window, 0)
-    assert (rows, stretches > 1) == SHAPES[shape][:2]
+    assert (rows, stretches > 1) == {**SHAPES, **FEW}[shape][:2]
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
@@ -195,3 +202,13 @@ def test_offsets_past_32_bits(dev):
         out = _C.kv8_attention(bt.q.to(dev), k, v, ks, vs, table, i32([300], dev), cu_q=i32([0, 300], dev)).cpu().double()
         ref, A, E = plain.attention(bt.q, *bt.cache.sequence(bt.pages[0], 300), 0, D ** -0.5)
         assert bool(((out - ref).abs() <= plain.attention_bound(ref, A, E, BF)).all())
+
+
+@pytest.mark.parametrize("shape", ["16", "16-joined", "128-64", "128-128-joined", "256-128"])
+@pytest.mark.parametrize("dtype,size", [(HF, 4e4), (BF, 1e6), (BF, 1e8), (BF, 4e8), (BF, 1e9), (BF, 1e18), (BF, 1e30), (BF, 1e-30), (BF, 1e-38)])
+def test_scores_of_every_size(dev, shape, dtype, size):
+    # queries whose scores leave one token a row, or all of them alike
+    bt = batch(shape, dtype, 58)
+    assert_plan(bt, shape)
+    bt.q = (bt.q.float().clamp(-1.5, 1.5) * size).to(dtype)
+    check_attention(dev, bt)

@@ -20,7 +20,7 @@ struct AttnArgs {
     int round;                                    // sequences whose workgroups make one round of the CUs; 0: taken as they come
     float scale, cap;                             // cap 0: none
     uint16_t* out;
-    float* part;                                  // (token, head, split): D sums, maximum, sum of weights, 2 unused
+    float* part;                                  // (token, head, split): D sums, the weights' base, their sum, 2 unused
 };
 
 constexpr int kPartExtra = 4;                     // floats of a partial result behind its D sums
@@ -31,8 +31,9 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTile = 64;                         // tokens taken at a time
-constexpr float kLow = -3e38f;                    // running maximum before any token: below every score
+constexpr float kLow = -3e38f;                    // the weights' base before any token: below every score
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kMostWeight = 15.0f;              // weights reach 2^15: fp16 ends at 65504
 constexpr float kValueFloor = 0x1p-40f;           // smallest scale of a page
 constexpr float kMostScale = 0x1p89f;             // times 2^23 * 127 * 128: scores stay finite
 
@@ -46,6 +47,14 @@ __device__ __forceinline__ h8 codes8(uint32_t a, uint32_t b) {
     const h2 r2 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) - bias;
     const h2 r3 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) - bias;
     return (h8){r0[0], r0[1], r1[0], r1[1], r2[0], r2[1], r3[0], r3[1]};
+}
+
+// Base of weights exp2(score - base) whose largest score is top: 2^12 below it, so that weights are
+// normal in fp16 down to 2^-26 of the largest.  Far from zero (from 2^26 on) the difference is rounded, to 16 or to
+// none: then the largest weight is 1.
+__device__ __forceinline__ float base_of(float top) {
+    const float base = top - 12.0f;
+    return top - base > kMostWeight ? top : base;
 }
 
 // A score in powers of two.  With a cap, x is 2 log2(e) score / cap: cap tanh(u) =

@@ -22,10 +22,10 @@
 // on values converted exactly, needs: the probabilities never leave their lanes.
 //
 // A token's value scale is folded into its exponent: with t = log2(e) s +
-// log2(v_scale), weights are exp2(t - maximum + 12), rounded once to fp16 (11 bits, normal
+// log2(v_scale), weights are exp2(t - base), rounded once to fp16 (11 bits, normal
 // down to 2^-26 of the largest), and the sum of the probabilities takes them, unrounded,
-// times 1 / v_scale, in fp32.  The maximum follows lazily: it moves, and the sums are
-// rescaled, only when a score passes it by 2^3.
+// times 1 / v_scale, in fp32.  The base follows the running maximum lazily, 2^12 below it: it
+// moves, and the sums are rescaled, only when a weight would pass 2^15.
 //
 // Bound by HBM where the cache fills the chip (one token behind 131072, 8 heads of 128:
 // 268 MB in 57 us with 6 to join, 4.8 TB/s; 64 ragged sequences up to 4096: 344 MB in 66 us,
@@ -40,7 +40,6 @@ namespace {
 typedef int v4i __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
-constexpr float kHead = 12.0f, kSlack = 3.0f;       // weights reach 2^15
 
 __device__ __forceinline__ float quarters_max(float v) {
     v = fmaxf(v, __shfl_xor(v, 16));
@@ -154,7 +153,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
     v4f acc[NB];
 #pragma unroll
     for (int d = 0; d < NB; ++d) acc[d] = zero;
-    float m = kLow, l = 0.0f;
+    float m = kLow, l = 0.0f;                     // the weights' base, their sum
     const int64_t tile_bytes = (int64_t)D << lg;
     const int32_t* table = t.table + (int64_t)b * t.table_stride;
     constexpr int kStep = kWaves * kTile;
@@ -234,21 +233,20 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
 #pragma unroll
             for (int e = 0; e < 4; ++e) top = fmaxf(top, sc[n][e]);
         top = quarters_max(top);
-        if (__any(top > m + kSlack)) {
-            const float mn = fmaxf(m, top), fade = __builtin_amdgcn_exp2f(m - mn);
+        if (__any(top - m > kMostWeight)) {
+            const float mn = fmaxf(m, base_of(top)), fade = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= fade;
 #pragma unroll
             for (int d = 0; d < NB; ++d) acc[d] *= fade;
         }
-        const float less = m - kHead;
         float sum = 0.0f;
         h8 p[2];
 #pragma unroll
         for (int n = 0; n < 4; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float w = __builtin_amdgcn_exp2f(sc[n][e] - less);
+                const float w = __builtin_amdgcn_exp2f(sc[n][e] - m);
                 sum += w;
                 p[n >> 1][4 * (n & 1) + e] = (_Float16)w;
             }

@@ -14,8 +14,8 @@
 // barrier between phases: of a SIMD's two wavefronts one feeds the matrix cores while the
 // other computes.
 //
-// The running maximum follows lazily: it moves, and the sums are rescaled, only
-// when a score passes it by 2^3; weights are exp2(t - maximum + 12), at most 2^15,
+// The base of the weights exp2(t - base), 2^12 below the running maximum, follows it lazily: it
+// moves, and the sums are rescaled, only when a weight would pass 2^15; weights are
 // rounded once to fp16 (11 bits, normal down to 2^-26 of the largest) for the product;
 // their sum takes them unrounded (pages whose values are far smaller than others' have
 // weights below fp16's range, and count in it all the same).
@@ -32,7 +32,7 @@ namespace {
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 
-constexpr float kHead = 12.0f, kSlack = 3.0f;
+constexpr float kFar = 0x1p12f;                   // a base up to it is off by 2^-12 at most
 // a row's factor times a key scale, both kept in these ranges, stays finite and
 // normal, and so does a score: 2^37 * 2^60 * 2^15 * 127 * 128 < 2^128
 constexpr float kLeastKeyScale = 0x1p-60f, kMostKeyScale = 0x1p60f, kLeastRow = 0x1p-66f, kMostRow = 0x1p37f;
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
     for (int d = 0; d < NB; ++d) o[d] = 0.0f;
 #pragma unroll
     for (int g = 0; g < 4; ++g) p[g] = (_Float16)0.0f;
-    float m = kLow, l = 0.0f;
+    float m = kLow, l = 0.0f;                     // the weights' base, their sum
     // The matrix phase: the second product of a tile and (QK) the first of the next,
     // their operands read kAhead fragments ahead of the MFMAs, and the staging: keys
     // into the buffer that kbuf is not, values into the one that kbuf is.
@@ -289,16 +289,27 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
         }
         const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
         top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
-        if (__any(top > m + kSlack)) {
-            const float mn = fmaxf(m, top), fade = __builtin_amdgcn_exp2f(m - mn);
+        if (__any(top - m > kMostWeight)) {
+            const float mn = fmaxf(m, base_of(top)), fade = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= fade;
 #pragma unroll
             for (int d = 0; d < NB; ++d) o[d] *= fade;
         }
+        // Far from zero the rounding of the base may exceed the weights' head-room: scores are
+        // rounded as the maximum was, so that none passes it (with a cap they have been).
+        if (!CAP && __any(fabsf(m) > kFar)) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sc[g >> 1][8 * (g & 1) + e] = __builtin_fmaf(sc[g >> 1][8 * (g & 1) + e], cg[g], lv[g]);
+                cg[g] = 1.0f;
+                lv[g] = 0.0f;
+            }
+        }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const float base = lv[g] - (m - kHead);
+            const float base = lv[g] - m;
             float sum;
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
