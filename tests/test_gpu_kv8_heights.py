@@ -212,3 +212,20 @@ def test_scores_of_every_size(dev, shape, dtype, size):
     assert_plan(bt, shape)
     bt.q = (bt.q.float().clamp(-1.5, 1.5) * size).to(dtype)
     check_attention(dev, bt)
+
+
+@pytest.mark.parametrize("shape", ["16", "16-joined", "128-64", "128-128-joined", "256-128"])
+@pytest.mark.parametrize("power", [-100, -64, 64, 100])
+def test_key_scales_of_every_size(dev, shape, power):
+    # queries and key scales far from one on opposite sides: the same scores, and the same choice
+    # between pages, at every tile height; and a page of keys that are all zero
+    bt = batch(shape, BF, 59)
+    assert_plan(bt, shape)
+    bt.fill(bt.lens)
+    bt.q = (bt.q.float() * 2.0 ** power).to(BF)
+    for pages in bt.pages:
+        for i, p in enumerate(pages):
+            bt.cache.ks[p] *= 2.0 ** -power * (1.0, 4.0, 0.25)[i % 3]
+        if len(pages) > 4:
+            bt.cache.ks[pages[3]] = 0
+    check_attention(dev, bt, filled=False)

@@ -35,7 +35,6 @@ constexpr float kLow = -3e38f;                    // the weights' base before an
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kMostWeight = 15.0f;              // weights reach 2^15: fp16 ends at 65504
 constexpr float kValueFloor = 0x1p-40f;           // smallest scale of a page
-constexpr float kMostScale = 0x1p89f;             // times 2^23 * 127 * 128: scores stay finite
 
 // 8 int8 codes -> fp16, exact: code ^ 0x80 = code + 128 in the low byte of 1024.0
 __device__ __forceinline__ h8 codes8(uint32_t a, uint32_t b) {
@@ -47,6 +46,15 @@ __device__ __forceinline__ h8 codes8(uint32_t a, uint32_t b) {
     const h2 r2 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) - bias;
     const h2 r3 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) - bias;
     return (h8){r0[0], r0[1], r1[0], r1[1], r2[0], r2[1], r3[0], r3[1]};
+}
+
+// A row's factor, by which q was scaled: finite, so that a key scale of 0 gives scores of 0
+__device__ __forceinline__ float row_factor(float c) {
+    return __builtin_amdgcn_fmed3f(c, -3e38f, 3e38f);
+}
+// A row's factor times a key scale, below which scores stay finite: 2^89 * 2^23 * 127 * 128 = 2^126.  A NaN stays one.
+__device__ __forceinline__ float kept_finite(float cs) {
+    return fabsf(cs) > 0x1p89f ? __builtin_copysignf(0x1p89f, cs) : cs;
 }
 
 // Base of weights exp2(score - base) whose largest score is top: 2^12 below it, so that weights are

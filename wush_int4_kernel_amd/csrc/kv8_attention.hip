@@ -130,7 +130,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
         mx = quarters_max(mx);
         int ex = mx > 0.0f ? 23 - __builtin_amdgcn_frexp_expf(mx) : 0;
         if (__builtin_amdgcn_ldexpf(mx, ex) > 8355711.0f) --ex;   // 127 in each byte
-        c = __builtin_amdgcn_ldexpf(a.scale * (CAP ? 2.0f * kLog2e / a.cap : kLog2e), -ex);
+        c = row_factor(__builtin_amdgcn_ldexpf(a.scale * (CAP ? 2.0f * kLog2e / a.cap : kLog2e), -ex));
         if (quarters_max(bad ? 1.0f : 0.0f) > 0.0f) c = __builtin_nanf("");
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
@@ -201,8 +201,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
                 sl[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[n][j], ql[j], sl[n], 0, 0, 0);
             }
         // the lane's 16 tokens, of one page
-        float cs = c * ks;
-        if (fabsf(cs) > kMostScale) cs = __builtin_copysignf(kMostScale, cs);
+        const float cs = kept_finite(c * ks);
         const float fv = vs < kValueFloor ? kValueFloor : vs;
         const float lv = __builtin_amdgcn_logf(fv);
         __builtin_amdgcn_sched_barrier(0);

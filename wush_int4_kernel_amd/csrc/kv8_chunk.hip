@@ -33,9 +33,6 @@ namespace {
 typedef float v16f __attribute__((ext_vector_type(16)));
 
 constexpr float kFar = 0x1p12f;                   // a base up to it is off by 2^-12 at most
-// a row's factor times a key scale, both kept in these ranges, stays finite and
-// normal, and so does a score: 2^37 * 2^60 * 2^15 * 127 * 128 < 2^128
-constexpr float kLeastKeyScale = 0x1p-60f, kMostKeyScale = 0x1p60f, kLeastRow = 0x1p-66f, kMostRow = 0x1p37f;
 
 template <int DT, int D, int NW, bool CAP>
 __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a) {
@@ -73,7 +70,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
     const int hq = h * G + r % G;
 
     h8 q[NS];
-    float c;                                      // scores in powers of two, per unit of key scale; positive
+    float c;                                      // scores in powers of two, per unit of key scale; not negative
     {
         const uint16_t* p = a.q + tok * a.qt + hq * a.qh + 8 * hf;
         float mx = 0.0f;
@@ -91,16 +88,14 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         bad |= __shfl_xor((int)bad, 32) != 0;
         const int ex = mx > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(mx) : 0;
-        const float up = __builtin_amdgcn_ldexpf(1.0f, ex > 100 ? 100 : ex);
-        c = fabsf(a.scale) * (CAP ? 2.0f * kLog2e / a.cap : kLog2e) / up;
-        c = bad ? __builtin_nanf("") : __builtin_amdgcn_fmed3f(c, kLeastRow, kMostRow);
-        const float sup = a.scale < 0.0f ? -up : up;
+        c = row_factor(__builtin_amdgcn_ldexpf(fabsf(a.scale) * (CAP ? 2.0f * kLog2e / a.cap : kLog2e), -ex));
+        if (bad) c = __builtin_nanf("");
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
             float x[8];
             load8<DT>(p + 16 * j, x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) q[j][e] = bad ? (_Float16)0.0f : (_Float16)(x[e] * sup);
+            for (int e = 0; e < 8; ++e) q[j][e] = bad ? (_Float16)0.0f : (_Float16)__builtin_amdgcn_ldexpf(a.scale < 0.0f ? -x[e] : x[e], ex);
         }
     }
 
@@ -122,7 +117,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
         r.tile = has ? id * a.cache.heads + h : 0;
         const float ks = a.cache.ks[r.tile];
         float vs = a.cache.vs[r.tile];
-        r.ks = !has || ks < kLeastKeyScale ? kLeastKeyScale : ks > kMostKeyScale ? kMostKeyScale : ks;
+        r.ks = has ? ks : 0.0f;
         if (vs < kValueFloor) vs = kValueFloor;
         r.lv = has ? __builtin_amdgcn_logf(vs) : -__builtin_inff();
         r.rv = has && vs == vs ? 1.0f / vs : 0.0f;
@@ -244,7 +239,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
             const bool half = e < 64;
             const float ks = half ? page0.ks : page1.ks, ls = half ? page0.lv : page1.lv, rs = half ? page0.rv : page1.rv;
             auto of = [&](float v, int at) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), at)); };
-            cg[0] = c * of(ks, e & 63);
+            cg[0] = kept_finite(c * of(ks, e & 63));
             lv[0] = of(ls, e & 63);
             rv[0] = of(rs, e & 63);
 #pragma unroll
@@ -257,7 +252,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
 #pragma unroll
                 for (int g = 1; g < 4; ++g) {
                     const int at = (e & 63) + (16 * g >> lg);
-                    cg[g] = c * of(ks, at);
+                    cg[g] = kept_finite(c * of(ks, at));
                     lv[g] = of(ls, at);
                     rv[g] = of(rs, at);
                 }
