@@ -229,3 +229,21 @@ def test_key_scales_of_every_size(dev, shape, power):
         if len(pages) > 4:
             bt.cache.ks[pages[3]] = 0
     check_attention(dev, bt, filled=False)
+
+
+@pytest.mark.parametrize("shape", ["16", "16-joined", "128-64", "128-128-joined", "256-128"])
+def test_non_finite_queries_that_see_nothing(dev, shape):
+    # zeros where there is no page to see, as for any other query; NaN where there is one
+    from my_int4 import _C
+    bt = batch(shape, BF, 60)
+    assert_plan(bt, shape)
+    bt.fill(bt.lens)
+    bt.q[::3, :, 0] = math.nan
+    bt.q[1::3, :, -1] = math.inf
+    table, lens, cu = bt.meta(dev)
+    table[0] = -1
+    out = _C.kv8_attention(bt.q.to(dev), *bt.cache.to(dev), table, lens, cu_q=cu).float().cpu()
+    assert not out[:bt.n[0]].any()
+    bad = torch.arange(sum(bt.n)) % 3 < 2
+    seen = torch.arange(sum(bt.n)) >= bt.n[0]
+    assert torch.equal(torch.isnan(out).all(-1).all(-1), bad & seen) and torch.equal(torch.isnan(out).any(-1).any(-1), bad & seen)

@@ -71,10 +71,10 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
 
     h8 q[NS];
     float c;                                      // scores in powers of two, per unit of key scale; not negative
+    bool bad = false;                             // a value is not finite: scores of 0, and NaN for what sees a token
     {
         const uint16_t* p = a.q + tok * a.qt + hq * a.qh + 8 * hf;
         float mx = 0.0f;
-        bool bad = false;
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
             float x[8];
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
         bad |= __shfl_xor((int)bad, 32) != 0;
         const int ex = mx > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(mx) : 0;
         c = row_factor(__builtin_amdgcn_ldexpf(fabsf(a.scale) * (CAP ? 2.0f * kLog2e / a.cap : kLog2e), -ex));
-        if (bad) c = __builtin_nanf("");
+        if (bad) c = 0.0f;
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
             float x[8];
@@ -370,6 +370,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
     }
 
     l += __shfl_xor(l, 32);
+    if (bad && l != 0.0f) l = __builtin_nanf("");
     // register e of block d: channel 32 d + 8 (e / 4) + 4 hf + e % 4
     const bool mine = wrow + l32 < rows;
     if (a.splits > 1) {
