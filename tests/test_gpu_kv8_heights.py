@@ -247,3 +247,28 @@ def test_non_finite_queries_that_see_nothing(dev, shape):
     bad = torch.arange(sum(bt.n)) % 3 < 2
     seen = torch.arange(sum(bt.n)) >= bt.n[0]
     assert torch.equal(torch.isnan(out).all(-1).all(-1), bad & seen) and torch.equal(torch.isnan(out).any(-1).any(-1), bad & seen)
+
+
+@pytest.mark.parametrize("shape", ["16", "16-joined", "128-64", "128-128-joined", "256-128"])
+@pytest.mark.parametrize("cap", [256.0, 257.0, 1e3, 1e5, 1e7, 1e30, 3e38])
+@pytest.mark.parametrize("size", [1.0, 40.0])
+def test_wide_caps(dev, shape, cap, size):
+    """Caps far above the scores leave them as they are.  A capped score may be off by
+    2^-22 of a cap up to 256, else by 2^-20 of itself: twice what the bound without a cap has for the
+    rounding of scores and exponents, on scores that a cap only makes smaller."""
+    from my_int4 import _C
+    bt = batch(shape, HF, 61, size=1.0)
+    assert_plan(bt, shape)
+    bt.fill(bt.lens)
+    bt.q = (bt.q.float() * size).to(HF)
+    table, lens, cu = bt.meta(dev)
+    out = _C.kv8_attention(bt.q.to(dev), *bt.cache.to(dev), table, lens, cu_q=cu, softcap=cap).cpu().double()
+    at = 0
+    for b, n in enumerate(bt.n):
+        q = bt.q[at:at + n]
+        args = q, *bt.cache.sequence(bt.pages[b], bt.lens[b]), bt.lens[b] - n, bt.D ** -0.5
+        ref, A, _ = plain.attention(*args, cap=cap)
+        E = 2 * plain.attention(*args)[2] + (2.0 ** -22 * cap if cap <= 256 else 0.0)
+        assert bool((E < 1 / 16).all())
+        assert bool(((out[at:at + n] - ref).abs() <= plain.attention_bound(ref, A, E, HF)).all()), b
+        at += n

@@ -65,13 +65,32 @@ __device__ __forceinline__ float base_of(float top) {
     return top - base > kMostWeight ? top : base;
 }
 
-// A score in powers of two.  With a cap, x is 2 log2(e) score / cap: cap tanh(u) =
-// cap (1 - 2 / (1 + exp(2 u))), off by a few 2^-24 of the cap.
-template <bool CAP>
+// How scores are capped.  kCap's formula is off by up to 2^-22 of the cap, which up to kMostPlainCap is no more
+// than a quarter of a weight's rounding; kWideCap's by 2^-20 of the score, for 11 more
+// instructions a score (decode of 32 sequences of 4096 47.8 us, not 46.0, 2 x 4096 new tokens 653, not 403).
+enum { kNoCap, kCap, kWideCap };
+constexpr float kMostPlainCap = 256.0f;
+
+// What a score in natural units is multiplied by before capped takes it
+template <int CAP>
+__device__ __forceinline__ float score_unit(const AttnArgs& a) {
+    return CAP == kCap ? 2.0f * kLog2e / a.cap : kLog2e;
+}
+
+// A score in powers of two, cap tanh(score / cap) if there is a cap.
+template <int CAP>
 __device__ __forceinline__ float capped(const AttnArgs& a, float x) {
-    if constexpr (!CAP) return x;
-    const float top = a.cap * kLog2e;
-    return __builtin_fmaf(-2.0f * top, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x)), top);
+    if constexpr (CAP == kNoCap) return x;
+    if constexpr (CAP == kCap) {                  // cap tanh(u) = cap (1 - 2 / (1 + exp(2 u)))
+        const float top = a.cap * kLog2e;
+        return __builtin_fmaf(-2.0f * top, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x)), top);
+    }
+    // the same for |u| of 1/4 and more; below, tanh(u) = u (1 - u^2/3 + 2 u^4/15 - 17 u^6/315 + 62 u^8/2835 - ...)
+    const float top = fminf(a.cap * kLog2e, 3e38f), v = x * (2.0f / a.cap);
+    const float u = v * 0.34657359f, w = u * u;   // ln(2) / 2
+    const float far = top * __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(fabsf(v))), 1.0f);
+    const float p = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(62.0f / 2835, w, -17.0f / 315), w, 2.0f / 15), w, -1.0f / 3);
+    return fabsf(u) < 0.25f ? __builtin_fmaf(x * w, p, x) : __builtin_copysignf(far, x);
 }
 
 // Tokens that a work item's rows, beginning at row0 of their sequence, may see:

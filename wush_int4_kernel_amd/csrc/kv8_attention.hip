@@ -81,7 +81,7 @@ __device__ __forceinline__ int by_length(const AttnArgs& a, int w) {
     return __builtin_amdgcn_readfirstlane(found);
 }
 
-template <int DT, int D, bool CAP>
+template <int DT, int D, int CAP>
 __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a) {
     constexpr int NJ = D / 64, NB = D / 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_rows_kernel(const AttnArgs a)
         mx = quarters_max(mx);
         int ex = mx > 0.0f ? 23 - __builtin_amdgcn_frexp_expf(mx) : 0;
         if (__builtin_amdgcn_ldexpf(mx, ex) > 8355711.0f) --ex;   // 127 in each byte
-        c = row_factor(__builtin_amdgcn_ldexpf(a.scale * (CAP ? 2.0f * kLog2e / a.cap : kLog2e), -ex));
+        c = row_factor(__builtin_amdgcn_ldexpf(a.scale * score_unit<CAP>(a), -ex));
         if (quarters_max(bad ? 1.0f : 0.0f) > 0.0f) c = __builtin_nanf("");
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
@@ -470,6 +470,13 @@ Plan plan_of(const Kv8Cache& c, int64_t seqs, int64_t tokens, bool ragged, int g
     return best;
 }
 
+template <int DT, int D>
+void launch_rows(const AttnArgs& a, unsigned grid, hipStream_t stream) {
+    if (a.cap > kMostPlainCap) kv8_rows_kernel<DT, D, kWideCap><<<grid, 64 * kWaves, 0, stream>>>(a);
+    else if (a.cap > 0.0f) kv8_rows_kernel<DT, D, kCap><<<grid, 64 * kWaves, 0, stream>>>(a);
+    else kv8_rows_kernel<DT, D, kNoCap><<<grid, 64 * kWaves, 0, stream>>>(a);
+}
+
 template <int DT>
 int launch(const AttnArgs& a, hipStream_t stream) {
     const int64_t blocks = (int64_t)a.items * a.cache.heads * a.splits;
@@ -479,16 +486,12 @@ int launch(const AttnArgs& a, hipStream_t stream) {
         const int st = launch_kv8_chunk(a, DT, stream);
         if (st) return st;
     }
-    const dim3 grid((unsigned)blocks), join((unsigned)(a.splits <= kFewSplits ? (rows + 3) / 4 : rows));
+    const dim3 join((unsigned)(a.splits <= kFewSplits ? (rows + 3) / 4 : rows));
     if (a.cache.dim == 64) {
-        if (a.tile_rows > 16) {}
-        else if (a.cap > 0.0f) kv8_rows_kernel<DT, 64, true><<<grid, 64 * kWaves, 0, stream>>>(a);
-        else kv8_rows_kernel<DT, 64, false><<<grid, 64 * kWaves, 0, stream>>>(a);
+        if (a.tile_rows == 16) launch_rows<DT, 64>(a, (unsigned)blocks, stream);
         if (a.splits > 1) kv8_join_kernel<DT, 64><<<join, 256, 0, stream>>>(a);
     } else {
-        if (a.tile_rows > 16) {}
-        else if (a.cap > 0.0f) kv8_rows_kernel<DT, 128, true><<<grid, 64 * kWaves, 0, stream>>>(a);
-        else kv8_rows_kernel<DT, 128, false><<<grid, 64 * kWaves, 0, stream>>>(a);
+        if (a.tile_rows == 16) launch_rows<DT, 128>(a, (unsigned)blocks, stream);
         if (a.splits > 1) kv8_join_kernel<DT, 128><<<join, 256, 0, stream>>>(a);
     }
     return (int)hipGetLastError();

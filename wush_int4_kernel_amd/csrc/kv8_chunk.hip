@@ -34,7 +34,7 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 
 constexpr float kFar = 0x1p12f;                   // a base up to it is off by 2^-12 at most
 
-template <int DT, int D, int NW, bool CAP>
+template <int DT, int D, int NW, int CAP>
 __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a) {
     constexpr int kThreads = 64 * NW;
     constexpr int NS = D / 16, NB = D / 32;       // steps of the first product, channel blocks of the second
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         bad |= __shfl_xor((int)bad, 32) != 0;
         const int ex = mx > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(mx) : 0;
-        c = row_factor(__builtin_amdgcn_ldexpf(fabsf(a.scale) * (CAP ? 2.0f * kLog2e / a.cap : kLog2e), -ex));
+        c = row_factor(__builtin_amdgcn_ldexpf(fabsf(a.scale) * score_unit<CAP>(a), -ex));
         if (bad) c = 0.0f;
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
@@ -415,8 +415,9 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_chunk_kernel(const AttnArgs a)
 
 template <int DT, int D, int NW>
 void launch_one(const AttnArgs& a, unsigned grid, hipStream_t stream) {
-    if (a.cap > 0.0f) kv8_chunk_kernel<DT, D, NW, true><<<grid, 64 * NW, 0, stream>>>(a);
-    else kv8_chunk_kernel<DT, D, NW, false><<<grid, 64 * NW, 0, stream>>>(a);
+    if (a.cap > kMostPlainCap) kv8_chunk_kernel<DT, D, NW, kWideCap><<<grid, 64 * NW, 0, stream>>>(a);
+    else if (a.cap > 0.0f) kv8_chunk_kernel<DT, D, NW, kCap><<<grid, 64 * NW, 0, stream>>>(a);
+    else kv8_chunk_kernel<DT, D, NW, kNoCap><<<grid, 64 * NW, 0, stream>>>(a);
 }
 
 template <int DT>
