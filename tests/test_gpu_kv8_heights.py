@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import _int8 as plain
-from test_gpu_kv8 import BF, HF, Batch, check_attention, i32
+from test_gpu_kv8 import BF, HF, Batch, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -44,6 +44,37 @@ def assert_plan(bt, shape, window=0):
     rows, stretches, _, _ = capi.kv8_attention_plan(bt.cache.k.shape[0], bt.Hkv, bt.page, bt.D, len(bt.lens), sum(bt.n), True,
                                                     bt.Hq, bt.table.shape[1], window, 0)
     assert (rows, stretches > 1) == {**SHAPES, **FEW}[shape][:2]
+
+
+def reference(dev, bt, b, q, scale=None, window=0, cap=0.0):
+    """plain.attention of sequence b's queries, in fp64 on the GPU."""
+    k, v, seen = bt.cache.sequence(bt.pages[b], min(bt.lens[b], bt.table.shape[1] * bt.page))
+    with torch.device(dev):
+        return plain.attention(q, k.to(dev), v.to(dev), seen.to(dev), bt.lens[b] - bt.n[b],
+                               bt.D ** -0.5 if scale is None else scale, window, cap)
+
+
+def within(got, ref, bound):
+    same_nan = torch.equal(torch.isnan(got), torch.isnan(ref))
+    return same_nan and bool((torch.nan_to_num((got - ref).abs()) <= torch.nan_to_num(bound)).all())
+
+
+def run(dev, bt, scale=None, window=0, cap=0.0):
+    from my_int4 import _C
+    table, lens, cu = bt.meta(dev)
+    kw = {} if scale is None else {"scale": scale}
+    return _C.kv8_attention(bt.q.to(dev), *bt.cache.to(dev), table, lens, cu_q=cu, window=window, softcap=cap, **kw)
+
+
+def check_attention(dev, bt, scale=None, window=0, cap=0.0, filled=True):
+    if filled:
+        bt.fill(bt.lens)
+    out, q, at = run(dev, bt, scale, window, cap), bt.q.to(dev), 0
+    for b, n in enumerate(bt.n):
+        ref, A, E = reference(dev, bt, b, q[at:at + n], scale, window, cap)
+        assert within(out[at:at + n].double(), ref, plain.attention_bound(ref, A, E, bt.dtype)), b
+        at += n
+    return out.cpu()
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
@@ -95,21 +126,21 @@ def test_missing_pages_are_not_seen(dev, shape):
     assert torch.equal(out[at:], torch.zeros_like(out[at:]))
 
 
-def small_weights(bt, b, q):
+def small_weights(dev, bt, b, q):
     """What one sequence's outputs may lose with the bits of small weights, (n, Hq, D): a
     weight is p * v_scale, at least 2^12 for a row's largest, rounded to fp16, below
     2^-14 to multiples of 2^-24: off by 2^-25, times its code."""
     pages = [p for p in bt.pages[b] if 0 <= p < bt.cache.k.shape[0]]
     assert len(pages) * bt.page >= bt.lens[b]
     k, v, _ = bt.cache.sequence(bt.pages[b], bt.lens[b])
-    vs = bt.cache.vs[pages].double().repeat_interleave(bt.page, 0)[:bt.lens[b]]           # (L, Hkv)
-    codes = (v / vs[..., None]).abs().sum(0)                                              # (Hkv, D)
-    pos = bt.lens[b] - bt.n[b] + torch.arange(bt.n[b])[:, None]
-    out = torch.empty(bt.n[b], bt.Hq, bt.D, dtype=torch.float64)
+    vs = bt.cache.vs[pages].double().repeat_interleave(bt.page, 0)[:bt.lens[b]].to(dev)       # (L, Hkv)
+    k, codes = k.to(dev), (v.to(dev) / vs[..., None]).abs().sum(0)                            # codes: (Hkv, D)
+    pos = bt.lens[b] - bt.n[b] + torch.arange(bt.n[b], device=dev)[:, None]
+    out = torch.empty(bt.n[b], bt.Hq, bt.D, dtype=torch.float64, device=dev)
     for hq in range(bt.Hq):
         h = hq // (bt.Hq // bt.Hkv)
         s = (q[:, hq].double() @ k[:, h].t()) * bt.D ** -0.5
-        p = s.masked_fill(torch.arange(bt.lens[b]) > pos, -math.inf).softmax(-1)
+        p = s.masked_fill(torch.arange(bt.lens[b], device=dev) > pos, -math.inf).softmax(-1)
         out[:, hq] = (p * vs[:, h]).amax(-1, keepdim=True) * codes[h] * 2.0 ** (-25 - 12)
     return out
 
@@ -117,7 +148,6 @@ def small_weights(bt, b, q):
 @pytest.mark.parametrize("shape", SHAPES)
 def test_scales_of_every_size(dev, shape):
     # pages of zeros, of tiny and of large values side by side, scores in the hundreds
-    from my_int4 import _C
     bt = batch(shape, BF, 55)
     assert_plan(bt, shape)
     bt.fill(bt.lens)
@@ -130,14 +160,10 @@ def test_scales_of_every_size(dev, shape):
                 bt.cache.v[p] = 0
                 bt.cache.vs[p] = plain.FLOOR
             bt.cache.ks[p] *= (1.0, 40.0, 0.01)[i % 3]
-    table, lens, cu = bt.meta(dev)
-    out = _C.kv8_attention(bt.q.to(dev), *bt.cache.to(dev), table, lens, cu_q=cu).cpu().double()
-    at = 0
+    out, q, at = run(dev, bt), bt.q.to(dev), 0
     for b, n in enumerate(bt.n):
-        q = bt.q[at:at + n]
-        ref, A, E = plain.attention(q, *bt.cache.sequence(bt.pages[b], bt.lens[b]), bt.lens[b] - n, bt.D ** -0.5)
-        bound = plain.attention_bound(ref, A, E, BF) + small_weights(bt, b, q)
-        assert bool(((out[at:at + n] - ref).abs() <= bound).all()), b
+        ref, A, E = reference(dev, bt, b, q[at:at + n])
+        assert within(out[at:at + n].double(), ref, plain.attention_bound(ref, A, E, BF) + small_weights(dev, bt, b, q[at:at + n])), b
         at += n
 
 
@@ -199,9 +225,9 @@ def test_offsets_past_32_bits(dev):
             t[at] = c[bt.pages[0]].to(dev)
         assert capi.kv8_attention_plan(pages, Hkv, page, D, 1, 300, True, Hq, 3 + room)[0] == rows
         table = i32([at + [-1] * room], dev)
-        out = _C.kv8_attention(bt.q.to(dev), k, v, ks, vs, table, i32([300], dev), cu_q=i32([0, 300], dev)).cpu().double()
-        ref, A, E = plain.attention(bt.q, *bt.cache.sequence(bt.pages[0], 300), 0, D ** -0.5)
-        assert bool(((out - ref).abs() <= plain.attention_bound(ref, A, E, BF)).all())
+        out = _C.kv8_attention(bt.q.to(dev), k, v, ks, vs, table, i32([300], dev), cu_q=i32([0, 300], dev))
+        ref, A, E = reference(dev, bt, 0, bt.q.to(dev))
+        assert within(out.double(), ref, plain.attention_bound(ref, A, E, BF))
 
 
 @pytest.mark.parametrize("shape", ["16", "16-joined", "128-64", "128-128-joined", "256-128"])
@@ -256,19 +282,14 @@ def test_wide_caps(dev, shape, cap, size):
     """Caps far above the scores leave them as they are.  A capped score may be off by
     2^-22 of a cap up to 256, else by 2^-20 of itself: twice what the bound without a cap has for the
     rounding of scores and exponents, on scores that a cap only makes smaller."""
-    from my_int4 import _C
     bt = batch(shape, HF, 61, size=1.0)
     assert_plan(bt, shape)
     bt.fill(bt.lens)
     bt.q = (bt.q.float() * size).to(HF)
-    table, lens, cu = bt.meta(dev)
-    out = _C.kv8_attention(bt.q.to(dev), *bt.cache.to(dev), table, lens, cu_q=cu, softcap=cap).cpu().double()
-    at = 0
+    out, q, at = run(dev, bt, cap=cap), bt.q.to(dev), 0
     for b, n in enumerate(bt.n):
-        q = bt.q[at:at + n]
-        args = q, *bt.cache.sequence(bt.pages[b], bt.lens[b]), bt.lens[b] - n, bt.D ** -0.5
-        ref, A, _ = plain.attention(*args, cap=cap)
-        E = 2 * plain.attention(*args)[2] + (2.0 ** -22 * cap if cap <= 256 else 0.0)
+        ref, A, _ = reference(dev, bt, b, q[at:at + n], cap=cap)
+        E = 2 * reference(dev, bt, b, q[at:at + n])[2] + (2.0 ** -22 * cap if cap <= 256 else 0.0)
         assert bool((E < 1 / 16).all())
-        assert bool(((out[at:at + n] - ref).abs() <= plain.attention_bound(ref, A, E, HF)).all()), b
+        assert within(out[at:at + n].double(), ref, plain.attention_bound(ref, A, E, HF)), b
         at += n
