@@ -120,3 +120,24 @@ def test_queries_with_an_outlier_channel(dev, rows, D, Hq, Hkv, n, times, keys):
         E = E + (2.0 ** -23 * q.double().abs().amax(-1) * most * D ** -0.5)[..., None]
         assert bool(((out[at:at + m] - ref).abs() <= plain.attention_bound(ref, A, E, HF)).all()), b
         at += m
+
+
+def test_reading_more_pages_than_a_launch(dev):
+    # 2^22 (page, head)s are one launch, and 2^23 have 2^32 threads; 34 GB of output
+    from my_int4 import _C
+    H, n = 2 ** 9, 2 ** 14 + 5
+    g = torch.Generator().manual_seed(46)
+    c = plain.Cache(3, H, 16, 64)
+    c.k.copy_(torch.randint(-127, 128, c.k.shape, generator=g))
+    c.v.copy_(torch.randint(-127, 128, c.v.shape, generator=g))
+    c.ks.copy_(torch.rand(3, H, generator=g))
+    c.vs.copy_(torch.rand(3, H, generator=g))
+    ids = (torch.arange(n) * 7 % 3).to(torch.int32)
+    k, v = _C.kv8_read(*c.to(dev), ids.to(dev), BF)
+    kr = (c.k.float() * c.ks[..., None, None]).to(BF).to(dev)
+    vr = (c.v.float() * c.vs[..., None, None]).to(BF).transpose(2, 3).contiguous().to(dev)
+    for at in (0, 2 ** 13 - 2, 2 ** 14 - 2, n - 5):
+        i = ids[at:at + 5].long().to(dev)
+        assert torch.equal(k[at:at + 5], kr[i]) and torch.equal(v[at:at + 5], vr[i])
+    del k, v
+    torch.cuda.empty_cache()

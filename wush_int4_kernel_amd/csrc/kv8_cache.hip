@@ -345,6 +345,20 @@ int launch_append(const AppendArgs& a, dim3 grid, hipStream_t stream) {
     return (int)hipGetLastError();
 }
 
+// Pages of at most 2^22 (page, head)s a launch: a launch has fewer than 2^32 threads.
+template <int DT>
+int launch_read(const Kv8Cache& c, const int32_t* pages, int64_t n, uint16_t* k, uint16_t* v, hipStream_t stream) {
+    const int64_t most = (1 << 22) / c.heads, page = (int64_t)c.heads * (c.dim << c.page_log2);
+    for (int64_t at = 0; at < n; at += most, pages += most, k += most * page, v += most * page) {
+        const dim3 grid((unsigned)((n - at < most ? n - at : most) * c.heads * 2));
+        if (c.dim == 64) kv8_read_kernel<DT, 64><<<grid, kThreads, 0, stream>>>(c, pages, k, v);
+        else kv8_read_kernel<DT, 128><<<grid, kThreads, 0, stream>>>(c, pages, k, v);
+        const int st = (int)hipGetLastError();
+        if (st) return st;
+    }
+    return (int)hipSuccess;
+}
+
 }  // namespace
 
 int kv8_cache_of(const wush_kv8_cache* c, Kv8Cache* out) {
@@ -419,16 +433,9 @@ int wush_kv8_read(const wush_kv8_cache* cache, const int32_t* pages, int64_t n, 
     if (n == 0) return (int)hipSuccess;
     WUSH_REQUIRE(pages && k && v && (((uintptr_t)k | (uintptr_t)v) & 15u) == 0);
     WUSH_REQUIRE(n <= 0x3fffffffLL / c.heads);
-    const dim3 grid((unsigned)(n * c.heads * 2));
     uint16_t *ko = static_cast<uint16_t*>(k), *vo = static_cast<uint16_t*>(v);
-    if (dtype == WUSH_DTYPE_BF16) {
-        if (c.dim == 64) wush::kv8_read_kernel<WUSH_DTYPE_BF16, 64><<<grid, wush::kThreads, 0, stream>>>(c, pages, ko, vo);
-        else wush::kv8_read_kernel<WUSH_DTYPE_BF16, 128><<<grid, wush::kThreads, 0, stream>>>(c, pages, ko, vo);
-    } else {
-        if (c.dim == 64) wush::kv8_read_kernel<WUSH_DTYPE_F16, 64><<<grid, wush::kThreads, 0, stream>>>(c, pages, ko, vo);
-        else wush::kv8_read_kernel<WUSH_DTYPE_F16, 128><<<grid, wush::kThreads, 0, stream>>>(c, pages, ko, vo);
-    }
-    return (int)hipGetLastError();
+    return dtype == WUSH_DTYPE_BF16 ? wush::launch_read<WUSH_DTYPE_BF16>(c, pages, n, ko, vo, stream)
+                                    : wush::launch_read<WUSH_DTYPE_F16>(c, pages, n, ko, vo, stream);
 }
 
 }  // extern "C"
