@@ -254,7 +254,7 @@ int wush_quant_int8_token(const void *x, int dtype, int8_t *q, float *s, int64_t
 
 /* W8A8 product: y[m][n] = (sum_k xq[m][k] wq[n][k]) * xs[m] * ws[n], the sum
  * exact in int32, then two fp32 products and one rounding to `dtype` (bf16 or
- * fp16).  xq (M, K), wq (N, K) int8; xs M, ws N fp32; y (M, N).  Any M, N;
+ * fp16).  xq (M, K), wq (N, K) int8; xs M, ws N fp32; y (M, N).  Any M, N up to 2^26;
  * K % 16 == 0, K <= WUSH_W8A8_MAX_K; xq and wq 16-byte aligned.  The result's
  * bits depend on neither the workspace nor the plan.  Bytes of workspace with which
  * it runs its fastest plan (int32 partial sums of a split K) are asked of
@@ -288,7 +288,8 @@ int wush_linear_w8a8(const void *x, int64_t row_stride, const int8_t *wq, const 
  *   k        int8 (pages, heads, page_size, head_dim)
  *   v        int8 (pages, heads, head_dim, page_size): channel by channel, the
  *            order in which the attention's second product reads it
- *   k_scale, v_scale  fp32 (pages, heads): a code stands for code * scale
+ *   k_scale, v_scale  fp32 (pages, heads), not negative: a code stands for code * scale
+ *            (in attention a value scale below 2^-40, the least that append writes, counts as 2^-40)
  * k and v 16-byte aligned. */
 typedef struct wush_kv8_cache {
     int8_t *k, *v;
@@ -336,11 +337,17 @@ int wush_kv8_append(const void *q, const void *k, const void *v, int dtype, cons
  * head hq / (q_heads / heads),
  *   out = sum_t softmax_t(cap(scale * q . k_t)) v_t over t in [max(0, p - window + 1), p]
  * with window 0 for all t <= p, and cap(x) = softcap * tanh(x / softcap), softcap 0 for
- * none; scale finite, of either sign.  A query that sees no token gets zeros.  q (tokens, q_heads, head_dim)
+ * none; scale finite, of either sign.  A query that sees no token gets zeros; one with a non-finite value
+ * NaN if it sees any.  q (tokens, q_heads, head_dim)
  * bf16 or fp16 with a token and a head stride (multiples of 8, 16-byte aligned);
  * out (tokens, q_heads, head_dim) contiguous, of the same type.
+ *   Scores, sums and outputs are held in fp32.  Fewer bits than that: of q, 2^-23 of its row's
+ * largest value; of a score with softcap, 2^-22 of a softcap up to 256, above it 2^-20 of the score; and the
+ * weights p_t * v_scale of the sum over v, rounded to 11 bits (fp16), to fewer below 2^-26 of the row's
+ * largest and to none from 2^-37 on.  How the work is split, and with it the order of sums, depends on the
+ * sizes, window and max_len, not on the values.
  *   max_len: a bound of seq_lens that the host knows (0: the table's room). It only
- * decides how the work is split.  The workspace, of at least
+ * decides how the work is split (a captured call keeps the split that it was captured with).  The workspace, of at least
  * wush_kv8_attention_workspace_bytes for the same arguments (ragged: whether
  * cu_q is given), 16-byte aligned, holds partial results. */
 size_t wush_kv8_attention_workspace_bytes(const wush_kv8_cache *cache, int64_t seqs, int64_t tokens, int ragged,

@@ -28,8 +28,8 @@
 // moves, and the sums are rescaled, only when a weight would pass 2^15.
 //
 // Bound by HBM where the cache fills the chip (one token behind 131072, 8 heads of 128:
-// 268 MB in 57 us with 6 to join, 4.8 TB/s; 64 ragged sequences up to 4096: 344 MB in 66 us,
-// the CUs not quite evenly loaded), by a wavefront's instructions and latencies otherwise (3 x 300: 6 us).  Two
+// 268 MB in 57 us with 6 to join, 4.7 TB/s; 64 ragged sequences up to 4096: 344 MB in 66 us,
+// the CUs not quite evenly loaded), by a wavefront's instructions and latencies otherwise (3 x 300: 6.1 us).  Two
 // tiles' loads in flight instead of one changed nothing; without the non-temporal hint
 // 131072 tokens took 2 us more, but 8192-token stretches 20% less, so loads have none.
 #include "kv8_attention.h"
@@ -411,17 +411,20 @@ struct Plan {
 };
 
 // For each tile height, 16 (kv8_rows_kernel), 128 and 256 (kv8_chunk.hip), the
-// stretches of the cache per item with the least estimated time, in microseconds: a
+// stretches of the cache per item with the least estimated time: a
 // workgroup's pass over `step` tokens (`split` alone on its CU, `more` for each where several
 // share it: the loads of one cover the latencies of another), `ends` passes' worth for its beginning
 // and end, and where there is more than one stretch the joining.  `more` below `split`
-// halves the stretches of long caches: 8 ragged sequences up to 32768 79 us, not 91 (8 heads of
+// (16 rows only; for tall tiles `pass` below `alone` says the same, and their stretches have not been
+// chosen by it) halves the stretches of long caches: 8 ragged sequences up to 32768 79 us, not 91 (8 heads of
 // 128; of 64 48, not 61), 16 up to 8192 46, not 51, one of 131072 58 to 59 in both; over 104 shapes of decode and few new
 // tokens 2.4% faster on average, 28% at best, 5% slower at worst (5 of 12000, page of 16); without `ends`
 // 12 of 3000 took 18.0 us, not 15.1.  Of the three, the height with the least time: a
 // start, and passes that take `alone` where a CU has one workgroup and `pass` for each where it has
 // more.  Those constants are fitted to 72 shapes, 1 and 16 sequences of 1024 and 8192 with 41 to 1024 rows of
-// new tokens: 1% slower than the fastest height on average, 19% at worst; 16 rows below
+// new tokens, none with a cap: 1% slower than the fastest height on average, 19% at worst.  The estimates rank heights
+// and are no times: neither what causality leaves out nor a cap's exponentials are in them (1 x 8192 new tokens 1092,
+// measured 540; 5 x 700 with window and cap 21, measured 56).  16 rows below
 // a fixed number of rows a sequence, tall ones above, was 15% slower on average and 98% at
 // worst (16 sequences of 8192 with 32 heads of 64 and 170 new tokens: 467 us, now 267).
 Plan plan_of(const Kv8Cache& c, int64_t seqs, int64_t tokens, bool ragged, int group, int64_t table_stride, int window,

@@ -20,10 +20,10 @@
 // their sum takes them unrounded (pages whose values are far smaller than others' have
 // weights below fp16's range, and count in it all the same).
 //
-// 8192 new tokens, 32 query and 8 key/value heads of 128: 540-565 us, 1.0 PFLOP/s (a large
+// 8192 new tokens, 32 query and 8 key/value heads of 128: 540-570 us, 1.0 PFLOP/s (a large
 // fp16 matrix product reaches 1.43 on this card).  The matrix cores are busy for 47% of the
-// time and the vector units for 60%: one phase's 32 exponentials a lane and tile, and about 130 other vector
-// instructions, take as long as the other's MFMAs.  All wavefronts in step took 613 us, no higher
+// time and the vector units for 60%, neither in full: a tile has 32 MFMAs and about 260 vector instructions a wavefront (32 of
+// them exponentials, 80 between the MFMAs), and the halves wait for each other at the barriers.  All wavefronts in step took 613 us, no higher
 // priority for the matrix phase 16% more, loads in the vector phase 5%.
 #include "kv8_attention.h"
 

@@ -7,7 +7,9 @@
 //
 // A row of x with a non-finite value gets s = NaN and zero codes, so its
 // outputs are NaN.  Every step is one IEEE operation, so codes and scales are
-// the same bits in any implementation of these formulas; the integer sum does
+// the same bits wherever these are (a product with 1 / 127 in place of the division, which
+// tensor libraries make of one by a constant on the GPU, is an ulp off now and then, and codes
+// at ties with it); the integer sum does
 // not depend on its order, so the product is the same bits for every split of K.
 #include "w8a8.h"
 #include "wush_device.h"
@@ -249,7 +251,9 @@ __global__ __launch_bounds__(256) void w8a8_dot_kernel(const int8_t* __restrict_
 // (grid.x), K split over the workgroup's KW wavefronts, whose int32 partial
 // sums meet in LDS.  v_mfma_i32_16x16x64_i8 with the weights as row operand: a
 // lane loads 16 bytes of its row, straight from HBM into the operand register.
-// Any K % 16 == 0: past the end of a row the weights count as zero.
+// Any K % 16 == 0: past the end of a row the weights count as zero.  Every 16 rows
+// load all weights again: right for few rows only (5 x 8192 x 4112 10.4 us, tiles at K = 4096 12.6; 32
+// rows 17.0 and 12.6, 300 rows 102 and 21, 2000 rows 623 and 69).
 template <int CB, int KW>
 __global__ __launch_bounds__(64 * KW) void w8a8_stream_kernel(const int8_t* __restrict__ xq,
                                                               const float* __restrict__ xs,
@@ -330,7 +334,7 @@ struct Plan {
 // time, in microseconds.  A workgroup's stage of 128 codes takes `stage` on a full
 // chip, 0.6 of it on an empty one, and no less than HBM's latency over the stages in flight;
 // the whole takes no less than the weights' way from HBM.  A split costs a launch and its
-// partial sums both ways.  The constants are fitted to 60 shapes from 5 x 8192 x 28672 to 300 rows, weights
+// partial sums both ways.  The estimates are there to be compared with each other.  The constants are fitted to 60 shapes from 5 x 8192 x 28672 to 300 rows, weights
 // from HBM: 1.6% slower than the fastest of all tiles and splits on average, 15% at worst; without the
 // latency 5.4% and 50%.  Other K take the streaming kernel, which any K % 16 == 0 suits (tiles need
 // whole steps of 64 codes).
