@@ -374,12 +374,15 @@ int launch_quant(const void* x, int8_t* q, float* s, int64_t rows, int64_t K, in
     const int64_t units = K / 8;
     const unsigned threads = units < kQuantThreads ? (unsigned)((units + 63) / 64 * 64) : kQuantThreads;
     // a launch has fewer than 2^32 threads
-    for (int64_t r = 0; r < rows; r += kQuantRows, p += kQuantRows * stride, q += kQuantRows * K, s += kQuantRows) {
+    for (int64_t r = 0; r < rows; r += kQuantRows) {
+        const uint16_t* xr = r ? p + r * stride : p;              // one row's stride may be anything
+        int8_t* qr = q + r * K;
+        float* sr = s + r;
         const dim3 grid((unsigned)(rows - r < kQuantRows ? rows - r : kQuantRows));
-        if (units <= threads) quant_int8_token_kernel<DT, 1><<<grid, threads, 0, stream>>>(p, q, s, (int)K, stride);
-        else if (units <= 2 * threads) quant_int8_token_kernel<DT, 2><<<grid, threads, 0, stream>>>(p, q, s, (int)K, stride);
-        else if (units <= 4 * threads) quant_int8_token_kernel<DT, 4><<<grid, threads, 0, stream>>>(p, q, s, (int)K, stride);
-        else quant_int8_token_kernel<DT, 0><<<grid, threads, 0, stream>>>(p, q, s, (int)K, stride);
+        if (units <= threads) quant_int8_token_kernel<DT, 1><<<grid, threads, 0, stream>>>(xr, qr, sr, (int)K, stride);
+        else if (units <= 2 * threads) quant_int8_token_kernel<DT, 2><<<grid, threads, 0, stream>>>(xr, qr, sr, (int)K, stride);
+        else if (units <= 4 * threads) quant_int8_token_kernel<DT, 4><<<grid, threads, 0, stream>>>(xr, qr, sr, (int)K, stride);
+        else quant_int8_token_kernel<DT, 0><<<grid, threads, 0, stream>>>(xr, qr, sr, (int)K, stride);
         const int st = (int)hipGetLastError();
         if (st) return st;
     }
