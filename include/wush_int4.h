@@ -371,6 +371,82 @@ int wush_kv8_attention_plan(const wush_kv8_cache *cache, int64_t seqs, int64_t t
 int wush_kv8_read(const wush_kv8_cache *cache, const int32_t *pages, int64_t n, int dtype, void *k, void *v,
                   hipStream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Products in 8-bit floating point, and layers of experts on them.  Codes are e4m3 bytes (four
+ * exponent bits, three fraction bits, no infinities, largest 448).
+ * ------------------------------------------------------------------------ */
+
+/* Largest K of the e4m3 entry points. */
+#define WUSH_FP8_MAX_K 131056
+
+/* Quantization of x (rows, K), bf16 or fp16, rows `row_stride` elements apart, with a scale for each
+ * row and block b of 128 channels (the last one may be shorter):
+ *   A = max(amax |x[m][k in b]|, 448 * 2^-126),  s[b][m] = A / 448,  q[m][k] = e4m3(448 x[m][k] / A)
+ * A / 448 rounded to fp32, the code the one nearest to the quotient itself, halves to even.  A block with a
+ * non-finite value gets s = NaN and zero codes.  q: rows*K bytes; s: (K / 128, rows) fp32, block by block.
+ * K % 16 == 0, K <= WUSH_FP8_MAX_K, at most 2^26 rows, x and q 16-byte aligned, row_stride a multiple of 8. */
+int wush_quant_fp8_block(const void *x, int dtype, uint8_t *q, float *s, int64_t rows, int64_t K,
+                         int64_t row_stride, hipStream_t stream);
+
+/* Product with a scale for each row of x and block of 128 channels, and each block of 128 x 128 weights:
+ *   y[m][n] = sum_b (sum_{k in b} xq[m][k] wq[n][k]) * xs[b][m] * ws[n / 128][b]
+ * sums in fp32, rounded once to `dtype` (bf16 or fp16).  xq (M, K), wq (N, K) codes; xs (K / 128, M), ws
+ * (N / 128, K / 128) fp32, sizes rounded up; y (M, N).  M, N up to 2^26, K % 16 == 0, K <= WUSH_FP8_MAX_K;
+ * xq and wq 16-byte aligned.  The order of the sums depends on M, N, K and the workspace: of the size asked of
+ * wush_gemm_fp8_workspace_bytes it holds partial sums of a split K; with less, K is not split. */
+size_t wush_gemm_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int wush_gemm_fp8(const uint8_t *xq, const float *xs, const uint8_t *wq, const float *ws, void *y, int dtype,
+                  int64_t M, int64_t N, int64_t K, void *workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* Kernels of wush_gemm_fp8, as its plan query names them. */
+enum wush_fp8_kernel {
+    WUSH_FP8_TILES = 0              /* MFMA tiles through LDS */
+};
+
+/* The plan wush_gemm_fp8 runs with `workspace_bytes` of 16-byte aligned workspace:
+ * plan = {kernel, output rows of a workgroup, columns, K slices}.  Host only, no device is
+ * touched; for tests and tuning. */
+int wush_gemm_fp8_plan(int64_t M, int64_t N, int64_t K, size_t workspace_bytes, int32_t plan[4]);
+
+/* Both in one call: y = product of x (M, K), bf16 or fp16 as y, rows row_stride elements apart, quantized
+ * as above.  The workspace (16-byte aligned, of at least wush_linear_fp8_workspace_bytes) holds the codes. */
+size_t wush_linear_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int wush_linear_fp8(const void *x, int64_t row_stride, const uint8_t *wq, const float *ws, void *y, int dtype,
+                    int64_t M, int64_t N, int64_t K, void *workspace, size_t workspace_bytes, hipStream_t stream);
+
+#define WUSH_MOE_MAX_EXPERTS 1024
+#define WUSH_MOE_MAX_CHOICES 64
+
+/* How a router chooses: k experts of those of the best keep_groups of `groups` groups of equal size
+ * (experts one after another), a group's score being the sum of its group_best (1 or 2) largest. */
+typedef struct wush_moe_choice {
+    int32_t k, groups, keep_groups, group_best;
+    int32_t sigmoid;                /* scores sigmoid(x), else softmax(x) over all experts */
+    int32_t renorm;                 /* weights divided by their sum */
+    float scale;                    /* factor of the weights */
+} wush_moe_choice;
+
+/* The router's choice for each row of logits (rows, experts), bf16, fp16 or fp32, rows `row_stride`
+ * elements apart: scores s, choices by c = s + bias (experts fp32, or NULL), all in 64 bits; ids (rows, k) the k experts of
+ * the largest c in the groups that stay, in falling order, equal ones by rising index; weights (rows, k) =
+ * s[ids], with renorm divided by their sum (a sum of 0 gives zeros), times scale, rounded once.  A NaN counts below
+ * every number.  A row of nothing but -inf has scores of 0; with softmax a NaN or +inf makes all of the row's scores NaN.
+ * experts <= 1024, groups <= 64, k <= 64. */
+int wush_moe_route(const void *logits, int dtype, int64_t row_stride, const float *bias, int64_t rows, int64_t experts,
+                   const wush_moe_choice *choice, float *weights, int32_t *ids, hipStream_t stream);
+
+/* A layer of E gated experts: y[t] = sum_j weights[t][j] * down_e(silu(gate_e(x[t])) * up_e(x[t])), e = ids[t][j]
+ * (an id out of [0, E) adds nothing).  x (T, H), rows row_stride elements apart, and y (T, H) bf16 or fp16; weights fp32
+ * and ids int32 (T, k).  w_up codes (E, 2 I, H), the gate's I rows before the up projection's, s_up
+ * (E, 2 I / 128, H / 128); w_down (E, H, I), s_down (E, H / 128, I / 128).  Both inner inputs are quantized as by
+ * wush_quant_fp8_block, all between in fp32, y rounded once.  H % 16 == 0, I % 128 == 0, E <= 1024, k <= 64.  The workspace is 16-byte
+ * aligned, of at least wush_moe_experts_fp8_workspace_bytes. */
+size_t wush_moe_experts_fp8_workspace_bytes(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I);
+int wush_moe_experts_fp8(const void *x, int dtype, int64_t row_stride, const float *weights, const int32_t *ids,
+                         const uint8_t *w_up, const float *s_up, const uint8_t *w_down, const float *s_down, void *y,
+                         int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, void *workspace,
+                         size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,6 +23,12 @@ class Kv8Cache(ctypes.Structure):
                 ("heads", ctypes.c_int32), ("page_size", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
 
 
+class MoeChoice(ctypes.Structure):
+    """``wush_moe_choice``: how a router chooses."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("k", "groups", "keep_groups", "group_best", "sigmoid", "renorm")] + [
+        ("scale", ctypes.c_float)]
+
+
 _KV = ctypes.POINTER(Kv8Cache)
 SIGNATURES = {
     "wush_abi_version": ([], _I),
@@ -57,6 +63,15 @@ SIGNATURES = {
     "wush_kv8_attention": ([_P, _I, _I64, _I64, _KV, _P, _I64, _P, _P, _I64, _I64, _I64, _F, _I64, _F, _I64, _P, _P,
                             _SZ, _P], _I),
     "wush_kv8_read": ([_KV, _P, _I64, _I, _P, _P, _P], _I),
+    "wush_quant_fp8_block": ([_P, _I, _P, _P, _I64, _I64, _I64, _P], _I),
+    "wush_gemm_fp8_workspace_bytes": ([_I64, _I64, _I64], _SZ),
+    "wush_gemm_fp8_plan": ([_I64, _I64, _I64, _SZ, ctypes.POINTER(ctypes.c_int32)], _I),
+    "wush_gemm_fp8": ([_P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _P, _SZ, _P], _I),
+    "wush_linear_fp8_workspace_bytes": ([_I64, _I64, _I64], _SZ),
+    "wush_linear_fp8": ([_P, _I64, _P, _P, _P, _I, _I64, _I64, _I64, _P, _SZ, _P], _I),
+    "wush_moe_route": ([_P, _I, _I64, _P, _I64, _I64, ctypes.POINTER(MoeChoice), _P, _P, _P], _I),
+    "wush_moe_experts_fp8_workspace_bytes": ([_I64, _I64, _I64, _I64, _I64], _SZ),
+    "wush_moe_experts_fp8": ([_P, _I, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _SZ, _P], _I),
 }
 
 DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
@@ -190,4 +205,17 @@ def kv8_attention_plan(pages, heads, page_size, head_dim, seqs, tokens, ragged, 
     plan = (ctypes.c_int32 * 4)()
     _check(load().wush_kv8_attention_plan(ctypes.byref(cache), seqs, tokens, ragged, q_heads, table_stride, window,
                                           max_len, plan), "wush_kv8_attention_plan")
+    return tuple(plan)
+
+
+# kernels of gemm_fp8_plan
+FP8_TILES, = range(1)
+
+
+def gemm_fp8_plan(M, N, K, workspace_bytes=None) -> tuple:
+    """(kernel, rows, columns, K slices) of gemm_fp8 with that much workspace (None: what it asks for)."""
+    if workspace_bytes is None:
+        workspace_bytes = load().wush_gemm_fp8_workspace_bytes(M, N, K)
+    plan = (ctypes.c_int32 * 4)()
+    _check(load().wush_gemm_fp8_plan(M, N, K, workspace_bytes, plan), "wush_gemm_fp8_plan")
     return tuple(plan)

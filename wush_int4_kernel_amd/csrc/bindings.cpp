@@ -4,7 +4,8 @@
 // validates and allocates with torch on the input's device, takes torch's
 // current HIP stream, and calls the C ABI of libwush_int4.so
 // (include/wush_int4.h).  No computation happens here.  Behind them, the 8-bit
-// operators that the reference lacks (quant_int8_token, w8a8_*, kv8_*).
+// operators that the reference lacks (quant_int8_token, w8a8_*, kv8_*, quant_fp8_block,
+// fp8_*, moe_route).
 #include <torch/extension.h>
 
 #include <ATen/hip/EmptyTensor.h>
@@ -590,6 +591,154 @@ std::vector<torch::Tensor> kv8_read(torch::Tensor k_cache, torch::Tensor v_cache
     return {k, v};
 }
 
+// ------------------------------------------------------- 8-bit floating point, experts
+void check_e4m3(const torch::Tensor& t, const char* name) {
+    TORCH_CHECK(t.scalar_type() == torch::kFloat8_e4m3fn && t.is_contiguous(), name, " must be contiguous float8_e4m3fn");
+    TORCH_CHECK(aligned16(t), name, " must be 16-byte aligned");
+}
+
+int64_t blocks128(int64_t n) { return (n + 127) / 128; }
+
+void check_k(int64_t K, const char* name) {
+    TORCH_CHECK(K > 0 && K % 16 == 0 && K <= WUSH_FP8_MAX_K, name, " must be a multiple of 16 and at most ", WUSH_FP8_MAX_K);
+}
+
+// codes (lead..., N, K) and their scales (lead..., N / 128, K / 128)
+void check_fp8_weights(const torch::Tensor& w, const char* wname, const torch::Tensor& s, const char* sname,
+                       const torch::Tensor& like, int64_t dims) {
+    check_gpu(w, wname, like);
+    check_gpu(s, sname, like);
+    check_e4m3(w, wname);
+    check_f32(s, sname);
+    TORCH_CHECK(w.dim() == dims && s.dim() == dims, wname, " must be ", dims, "D (", dims == 3 ? "experts, " : "", "N, K) and ",
+                sname, " ", dims, "D");
+    TORCH_CHECK((dims == 2 || s.size(0) == w.size(0)) && s.size(-2) == blocks128(w.size(-2)) && s.size(-1) == blocks128(w.size(-1)),
+                sname, " must hold one scale per 128 x 128 block of ", wname);
+}
+
+std::vector<torch::Tensor> quant_fp8_block(torch::Tensor x) {
+    TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    const int dt = half_code(x.scalar_type(), "x");
+    TORCH_CHECK(x.dim() >= 1, "x must have a last dimension");
+    const int64_t K = x.size(-1);
+    check_k(K, "last dim");
+    const at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    int64_t rows, stride;
+    const auto xr = token_rows(x, rows, stride);
+    auto q = new_tensor(x.sizes(), torch::kFloat8_e4m3fn, x);
+    auto s = new_tensor({blocks128(K), rows}, torch::kFloat32, x);
+    check_status(wush_quant_fp8_block(xr.data_ptr(), dt, ptr<uint8_t>(q), ptr<float>(s), rows, K, stride, current_stream(x)),
+                 "quant_fp8_block");
+    return {q, s};
+}
+
+torch::Tensor fp8_gemm(torch::Tensor xq, torch::Tensor xs, torch::Tensor wq, torch::Tensor ws, at::ScalarType dtype) {
+    TORCH_CHECK(xq.is_cuda(), "xq must be a CUDA tensor");
+    const int dt = half_code(dtype, "dtype");
+    check_fp8_weights(wq, "wq", ws, "ws", xq, 2);
+    check_gpu(xs, "xs", xq);
+    check_e4m3(xq, "xq");
+    check_f32(xs, "xs");
+    const int64_t K = wq.size(1), N = wq.size(0);
+    check_k(K, "K");
+    TORCH_CHECK(xq.dim() >= 1 && xq.size(-1) == K, "K mismatch: xq must have wq's ", K, " columns");
+    const int64_t M = xq.numel() / K;
+    TORCH_CHECK(xs.dim() == 2 && xs.size(0) == blocks128(K) && xs.size(1) == M, "xs must be (K / 128, rows)");
+    const at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(xq.device());
+    auto y = new_tensor(with_last(xq, N), dtype, xq);
+    const size_t wsb = wush_gemm_fp8_workspace_bytes(M, N, K);
+    auto work = bytes_like(wsb, xq);
+    check_status(wush_gemm_fp8(ptr<uint8_t>(xq), ptr<float>(xs), ptr<uint8_t>(wq), ptr<float>(ws), y.data_ptr(), dt, M, N, K,
+                               wsb ? work.data_ptr() : nullptr, wsb, current_stream(xq)),
+                 "fp8_gemm");
+    return y;
+}
+
+torch::Tensor fp8_linear(torch::Tensor x, torch::Tensor wq, torch::Tensor ws) {
+    TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    const int dt = half_code(x.scalar_type(), "x");
+    check_fp8_weights(wq, "wq", ws, "ws", x, 2);
+    const int64_t K = wq.size(1), N = wq.size(0);
+    check_k(K, "K");
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) == K, "K mismatch: x must have wq's ", K, " columns");
+    const at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    int64_t M, stride;
+    const auto xr = token_rows(x, M, stride);
+    auto y = new_tensor(with_last(x, N), x.scalar_type(), x);
+    const size_t wsb = wush_linear_fp8_workspace_bytes(M, N, K);
+    auto work = bytes_like(wsb, x);
+    check_status(wush_linear_fp8(xr.data_ptr(), stride, ptr<uint8_t>(wq), ptr<float>(ws), y.data_ptr(), dt, M, N, K,
+                                 wsb ? work.data_ptr() : nullptr, wsb, current_stream(x)),
+                 "fp8_linear");
+    return y;
+}
+
+std::vector<torch::Tensor> moe_route(torch::Tensor logits, int64_t k, std::optional<torch::Tensor> bias, bool sigmoid,
+                                     int64_t groups, int64_t keep_groups, int64_t group_best, bool renorm, double scale) {
+    TORCH_CHECK(logits.is_cuda(), "logits must be a CUDA tensor");
+    const auto t = logits.scalar_type();
+    TORCH_CHECK(t == torch::kBFloat16 || t == torch::kHalf || t == torch::kFloat32, "logits must be bf16, fp16 or fp32, got ", t);
+    TORCH_CHECK(logits.dim() >= 1, "logits must have a last dimension");
+    const int64_t E = logits.size(-1);
+    TORCH_CHECK(E >= 1 && E <= WUSH_MOE_MAX_EXPERTS, "there must be 1 to ", WUSH_MOE_MAX_EXPERTS, " experts, got ", E);
+    TORCH_CHECK(groups >= 1 && groups <= 64 && E % groups == 0, "groups must be 1 to 64 and divide the ", E, " experts");
+    TORCH_CHECK(keep_groups >= 1 && keep_groups <= groups, "keep_groups must be 1 to groups");
+    TORCH_CHECK((group_best == 1 || group_best == 2) && group_best <= E / groups, "group_best must be 1 or 2, and no more than a group holds");
+    TORCH_CHECK(k >= 1 && k <= WUSH_MOE_MAX_CHOICES && k <= keep_groups * (E / groups), "k must be 1 to ", WUSH_MOE_MAX_CHOICES,
+                ", and no more than the kept groups hold");
+    TORCH_CHECK(std::isfinite((float)scale), "scale must be finite");
+    if (bias.has_value()) {
+        check_gpu(*bias, "bias", logits);
+        check_f32(*bias, "bias");
+        TORCH_CHECK(bias->dim() == 1 && bias->size(0) == E, "bias must hold one value per expert");
+    }
+    const at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(logits.device());
+    const int64_t rows = logits.numel() / E;
+    const bool even = logits.dim() == 2 && logits.stride(1) == 1 && logits.stride(0) >= 0;
+    const auto l = even ? logits : logits.contiguous();
+    auto w = new_tensor(with_last(logits, k), torch::kFloat32, logits), ids = new_tensor(with_last(logits, k), torch::kInt32, logits);
+    const wush_moe_choice c = {(int32_t)k, (int32_t)groups, (int32_t)keep_groups, (int32_t)group_best, sigmoid, renorm, (float)scale};
+    check_status(wush_moe_route(l.data_ptr(), t == torch::kBFloat16 ? WUSH_DTYPE_BF16 : t == torch::kHalf ? WUSH_DTYPE_F16 : WUSH_DTYPE_F32,
+                                even ? l.stride(0) : E, bias.has_value() ? ptr<float>(*bias) : nullptr, rows, E, &c,
+                                ptr<float>(w), ptr<int32_t>(ids), current_stream(logits)),
+                 "moe_route");
+    return {w, ids};
+}
+
+torch::Tensor fp8_experts(torch::Tensor x, torch::Tensor weights, torch::Tensor ids, torch::Tensor w_up, torch::Tensor s_up,
+                          torch::Tensor w_down, torch::Tensor s_down) {
+    TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    const int dt = half_code(x.scalar_type(), "x");
+    check_fp8_weights(w_up, "w_up", s_up, "s_up", x, 3);
+    check_fp8_weights(w_down, "w_down", s_down, "s_down", x, 3);
+    const int64_t E = w_up.size(0), H = w_up.size(2), I = w_down.size(2);
+    TORCH_CHECK(E >= 1 && E <= WUSH_MOE_MAX_EXPERTS, "there must be 1 to ", WUSH_MOE_MAX_EXPERTS, " experts, got ", E);
+    check_k(H, "H");
+    TORCH_CHECK(I > 0 && I % 128 == 0 && I <= WUSH_FP8_MAX_K, "I must be a multiple of 128 and at most ", WUSH_FP8_MAX_K);
+    TORCH_CHECK(w_up.size(1) == 2 * I && w_down.size(0) == E && w_down.size(1) == H,
+                "w_up must be (experts, 2 I, H) and w_down (experts, H, I)");
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) == H, "x must have w_up's ", H, " columns");
+    check_gpu(weights, "weights", x);
+    check_f32(weights, "weights");
+    check_int32(ids, "ids", x);
+    const int64_t T = x.numel() / H;
+    TORCH_CHECK(ids.dim() >= 1 && ids.sizes() == weights.sizes() && ids.size(-1) >= 1 && ids.size(-1) <= WUSH_MOE_MAX_CHOICES &&
+                    ids.numel() == T * ids.size(-1),
+                "weights and ids must be (tokens, k), k from 1 to ", WUSH_MOE_MAX_CHOICES);
+    const int64_t k = ids.size(-1);
+    const at::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    int64_t rows, stride;
+    const auto xr = token_rows(x, rows, stride);
+    auto y = new_tensor(x.sizes(), x.scalar_type(), x);
+    const size_t wsb = wush_moe_experts_fp8_workspace_bytes(T, k, E, H, I);
+    auto work = bytes_like(wsb, x);
+    check_status(wush_moe_experts_fp8(xr.data_ptr(), dt, stride, ptr<float>(weights), ptr<int32_t>(ids), ptr<uint8_t>(w_up),
+                                      ptr<float>(s_up), ptr<uint8_t>(w_down), ptr<float>(s_down), y.data_ptr(), T, k, E, H, I,
+                                      wsb ? work.data_ptr() : nullptr, wsb, current_stream(x)),
+                 "fp8_experts");
+    return y;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -650,5 +799,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("kv8_read", &kv8_read, "pages of the 8-bit cache as values: (k, v), each (pages, heads, page_size, head_dim)",
           py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("pages"),
           py::arg("dtype") = at::kBFloat16);
+    m.def("quant_fp8_block", &quant_fp8_block,
+          "e4m3 quantize with a scale per row and 128 channels: (codes, scales fp32 (K / 128, rows))", py::arg("x"));
+    m.def("fp8_gemm", &fp8_gemm, "e4m3 matmul, scales per row and 128 channels of x and per 128 x 128 weights", py::arg("xq"),
+          py::arg("xs"), py::arg("wq"), py::arg("ws"), py::arg("dtype") = at::kBFloat16);
+    m.def("fp8_linear", &fp8_linear, "quant_fp8_block and fp8_gemm in one call; y of x's type", py::arg("x"), py::arg("wq"),
+          py::arg("ws"));
+    m.def("moe_route", &moe_route, "a router's choice: (weights fp32, ids int32), each (tokens, k)", py::arg("logits"),
+          py::arg("k"), py::arg("bias") = py::none(), py::arg("sigmoid") = false, py::arg("groups") = 1,
+          py::arg("keep_groups") = 1, py::arg("group_best") = 1, py::arg("renorm") = true, py::arg("scale") = 1.0);
+    m.def("fp8_experts", &fp8_experts, "gated e4m3 experts: the weighted sum of each token's", py::arg("x"), py::arg("weights"),
+          py::arg("ids"), py::arg("w_up"), py::arg("s_up"), py::arg("w_down"), py::arg("s_down"));
     m.def("abi_version", &wush_abi_version, "C ABI version of libwush_int4.so");
 }

@@ -1,0 +1,182 @@
+// fp8.hip -- linear layers in 8-bit floating point (e4m3: four exponent and three
+// fraction bits, largest 448): activations scaled for each token and block of 128 channels,
+// weights for each block of 128 x 128.
+//
+//   A_bm = max(amax_{k in b} |x_mk|, 448 * 2^-126),  xs_bm = A_bm / 448,  q_mk = e4m3(448 x_mk / A_bm)
+//   y_mn = sum_b (sum_{k in b} q_mk w_nk) xs_bm ws_{n / 128, b}        (fp32 sums, rounded once)
+//
+// Scales lie block by block, (K / 128, rows): a tile's rows of one block are then one load.
+#include "fp8.h"
+#include "fp8_device.h"
+#include "../../include/wush_int4.h"
+
+namespace wush {
+namespace {
+
+// A workgroup takes ROWS rows and 16 / ROWS blocks of each, a row of 16 lanes a block, and
+// kQuantSteps times that along K.  Sixteen rows together write a block's scales as 64 bytes.
+constexpr int kQuantSteps = 4;
+
+template <int DT, int ROWS>
+__global__ __launch_bounds__(256) void quant_fp8_block_kernel(const uint16_t* __restrict__ x, uint8_t* __restrict__ q,
+                                                              float* __restrict__ s, int64_t rows, int K, int64_t stride) {
+    constexpr int BLOCKS = 16 / ROWS;
+    const int group = threadIdx.x >> 4, l16 = threadIdx.x & 15;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + group % ROWS;
+    const int KB = (K + 127) >> 7;
+    const int64_t at = row < rows ? row : rows - 1;
+    const uint16_t* px = x + at * stride;
+    uint4 w[kQuantSteps];
+    const int b0 = (int)blockIdx.y * BLOCKS * kQuantSteps + group / ROWS;
+#pragma unroll
+    for (int u = 0; u < kQuantSteps; ++u) {
+        const int k = (b0 + u * BLOCKS) * 128 + 8 * l16;
+        w[u] = k < K ? *reinterpret_cast<const uint4*>(px + k) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < kQuantSteps; ++u) {
+        const int b = b0 + u * BLOCKS, k = b * 128 + 8 * l16;
+        float v[8];
+        fp8_unpack8<DT>(w[u], v);
+        const float amax = fp8_amax(row16_max(fp8_largest8(v)));
+        if (row >= rows || b >= KB) continue;
+        if (l16 == 0) s[(size_t)b * rows + row] = fp8_scale(amax);
+        if (k < K)
+            *reinterpret_cast<uint2*>(q + row * K + k) =
+                make_uint2(fp8_codes4(v[0], v[1], v[2], v[3], amax), fp8_codes4(v[4], v[5], v[6], v[7], amax));
+    }
+}
+
+template <int DT>
+int launch_quant(const void* x, uint8_t* q, float* s, int64_t rows, int64_t K, int64_t stride, hipStream_t stream) {
+    const uint16_t* p = static_cast<const uint16_t*>(x);
+    const int64_t KB = (K + 127) / 128;
+    if (rows < 16) {
+        const dim3 grid((unsigned)rows, (unsigned)((KB + 16 * kQuantSteps - 1) / (16 * kQuantSteps)));
+        quant_fp8_block_kernel<DT, 1><<<grid, 256, 0, stream>>>(p, q, s, rows, (int)K, stride);
+    } else {
+        const dim3 grid((unsigned)((rows + 15) / 16), (unsigned)((KB + kQuantSteps - 1) / kQuantSteps));
+        quant_fp8_block_kernel<DT, 16><<<grid, 256, 0, stream>>>(p, q, s, rows, (int)K, stride);
+    }
+    return (int)hipGetLastError();
+}
+
+// ---------------------------------------------------------------- the choice
+struct Plan {
+    int kernel, rows, cols, splits;
+};
+
+// The tile and the split of K with the least estimated time, in microseconds.
+Plan plan_of(int64_t M, int64_t N, int64_t K, size_t room) {
+    Plan best = {WUSH_FP8_TILES, 32, 64, 1};
+    const int64_t stages = (K + 127) / 128;
+    double least = 1e30;
+    for (const auto& t : kFp8Tiles) {
+        if (t.rows > 32 && t.rows >= 2 * M) continue;
+        const int64_t tiles = ((M + t.rows - 1) / t.rows) * ((N + t.cols - 1) / t.cols);
+        for (int s = 1; s <= 8 && (s == 1 || stages / s >= 4); ++s) {
+            if (s > 1 && (size_t)M * N * 4 * s > room) break;
+            const double groups = (double)tiles * s, full = groups / 256 < 1 ? groups / 256 : 1;
+            const double rounds = groups <= 1024 ? (double)(int64_t)((groups + 255) / 256) : groups / 256;
+            const double busy = t.stage * (0.6 + 0.4 * full), idle = 0.72 / (t.depth - 1);
+            const double work = rounds * (double)((stages + s - 1) / s) * (busy > idle ? busy : idle);
+            const double hbm = (double)N * K / 7e6;
+            double us = 4.0 + 1.0 * rounds + (work > hbm ? work : hbm);
+            if (s > 1) us += 3.3 + (double)M * N * (8.0 * s + 2) / 4.5e6;
+            if (us < least) {
+                least = us;
+                best = {WUSH_FP8_TILES, t.rows, t.cols, s};
+            }
+        }
+    }
+    return best;
+}
+
+}  // namespace
+}  // namespace wush
+
+extern "C" {
+
+static constexpr int64_t kMostRows = 1 << 26;
+
+static bool fp8_sizes(int64_t M, int64_t N, int64_t K) {
+    return M >= 0 && N >= 0 && K > 0 && K % 16 == 0 && K <= WUSH_FP8_MAX_K && M <= kMostRows && N <= kMostRows;
+}
+
+int wush_quant_fp8_block(const void* x, int dtype, uint8_t* q, float* s, int64_t rows, int64_t K, int64_t row_stride,
+                         hipStream_t stream) {
+    WUSH_REQUIRE(fp8_sizes(rows, 0, K));
+    WUSH_REQUIRE(dtype == WUSH_DTYPE_BF16 || dtype == WUSH_DTYPE_F16);
+    if (rows == 0) return (int)hipSuccess;
+    WUSH_REQUIRE(x && q && s);
+    WUSH_REQUIRE(((uintptr_t)x & 15u) == 0 && ((uintptr_t)q & 15u) == 0 && ((uintptr_t)s & 3u) == 0);
+    WUSH_REQUIRE(rows == 1 || (row_stride >= 0 && row_stride % 8 == 0));
+    if (rows == 1) row_stride = 0;                // the stride of a single row does not enter any address
+    return dtype == WUSH_DTYPE_BF16 ? wush::launch_quant<WUSH_DTYPE_BF16>(x, q, s, rows, K, row_stride, stream)
+                                    : wush::launch_quant<WUSH_DTYPE_F16>(x, q, s, rows, K, row_stride, stream);
+}
+
+size_t wush_gemm_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    if (!fp8_sizes(M, N, K) || M == 0 || N == 0) return 0;
+    const wush::Plan p = wush::plan_of(M, N, K, SIZE_MAX);
+    return p.splits > 1 ? (size_t)p.splits * M * N * 4 : 0;
+}
+
+int wush_gemm_fp8_plan(int64_t M, int64_t N, int64_t K, size_t workspace_bytes, int32_t plan[4]) {
+    WUSH_REQUIRE(plan && M > 0 && N > 0 && fp8_sizes(M, N, K));
+    const wush::Plan p = wush::plan_of(M, N, K, workspace_bytes);
+    plan[0] = p.kernel;
+    plan[1] = p.rows;
+    plan[2] = p.cols;
+    plan[3] = p.splits;
+    return (int)hipSuccess;
+}
+
+int wush_gemm_fp8(const uint8_t* xq, const float* xs, const uint8_t* wq, const float* ws, void* y, int dtype, int64_t M,
+                  int64_t N, int64_t K, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    WUSH_REQUIRE(fp8_sizes(M, N, K));
+    WUSH_REQUIRE(dtype == WUSH_DTYPE_BF16 || dtype == WUSH_DTYPE_F16);
+    if (M == 0 || N == 0) return (int)hipSuccess;
+    WUSH_REQUIRE(xq && xs && wq && ws && y);
+    WUSH_REQUIRE((((uintptr_t)xq | (uintptr_t)wq) & 15u) == 0 && (((uintptr_t)xs | (uintptr_t)ws) & 3u) == 0 && ((uintptr_t)y & 1u) == 0);
+    const bool usable = workspace && ((uintptr_t)workspace & 15u) == 0;
+    const wush::Plan p = wush::plan_of(M, N, K, usable ? workspace_bytes : 0);
+    wush::Fp8Gemm g = {};
+    g.x = xq;
+    g.xs = xs;
+    g.ldx = M;
+    g.w = wq;
+    g.ws = ws;
+    g.y = y;
+    g.out = dtype;
+    g.part = static_cast<float*>(workspace);
+    g.M = (int)M;
+    g.N = (int)N;
+    g.K = (int)K;
+    g.splits = p.splits;
+    return wush::launch_gemm_fp8(g, p.rows, p.cols, stream);
+}
+
+static size_t fp8_scale_bytes(int64_t M, int64_t K) { return ((size_t)M * ((K + 127) / 128) * 4 + 15) & ~(size_t)15; }
+
+size_t wush_linear_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    if (!fp8_sizes(M, N, K) || M == 0 || N == 0) return 0;
+    return (size_t)M * K + fp8_scale_bytes(M, K) + wush_gemm_fp8_workspace_bytes(M, N, K);
+}
+
+int wush_linear_fp8(const void* x, int64_t row_stride, const uint8_t* wq, const float* ws, void* y, int dtype, int64_t M,
+                    int64_t N, int64_t K, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    WUSH_REQUIRE(fp8_sizes(M, N, K));
+    WUSH_REQUIRE(dtype == WUSH_DTYPE_BF16 || dtype == WUSH_DTYPE_F16);
+    if (M == 0 || N == 0) return (int)hipSuccess;
+    const size_t need = wush_linear_fp8_workspace_bytes(M, N, K);
+    WUSH_REQUIRE(x && wq && ws && y && workspace_bytes >= need && (need == 0 || (workspace && ((uintptr_t)workspace & 15u) == 0)));
+    uint8_t* q = static_cast<uint8_t*>(workspace);
+    float* s = reinterpret_cast<float*>(q + (size_t)M * K);
+    const int st = wush_quant_fp8_block(x, dtype, q, s, M, K, row_stride, stream);
+    if (st) return st;
+    const size_t held = (size_t)M * K + fp8_scale_bytes(M, K);
+    return wush_gemm_fp8(q, s, wq, ws, y, dtype, M, N, K, q + held, workspace_bytes - held, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,71 @@
+// fp8_device.h -- e4m3 codes of a block of 128 channels, shared by the kernels
+// that quantize activations.
+//
+//   A = max(amax |x|, 448 * 2^-126),  scale = A / 448,  code = e4m3(448 x / A)
+//
+// The code is the nearest to the quotient itself, halves to even: 0.875 x is exact for bf16 and fp16
+// values (7 x has 3 more bits), the division is correctly rounded and 512 a power of two, and
+// no quotient of two such values is within 2^-23 of half a code's step without being it.  A
+// product with the rounded reciprocal instead falls to one or the other side of those
+// halves, which values of 8 bits meet often.  A block with a non-finite value gets the
+// scale NaN and zero codes.
+#pragma once
+
+#include "wush_device.h"
+
+namespace wush {
+namespace {
+
+constexpr float kFp8Largest = 448.0f;
+constexpr float kFp8Floor = 448.0f * 0x1p-126f;
+
+// largest: amax as fp32 bits, sign cleared (a NaN's are above infinity's)
+__device__ __forceinline__ float fp8_amax(uint32_t largest) {
+    return largest >= 0x7f800000u ? __builtin_nanf("") : fmaxf(__uint_as_float(largest), kFp8Floor);
+}
+__device__ __forceinline__ float fp8_scale(float amax) { return amax / kFp8Largest; }
+__device__ __forceinline__ float fp8_arg(float v, float amax) { return v * 0.875f / amax * 512.0f; }
+
+// four codes
+__device__ __forceinline__ uint32_t fp8_codes4(float a, float b, float c, float d, float amax) {
+    if (amax != amax) return 0;
+    int p = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_arg(a, amax), fp8_arg(b, amax), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(fp8_arg(c, amax), fp8_arg(d, amax), p, true);
+}
+
+// maximum over the 16 lanes of a row (of a block, where a lane holds 8 channels)
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
+    v = dpp_max<0xB1>(v);        // quad_perm [1,0,3,2]
+    v = dpp_max<0x4E>(v);        // quad_perm [2,3,0,1]
+    v = dpp_max<0x141>(v);       // row_half_mirror
+    return dpp_max<0x140>(v);    // row_mirror
+}
+
+// eight bf16 or fp16 values as fp32
+template <int DT>
+__device__ __forceinline__ void fp8_unpack8(const uint4& w, float (&v)[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (DT == 0) {
+            v[2 * i] = __uint_as_float(u[i] << 16);
+            v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        } else {
+            v[2 * i] = f16_to_f32(u[i] & 0xffffu);
+            v[2 * i + 1] = f16_to_f32(u[i] >> 16);
+        }
+    }
+}
+__device__ __forceinline__ uint32_t fp8_largest8(const float (&v)[8]) {
+    uint32_t mx = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mx = max(mx, __float_as_uint(v[i]) & 0x7fffffffu);
+    return mx;
+}
+
+}  // namespace
+}  // namespace wush

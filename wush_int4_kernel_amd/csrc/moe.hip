@@ -1,0 +1,473 @@
+// moe.hip -- a feed-forward layer of experts: the router's choice, and the experts'
+// gated layers in e4m3.
+//
+// Route: s = softmax(x) or sigmoid(x), c = s + bias; of each group of experts the sum of its best one or
+// two c, the best groups stay; ids are the k largest c left, equal ones by the lowest
+// index; weights s[ids], divided by their sum or not, times a factor.  Scores and sums are in 64
+// bits: in 32, of 16384 x 256 choices some would hang on a rounding.
+//
+// Experts: rows of x by expert; a = q(x) up_e^T, h = silu(a_gate) a_up, o = q(h) down_e^T, y = sum of w o over a
+// token's experts.  a, h and o are kept in fp32, h and x quantized as in fp8_device.h.
+#include "fp8.h"
+#include "fp8_device.h"
+#include "../../include/wush_int4.h"
+
+namespace wush {
+namespace {
+
+// ------------------------------------------------------------------- the router
+typedef unsigned long long u64;
+
+// Order of doubles as that of unsigned integers; NaN below all, 0 left for "not there".
+__device__ __forceinline__ u64 order_key(double c) {
+    if (c != c) return 1;
+    const u64 b = __builtin_bit_cast(u64, c + 0.0);              // -0 is 0
+    return b >> 63 ? ~b : b | 1ull << 63;
+}
+__device__ __forceinline__ double order_value(u64 key) {
+    if (key <= 1) return __builtin_nan("");
+    return __builtin_bit_cast(double, key >> 63 ? key & ~(1ull << 63) : ~key);
+}
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+__device__ __forceinline__ double lane_value(double v, int lane) {
+    const u64 b = __builtin_bit_cast(u64, v);
+    return __builtin_bit_cast(double, (u64)lane_value((uint32_t)(b >> 32), lane) << 32 | lane_value((uint32_t)b, lane));
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d));
+    return v;
+}
+
+struct RouteArgs {
+    const void* logits;
+    int64_t stride;
+    const float* bias;
+    float* weights;
+    int32_t* ids;
+    int64_t rows;
+    int E, k, groups, size, keep, best, lanes;   // size: experts of a group; lanes: of a group, a power of two
+    int sigmoid, renorm;
+    float scale;
+};
+
+// A wavefront per row.  Lane group * lanes + sub holds experts group * size + sub + lanes * i.
+template <int V, int DT>
+__global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs p) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= p.rows) return;
+    const int group = lane / p.lanes, sub = lane % p.lanes;
+    float x[V];
+    bool in[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int o = sub + p.lanes * i, e = group * p.size + o;
+        in[i] = group < p.groups && o < p.size;
+        x[i] = -__builtin_inff();
+        if (in[i]) {
+            if constexpr (DT == WUSH_DTYPE_F32) x[i] = static_cast<const float*>(p.logits)[row * p.stride + e];
+            else {
+                const uint32_t w = static_cast<const uint16_t*>(p.logits)[row * p.stride + e];
+                x[i] = DT == WUSH_DTYPE_BF16 ? bf16_to_f32(w) : f16_to_f32(w);
+            }
+        }
+    }
+    double s[V], total = 1.0;
+    if (p.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i] = 1.0 / (1.0 + exp(-(double)x[i]));
+    } else {
+        float mx = x[0];
+        bool nan = x[0] != x[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) {
+            mx = fmaxf(mx, x[i]);
+            nan |= x[i] != x[i];
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
+        nan = __any(nan) || mx == __builtin_inff();              // inf - inf
+        const bool none = mx == -__builtin_inff();               // nothing but -inf: every score 0
+        total = 0.0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            s[i] = nan ? __builtin_nan("") : none ? 0.0 : exp((double)x[i] - (double)mx);
+            total += in[i] ? s[i] : 0.0;
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+        if (none && !nan) total = 1.0;
+    }
+    // without a bias the order of exp(x - max) is that of the scores
+    u64 key[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int e = group * p.size + sub + p.lanes * i;
+        double c = s[i];
+        if (p.bias && in[i]) c = (p.sigmoid ? s[i] : s[i] / total) + (double)p.bias[e];
+        key[i] = in[i] ? order_key(c) : 0;
+    }
+    if (p.groups > 1) {
+        u64 a = 0, b = 0;                        // the group's two largest
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            b = max(b, min(a, key[i]));
+            a = max(a, key[i]);
+        }
+        for (int d = 1; d < p.lanes; d <<= 1) {
+            const u64 oa = __shfl_xor(a, d), ob = __shfl_xor(b, d);
+            b = max(min(a, oa), max(b, ob));
+            a = max(a, oa);
+        }
+        const u64 score = p.best == 2 ? order_key(order_value(a) + order_value(b)) : a;
+        int above = 0;
+        for (int g = 0; g < p.groups; ++g) {
+            const u64 o = (u64)lane_value((uint32_t)(score >> 32), g * p.lanes) << 32 | lane_value((uint32_t)score, g * p.lanes);
+            above += o > score || (o == score && g < group);
+        }
+        if (above >= p.keep) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) key[i] = 0;
+        }
+    }
+    int id = 0;                                  // lane j: choice j
+    double w = 0.0, sum = 0.0;
+    for (int j = 0; j < p.k; ++j) {
+        u64 top = key[0];
+        int at = 0;
+        double sc = s[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i)
+            if (key[i] > top) {
+                top = key[i];
+                at = i;
+                sc = s[i];
+            }
+        const uint32_t hi = wave_max_u32((uint32_t)(top >> 32));
+        u64 who = __ballot((uint32_t)(top >> 32) == hi);
+        int e = group * p.size + sub + p.lanes * at;
+        if (who & (who - 1)) {                   // several lanes: the low words, then the index
+            const bool me = (uint32_t)(top >> 32) == hi;
+            const uint32_t lo = wave_max_u32(me ? (uint32_t)top : 0);
+            const bool still = me && (uint32_t)top == lo;
+            const uint32_t least = ~wave_max_u32(still ? ~(uint32_t)e : 0);
+            who = __ballot(still && (uint32_t)e == least);
+        }
+        const int winner = (int)__builtin_ctzll(who);
+        const int chosen = (int)lane_value((uint32_t)e, winner);
+        const double score = lane_value(sc, winner);
+        sum += score;
+        if (lane == j) {
+            id = chosen;
+            w = score;
+        }
+        if (lane == winner) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i == at) key[i] = 0;
+        }
+    }
+    if (lane < p.k) {
+        if (p.renorm) w = sum > 0.0 || sum != sum ? w / sum : 0.0;
+        else if (!p.sigmoid) w = w / total;
+        p.weights[row * p.k + lane] = (float)(w * (double)p.scale);
+        p.ids[row * p.k + lane] = id;
+    }
+}
+
+template <int DT>
+int launch_route(const RouteArgs& a, hipStream_t stream) {
+    const int v = (a.size + a.lanes - 1) / a.lanes;
+    const unsigned grid = (unsigned)((a.rows + 3) / 4);
+    if (v <= 1) moe_route_kernel<1, DT><<<grid, 256, 0, stream>>>(a);
+    else if (v <= 2) moe_route_kernel<2, DT><<<grid, 256, 0, stream>>>(a);
+    else if (v <= 4) moe_route_kernel<4, DT><<<grid, 256, 0, stream>>>(a);
+    else if (v <= 8) moe_route_kernel<8, DT><<<grid, 256, 0, stream>>>(a);
+    else if (v <= 16) moe_route_kernel<16, DT><<<grid, 256, 0, stream>>>(a);
+    else moe_route_kernel<32, DT><<<grid, 256, 0, stream>>>(a);
+    return (int)hipGetLastError();
+}
+
+// ------------------------------------------------------------------- the experts
+// Rows by expert.  One workgroup per kSortPairs (token, choice) pairs; each counts all
+// pairs' experts for itself, those before its own apart, and so needs no other: row = the
+// expert's first + its pairs in earlier workgroups + the rank among this one's.  The last two come
+// from an LDS counter: which of an expert's rows a pair gets may differ from call to call, what
+// is computed in that row does not depend on it.
+constexpr int kSortThreads = 1024, kSortPairs = 1024, kMostExperts = 1024;
+
+__global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(const int32_t* __restrict__ ids, int P, int k, int E,
+                                                                int tile_rows, int* __restrict__ row_of,
+                                                                int* __restrict__ pos, int4* __restrict__ tiles,
+                                                                int* __restrict__ ntiles) {
+    __shared__ int all[kMostExperts], before[kMostExperts], start[kMostExperts], tile0[kMostExperts];
+    __shared__ int wave_rows[kSortThreads / 64], wave_tiles[kSortThreads / 64];
+    const int tid = threadIdx.x, first = blockIdx.x * kSortPairs;
+    all[tid] = before[tid] = 0;
+    __syncthreads();
+    int mine = -1;
+    for (int p = tid; p < P; p += kSortThreads) {
+        const int e = ids[p];
+        if ((unsigned)e >= (unsigned)E) continue;
+        if (p >= first && p < first + kSortPairs) mine = e;
+        else if (p < first) atomicAdd(&before[e], 1);
+        else atomicAdd(&all[e], 1);
+    }
+    __syncthreads();
+    int rank = 0;                                // among the expert's pairs up to this workgroup's
+    if (mine >= 0) rank = atomicAdd(&before[mine], 1);
+    __syncthreads();
+    // exclusive sums over the experts, one a thread
+    const int n = before[tid] + all[tid], t = (n + tile_rows - 1) / tile_rows;
+    int sn = n, stl = t;
+    const int lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int a = __shfl_up(sn, d), c = __shfl_up(stl, d);
+        if (lane >= d) {
+            sn += a;
+            stl += c;
+        }
+    }
+    if (lane == 63) {
+        wave_rows[wave] = sn;
+        wave_tiles[wave] = stl;
+    }
+    __syncthreads();
+    int on = 0, ot = 0;
+    for (int w = 0; w < wave; ++w) {
+        on += wave_rows[w];
+        ot += wave_tiles[w];
+    }
+    start[tid] = on + sn - n;
+    tile0[tid] = ot + stl - t;
+    __syncthreads();
+    if (first + tid < P) {
+        int r = -1;
+        if (mine >= 0) {
+            r = start[mine] + rank;
+            row_of[r] = (first + tid) / k;
+        }
+        pos[first + tid] = r;
+    }
+    if (blockIdx.x == 0) {
+        if (tid < E)
+            for (int i = 0; i < t; ++i) tiles[tile0[tid] + i] = make_int4(tid, start[tid] + i * tile_rows, start[tid] + n, 0);
+        if (tid == kSortThreads - 1) *ntiles = ot + stl;
+    }
+}
+
+// h = silu(gate) * up of a row's 128 channels, quantized: 16 lanes a block
+__global__ __launch_bounds__(256) void moe_act_kernel(const float* __restrict__ a, uint8_t* __restrict__ q,
+                                                      float* __restrict__ s, int I, int64_t ld,
+                                                      const int4* __restrict__ tiles, const int* __restrict__ ntiles) {
+    const int nt = *ntiles, rows = nt ? tiles[nt - 1].z : 0;
+    const int l16 = threadIdx.x & 15, blocks = I >> 7;
+    const int64_t total = (int64_t)rows * blocks;
+    for (int64_t u = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); u < total; u += (int64_t)gridDim.x * 16) {
+        const int64_t row = u / blocks;
+        const int b = (int)(u - row * blocks), c = b * 128 + 8 * l16;
+        const float4* g = reinterpret_cast<const float4*>(a + row * 2 * I + c);
+        const float4* p = reinterpret_cast<const float4*>(a + row * 2 * I + I + c);
+        const float4 g0 = g[0], g1 = g[1], p0 = p[0], p1 = p[1];
+        const float gate[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+        const float up[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = gate[i] / (1.0f + expf(-gate[i])) * up[i];
+        const float amax = fp8_amax(row16_max(fp8_largest8(v)));
+        if (l16 == 0) s[b * ld + row] = fp8_scale(amax);
+        *reinterpret_cast<uint2*>(q + row * I + c) =
+            make_uint2(fp8_codes4(v[0], v[1], v[2], v[3], amax), fp8_codes4(v[4], v[5], v[6], v[7], amax));
+    }
+}
+
+__device__ __forceinline__ uint16_t out_bits(float f, int dt) {
+    return dt == WUSH_DTYPE_F16 ? f32_to_f16_bits(f) : (uint16_t)(f != f ? 0x7fc0u : f32_to_bf16_rne(f));
+}
+
+// y of a token: the sum of its experts' rows, in the order of its choices
+__global__ __launch_bounds__(256) void moe_sum_kernel(const float* __restrict__ o, const int* __restrict__ pos,
+                                                      const float* __restrict__ weights, uint16_t* __restrict__ y, int dt,
+                                                      int k, int H) {
+    const int64_t t = blockIdx.x;
+    const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
+    if (c >= H) return;
+    float v[4] = {0, 0, 0, 0};
+    for (int j = 0; j < k; ++j) {
+        const int r = pos[t * k + j];
+        if (r < 0) continue;
+        const float w = weights[t * k + j];
+        const float4 f = *reinterpret_cast<const float4*>(o + (int64_t)r * H + c);
+        v[0] = __builtin_fmaf(w, f.x, v[0]);
+        v[1] = __builtin_fmaf(w, f.y, v[1]);
+        v[2] = __builtin_fmaf(w, f.z, v[2]);
+        v[3] = __builtin_fmaf(w, f.w, v[3]);
+    }
+    uint16_t* out = y + t * H + c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = out_bits(v[i], dt);
+}
+
+// ------------------------------------------------------------ sizes of a call
+// Tokens go through in runs of at most kRunPairs pairs: the workspace does not grow beyond that,
+// and offsets of rows of x and h within a run stay below 2^32.
+constexpr int64_t kRunPairs = 65536;
+
+struct ExpertsPlan {
+    int64_t tokens, pairs;                       // of a run
+    int tile_rows, tile_cols, most_tiles;
+    size_t xq, xs, row_of, pos, tiles, ntiles, a, hq, hs, o, bytes;
+};
+
+ExpertsPlan experts_plan(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) {
+    ExpertsPlan p = {};
+    int64_t most = kRunPairs / k;
+    if (most * H > 0x7fffffffLL) most = 0x7fffffffLL / H;
+    if (most * k * I > 0x7fffffffLL) most = 0x7fffffffLL / (k * I);
+    p.tokens = T < most ? T : most;
+    p.pairs = p.tokens * k;
+    const double rows = (double)p.pairs / (double)E;
+    p.tile_rows = rows <= 24 ? 32 : rows <= 64 ? 64 : 128;
+    p.tile_cols = rows <= 24 ? 64 : 128;
+    p.most_tiles = (int)(p.pairs / p.tile_rows + (p.pairs < E ? p.pairs : E));
+    auto take = [&](size_t n) {
+        const size_t at = p.bytes;
+        p.bytes += (n + 255) & ~(size_t)255;
+        return at;
+    };
+    p.xq = take((size_t)p.tokens * H);
+    p.xs = take((size_t)p.tokens * ((H + 127) / 128) * 4);
+    p.row_of = take((size_t)p.pairs * 4);
+    p.pos = take((size_t)p.pairs * 4);
+    p.tiles = take((size_t)p.most_tiles * 16);
+    p.ntiles = take(4);
+    p.a = take((size_t)p.pairs * 2 * I * 4);
+    p.hq = take((size_t)p.pairs * I);
+    p.hs = take((size_t)p.pairs * (I / 128) * 4);
+    p.o = take((size_t)p.pairs * H * 4);
+    return p;
+}
+
+bool experts_sizes(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) {
+    return T >= 0 && T <= (1 << 26) && k >= 1 && k <= 64 && E >= 1 && E <= kMostExperts && H > 0 && H % 16 == 0 &&
+           H <= WUSH_FP8_MAX_K && I > 0 && I % 128 == 0 && I <= WUSH_FP8_MAX_K;
+}
+
+}  // namespace
+}  // namespace wush
+
+extern "C" {
+
+int wush_moe_route(const void* logits, int dtype, int64_t row_stride, const float* bias, int64_t rows, int64_t experts,
+                   const wush_moe_choice* choice, float* weights, int32_t* ids, hipStream_t stream) {
+    WUSH_REQUIRE(choice && rows >= 0 && rows <= 0x7fffffffLL && experts >= 1 && experts <= WUSH_MOE_MAX_EXPERTS);
+    const wush_moe_choice& c = *choice;
+    WUSH_REQUIRE(dtype == WUSH_DTYPE_BF16 || dtype == WUSH_DTYPE_F16 || dtype == WUSH_DTYPE_F32);
+    WUSH_REQUIRE(c.groups >= 1 && c.groups <= 64 && experts % c.groups == 0 && c.keep_groups >= 1 && c.keep_groups <= c.groups);
+    const int64_t size = experts / c.groups;
+    WUSH_REQUIRE(c.k >= 1 && c.k <= WUSH_MOE_MAX_CHOICES && c.k <= c.keep_groups * size);
+    WUSH_REQUIRE((c.group_best == 1 || c.group_best == 2) && c.group_best <= size);
+    WUSH_REQUIRE(c.scale - c.scale == 0.0f);
+    if (rows == 0) return (int)hipSuccess;
+    WUSH_REQUIRE(logits && weights && ids && (rows == 1 || row_stride >= 0));
+    WUSH_REQUIRE(((uintptr_t)logits & (dtype == WUSH_DTYPE_F32 ? 3u : 1u)) == 0 &&
+                 (((uintptr_t)bias | (uintptr_t)weights | (uintptr_t)ids) & 3u) == 0);
+    wush::RouteArgs a;
+    a.logits = logits;
+    a.stride = rows == 1 ? 0 : row_stride;
+    a.bias = bias;
+    a.weights = weights;
+    a.ids = ids;
+    a.rows = rows;
+    a.E = (int)experts;
+    a.k = c.k;
+    a.groups = c.groups;
+    a.size = (int)size;
+    a.keep = c.keep_groups;
+    a.best = c.group_best;
+    a.lanes = 64;
+    while (a.lanes * c.groups > 64) a.lanes >>= 1;
+    a.sigmoid = c.sigmoid != 0;
+    a.renorm = c.renorm != 0;
+    a.scale = c.scale;
+    if (dtype == WUSH_DTYPE_BF16) return wush::launch_route<WUSH_DTYPE_BF16>(a, stream);
+    if (dtype == WUSH_DTYPE_F16) return wush::launch_route<WUSH_DTYPE_F16>(a, stream);
+    return wush::launch_route<WUSH_DTYPE_F32>(a, stream);
+}
+
+size_t wush_moe_experts_fp8_workspace_bytes(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) {
+    if (!wush::experts_sizes(T, k, E, H, I) || T == 0) return 0;
+    return wush::experts_plan(T, k, E, H, I).bytes;
+}
+
+int wush_moe_experts_fp8(const void* x, int dtype, int64_t row_stride, const float* weights, const int32_t* ids,
+                         const uint8_t* w_up, const float* s_up, const uint8_t* w_down, const float* s_down, void* y,
+                         int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, void* workspace, size_t workspace_bytes,
+                         hipStream_t stream) {
+    WUSH_REQUIRE(wush::experts_sizes(T, k, E, H, I));
+    WUSH_REQUIRE(dtype == WUSH_DTYPE_BF16 || dtype == WUSH_DTYPE_F16);
+    if (T == 0) return (int)hipSuccess;
+    const wush::ExpertsPlan p = wush::experts_plan(T, k, E, H, I);
+    WUSH_REQUIRE(x && weights && ids && w_up && s_up && w_down && s_down && y && workspace && workspace_bytes >= p.bytes);
+    WUSH_REQUIRE((((uintptr_t)x | (uintptr_t)w_up | (uintptr_t)w_down | (uintptr_t)workspace) & 15u) == 0 && ((uintptr_t)y & 1u) == 0);
+    WUSH_REQUIRE((((uintptr_t)weights | (uintptr_t)ids | (uintptr_t)s_up | (uintptr_t)s_down) & 3u) == 0);
+    WUSH_REQUIRE(T == 1 || (row_stride >= 0 && row_stride % 8 == 0));
+    if (T == 1) row_stride = 0;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    const uint16_t* px = static_cast<const uint16_t*>(x);
+    uint16_t* py = static_cast<uint16_t*>(y);
+    int* row_of = reinterpret_cast<int*>(ws + p.row_of);
+    int* pos = reinterpret_cast<int*>(ws + p.pos);
+    int4* tiles = reinterpret_cast<int4*>(ws + p.tiles);
+    int* ntiles = reinterpret_cast<int*>(ws + p.ntiles);
+    float* a = reinterpret_cast<float*>(ws + p.a);
+    float* o = reinterpret_cast<float*>(ws + p.o);
+    for (int64_t t = 0; t < T; t += p.tokens) {
+        const int64_t n = T - t < p.tokens ? T - t : p.tokens;
+        int st = wush_quant_fp8_block(px + t * row_stride, dtype, ws + p.xq, reinterpret_cast<float*>(ws + p.xs), n, H, row_stride, stream);
+        if (st) return st;
+        const int P = (int)(n * k);
+        wush::moe_sort_kernel<<<(unsigned)((P + wush::kSortPairs - 1) / wush::kSortPairs), wush::kSortThreads, 0, stream>>>(
+            ids + t * k, P, (int)k, (int)E, p.tile_rows, row_of, pos, tiles, ntiles);
+        if ((st = (int)hipGetLastError())) return st;
+        wush::Fp8Gemm g = {};
+        g.x = ws + p.xq;
+        g.xs = reinterpret_cast<float*>(ws + p.xs);
+        g.ldx = n;
+        g.w = w_up;
+        g.ws = s_up;
+        g.y = a;
+        g.out = wush::kOutF32;
+        g.M = P;
+        g.N = (int)(2 * I);
+        g.K = (int)H;
+        g.splits = 1;
+        g.tiles = tiles;
+        g.ntiles = ntiles;
+        g.row_of = row_of;
+        g.most_tiles = p.most_tiles;
+        if ((st = wush::launch_gemm_fp8(g, p.tile_rows, p.tile_cols, stream))) return st;
+        const int64_t blocks = ((int64_t)P * (I / 128) + 15) / 16;
+        wush::moe_act_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, stream>>>(
+            a, ws + p.hq, reinterpret_cast<float*>(ws + p.hs), (int)I, p.pairs, tiles, ntiles);
+        if ((st = (int)hipGetLastError())) return st;
+        g.x = ws + p.hq;
+        g.xs = reinterpret_cast<float*>(ws + p.hs);
+        g.ldx = p.pairs;
+        g.w = w_down;
+        g.ws = s_down;
+        g.y = o;
+        g.N = (int)H;
+        g.K = (int)I;
+        g.row_of = nullptr;
+        if ((st = wush::launch_gemm_fp8(g, p.tile_rows, p.tile_cols, stream))) return st;
+        const dim3 grid((unsigned)n, (unsigned)((H / 4 + 255) / 256));
+        wush::moe_sum_kernel<<<grid, 256, 0, stream>>>(o, pos, weights + t * k, py + t * H, dtype, (int)k, (int)H);
+        if ((st = (int)hipGetLastError())) return st;
+    }
+    return (int)hipSuccess;
+}
+
+}  // extern "C"
