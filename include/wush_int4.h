@@ -392,7 +392,7 @@ int wush_quant_fp8_block(const void *x, int dtype, uint8_t *q, float *s, int64_t
  *   y[m][n] = sum_b (sum_{k in b} xq[m][k] wq[n][k]) * xs[b][m] * ws[n / 128][b]
  * sums in fp32, rounded once to `dtype` (bf16 or fp16).  xq (M, K), wq (N, K) codes; xs (K / 128, M), ws
  * (N / 128, K / 128) fp32, sizes rounded up; y (M, N).  M, N up to 2^26, K % 16 == 0, K <= WUSH_FP8_MAX_K;
- * xq and wq 16-byte aligned.  The order of the sums depends on M, N, K and the workspace: of the size asked of
+ * xq and wq 16-byte aligned, and y too where N % 8 == 0.  The order of the sums depends on M, N, K and the workspace: of the size asked of
  * wush_gemm_fp8_workspace_bytes it holds partial sums of a split K; with less, K is not split. */
 size_t wush_gemm_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int wush_gemm_fp8(const uint8_t *xq, const float *xs, const uint8_t *wq, const float *ws, void *y, int dtype,
@@ -441,7 +441,7 @@ int wush_moe_route(const void *logits, int dtype, int64_t row_stride, const floa
  * (E, 2 I / 128, H / 128); w_down (E, H, I), s_down (E, H / 128, I / 128).  Both inner inputs are quantized as by
  * wush_quant_fp8_block, all between in fp32, y rounded once.  H % 16 == 0, I % 128 == 0, E <= 1024, k <= 64.  The workspace is 16-byte
  * aligned, of at least wush_moe_experts_fp8_workspace_bytes. */
-size_t wush_moe_experts_fp8_workspace_bytes(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I);
+size_t wush_moe_experts_fp8_workspace_bytes(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, int dtype);
 int wush_moe_experts_fp8(const void *x, int dtype, int64_t row_stride, const float *weights, const int32_t *ids,
                          const uint8_t *w_up, const float *s_up, const uint8_t *w_down, const float *s_down, void *y,
                          int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, void *workspace,

@@ -130,10 +130,11 @@ def route(x, k, bias=None, sigmoid=False, groups=1, keep=1, best=1, renorm=True,
     return w * scale, ids
 
 
-def experts(x, wts, ids, w_up, s_up, w_down, s_down, matrix=True):
+def experts(x, wts, ids, w_up, s_up, w_down, s_down, up_matrix, down_matrix, rows=0.0):
     """(y, bound of its error before rounding).  The hidden values' codes may fall to either side of a half where the
     kernel's sums leave that open: such a code counts a whole step, and its row's cut products whatever they may (7 of 8
-    products, each by less than 2^-13 of the group's largest)."""
+    products, each by less than 2^-13 of the group's largest).  up_matrix, down_matrix: which products are cut; rows:
+    half a unit, of the value, of the type that experts' rows are kept in."""
     E, N2, H = w_up.shape
     I = N2 // 2
     y = torch.zeros(x.shape, dtype=torch.float64, device=x.device)
@@ -142,7 +143,7 @@ def experts(x, wts, ids, w_up, s_up, w_down, s_down, matrix=True):
         t, j = (ids == e).nonzero(as_tuple=True)
         if not t.numel():
             continue
-        a, ea = product(*quant(x[t]), w_up[e], s_up[e], matrix)
+        a, ea = product(*quant(x[t]), w_up[e], s_up[e], up_matrix)
         g, u, eg, eu = a[:, :I], a[:, I:], ea[:, :I], ea[:, I:]
         h = g * torch.sigmoid(g) * u
         eh = 1.1 * u.abs() * eg + (g * torch.sigmoid(g)).abs() * eu + 1.1 * eg * eu + 2.0 ** -21 * h.abs()
@@ -156,13 +157,13 @@ def experts(x, wts, ids, w_up, s_up, w_down, s_down, matrix=True):
         code = nearest(v)
         step = torch.maximum((hi - code).abs(), (code - lo).abs())
         dh = (step * s + code.abs() * s * (ea_max / amax + 2.0 ** -22)).flatten(-2)
-        o, eo = product(code.flatten(-2), s[..., 0], w_down[e], s_down[e], matrix)
+        o, eo = product(code.flatten(-2), s[..., 0], w_down[e], s_down[e], down_matrix)
         hv = (code * s).flatten(-2).abs()
         wd = (w_down[e].float().double() * spread(s_down[e], H, I)).abs()
         eo = eo + dh @ wd.t()
-        if matrix:
+        if down_matrix:
             eo = eo + (step.amax((1, 2)) > 0)[:, None] * 7 * 2.0 ** -13 * (hv @ wd.t())
         w = wts[t, j].double()[:, None]
         y.index_add_(0, t, o * w)
-        err.index_add_(0, t, (eo + 2.0 ** -22 * o.abs()) * w.abs())
+        err.index_add_(0, t, (eo + (2.0 ** -22 + rows) * o.abs()) * w.abs())
     return y, err

@@ -107,6 +107,22 @@ def test_product(dev, M, N, K):
     check_product(_C, dev, M, N, K)
 
 
+@pytest.mark.parametrize("M,N,K", [(2050, 8200, 128), (4096, 8192, 384), (2049, 12296, 272), (1900, 20480, 1040), (5000, 4104, 512),
+                                   (4097, 4100, 256), (3000, 3333, 144)])
+def test_more_tiles_than_workgroups(dev, M, N, K):
+    # tiles one after another in a workgroup, of one block of K on; rows in every tile
+    from my_int4 import _C
+    g = gen(M + N + K)
+    xq = (torch.randn(M, K, generator=g) * 100).clamp(-448, 448).to(plain.E4M3).to(dev)
+    xs = torch.exp(torch.randn(-(-K // 128), M, generator=g)).to(dev) * 2.0 ** -10
+    w, ws = plain.weights(g, N, K, dev=dev)
+    rows = torch.cat((torch.arange(0, M, 61), torch.tensor([M - 2, M - 1]))).to(dev)
+    for dtype in DTYPES:
+        y = _C.fp8_gemm(xq, xs, w, ws, dtype=dtype)
+        check(y[rows], xq[rows].float().double(), xs.t()[rows].double(), w, ws, (M, N, K))
+        assert torch.equal(y, _C.fp8_gemm(xq, xs, w, ws, dtype=dtype))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("M,N,K", [(1, 70, 96), (1, 4096, 4096), (3, 520, 1024), (7, 33, 16), (12, 515, 8192), (66, 200, 640),
                                    (260, 520, 1024)])

@@ -135,18 +135,22 @@ def check_experts(_C, args):
 
 
 def within(y, args):
-    """The bound of exact products (few tokens), or of the matrix instruction's; both say something: they are
-    a small part of the outputs."""
-    both = [plain.experts(*args, matrix=m) for m in (True, False)]
-    for ref, err in both:
-        assert float(err.norm()) <= 0.03 * float(ref.norm())
-    assert min(plain.off(y, ref, err, y.dtype) for ref, err in both) <= 1
+    """The bound of one of the three ways: all products exact (few tokens); the down projection's cut; both's, and an
+    expert's rows kept in fp16.  Each says something: it is a small part of the outputs (a single token whose one
+    open code lets all of a row's cut products count: 7 * 2^-13 * sum |h w| / |y|, some 2% for hundreds of terms, and the code)."""
+    ratios = []
+    for way in ((False, False), (False, True), (True, True, 2.0 ** -11)):
+        ref, err = plain.experts(*args, *way)
+        assert float(err.norm()) <= 0.1 * float(ref.norm())
+        ratios.append(plain.off(y, ref, err, y.dtype))
+    assert min(ratios) <= 1, ratios
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T,E,k,H,I", [(1, 1, 1, 16, 128), (1, 8, 2, 256, 128), (1, 64, 6, 1024, 384), (2, 16, 4, 272, 128), (4, 8, 8, 512, 256),
                                        (5, 40, 3, 1040, 256), (33, 16, 2, 512, 384), (64, 64, 8, 768, 128), (200, 8, 2, 640, 256),
-                                       (300, 4, 1, 400, 128), (777, 16, 4, 256, 256), (513, 3, 2, 1024, 512), (1500, 2, 1, 512, 128)])
+                                       (300, 4, 1, 400, 128), (777, 16, 4, 256, 256), (513, 3, 2, 1024, 512), (1500, 2, 1, 512, 128),
+                                       (2000, 6, 3, 656, 640), (3100, 40, 2, 128, 2048)])
 def test_experts(dev, dtype, T, E, k, H, I):
     from my_int4 import _C
     args = case(T + E + H, T, E, k, H, I, dev, dtype)

@@ -70,7 +70,7 @@ SIGNATURES = {
     "wush_linear_fp8_workspace_bytes": ([_I64, _I64, _I64], _SZ),
     "wush_linear_fp8": ([_P, _I64, _P, _P, _P, _I, _I64, _I64, _I64, _P, _SZ, _P], _I),
     "wush_moe_route": ([_P, _I, _I64, _P, _I64, _I64, ctypes.POINTER(MoeChoice), _P, _P, _P], _I),
-    "wush_moe_experts_fp8_workspace_bytes": ([_I64, _I64, _I64, _I64, _I64], _SZ),
+    "wush_moe_experts_fp8_workspace_bytes": ([_I64, _I64, _I64, _I64, _I64, _I], _SZ),
     "wush_moe_experts_fp8": ([_P, _I, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _SZ, _P], _I),
 }
 

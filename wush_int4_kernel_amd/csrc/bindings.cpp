@@ -730,7 +730,7 @@ torch::Tensor fp8_experts(torch::Tensor x, torch::Tensor weights, torch::Tensor 
     int64_t rows, stride;
     const auto xr = token_rows(x, rows, stride);
     auto y = new_tensor(x.sizes(), x.scalar_type(), x);
-    const size_t wsb = wush_moe_experts_fp8_workspace_bytes(T, k, E, H, I);
+    const size_t wsb = wush_moe_experts_fp8_workspace_bytes(T, k, E, H, I, dt);
     auto work = bytes_like(wsb, x);
     check_status(wush_moe_experts_fp8(xr.data_ptr(), dt, stride, ptr<float>(weights), ptr<int32_t>(ids), ptr<uint8_t>(w_up),
                                       ptr<float>(s_up), ptr<uint8_t>(w_down), ptr<float>(s_down), y.data_ptr(), T, k, E, H, I,

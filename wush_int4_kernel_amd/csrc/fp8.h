@@ -9,7 +9,9 @@ namespace wush {
 
 constexpr int kFp8Block = 128;                   // channels (and weight rows) that share a scale
 
-constexpr int kOutF32 = 2;                       // beside WUSH_DTYPE_BF16 and WUSH_DTYPE_F16
+// Types of y beside WUSH_DTYPE_BF16 and WUSH_DTYPE_F16; kOutShared: fp16 with a power of two for each
+// row's 64 columns.
+constexpr int kOutF32 = 2, kOutShared = 3;
 
 // y = x w^T of one matrix, or of one for each expert.
 struct Fp8Gemm {
@@ -28,15 +30,31 @@ struct Fp8Gemm {
     const int* ntiles;
     const int* row_of;
     int most_tiles;
+    // experts' outputs: fp32; act: codes of silu(gate) * up, N / 2 a row, with their scales in hs (N / 256, ldh);
+    // shared: fp16, with powers of two in hs (rows, N / 64)
+    int act, shared;
+    float* hs;
+    int64_t ldh;
+    int wide;                                    // products in fp16 matrix instructions, which cut none
 };
 
 struct Fp8Tile {
     int rows, cols, depth;
+    bool runs;                                   // N % 8 == 0 only
     double stage;                                // us that a K block takes a workgroup on a full chip
 };
-constexpr Fp8Tile kFp8Tiles[] = {{256, 256, 2, 1.6}, {128, 128, 4, 0.6}, {64, 128, 3, 0.43}, {32, 128, 3, 0.39}, {32, 64, 4, 0.2}};
+constexpr Fp8Tile kFp8Tiles[] = {{256, 256, 2, false, 1.5}, {128, 256, 3, true, 0.85}, {128, 128, 4, false, 0.6},
+                                 {64, 128, 3, false, 0.43}, {32, 128, 3, false, 0.39}, {32, 64, 4, false, 0.2}};
 
 // Tiles of tile_rows x tile_cols, one of kFp8Tiles; K % 16 == 0.
 int launch_gemm_fp8(const Fp8Gemm& g, int tile_rows, int tile_cols, hipStream_t stream);
+
+// The same over experts, fp32 out: tiles of 32 x 64, 64 x 128, 128 x 128.
+int launch_gemm_fp8_rows(const Fp8Gemm& g, int tile_rows, int tile_cols, hipStream_t stream);
+
+// Tiles of 128 x 256 by workgroups that take one after another: one matrix with N % 8 == 0 and
+// 16-byte aligned y, or experts with act or shared.
+constexpr int kFp8Workgroups = 256;              // one for each of the chip's CUs
+int launch_gemm_fp8_runs(const Fp8Gemm& g, hipStream_t stream);
 
 }  // namespace wush

@@ -72,9 +72,9 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, size_t room) {
     const int64_t stages = (K + 127) / 128;
     double least = 1e30;
     for (const auto& t : kFp8Tiles) {
-        if (t.rows > 32 && t.rows >= 2 * M) continue;
+        if ((t.rows > 32 && t.rows >= 2 * M) || (t.runs && N % 8 != 0)) continue;
         const int64_t tiles = ((M + t.rows - 1) / t.rows) * ((N + t.cols - 1) / t.cols);
-        for (int s = 1; s <= 8 && (s == 1 || stages / s >= 4); ++s) {
+        for (int s = 1; s <= 8 && (s == 1 || (stages / s >= 4 && t.cols < 256)); ++s) {
             if (s > 1 && (size_t)M * N * 4 * s > room) break;
             const double groups = (double)tiles * s, full = groups / 256 < 1 ? groups / 256 : 1;
             const double rounds = groups <= 1024 ? (double)(int64_t)((groups + 255) / 256) : groups / 256;
@@ -138,7 +138,7 @@ int wush_gemm_fp8(const uint8_t* xq, const float* xs, const uint8_t* wq, const f
     WUSH_REQUIRE(dtype == WUSH_DTYPE_BF16 || dtype == WUSH_DTYPE_F16);
     if (M == 0 || N == 0) return (int)hipSuccess;
     WUSH_REQUIRE(xq && xs && wq && ws && y);
-    WUSH_REQUIRE((((uintptr_t)xq | (uintptr_t)wq) & 15u) == 0 && (((uintptr_t)xs | (uintptr_t)ws) & 3u) == 0 && ((uintptr_t)y & 1u) == 0);
+    WUSH_REQUIRE((((uintptr_t)xq | (uintptr_t)wq) & 15u) == 0 && (((uintptr_t)xs | (uintptr_t)ws) & 3u) == 0 && ((uintptr_t)y & (N % 8 == 0 ? 15u : 1u)) == 0);
     const bool usable = workspace && ((uintptr_t)workspace & 15u) == 0;
     const wush::Plan p = wush::plan_of(M, N, K, usable ? workspace_bytes : 0);
     wush::Fp8Gemm g = {};
@@ -154,6 +154,7 @@ int wush_gemm_fp8(const uint8_t* xq, const float* xs, const uint8_t* wq, const f
     g.N = (int)N;
     g.K = (int)K;
     g.splits = p.splits;
+    if (p.rows == 128 && p.cols == 256) return wush::launch_gemm_fp8_runs(g, stream);
     return wush::launch_gemm_fp8(g, p.rows, p.cols, stream);
 }
 

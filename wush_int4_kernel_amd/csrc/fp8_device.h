@@ -33,6 +33,24 @@ __device__ __forceinline__ uint32_t fp8_codes4(float a, float b, float c, float 
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(fp8_arg(c, amax), fp8_arg(d, amax), p, true);
 }
 
+// The same for values that are sums in fp32: a product with the rounded quotient 448 / A, off by less than
+// 2^-22 of a code's value, since nothing puts such values onto the halves.
+__device__ __forceinline__ float fp8_factor(float amax) { return kFp8Largest / amax; }
+__device__ __forceinline__ uint32_t fp8_codes4_by(float a, float b, float c, float d, float factor) {
+    if (factor != factor) return 0;
+    int p = __builtin_amdgcn_cvt_pk_fp8_f32(a * factor, b * factor, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * factor, d * factor, p, true);
+}
+
+// x / (1 + exp(-x)): the hardware's exponential and reciprocal, each good to an ulp, with the exponent's
+// rounding made up for, within 2^-21
+__device__ __forceinline__ float fp8_silu(float x) {
+    const float hi = x * -1.44269504f, lo = __builtin_fmaf(x, -1.44269504f, -hi) - x * 1.92596303e-8f;
+    const float e = __builtin_amdgcn_exp2f(hi);
+    // 0 and infinity as they are
+    return x * __builtin_amdgcn_rcpf(1.0f + (__builtin_fabsf(hi) < 126.0f ? __builtin_fmaf(e, lo * 0.693147182f, e) : e));
+}
+
 // maximum over the 16 lanes of a row (of a block, where a lane holds 8 channels)
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {

@@ -11,6 +11,7 @@
 // column, by the next stage's.  The multiply-adds run kLag products behind the MFMAs, so that
 // none waits for its result.
 #include "fp8.h"
+#include "fp8_device.h"
 #include "gemm_h16_device.h"
 #include "../../include/wush_int4.h"
 
@@ -45,7 +46,10 @@ __device__ __forceinline__ void wait_all_but(int stages) {
     }
 }
 
-template <int RB, int CB, int WR, int WC, int NB, int BR, int OCC, int OUT, bool GROUPED>
+// kPlain: one matrix.  kRows: each expert's, over its rows.
+enum { kPlain, kRows };
+
+template <int RB, int CB, int WR, int WC, int NB, int BR, int OCC, int MODE, int OUT, bool F16>
 __global__ __launch_bounds__(64 * WR * WC) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
 void gemm_fp8_kernel(const Fp8Gemm g) {
     constexpr int NW = WR * WC, TR = 16 * RB * WR, TC = 16 * CB * WC;
@@ -53,6 +57,7 @@ void gemm_fp8_kernel(const Fp8Gemm g) {
     constexpr int kChunksA = (TR + 63) / 64;                     // wavefronts that fetch x's scales, the others w's
     constexpr int kA = TR * 128, kSx = kA + TC * 128, kSw = kSx + kChunksA * 256, kBuf = kSw + 256;
     constexpr int kStage = NW * (16 * RB) * (32 * CB);           // outputs staged, 32 CB bytes a row
+    constexpr bool GROUPED = MODE != kPlain;
     constexpr int kSmem = NB * kBuf > kStage ? NB * kBuf : kStage;
     constexpr int kMf = RB * CB, kLag = 3, kTmp = 4;
     static_assert(DA * 8 * NW == TR && DB * 8 * NW == TC && kChunksA < NW && CB % BR == 0 && BR >= 2 && CB >= 2);
@@ -71,7 +76,12 @@ void gemm_fp8_kernel(const Fp8Gemm g) {
     if constexpr (GROUPED) {
         const int NR = *g.ntiles;
         if ((int)blockIdx.x >= NR * NC) return;
-        h16_tile((int)blockIdx.x, NR, NC, tm, tn);
+        // An XCD (workgroups i, i + 8, ...) takes a run of row tiles, all columns of one
+        // before the next: an expert's row tiles share its weights in the XCD's L2.
+        const int q = (NR * NC) >> 3, r = (NR * NC) & 7, xcd = (int)blockIdx.x & 7;
+        const int s = xcd * q + min(xcd, r) + ((int)blockIdx.x >> 3);
+        tm = s / NC;
+        tn = s - tm * NC;
         const int4 t = g.tiles[tm];
         m0 = __builtin_amdgcn_readfirstlane(t.y);
         M = __builtin_amdgcn_readfirstlane(t.z);
@@ -155,9 +165,9 @@ void gemm_fp8_kernel(const Fp8Gemm g) {
         else dma16_uniform(bbase + o, v, dst + kA + (wave * DB + k - DA) * 1024);
     };
 
-    v4f acc[RB][CB], tmp[kTmp];
+    v4f acc[RB][CB];
     v8i a[RB], b[BR];
-    float sc[RB], old[RB];                       // product of the scales: this stage's, the last one's
+    float sc[RB], old[RB];                       // products of the scales: this stage's, the last one's
     const int fsw = (l16 >> 1) & 7;
     const uint8_t* arow = smem + (wr * RB * 16 + l16) * 128;
     const uint8_t* brow = smem + kA + (wc * CB * 16 + l16) * 128;
@@ -187,8 +197,6 @@ void gemm_fp8_kernel(const Fp8Gemm g) {
 #pragma unroll
         for (int j = 0; j < CB; ++j) acc[i][j] = (v4f){0, 0, 0, 0};
     }
-#pragma unroll
-    for (int t = 0; t < kTmp; ++t) tmp[t] = (v4f){0, 0, 0, 0};
     wait_all_but<ND, NB - 1>(last - first - 1);
     WUSH_LDS_BARRIER();
     __builtin_amdgcn_sched_barrier(0);
@@ -201,15 +209,8 @@ void gemm_fp8_kernel(const Fp8Gemm g) {
 
     int buf = 0;                                 // LDS buffer of stage st
     int st = first;
-    auto add = [&](int m, const float (&s)[RB]) {
-        const int i = m % RB, j = m / RB;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(tmp[m % kTmp][r], s[i], acc[i][j][r]);
-    };
-    // one stage; REFILL: its buffer takes stage st + NB.  Operands read past the
-    // last stage are what the buffer happens to hold, and are not used.
-    auto stage = [&](auto refill) {
-        const int nbuf = buf + 1 == NB ? 0 : buf + 1;
+    // what both forms of a stage begin with
+    auto begin = [&] {
 #pragma unroll
         for (int i = 0; i < RB; ++i) {
             old[i] = sc[i];
@@ -224,37 +225,117 @@ void gemm_fp8_kernel(const Fp8Gemm g) {
                 a[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
             }
         }
-        static_for<kMf>([&](auto mc) {
-            constexpr int m = mc.value, i = m % RB, j = m / RB;
-            if constexpr (i == 0 && j == CB - BR + 1) {
-                // stage st + 1 has landed in all wavefronts' view, and all have read this one's columns
-                if constexpr (refill.value) WUSH_WAIT_VMCNT((NB - 2) * ND);
-                else wait_all_but<ND, NB - 2>(last - st - 2);
-                WUSH_LDS_BARRIER();
+    };
+    // stage st + 1 has landed in all wavefronts' view, and all have read this one's columns
+    auto landed = [&](auto refill) {
+        if constexpr (refill.value) WUSH_WAIT_VMCNT((NB - 2) * ND);
+        else wait_all_but<ND, NB - 2>(last - st - 2);
+        WUSH_LDS_BARRIER();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // share q of n of the refill's DMAs
+    auto refill_part = [&](auto qc, auto nc) {
+        constexpr int q = qc.value, n = nc.value;
+        static_for<(q + 1) * ND / n - q * ND / n>([&](auto dc) { issue(st + NB, buf, q * ND / n + dc.value); });
+    };
+    constexpr int kTurn = CB - BR + 1;           // the column from which on the next stage is read
+    if constexpr (!F16) {
+        v4f tmp[kTmp];
+#pragma unroll
+        for (int t = 0; t < kTmp; ++t) tmp[t] = (v4f){0, 0, 0, 0};
+        auto add = [&](int m, const float (&s)[RB]) {
+            const int i = m % RB, j = m / RB;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(tmp[m % kTmp][r], s[i], acc[i][j][r]);
+        };
+        // one stage; REFILL: its buffer takes stage st + NB.  Operands read past the
+        // last stage are what the buffer happens to hold, and are not used.
+        auto stage = [&](auto refill) {
+            const int nbuf = buf + 1 == NB ? 0 : buf + 1;
+            begin();
+            static_for<kMf>([&](auto mc) {
+                constexpr int m = mc.value, i = m % RB, j = m / RB;
+                if constexpr (i == 0 && j == kTurn) landed(refill);
+                tmp[m % kTmp] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j % BR], a[i], (v4f){0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+                if constexpr (i == 0) {
+                    constexpr int jn = j + BR - 1;
+                    if constexpr (jn < CB) read_b(buf, jn);
+                    else read_b(nbuf, jn - CB);
+                }
+                if constexpr (j == CB - 1) read_a(nbuf, i);
+                if constexpr (m == kMf - 1) read_s(nbuf);
+                if constexpr (m >= kLag) add(m - kLag, sc);
+                else add(kMf + m - kLag, old);
+                if constexpr (refill.value && j >= kTurn)
+                    refill_part(std::integral_constant<int, m - kTurn * RB>{}, std::integral_constant<int, (BR - 1) * RB>{});
                 __builtin_amdgcn_sched_barrier(0);
+            });
+            buf = nbuf;
+        };
+        for (; st + NB < last; ++st) stage(std::true_type{});
+        for (; st < last; ++st) stage(std::false_type{});
+#pragma unroll
+        for (int m = kMf - kLag; m < kMf; ++m) add(m, sc);
+    } else {
+        // Operands widened to fp16, which is exact, and four v_mfma_f32_16x16x32_f16 a block; a column's
+        // multiply-adds run behind the next column's MFMAs.
+        v4f tmp[2][RB];
+        h8 wa[RB][4], wb[4];
+#pragma unroll
+        for (int i = 0; i < RB; ++i) tmp[(CB - 1) & 1][i] = (v4f){0, 0, 0, 0};
+        auto widen = [&](const v8i& v, h8 (&o)[4]) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                h2 p[4];
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    p[2 * d] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[2 * q + d], 1.0f, false);
+                    p[2 * d + 1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[2 * q + d], 1.0f, true);
+                }
+                o[q] = (h8){p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
             }
-            tmp[m % kTmp] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j % BR], a[i], (v4f){0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
-            if constexpr (i == 0) {
-                constexpr int jn = j + BR - 1;
+        };
+        auto add = [&](int j, int i, const float (&s)[RB]) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(tmp[j & 1][i][r], s[i], acc[i][j][r]);
+        };
+        auto stage = [&](auto refill) {
+            const int nbuf = buf + 1 == NB ? 0 : buf + 1;
+            begin();
+#pragma unroll
+            for (int i = 0; i < RB; ++i) widen(a[i], wa[i]);
+            static_for<CB>([&](auto jc) {
+                constexpr int j = jc.value, jn = j + BR - 1;
+                if constexpr (j == kTurn) {
+                    landed(refill);
+#pragma unroll
+                    for (int i = 0; i < RB; ++i) read_a(nbuf, i);
+                    read_s(nbuf);
+                }
+                widen(b[j % BR], wb);
                 if constexpr (jn < CB) read_b(buf, jn);
                 else read_b(nbuf, jn - CB);
-            }
-            if constexpr (j == CB - 1) read_a(nbuf, i);
-            if constexpr (m == kMf - 1) read_s(nbuf);
-            if constexpr (m >= kLag) add(m - kLag, sc);
-            else add(kMf + m - kLag, old);
-            if constexpr (refill.value && j >= CB - BR + 1) {
-                constexpr int n = (BR - 1) * RB, q = m - (CB - BR + 1) * RB;
-                static_for<(q + 1) * ND / n - q * ND / n>([&](auto dc) { issue(st + NB, buf, q * ND / n + dc.value); });
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        });
-        buf = nbuf;
-    };
-    for (; st + NB < last; ++st) stage(std::true_type{});
-    for (; st < last; ++st) stage(std::false_type{});
+                __builtin_amdgcn_sched_barrier(0);
+                static_for<4 * RB>([&](auto mc) {
+                    constexpr int q = mc.value / RB, i = mc.value % RB;
+                    tmp[j & 1][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wb[q], wa[i][q], q ? tmp[j & 1][i] : (v4f){0, 0, 0, 0}, 0, 0, 0);
+                    if constexpr (q == 1) {
+                        if constexpr (j > 0) add(j - 1, i, sc);
+                        else add(CB - 1, i, old);
+                    }
+                    if constexpr (refill.value && j >= kTurn)
+                        refill_part(std::integral_constant<int, (j - kTurn) * 4 * RB + mc.value>{},
+                                    std::integral_constant<int, (BR - 1) * 4 * RB>{});
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+            });
+            buf = nbuf;
+        };
+        for (; st + NB < last; ++st) stage(std::true_type{});
+        for (; st < last; ++st) stage(std::false_type{});
 #pragma unroll
-    for (int m = kMf - kLag; m < kMf; ++m) add(m, sc);
+        for (int i = 0; i < RB; ++i) add(CB - 1, i, sc);
+    }
     WUSH_WAIT_VMCNT(0);
     __syncthreads();
 
@@ -334,31 +415,53 @@ __global__ __launch_bounds__(256) void fp8_sum_kernel(const float* __restrict__ 
 }
 
 template <int RB, int CB, int WR, int WC, int NB, int BR, int OCC>
-void launch_tile(const Fp8Gemm& g, unsigned grid, hipStream_t stream) {
+int launch_plain(const Fp8Gemm& g, unsigned grid, hipStream_t stream) {
     constexpr int T = 64 * WR * WC;
-    if (g.tiles) gemm_fp8_kernel<RB, CB, WR, WC, NB, BR, OCC, kOutF32, true><<<grid, T, 0, stream>>>(g);
-    else if (g.out == WUSH_DTYPE_BF16) gemm_fp8_kernel<RB, CB, WR, WC, NB, BR, OCC, WUSH_DTYPE_BF16, false><<<grid, T, 0, stream>>>(g);
-    else gemm_fp8_kernel<RB, CB, WR, WC, NB, BR, OCC, WUSH_DTYPE_F16, false><<<grid, T, 0, stream>>>(g);
+    if (g.out == WUSH_DTYPE_BF16)
+        gemm_fp8_kernel<RB, CB, WR, WC, NB, BR, OCC, kPlain, WUSH_DTYPE_BF16, false><<<grid, T, 0, stream>>>(g);
+    else
+        gemm_fp8_kernel<RB, CB, WR, WC, NB, BR, OCC, kPlain, WUSH_DTYPE_F16, false><<<grid, T, 0, stream>>>(g);
+    return (int)hipGetLastError();
+}
+
+template <int RB, int CB, int WR, int WC, int NB, int BR>
+int launch_rows(const Fp8Gemm& g, unsigned grid, hipStream_t stream) {
+    constexpr int T = 64 * WR * WC;
+    if (g.wide) gemm_fp8_kernel<RB, CB, WR, WC, NB, BR, 1, kRows, kOutF32, true><<<grid, T, 0, stream>>>(g);
+    else gemm_fp8_kernel<RB, CB, WR, WC, NB, BR, 1, kRows, kOutF32, false><<<grid, T, 0, stream>>>(g);
+    return (int)hipGetLastError();
 }
 
 }  // namespace
 
-int launch_gemm_fp8(const Fp8Gemm& g, int tile_rows, int tile_cols, hipStream_t stream) {
-    WUSH_REQUIRE(g.M > 0 && g.N > 0 && g.K > 0 && g.K % 16 == 0 && g.splits >= 1 && g.splits <= (g.K + 127) / 128);
-    WUSH_REQUIRE(g.splits == 1 || (!g.tiles && g.part));
-    const long long rows = g.tiles ? g.most_tiles : (g.M + tile_rows - 1) / tile_rows;
-    const long long tiles = rows * ((g.N + tile_cols - 1) / tile_cols) * g.splits;
-    WUSH_REQUIRE(tiles <= 0x7fffffffLL);
-    const unsigned grid = (unsigned)tiles;
+int launch_gemm_fp8_rows(const Fp8Gemm& g, int tile_rows, int tile_cols, hipStream_t stream) {
+    const long long cols = (g.N + tile_cols - 1) / tile_cols;
+    WUSH_REQUIRE(g.tiles && g.ntiles && g.N > 0 && g.K > 0 && g.K % 16 == 0 && g.splits == 1 && !g.act && !g.shared);
+    WUSH_REQUIRE(g.most_tiles * cols < (1 << 23));               // a launch has fewer than 2^32 threads
+    const unsigned grid = (unsigned)(g.most_tiles * cols);
     switch (tile_rows << 16 | tile_cols) {
-        case 256 << 16 | 256: launch_tile<4, 8, 4, 2, 2, 4, 2>(g, grid, stream); break;
-        case 128 << 16 | 128: launch_tile<4, 4, 2, 2, 4, 4, 1>(g, grid, stream); break;
-        case 64 << 16 | 128: launch_tile<2, 4, 2, 2, 3, 4, 1>(g, grid, stream); break;
-        case 32 << 16 | 128: launch_tile<1, 4, 2, 2, 3, 4, 1>(g, grid, stream); break;
-        case 32 << 16 | 64: launch_tile<2, 2, 1, 2, 4, 2, 1>(g, grid, stream); break;
+        case 128 << 16 | 128: return launch_rows<4, 4, 2, 2, 4, 4>(g, grid, stream);
+        case 64 << 16 | 128: return launch_rows<2, 4, 2, 2, 3, 4>(g, grid, stream);
+        case 32 << 16 | 64: return launch_rows<2, 2, 1, 2, 4, 2>(g, grid, stream);
         default: return (int)hipErrorInvalidValue;
     }
-    const int st = (int)hipGetLastError();
+}
+
+int launch_gemm_fp8(const Fp8Gemm& g, int tile_rows, int tile_cols, hipStream_t stream) {
+    WUSH_REQUIRE(g.M > 0 && g.N > 0 && g.K > 0 && g.K % 16 == 0 && g.splits >= 1 && g.splits <= (g.K + 127) / 128);
+    WUSH_REQUIRE(!g.tiles && (g.splits == 1 || g.part));
+    const long long tiles = (long long)((g.M + tile_rows - 1) / tile_rows) * ((g.N + tile_cols - 1) / tile_cols) * g.splits;
+    WUSH_REQUIRE(tiles < (1 << 23));                             // a launch has fewer than 2^32 threads
+    const unsigned grid = (unsigned)tiles;
+    int st;
+    switch (tile_rows << 16 | tile_cols) {
+        case 256 << 16 | 256: st = launch_plain<4, 8, 4, 2, 2, 4, 2>(g, grid, stream); break;
+        case 128 << 16 | 128: st = launch_plain<4, 4, 2, 2, 4, 4, 1>(g, grid, stream); break;
+        case 64 << 16 | 128: st = launch_plain<2, 4, 2, 2, 3, 4, 1>(g, grid, stream); break;
+        case 32 << 16 | 128: st = launch_plain<1, 4, 2, 2, 3, 4, 1>(g, grid, stream); break;
+        case 32 << 16 | 64: st = launch_plain<2, 2, 1, 2, 4, 2, 1>(g, grid, stream); break;
+        default: return (int)hipErrorInvalidValue;
+    }
     if (st || g.splits == 1) return st;
     const size_t total = (size_t)g.M * g.N;
     const int e = g.N % 4 == 0 ? 4 : 1;

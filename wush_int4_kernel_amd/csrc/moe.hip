@@ -206,13 +206,21 @@ __global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(const int32_t* _
     const int tid = threadIdx.x, first = blockIdx.x * kSortPairs;
     all[tid] = before[tid] = 0;
     __syncthreads();
-    int mine = -1;
-    for (int p = tid; p < P; p += kSortThreads) {
-        const int e = ids[p];
-        if ((unsigned)e >= (unsigned)E) continue;
-        if (p >= first && p < first + kSortPairs) mine = e;
-        else if (p < first) atomicAdd(&before[e], 1);
-        else atomicAdd(&all[e], 1);
+    const int own = first + tid < P ? ids[first + tid] : -1;
+    const int mine = (unsigned)own < (unsigned)E ? own : -1;
+    constexpr int kAhead = 8;                    // loads in flight
+    for (int p0 = 0; p0 < P; p0 += kAhead * kSortThreads) {
+        int e[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int p = p0 + u * kSortThreads + tid;
+            e[u] = p < P ? ids[p] : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int run = p0 + u * kSortThreads;               // one workgroup's
+            if (run != first && (unsigned)e[u] < (unsigned)E) atomicAdd(run < first ? &before[e[u]] : &all[e[u]], 1);
+        }
     }
     __syncthreads();
     int rank = 0;                                // among the expert's pairs up to this workgroup's
@@ -275,11 +283,11 @@ __global__ __launch_bounds__(256) void moe_act_kernel(const float* __restrict__ 
         const float up[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = gate[i] / (1.0f + expf(-gate[i])) * up[i];
-        const float amax = fp8_amax(row16_max(fp8_largest8(v)));
+        for (int i = 0; i < 8; ++i) v[i] = fp8_silu(gate[i]) * up[i];
+        const float amax = fp8_amax(row16_max(fp8_largest8(v))), factor = fp8_factor(amax);
         if (l16 == 0) s[b * ld + row] = fp8_scale(amax);
         *reinterpret_cast<uint2*>(q + row * I + c) =
-            make_uint2(fp8_codes4(v[0], v[1], v[2], v[3], amax), fp8_codes4(v[4], v[5], v[6], v[7], amax));
+            make_uint2(fp8_codes4_by(v[0], v[1], v[2], v[3], factor), fp8_codes4_by(v[4], v[5], v[6], v[7], factor));
     }
 }
 
@@ -287,27 +295,41 @@ __device__ __forceinline__ uint16_t out_bits(float f, int dt) {
     return dt == WUSH_DTYPE_F16 ? f32_to_f16_bits(f) : (uint16_t)(f != f ? 0x7fc0u : f32_to_bf16_rne(f));
 }
 
-// y of a token: the sum of its experts' rows, in the order of its choices
-__global__ __launch_bounds__(256) void moe_sum_kernel(const float* __restrict__ o, const int* __restrict__ pos,
-                                                      const float* __restrict__ weights, uint16_t* __restrict__ y, int dt,
-                                                      int k, int H) {
-    const int64_t t = blockIdx.x;
-    const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
-    if (c >= H) return;
-    float v[4] = {0, 0, 0, 0};
+// y of a token: the sum of its experts' rows, in the order of its choices; 8 columns a thread.
+// SHARED: rows are fp16 with a power of two for each 64 columns.
+template <bool SHARED>
+__global__ __launch_bounds__(256) void moe_sum_kernel(const void* __restrict__ o, const float* __restrict__ os,
+                                                      const int* __restrict__ pos, const float* __restrict__ weights,
+                                                      uint16_t* __restrict__ y, int dt, int64_t T, int k, int H) {
+    const int units = H >> 3;
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t t = at / units;
+    if (t >= T) return;
+    const int c = (int)(at - t * units) * 8;
+    float v[8] = {};
     for (int j = 0; j < k; ++j) {
         const int r = pos[t * k + j];
         if (r < 0) continue;
-        const float w = weights[t * k + j];
-        const float4 f = *reinterpret_cast<const float4*>(o + (int64_t)r * H + c);
-        v[0] = __builtin_fmaf(w, f.x, v[0]);
-        v[1] = __builtin_fmaf(w, f.y, v[1]);
-        v[2] = __builtin_fmaf(w, f.z, v[2]);
-        v[3] = __builtin_fmaf(w, f.w, v[3]);
-    }
-    uint16_t* out = y + t * H + c;
+        float w = weights[t * k + j], f[8];
+        if constexpr (SHARED) {
+            w *= os[(int64_t)r * ((H + 63) >> 6) + (c >> 6)];
+            fp8_unpack8<WUSH_DTYPE_F16>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(o) + (int64_t)r * H + c), f);
+        } else {
+            const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(o) + (int64_t)r * H + c);
+            const float4 a = p[0], b = p[1];
+            f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+        }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = out_bits(v[i], dt);
+        for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(w, f[i], v[i]);
+    }
+    uint32_t out[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = out_bits(v[2 * i], dt) | (uint32_t)out_bits(v[2 * i + 1], dt) << 16;
+    uint16_t* p = y + t * H + c;
+    if ((reinterpret_cast<uintptr_t>(y) & 15u) == 0) *reinterpret_cast<uint4*>(p) = make_uint4(out[0], out[1], out[2], out[3]);
+    else
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = (uint16_t)(out[i >> 1] >> (16 * (i & 1)));
 }
 
 // ------------------------------------------------------------ sizes of a call
@@ -317,11 +339,19 @@ constexpr int64_t kRunPairs = 65536;
 
 struct ExpertsPlan {
     int64_t tokens, pairs;                       // of a run
+    bool fused;
     int tile_rows, tile_cols, most_tiles;
-    size_t xq, xs, row_of, pos, tiles, ntiles, a, hq, hs, o, bytes;
+    size_t xq, xs, row_of, pos, tiles, ntiles, a, hq, hs, o, os, bytes;
 };
 
-ExpertsPlan experts_plan(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) {
+// Two ways.  Fused: tiles of 128 x 256 on e4m3 matrix instructions, whose epilogue makes the hidden codes, and
+// outputs in fp16 with shared powers of two: for many rows an expert, where operations and the traffic of
+// intermediate rows bound the time, and for bf16 only.  The e4m3 instruction cuts small products next
+// to large ones (at 2^-13 of the largest of 8), which turns one in some thousand of the hidden codes to
+// the other side of a half: 1.2e-3 of the output, below bf16's rounding (1.7e-3), above fp16's (2.1e-4).
+// Otherwise the gate and up projections take fp16 matrix instructions, at half the rate where the
+// weights' stream bounds the time anyway, and intermediate rows are fp32.
+ExpertsPlan experts_plan(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, int dtype) {
     ExpertsPlan p = {};
     int64_t most = kRunPairs / k;
     if (most * H > 0x7fffffffLL) most = 0x7fffffffLL / H;
@@ -329,8 +359,9 @@ ExpertsPlan experts_plan(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) 
     p.tokens = T < most ? T : most;
     p.pairs = p.tokens * k;
     const double rows = (double)p.pairs / (double)E;
+    p.fused = rows > 64 && dtype == WUSH_DTYPE_BF16;
     p.tile_rows = rows <= 24 ? 32 : rows <= 64 ? 64 : 128;
-    p.tile_cols = rows <= 24 ? 64 : 128;
+    p.tile_cols = p.fused ? 256 : rows <= 24 ? 64 : 128;
     p.most_tiles = (int)(p.pairs / p.tile_rows + (p.pairs < E ? p.pairs : E));
     auto take = [&](size_t n) {
         const size_t at = p.bytes;
@@ -343,10 +374,11 @@ ExpertsPlan experts_plan(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) 
     p.pos = take((size_t)p.pairs * 4);
     p.tiles = take((size_t)p.most_tiles * 16);
     p.ntiles = take(4);
-    p.a = take((size_t)p.pairs * 2 * I * 4);
+    p.a = take(p.fused ? 0 : (size_t)p.pairs * 2 * I * 4);
     p.hq = take((size_t)p.pairs * I);
     p.hs = take((size_t)p.pairs * (I / 128) * 4);
-    p.o = take((size_t)p.pairs * H * 4);
+    p.o = take((size_t)p.pairs * H * (p.fused ? 2 : 4));
+    p.os = take(p.fused ? (size_t)p.pairs * ((H + 63) / 64) * 4 : 0);
     return p;
 }
 
@@ -397,9 +429,9 @@ int wush_moe_route(const void* logits, int dtype, int64_t row_stride, const floa
     return wush::launch_route<WUSH_DTYPE_F32>(a, stream);
 }
 
-size_t wush_moe_experts_fp8_workspace_bytes(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) {
+size_t wush_moe_experts_fp8_workspace_bytes(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, int dtype) {
     if (!wush::experts_sizes(T, k, E, H, I) || T == 0) return 0;
-    return wush::experts_plan(T, k, E, H, I).bytes;
+    return wush::experts_plan(T, k, E, H, I, dtype).bytes;
 }
 
 int wush_moe_experts_fp8(const void* x, int dtype, int64_t row_stride, const float* weights, const int32_t* ids,
@@ -409,7 +441,7 @@ int wush_moe_experts_fp8(const void* x, int dtype, int64_t row_stride, const flo
     WUSH_REQUIRE(wush::experts_sizes(T, k, E, H, I));
     WUSH_REQUIRE(dtype == WUSH_DTYPE_BF16 || dtype == WUSH_DTYPE_F16);
     if (T == 0) return (int)hipSuccess;
-    const wush::ExpertsPlan p = wush::experts_plan(T, k, E, H, I);
+    const wush::ExpertsPlan p = wush::experts_plan(T, k, E, H, I, dtype);
     WUSH_REQUIRE(x && weights && ids && w_up && s_up && w_down && s_down && y && workspace && workspace_bytes >= p.bytes);
     WUSH_REQUIRE((((uintptr_t)x | (uintptr_t)w_up | (uintptr_t)w_down | (uintptr_t)workspace) & 15u) == 0 && ((uintptr_t)y & 1u) == 0);
     WUSH_REQUIRE((((uintptr_t)weights | (uintptr_t)ids | (uintptr_t)s_up | (uintptr_t)s_down) & 3u) == 0);
@@ -423,7 +455,8 @@ int wush_moe_experts_fp8(const void* x, int dtype, int64_t row_stride, const flo
     int4* tiles = reinterpret_cast<int4*>(ws + p.tiles);
     int* ntiles = reinterpret_cast<int*>(ws + p.ntiles);
     float* a = reinterpret_cast<float*>(ws + p.a);
-    float* o = reinterpret_cast<float*>(ws + p.o);
+    float* hs = reinterpret_cast<float*>(ws + p.hs);
+    float* os = reinterpret_cast<float*>(ws + p.os);
     for (int64_t t = 0; t < T; t += p.tokens) {
         const int64_t n = T - t < p.tokens ? T - t : p.tokens;
         int st = wush_quant_fp8_block(px + t * row_stride, dtype, ws + p.xq, reinterpret_cast<float*>(ws + p.xs), n, H, row_stride, stream);
@@ -438,7 +471,6 @@ int wush_moe_experts_fp8(const void* x, int dtype, int64_t row_stride, const flo
         g.ldx = n;
         g.w = w_up;
         g.ws = s_up;
-        g.y = a;
         g.out = wush::kOutF32;
         g.M = P;
         g.N = (int)(2 * I);
@@ -448,23 +480,35 @@ int wush_moe_experts_fp8(const void* x, int dtype, int64_t row_stride, const flo
         g.ntiles = ntiles;
         g.row_of = row_of;
         g.most_tiles = p.most_tiles;
-        if ((st = wush::launch_gemm_fp8(g, p.tile_rows, p.tile_cols, stream))) return st;
-        const int64_t blocks = ((int64_t)P * (I / 128) + 15) / 16;
-        wush::moe_act_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, stream>>>(
-            a, ws + p.hq, reinterpret_cast<float*>(ws + p.hs), (int)I, p.pairs, tiles, ntiles);
-        if ((st = (int)hipGetLastError())) return st;
+        g.act = p.fused;
+        g.wide = !p.fused;
+        g.y = p.fused ? static_cast<void*>(ws + p.hq) : a;
+        g.hs = hs;
+        g.ldh = p.pairs;
+        st = p.fused ? wush::launch_gemm_fp8_runs(g, stream) : wush::launch_gemm_fp8_rows(g, p.tile_rows, p.tile_cols, stream);
+        if (st) return st;
+        if (!p.fused) {
+            const int64_t blocks = ((int64_t)P * (I / 128) + 15) / 16;
+            wush::moe_act_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, stream>>>(a, ws + p.hq, hs, (int)I, p.pairs, tiles, ntiles);
+            if ((st = (int)hipGetLastError())) return st;
+        }
         g.x = ws + p.hq;
-        g.xs = reinterpret_cast<float*>(ws + p.hs);
+        g.xs = hs;
         g.ldx = p.pairs;
         g.w = w_down;
         g.ws = s_down;
-        g.y = o;
+        g.y = ws + p.o;
         g.N = (int)H;
         g.K = (int)I;
         g.row_of = nullptr;
-        if ((st = wush::launch_gemm_fp8(g, p.tile_rows, p.tile_cols, stream))) return st;
-        const dim3 grid((unsigned)n, (unsigned)((H / 4 + 255) / 256));
-        wush::moe_sum_kernel<<<grid, 256, 0, stream>>>(o, pos, weights + t * k, py + t * H, dtype, (int)k, (int)H);
+        g.act = g.wide = 0;
+        g.shared = p.fused;
+        g.hs = os;
+        st = p.fused ? wush::launch_gemm_fp8_runs(g, stream) : wush::launch_gemm_fp8_rows(g, p.tile_rows, p.tile_cols, stream);
+        if (st) return st;
+        const unsigned grid = (unsigned)((n * (H / 8) + 255) / 256);
+        if (p.fused) wush::moe_sum_kernel<true><<<grid, 256, 0, stream>>>(ws + p.o, os, pos, weights + t * k, py + t * H, dtype, n, (int)k, (int)H);
+        else wush::moe_sum_kernel<false><<<grid, 256, 0, stream>>>(ws + p.o, nullptr, pos, weights + t * k, py + t * H, dtype, n, (int)k, (int)H);
         if ((st = (int)hipGetLastError())) return st;
     }
     return (int)hipSuccess;
