@@ -400,7 +400,8 @@ int wush_gemm_fp8(const uint8_t *xq, const float *xs, const uint8_t *wq, const f
 
 /* Kernels of wush_gemm_fp8, as its plan query names them. */
 enum wush_fp8_kernel {
-    WUSH_FP8_TILES = 0              /* MFMA tiles through LDS */
+    WUSH_FP8_DOT = 0,               /* fp32 dot products of whole weight rows (M <= 4) */
+    WUSH_FP8_TILES = 1              /* MFMA tiles through LDS */
 };
 
 /* The plan wush_gemm_fp8 runs with `workspace_bytes` of 16-byte aligned workspace:

@@ -28,7 +28,7 @@ EXT = os.path.join(PKG, "_C" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 HIP_SOURCES = ["quant.hip", "fused_tq.hip", "gemv.hip", "gemm_s4.hip", "gemm_h16.hip", "gemm_h16q.hip", "gemm_h16s.hip",
                "gemm_pt.hip", "w8a8.hip", "gemm_w8a8.hip", "kv8_cache.hip", "kv8_attention.hip", "kv8_chunk.hip",
-               "fp8.hip", "gemm_fp8.hip", "gemm_fp8_runs.hip", "moe.hip", "setup.hip"]
+               "fp8.hip", "fp8_gemv.hip", "gemm_fp8.hip", "gemm_fp8_runs.hip", "moe.hip", "setup.hip"]
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [

@@ -209,7 +209,7 @@ def kv8_attention_plan(pages, heads, page_size, head_dim, seqs, tokens, ragged, 
 
 
 # kernels of gemm_fp8_plan
-FP8_TILES, = range(1)
+FP8_DOT, FP8_TILES = range(2)
 
 
 def gemm_fp8_plan(M, N, K, workspace_bytes=None) -> tuple:

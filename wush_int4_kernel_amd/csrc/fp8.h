@@ -1,5 +1,6 @@
 // fp8.h -- what the e4m3 sources share: fp8.hip (quantization, the choice between
-// the kernels), gemm_fp8.hip (tiles) and moe.hip (experts).
+// the kernels), gemm_fp8.hip and
+// gemm_fp8_runs.hip (tiles), fp8_gemv.hip (few rows) and moe.hip (experts).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -52,9 +53,31 @@ int launch_gemm_fp8(const Fp8Gemm& g, int tile_rows, int tile_cols, hipStream_t 
 // The same over experts, fp32 out: tiles of 32 x 64, 64 x 128, 128 x 128.
 int launch_gemm_fp8_rows(const Fp8Gemm& g, int tile_rows, int tile_cols, hipStream_t stream);
 
-// Tiles of 128 x 256 by workgroups that take one after another: one matrix with N % 8 == 0 and
+// Tiles of tile_rows (64 or 128) x 256 by workgroups that take one after another: one matrix with N % 8 == 0 and
 // 16-byte aligned y, or experts with act or shared.
 constexpr int kFp8Workgroups = 256;              // one for each of the chip's CUs
-int launch_gemm_fp8_runs(const Fp8Gemm& g, hipStream_t stream);
+int launch_gemm_fp8_runs(const Fp8Gemm& g, int tile_rows, hipStream_t stream);
+
+// Up to four rows (see fp8_gemv_shape) on dot products: x as bf16 or fp16 rows of y's type (xs null), or as codes with
+// scales xs (K / 128, M).
+bool fp8_gemv_shape(int64_t M, int64_t K);
+int launch_fp8_gemv(const void* x, int64_t row_stride, const float* xs, const uint8_t* w, const float* ws, uint16_t* y,
+                    int dtype, int64_t M, int64_t N, int64_t K, hipStream_t stream);
+
+// A layer of experts for few tokens; h: T * k * I fp32 of workspace.
+struct Fp8Experts {
+    const void* x;
+    int64_t row_stride;
+    const float* weights;
+    const int32_t* ids;
+    const uint8_t *w_up, *w_down;
+    const float *s_up, *s_down;
+    float* h;
+    void* y;
+    int dtype, T, k, E, H, I;
+};
+constexpr int kFp8GemvPairs = 512;                // of tokens and choices, at most
+bool fp8_experts_gemv_shape(int64_t T, int64_t k, int64_t H, int64_t I);
+int launch_fp8_experts_gemv(const Fp8Experts& a, hipStream_t stream);
 
 }  // namespace wush

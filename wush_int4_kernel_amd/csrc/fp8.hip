@@ -41,9 +41,10 @@ __global__ __launch_bounds__(256) void quant_fp8_block_kernel(const uint16_t* __
         const float amax = fp8_amax(row16_max(fp8_largest8(v)));
         if (row >= rows || b >= KB) continue;
         if (l16 == 0) s[(size_t)b * rows + row] = fp8_scale(amax);
+        const Fp8Divisor by = fp8_divisor(amax);
         if (k < K)
-            *reinterpret_cast<uint2*>(q + row * K + k) =
-                make_uint2(fp8_codes4(v[0], v[1], v[2], v[3], amax), fp8_codes4(v[4], v[5], v[6], v[7], amax));
+            *reinterpret_cast<uint2*>(q + row * K + k) = make_uint2(fp8_codes4(v[0], v[1], v[2], v[3], by, amax != amax),
+                                                                    fp8_codes4(v[4], v[5], v[6], v[7], by, amax != amax));
     }
 }
 
@@ -66,8 +67,9 @@ struct Plan {
     int kernel, rows, cols, splits;
 };
 
-// The tile and the split of K with the least estimated time, in microseconds.
+// Up to four rows take dot products, more the tile and the split of K with the least estimated time, in microseconds.
 Plan plan_of(int64_t M, int64_t N, int64_t K, size_t room) {
+    if (fp8_gemv_shape(M, K)) return {WUSH_FP8_DOT, (int)M, 1, 1};
     Plan best = {WUSH_FP8_TILES, 32, 64, 1};
     const int64_t stages = (K + 127) / 128;
     double least = 1e30;
@@ -141,6 +143,8 @@ int wush_gemm_fp8(const uint8_t* xq, const float* xs, const uint8_t* wq, const f
     WUSH_REQUIRE((((uintptr_t)xq | (uintptr_t)wq) & 15u) == 0 && (((uintptr_t)xs | (uintptr_t)ws) & 3u) == 0 && ((uintptr_t)y & (N % 8 == 0 ? 15u : 1u)) == 0);
     const bool usable = workspace && ((uintptr_t)workspace & 15u) == 0;
     const wush::Plan p = wush::plan_of(M, N, K, usable ? workspace_bytes : 0);
+    if (p.kernel == WUSH_FP8_DOT)
+        return wush::launch_fp8_gemv(xq, 0, xs, wq, ws, static_cast<uint16_t*>(y), dtype, M, N, K, stream);
     wush::Fp8Gemm g = {};
     g.x = xq;
     g.xs = xs;
@@ -154,14 +158,14 @@ int wush_gemm_fp8(const uint8_t* xq, const float* xs, const uint8_t* wq, const f
     g.N = (int)N;
     g.K = (int)K;
     g.splits = p.splits;
-    if (p.rows == 128 && p.cols == 256) return wush::launch_gemm_fp8_runs(g, stream);
+    if (p.rows < 256 && p.cols == 256) return wush::launch_gemm_fp8_runs(g, p.rows, stream);
     return wush::launch_gemm_fp8(g, p.rows, p.cols, stream);
 }
 
 static size_t fp8_scale_bytes(int64_t M, int64_t K) { return ((size_t)M * ((K + 127) / 128) * 4 + 15) & ~(size_t)15; }
 
 size_t wush_linear_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    if (!fp8_sizes(M, N, K) || M == 0 || N == 0) return 0;
+    if (!fp8_sizes(M, N, K) || M == 0 || N == 0 || wush::fp8_gemv_shape(M, K)) return 0;
     return (size_t)M * K + fp8_scale_bytes(M, K) + wush_gemm_fp8_workspace_bytes(M, N, K);
 }
 
@@ -172,6 +176,11 @@ int wush_linear_fp8(const void* x, int64_t row_stride, const uint8_t* wq, const 
     if (M == 0 || N == 0) return (int)hipSuccess;
     const size_t need = wush_linear_fp8_workspace_bytes(M, N, K);
     WUSH_REQUIRE(x && wq && ws && y && workspace_bytes >= need && (need == 0 || (workspace && ((uintptr_t)workspace & 15u) == 0)));
+    WUSH_REQUIRE((((uintptr_t)x | (uintptr_t)wq) & 15u) == 0 && ((uintptr_t)ws & 3u) == 0 && ((uintptr_t)y & (N % 8 == 0 ? 15u : 1u)) == 0);
+    WUSH_REQUIRE(M == 1 || (row_stride >= 0 && row_stride % 8 == 0));
+    if (M == 1) row_stride = 0;
+    if (wush::fp8_gemv_shape(M, K))
+        return wush::launch_fp8_gemv(x, row_stride, nullptr, wq, ws, static_cast<uint16_t*>(y), dtype, M, N, K, stream);
     uint8_t* q = static_cast<uint8_t*>(workspace);
     float* s = reinterpret_cast<float*>(q + (size_t)M * K);
     const int st = wush_quant_fp8_block(x, dtype, q, s, M, K, row_stride, stream);

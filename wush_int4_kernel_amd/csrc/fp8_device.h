@@ -4,8 +4,8 @@
 //   A = max(amax |x|, 448 * 2^-126),  scale = A / 448,  code = e4m3(448 x / A)
 //
 // The code is the nearest to the quotient itself, halves to even: 0.875 x is exact for bf16 and fp16
-// values (7 x has 3 more bits), the division is correctly rounded and 512 a power of two, and
-// no quotient of two such values is within 2^-23 of half a code's step without being it.  A
+// values (7 x has 3 more bits), and no quotient of two such values is within 2^-22 of half a
+// code's step without being it.  A
 // product with the rounded reciprocal instead falls to one or the other side of those
 // halves, which values of 8 bits meet often.  A block with a non-finite value gets the
 // scale NaN and zero codes.
@@ -24,13 +24,38 @@ __device__ __forceinline__ float fp8_amax(uint32_t largest) {
     return largest >= 0x7f800000u ? __builtin_nanf("") : fmaxf(__uint_as_float(largest), kFp8Floor);
 }
 __device__ __forceinline__ float fp8_scale(float amax) { return amax / kFp8Largest; }
-__device__ __forceinline__ float fp8_arg(float v, float amax) { return v * 0.875f / amax * 512.0f; }
+// The division made once for a block: with a = A / 2^e in [1, 2), r = RN(1 / a) and v' = 0.875 v 2^(9 - e) (exact, or
+// so small that its code is 0), q0 = RN(v' r) is within 1.5 ulps of v' / a, its remainder exact in an fma, and
+// q1 = RN(q0 + remainder r) within an ulp, and the quotient itself where that is representable, as
+// halves between codes are.
+struct Fp8Divisor {
+    float a, r;
+    int shift;
+};
+__device__ __forceinline__ Fp8Divisor fp8_divisor(float amax) {
+    Fp8Divisor d;
+    const uint32_t u = __float_as_uint(amax);                    // a normal number, or NaN
+    d.shift = 9 + 127 - (int)(u >> 23);
+    d.a = __uint_as_float((u & 0x7fffffu) | 0x3f800000u);
+    d.r = 1.0f / d.a;
+    return d;
+}
+__device__ __forceinline__ float fp8_arg(float v, const Fp8Divisor& d) {
+    const float w = __builtin_ldexpf(v * 0.875f, d.shift), q = w * d.r;
+    return __builtin_fmaf(__builtin_fmaf(-q, d.a, w), d.r, q);
+}
 
 // four codes
-__device__ __forceinline__ uint32_t fp8_codes4(float a, float b, float c, float d, float amax) {
-    if (amax != amax) return 0;
-    int p = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_arg(a, amax), fp8_arg(b, amax), 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(fp8_arg(c, amax), fp8_arg(d, amax), p, true);
+__device__ __forceinline__ uint32_t fp8_codes4(float a, float b, float c, float d, const Fp8Divisor& by, bool bad) {
+    if (bad) return 0;
+    int p = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_arg(a, by), fp8_arg(b, by), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(fp8_arg(c, by), fp8_arg(d, by), p, true);
+}
+
+// values of four codes
+__device__ __forceinline__ void fp8_values4(uint32_t codes, float (&v)[4]) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
+    v[0] = lo[0], v[1] = lo[1], v[2] = hi[0], v[3] = hi[1];
 }
 
 // The same for values that are sums in fp32: a product with the rounded quotient 448 / A, off by less than
@@ -51,17 +76,34 @@ __device__ __forceinline__ float fp8_silu(float x) {
     return x * __builtin_amdgcn_rcpf(1.0f + (__builtin_fabsf(hi) < 126.0f ? __builtin_fmaf(e, lo * 0.693147182f, e) : e));
 }
 
+// 32 codes as fp16, exactly (NaN stays NaN), in order
+typedef int fp8_v8i __attribute__((ext_vector_type(8)));
+typedef _Float16 fp8_h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 fp8_h8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ void fp8_widen(const fp8_v8i& v, fp8_h8 (&o)[4]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        fp8_h2 p[4];
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+            p[2 * d] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[2 * q + d], 1.0f, false);
+            p[2 * d + 1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[2 * q + d], 1.0f, true);
+        }
+        o[q] = (fp8_h8){p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
+    }
+}
+
 // maximum over the 16 lanes of a row (of a block, where a lane holds 8 channels)
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
     return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false));
 }
-__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
+__device__ __forceinline__ uint32_t row8_max(uint32_t v) {       // over each half of a row: where a lane holds 16 channels
     v = dpp_max<0xB1>(v);        // quad_perm [1,0,3,2]
     v = dpp_max<0x4E>(v);        // quad_perm [2,3,0,1]
-    v = dpp_max<0x141>(v);       // row_half_mirror
-    return dpp_max<0x140>(v);    // row_mirror
+    return dpp_max<0x141>(v);    // row_half_mirror
 }
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) { return dpp_max<0x140>(row8_max(v)); }    // row_mirror
 
 // eight bf16 or fp16 values as fp32
 template <int DT>

@@ -283,18 +283,6 @@ void gemm_fp8_kernel(const Fp8Gemm g) {
         h8 wa[RB][4], wb[4];
 #pragma unroll
         for (int i = 0; i < RB; ++i) tmp[(CB - 1) & 1][i] = (v4f){0, 0, 0, 0};
-        auto widen = [&](const v8i& v, h8 (&o)[4]) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                h2 p[4];
-#pragma unroll
-                for (int d = 0; d < 2; ++d) {
-                    p[2 * d] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[2 * q + d], 1.0f, false);
-                    p[2 * d + 1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[2 * q + d], 1.0f, true);
-                }
-                o[q] = (h8){p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
-            }
-        };
         auto add = [&](int j, int i, const float (&s)[RB]) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(tmp[j & 1][i][r], s[i], acc[i][j][r]);
@@ -303,7 +291,7 @@ void gemm_fp8_kernel(const Fp8Gemm g) {
             const int nbuf = buf + 1 == NB ? 0 : buf + 1;
             begin();
 #pragma unroll
-            for (int i = 0; i < RB; ++i) widen(a[i], wa[i]);
+            for (int i = 0; i < RB; ++i) fp8_widen(a[i], wa[i]);
             static_for<CB>([&](auto jc) {
                 constexpr int j = jc.value, jn = j + BR - 1;
                 if constexpr (j == kTurn) {
@@ -312,7 +300,7 @@ void gemm_fp8_kernel(const Fp8Gemm g) {
                     for (int i = 0; i < RB; ++i) read_a(nbuf, i);
                     read_s(nbuf);
                 }
-                widen(b[j % BR], wb);
+                fp8_widen(b[j % BR], wb);
                 if constexpr (jn < CB) read_b(buf, jn);
                 else read_b(nbuf, jn - CB);
                 __builtin_amdgcn_sched_barrier(0);
@@ -440,8 +428,6 @@ int launch_gemm_fp8_rows(const Fp8Gemm& g, int tile_rows, int tile_cols, hipStre
     WUSH_REQUIRE(g.most_tiles * cols < (1 << 23));               // a launch has fewer than 2^32 threads
     const unsigned grid = (unsigned)(g.most_tiles * cols);
     switch (tile_rows << 16 | tile_cols) {
-        case 128 << 16 | 128: return launch_rows<4, 4, 2, 2, 4, 4>(g, grid, stream);
-        case 64 << 16 | 128: return launch_rows<2, 4, 2, 2, 3, 4>(g, grid, stream);
         case 32 << 16 | 64: return launch_rows<2, 2, 1, 2, 4, 2>(g, grid, stream);
         default: return (int)hipErrorInvalidValue;
     }

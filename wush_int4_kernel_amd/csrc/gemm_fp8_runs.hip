@@ -2,7 +2,7 @@
 // CU takes tile after tile, and the loads of a tile's first stages are issued during the last stages of
 // the one before, so that neither its way from memory nor the outputs' way to it is waited for.
 //
-// Workgroup: eight wavefronts, WR x WC, each owning 64 x 256 / WC outputs.  Stages and their order as in gemm_fp8.hip.
+// Workgroup: eight wavefronts, WR x WC, each owning 16 RB x 256 / WC outputs.  Stages and their order as in gemm_fp8.hip.
 // Outputs leave straight from registers, four columns of a lane made 16 by swaps between the
 // lanes of a row: LDS belongs to the next tile by then.
 #include "fp8.h"
@@ -16,11 +16,12 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
-// One matrix (kPlain); each expert's, over its rows, outputs in fp16 with shared powers of two (kShared);
-// each expert's gate and up projection together, whose products leave as codes of
-// silu(gate) * up (kAct): a wavefront's columns are 64 of the gate and the same of the up projection.
-enum { kPlain, kShared, kAct };
+// One matrix (kPlain); each expert's, over its rows, outputs in fp32 (kWide) or in fp16 with shared powers of
+// two (kShared); each expert's gate and up projection together, whose products leave as codes of
+// silu(gate) * up (kAct): half of a wavefront's columns are the gate's, the other half the same ones of the up projection.
+enum { kPlain, kWide, kShared, kAct };
 
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -46,18 +47,18 @@ __device__ __forceinline__ void rows_transpose(uint32_t (&v)[4]) {
     }
 }
 
-template <int WR, int WC, int NB, int MODE, bool BF16>
+template <int RB, int WR, int WC, int NB, int MODE, bool BF16, bool F16>
 __global__ __launch_bounds__(64 * WR * WC) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void gemm_fp8_runs_kernel(const Fp8Gemm g) {
-    constexpr int NW = WR * WC, TR = 64 * WR, TC = 256;
-    constexpr int RB = 4, CB = 16 / WC, BR = 4, kMf = RB * CB, kLag = 3, kTmp = 4, kTurn = CB - BR + 1;
+    constexpr int NW = WR * WC, TR = 16 * RB * WR, TC = 256;
+    constexpr int CB = 16 / WC, BR = F16 ? 2 : 4, kMf = RB * CB, kLag = 3, kTmp = 4, kTurn = CB - BR + 1;
     constexpr int DA = TR / 8 / NW, DB = TC / 8 / NW, ND = DA + DB + 1;    // DMAs per wavefront and stage, one of scales
     constexpr int kChunksA = TR / 64;                            // wavefronts that fetch x's scales, the others w's
     constexpr int kA = TR * 128, kSx = kA + TC * 128, kSw = kSx + kChunksA * 256, kBuf = kSw + 256;
     constexpr int kSmem = NB * kBuf + (MODE == kAct ? TR * WC * 4 : 0);
     constexpr bool GROUPED = MODE != kPlain;
     constexpr int NSW = MODE == kAct ? 2 : 1;                    // scales of w that a wavefront's columns have
-    constexpr int kStores = MODE == kAct ? RB : RB * CB / 2;     // stores of a whole tile, at least
+    constexpr int kStores = MODE == kAct ? RB : MODE == kWide ? RB * CB : RB * CB / 2;    // stores of a whole tile, at least
     constexpr int kHalf = 8 * CB;                                // kAct: columns of the gate that a wavefront has
     static_assert(kSmem <= 160 * 1024 && (NB - 2) * ND + kStores < 64 && 8 * DB <= kHalf && kChunksA < NW);
     __shared__ __align__(16) uint8_t smem[kSmem];
@@ -88,7 +89,8 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
     size_t sstep = 0;
     uint32_t voff[DA + DB], soff = 0;
     const int r0 = 8 * DB * wave;                                // this wavefront's first LDS row of w
-    const uint32_t piece = ((uint32_t)lane & 7u) ^ (((uint32_t)lane >> 4) & 3u);     // of even DMAs; of odd ones ^ 4
+    const uint32_t piece = ((uint32_t)lane & 7u) ^ (((uint32_t)lane >> 4) & 3u);     // of even groups of 8 rows; of odd ones ^ 4
+    const uint32_t flip = DA & 1 ? 4u * (wave & 1) : 0u;         // this wavefront's first group of x
     auto place = [&](int s, int& tm, int& tn) {
         if constexpr (GROUPED) {
             tm = s / NC;
@@ -140,7 +142,7 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
             } else if (MODE != kAct) {
                 row = max(min(row, N - n0 - 1), 0);
             }
-            voff[k] = (uint32_t)row * (uint32_t)K + 16u * (piece ^ (k & 1 ? 4u : 0u));
+            voff[k] = (uint32_t)row * (uint32_t)K + 16u * (piece ^ (k < DA ? flip ^ (k & 1 ? 4u : 0u) : (k - DA) & 1 ? 4u : 0u));
         }
         if (wave < kChunksA) {
             int row = min(64 * wave + lane, iM - im0 - 1);
@@ -162,7 +164,7 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
     // f(r) = (r / 2) % 8, so that 16 consecutive rows' reads of one piece hit distinct banks.  Rows past the
     // end read the last one; pieces past a short block's end its first one, whose activations are zeroed before use.
     const uint8_t *ia, *ib, *is;                                 // this stage's addresses
-    uint32_t idst, past[2];
+    uint32_t idst, past[2], pastx;
     auto aim = [&](int buf) {
         const int at = ist >= whole ? ist : ist + iturn - (ist + iturn >= whole ? whole : 0);
         const bool cut = tail && at == KB - 1;
@@ -175,6 +177,7 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
             const uint32_t p = piece ^ (e ? 4u : 0u);
             past[e] = cut && p >= (uint32_t)tail ? 16u * p : 0u;
         }
+        pastx = flip ? past[1] : past[0];
     };
     auto issue = [&](auto kc) {
         constexpr int k = kc.value;
@@ -182,12 +185,12 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
             asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
                          : : "v"(soff), "s"(is), "s"(idst + (wave < kChunksA ? kSx + wave * 256 : kSw)) : "m0");
         } else if constexpr (k < DA) {
-            dma16_uniform(ia, voff[k] - past[k & 1], idst + (wave * DA + k) * 1024);
+            dma16_uniform(ia, voff[k] - (DA & 1 ? pastx : past[k & 1]), idst + (wave * DA + k) * 1024);
         } else {
-            dma16_uniform(ib, voff[k] - past[k & 1], idst + kA + (wave * DB + k - DA) * 1024);
+            dma16_uniform(ib, voff[k] - past[(k - DA) & 1], idst + kA + (wave * DB + k - DA) * 1024);
         }
     };
-    static_assert(DA % 2 == 0 && DB % 2 == 0);
+    static_assert((DA == 1 || DA % 2 == 0) && DB % 2 == 0);
     // The stage after this one; behind the last of all, that one again, so that every stage issues as many loads.
     auto advance = [&] {
         if (++ist < KB) return;
@@ -196,11 +199,11 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
     };
 
     // --------------------------------------------------------------- the pipeline's state
-    v4f acc[RB][CB], tmp[kTmp];
+    v4f acc[RB][CB], tmp[F16 ? 2 * RB : kTmp];                   // F16: column j's products at (j & 1) * RB
     v8i a[RB], b[BR];
     float sc[NSW][RB], old[RB], sx[RB], sw[NSW];
     const int fsw = (l16 >> 1) & 7;
-    const uint8_t* arow = smem + (wr * 64 + l16) * 128;
+    const uint8_t* arow = smem + (wr * RB * 16 + l16) * 128;
     const uint8_t* brow = smem + kA + (wc * CB * 16 + l16) * 128;
     const int p0 = 16 * (kq ^ fsw), p1 = 16 * ((4 + kq) ^ fsw);
     auto pieces = [&](const uint8_t* p) {
@@ -212,7 +215,7 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
     auto read_s = [&](int buf) {
         const uint8_t* p = smem + buf * kBuf;
 #pragma unroll
-        for (int i = 0; i < RB; ++i) sx[i] = *reinterpret_cast<const float*>(p + kSx + 4 * (wr * 64 + 16 * i + l16));
+        for (int i = 0; i < RB; ++i) sx[i] = *reinterpret_cast<const float*>(p + kSx + 4 * ((wr * RB + i) * 16 + l16));
         if constexpr (MODE == kAct) {
             sw[0] = *reinterpret_cast<const float*>(p + kSw);
             sw[1] = *reinterpret_cast<const float*>(p + kSw + 4);
@@ -236,7 +239,7 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
 #pragma unroll
             for (int j = 0; j < CB; ++j) acc[i][j] = (v4f){0, 0, 0, 0};
 #pragma unroll
-        for (int t = 0; t < kTmp; ++t) tmp[t] = (v4f){0, 0, 0, 0};
+        for (int t = 0; t < (F16 ? 2 * RB : kTmp); ++t) tmp[t] = (v4f){0, 0, 0, 0};
     };
     clear();
 #pragma unroll
@@ -254,8 +257,9 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
     int buf = 0, st = 0;                         // LDS buffer of stage st
     auto add = [&](int m, const float (&s)[RB]) {
         const int i = m % RB, j = m / RB;
+        const v4f& t = tmp[F16 ? (j & 1) * RB + i : m % kTmp];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(tmp[m % kTmp][r], s[i], acc[i][j][r]);
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(t[r], s[i], acc[i][j][r]);
         asm volatile("" : "+v"(acc[i][j]));      // here, and not where the compiler finds its next use
     };
     // One stage, whose buffer takes the next one to be issued.  Operands read past the last stage are not used.
@@ -278,38 +282,73 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
                 a[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
             }
         }
-        static_for<kMf>([&](auto mc) {
-            constexpr int m = mc.value, i = m % RB, j = m / RB;
-            if constexpr (i == 0 && j == kTurn) {
-                // the next stage has landed in all wavefronts' view, and all have read this one's columns
-                WUSH_WAIT_VMCNT((NB - 2) * ND + (first.value ? kStores : 0));
-                WUSH_LDS_BARRIER();
-                aim(buf);
+        // the next stage has landed in all wavefronts' view, and all have read this one's columns
+        auto landed = [&] {
+            WUSH_WAIT_VMCNT((NB - 2) * ND + (first.value ? kStores : 0));
+            WUSH_LDS_BARRIER();
+            aim(buf);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto refill_part = [&](auto qc, auto nc) {               // share q of n
+            constexpr int q = qc.value, n = nc.value;
+            static_for<(q + 1) * ND / n - q * ND / n>([&](auto dc) { issue(std::integral_constant<int, q * ND / n + dc.value>{}); });
+        };
+        if constexpr (!F16) {
+            static_for<kMf>([&](auto mc) {
+                constexpr int m = mc.value, i = m % RB, j = m / RB;
+                if constexpr (i == 0 && j == kTurn) landed();
+                tmp[m % kTmp] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j % BR], a[i], (v4f){0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+                if constexpr (i == 0) {
+                    constexpr int jn = j + BR - 1;
+                    if constexpr (jn < CB) read_b(buf, jn);
+                    else read_b(nbuf, jn - CB);
+                }
+                if constexpr (j == CB - 1) read_a(nbuf, i);
+                if constexpr (m == kMf - 1) read_s(nbuf);
+                if constexpr (m >= kLag) add(m - kLag, sc[(m - kLag) / RB * NSW / CB]);
+                else add(kMf + m - kLag, old);
+                if constexpr (j >= kTurn)
+                    refill_part(std::integral_constant<int, m - kTurn * RB>{}, std::integral_constant<int, (BR - 1) * RB>{});
                 __builtin_amdgcn_sched_barrier(0);
-            }
-            tmp[m % kTmp] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j % BR], a[i], (v4f){0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
-            if constexpr (i == 0) {
-                constexpr int jn = j + BR - 1;
+            });
+        } else {
+            h8 wa[RB][4], wb[4];
+#pragma unroll
+            for (int i = 0; i < RB; ++i) fp8_widen(a[i], wa[i]);
+            static_for<CB>([&](auto jc) {
+                constexpr int j = jc.value, jn = j + BR - 1;
+                if constexpr (j == kTurn) {
+                    landed();
+#pragma unroll
+                    for (int i = 0; i < RB; ++i) read_a(nbuf, i);
+                    read_s(nbuf);
+                }
+                fp8_widen(b[j % BR], wb);
                 if constexpr (jn < CB) read_b(buf, jn);
                 else read_b(nbuf, jn - CB);
-            }
-            if constexpr (j == CB - 1) read_a(nbuf, i);
-            if constexpr (m == kMf - 1) read_s(nbuf);
-            if constexpr (m >= kLag) add(m - kLag, sc[(m - kLag) / RB * NSW / CB]);
-            else add(kMf + m - kLag, old);
-            if constexpr (j >= kTurn) {
-                constexpr int n = (BR - 1) * RB, q = m - kTurn * RB;
-                static_for<(q + 1) * ND / n - q * ND / n>([&](auto dc) { issue(std::integral_constant<int, q * ND / n + dc.value>{}); });
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        });
+                __builtin_amdgcn_sched_barrier(0);
+                static_for<4 * RB>([&](auto mc) {
+                    constexpr int q = mc.value / RB, i = mc.value % RB, t = (j & 1) * RB + i;
+                    tmp[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wb[q], wa[i][q], q ? tmp[t] : (v4f){0, 0, 0, 0}, 0, 0, 0);
+                    if constexpr (q == 1) {
+                        if constexpr (j > 0) add((j - 1) * RB + i, sc[(j - 1) * NSW / CB]);
+                        else add((CB - 1) * RB + i, old);
+                    }
+                    if constexpr (j >= kTurn)
+                        refill_part(std::integral_constant<int, (j - kTurn) * 4 * RB + mc.value>{},
+                                    std::integral_constant<int, (BR - 1) * 4 * RB>{});
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+            });
+        }
+        asm volatile("" ::: "memory");           // the reads above stay above
         buf = nbuf;
         advance();
     };
     // The tile's outputs.  Rows past M hold what row M - 1 does, and are stored there.
     auto finish = [&] {
 #pragma unroll
-        for (int m = kMf - kLag; m < kMf; ++m) add(m, sc[NSW - 1]);
+        for (int m = kMf - (F16 ? RB : kLag); m < kMf; ++m) add(m, sc[NSW - 1]);
         __builtin_amdgcn_sched_barrier(0);
         const int nw = tn * TC + wc * CB * 16;
         const bool full = MODE == kAct || tn * TC + TC <= N;
@@ -329,12 +368,12 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
                     }
                 mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16));
                 mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32));
-                if (kq == 0) part[WC * (wr * 64 + 16 * i + l16) + wc] = mx;
+                if (kq == 0) part[WC * ((wr * RB + i) * 16 + l16) + wc] = mx;
             }
             WUSH_LDS_BARRIER();
 #pragma unroll
             for (int i = 0; i < RB; ++i) {
-                const int row = wr * 64 + 16 * i + l16, m = min(m0 + row, M - 1);
+                const int row = (wr * RB + i) * 16 + l16, m = min(m0 + row, M - 1);
                 uint32_t mx = part[WC * row];
 #pragma unroll
                 for (int w = 1; w < WC; ++w) mx = max(mx, part[WC * row + w]);
@@ -354,11 +393,21 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
                 }
             }
             WUSH_LDS_BARRIER();                  // part is read before the next tile's is written
+        } else if constexpr (MODE == kWide) {
+#pragma unroll
+            for (int i = 0; i < RB; ++i) {
+                const int m = min(m0 + (wr * RB + i) * 16 + l16, M - 1);
+                float* out = static_cast<float*>(g.y) + (size_t)m * N + nw + 4 * kq;
+#pragma unroll
+                for (int j = 0; j < CB; ++j)
+                    if (full || nw + 16 * j < N) *reinterpret_cast<v4f*>(out + 16 * j) = acc[i][j];
+                __builtin_amdgcn_sched_barrier(0);
+            }
         } else {
             uint16_t* y = static_cast<uint16_t*>(g.y);
 #pragma unroll
             for (int i = 0; i < RB; ++i) {
-                const int m = min(m0 + wr * 64 + 16 * i + l16, M - 1);
+                const int m = min(m0 + (wr * RB + i) * 16 + l16, M - 1);
 #pragma unroll
                 for (int h = 0; h < CB / 4; ++h) {
                     const int n0 = nw + 64 * h;
@@ -412,27 +461,29 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
     WUSH_WAIT_VMCNT(0);                          // no load may reach LDS that is another workgroup's by then
 }
 
-template <int WR, int WC, int NB>
+template <int RB>
 int launch(const Fp8Gemm& g, unsigned grid, hipStream_t stream) {
-    constexpr int T = 64 * WR * WC;
-    if (g.act) gemm_fp8_runs_kernel<WR, WC, NB, kAct, false><<<grid, T, 0, stream>>>(g);
-    else if (g.shared) gemm_fp8_runs_kernel<WR, WC, NB, kShared, false><<<grid, T, 0, stream>>>(g);
-    else if (g.out == WUSH_DTYPE_BF16) gemm_fp8_runs_kernel<WR, WC, NB, kPlain, true><<<grid, T, 0, stream>>>(g);
-    else gemm_fp8_runs_kernel<WR, WC, NB, kPlain, false><<<grid, T, 0, stream>>>(g);
+    constexpr int WR = 2, WC = 4, NB = 3, T = 64 * WR * WC;
+    if (g.act && g.wide) gemm_fp8_runs_kernel<RB, WR, WC, NB, kAct, false, true><<<grid, T, 0, stream>>>(g);
+    else if (g.act) gemm_fp8_runs_kernel<RB, WR, WC, NB, kAct, false, false><<<grid, T, 0, stream>>>(g);
+    else if (g.tiles && g.shared) gemm_fp8_runs_kernel<RB, WR, WC, NB, kShared, false, false><<<grid, T, 0, stream>>>(g);
+    else if (g.tiles) gemm_fp8_runs_kernel<RB, WR, WC, NB, kWide, false, false><<<grid, T, 0, stream>>>(g);
+    else if (g.out == WUSH_DTYPE_BF16) gemm_fp8_runs_kernel<RB, WR, WC, NB, kPlain, true, false><<<grid, T, 0, stream>>>(g);
+    else gemm_fp8_runs_kernel<RB, WR, WC, NB, kPlain, false, false><<<grid, T, 0, stream>>>(g);
     return (int)hipGetLastError();
 }
 
 }  // namespace
 
-int launch_gemm_fp8_runs(const Fp8Gemm& g, hipStream_t stream) {
-    WUSH_REQUIRE(g.M > 0 && g.N > 0 && g.N % 8 == 0 && g.K > 0 && g.K % 16 == 0 && ((uintptr_t)g.y & 15u) == 0);
-    WUSH_REQUIRE(!(g.act || g.shared) || (g.tiles && g.ntiles && g.hs && g.N % 16 == 0 && g.K <= (1 << 20)));
-    WUSH_REQUIRE(!g.act || (g.N % 256 == 0 && g.row_of));
-    const long long rows = g.act || g.shared ? g.most_tiles : (g.M + 127) / 128;
+int launch_gemm_fp8_runs(const Fp8Gemm& g, int tile_rows, hipStream_t stream) {
+    WUSH_REQUIRE((tile_rows == 64 || tile_rows == 128) && g.M > 0 && g.N > 0 && g.N % 8 == 0 && g.K > 0 && g.K % 16 == 0 && ((uintptr_t)g.y & 15u) == 0);
+    WUSH_REQUIRE(!g.tiles || (g.ntiles && g.N % 16 == 0 && (g.act || !g.wide)));
+    WUSH_REQUIRE(!g.act || (g.tiles && g.N % 256 == 0 && g.row_of && g.hs));
+    const long long rows = g.tiles ? g.most_tiles : (g.M + tile_rows - 1) / tile_rows;
     const long long tiles = rows * (g.act ? g.N / 256 : (g.N + 255) / 256);
     WUSH_REQUIRE(tiles <= 0x7fffffffLL);
     const unsigned grid = (unsigned)(tiles < kFp8Workgroups ? tiles : kFp8Workgroups);
-    return launch<2, 4, 3>(g, grid, stream);
+    return tile_rows == 64 ? launch<2>(g, grid, stream) : launch<4>(g, grid, stream);
 }
 
 }  // namespace wush

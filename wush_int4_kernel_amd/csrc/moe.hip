@@ -8,6 +8,8 @@
 //
 // Experts: rows of x by expert; a = q(x) up_e^T, h = silu(a_gate) a_up, o = q(h) down_e^T, y = sum of w o over a
 // token's experts.  a, h and o are kept in fp32, h and x quantized as in fp8_device.h.
+#include <cmath>
+
 #include "fp8.h"
 #include "fp8_device.h"
 #include "../../include/wush_int4.h"
@@ -339,29 +341,44 @@ constexpr int64_t kRunPairs = 65536;
 
 struct ExpertsPlan {
     int64_t tokens, pairs;                       // of a run
-    bool fused;
+    bool few, fused, shared;                     // see experts_plan
     int tile_rows, tile_cols, most_tiles;
     size_t xq, xs, row_of, pos, tiles, ntiles, a, hq, hs, o, os, bytes;
 };
 
-// Two ways.  Fused: tiles of 128 x 256 on e4m3 matrix instructions, whose epilogue makes the hidden codes, and
-// outputs in fp16 with shared powers of two: for many rows an expert, where operations and the traffic of
-// intermediate rows bound the time, and for bf16 only.  The e4m3 instruction cuts small products next
-// to large ones (at 2^-13 of the largest of 8), which turns one in some thousand of the hidden codes to
-// the other side of a half: 1.2e-3 of the output, below bf16's rounding (1.7e-3), above fp16's (2.1e-4).
-// Otherwise the gate and up projections take fp16 matrix instructions, at half the rate where the
-// weights' stream bounds the time anyway, and intermediate rows are fp32.
+// Three ways.
+// A few tokens: dot products that read an expert's weights for each choice (fp8_gemv.hip).
+// Fused: tiles of 64 or 128 x 256, one after another (gemm_fp8_runs.hip), whose epilogue makes the hidden codes.  For bf16 all
+// products are on the e4m3 matrix instruction and experts' rows in fp16 with shared powers of two.
+// That instruction cuts small products next to large ones (at 2^-13 of the largest of 8), which turns
+// one in some thousand of the hidden codes to the other side of a half: 1.2e-3 of the output, below bf16's rounding (1.7e-3)
+// but above fp16's (2.1e-4).  For fp16 the gate and up projections therefore take the fp16 matrix
+// instruction, and experts' rows are fp32.
+// Otherwise (few rows an expert, and few workgroups of the other kind): tiles of 32 x 64, the gate
+// and up projections on the fp16 instruction, at half the rate where the weights' stream bounds the time anyway, and
+// intermediate rows in fp32.
+// us, bf16, by tokens, three ways (dots, 32, 64 rows): 64 experts of 2048 x 1408, 6 choices: 4: 46, 53, 51;
+// 8: 77, 66, 69; 64: -, 108, 110; 256: -, 150, 124 (128 rows 142); 1024: -, 333, 185 (180).  8 of 4096 x
+// 1792, 2 choices: 4: 33, 43, 49; 8: 55, 44, 50; 48: -, 57, 58; 256: -, 108, 59 (70); 512: -, 150, 93 (71).
 ExpertsPlan experts_plan(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, int dtype) {
     ExpertsPlan p = {};
+    // us: every choice reads its expert's weights; tiles read each expert once that some choice meets, after some launches
+    const double each = 3.0 * (double)H * (double)I / 6.5e6, met = (double)E * (1.0 - std::pow(1.0 - (k < E ? (double)k / (double)E : 1.0), (double)T));
+    if ((p.few = fp8_experts_gemv_shape(T, k, H, I) && 9.0 + (double)(T * k) * each < 22.0 + 1.05 * met * each)) {
+        p.tokens = T;
+        p.bytes = (size_t)(T * k) * I * 4;       // h
+        return p;
+    }
     int64_t most = kRunPairs / k;
     if (most * H > 0x7fffffffLL) most = 0x7fffffffLL / H;
     if (most * k * I > 0x7fffffffLL) most = 0x7fffffffLL / (k * I);
     p.tokens = T < most ? T : most;
     p.pairs = p.tokens * k;
     const double rows = (double)p.pairs / (double)E;
-    p.fused = rows > 64 && dtype == WUSH_DTYPE_BF16;
-    p.tile_rows = rows <= 24 ? 32 : rows <= 64 ? 64 : 128;
-    p.tile_cols = p.fused ? 256 : rows <= 24 ? 64 : 128;
+    p.fused = rows > 12 || (dtype == WUSH_DTYPE_BF16 && met * (double)(I / 128) >= 512);
+    p.shared = p.fused && dtype == WUSH_DTYPE_BF16;
+    p.tile_rows = !p.fused ? 32 : rows <= 80 ? 64 : 128;
+    p.tile_cols = p.fused ? 256 : 64;
     p.most_tiles = (int)(p.pairs / p.tile_rows + (p.pairs < E ? p.pairs : E));
     auto take = [&](size_t n) {
         const size_t at = p.bytes;
@@ -377,8 +394,8 @@ ExpertsPlan experts_plan(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, 
     p.a = take(p.fused ? 0 : (size_t)p.pairs * 2 * I * 4);
     p.hq = take((size_t)p.pairs * I);
     p.hs = take((size_t)p.pairs * (I / 128) * 4);
-    p.o = take((size_t)p.pairs * H * (p.fused ? 2 : 4));
-    p.os = take(p.fused ? (size_t)p.pairs * ((H + 63) / 64) * 4 : 0);
+    p.o = take((size_t)p.pairs * H * (p.shared ? 2 : 4));
+    p.os = take(p.shared ? (size_t)p.pairs * ((H + 63) / 64) * 4 : 0);
     return p;
 }
 
@@ -447,6 +464,11 @@ int wush_moe_experts_fp8(const void* x, int dtype, int64_t row_stride, const flo
     WUSH_REQUIRE((((uintptr_t)weights | (uintptr_t)ids | (uintptr_t)s_up | (uintptr_t)s_down) & 3u) == 0);
     WUSH_REQUIRE(T == 1 || (row_stride >= 0 && row_stride % 8 == 0));
     if (T == 1) row_stride = 0;
+    if (p.few) {
+        const wush::Fp8Experts a = {x, row_stride, weights, ids, w_up, w_down, s_up, s_down, static_cast<float*>(workspace), y, dtype,
+                                    (int)T, (int)k, (int)E, (int)H, (int)I};
+        return wush::launch_fp8_experts_gemv(a, stream);
+    }
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     const uint16_t* px = static_cast<const uint16_t*>(x);
     uint16_t* py = static_cast<uint16_t*>(y);
@@ -481,11 +503,11 @@ int wush_moe_experts_fp8(const void* x, int dtype, int64_t row_stride, const flo
         g.row_of = row_of;
         g.most_tiles = p.most_tiles;
         g.act = p.fused;
-        g.wide = !p.fused;
+        g.wide = !p.shared;
         g.y = p.fused ? static_cast<void*>(ws + p.hq) : a;
         g.hs = hs;
         g.ldh = p.pairs;
-        st = p.fused ? wush::launch_gemm_fp8_runs(g, stream) : wush::launch_gemm_fp8_rows(g, p.tile_rows, p.tile_cols, stream);
+        st = p.fused ? wush::launch_gemm_fp8_runs(g, p.tile_rows, stream) : wush::launch_gemm_fp8_rows(g, p.tile_rows, p.tile_cols, stream);
         if (st) return st;
         if (!p.fused) {
             const int64_t blocks = ((int64_t)P * (I / 128) + 15) / 16;
@@ -502,12 +524,12 @@ int wush_moe_experts_fp8(const void* x, int dtype, int64_t row_stride, const flo
         g.K = (int)I;
         g.row_of = nullptr;
         g.act = g.wide = 0;
-        g.shared = p.fused;
+        g.shared = p.shared;
         g.hs = os;
-        st = p.fused ? wush::launch_gemm_fp8_runs(g, stream) : wush::launch_gemm_fp8_rows(g, p.tile_rows, p.tile_cols, stream);
+        st = p.fused ? wush::launch_gemm_fp8_runs(g, p.tile_rows, stream) : wush::launch_gemm_fp8_rows(g, p.tile_rows, p.tile_cols, stream);
         if (st) return st;
         const unsigned grid = (unsigned)((n * (H / 8) + 255) / 256);
-        if (p.fused) wush::moe_sum_kernel<true><<<grid, 256, 0, stream>>>(ws + p.o, os, pos, weights + t * k, py + t * H, dtype, n, (int)k, (int)H);
+        if (p.shared) wush::moe_sum_kernel<true><<<grid, 256, 0, stream>>>(ws + p.o, os, pos, weights + t * k, py + t * H, dtype, n, (int)k, (int)H);
         else wush::moe_sum_kernel<false><<<grid, 256, 0, stream>>>(ws + p.o, nullptr, pos, weights + t * k, py + t * H, dtype, n, (int)k, (int)H);
         if ((st = (int)hipGetLastError())) return st;
     }
