@@ -37,15 +37,16 @@ struct Fp8Gemm {
     float* hs;
     int64_t ldh;
     int wide;                                    // products in fp16 matrix instructions, which cut none
+    int once;                                    // weights are mostly read for one tile of rows only
 };
 
 struct Fp8Tile {
-    int rows, cols, depth;
-    bool runs;                                   // N % 8 == 0 only
+    int rows, cols;
+    bool runs;                                   // gemm_fp8_runs.hip: N % 8 == 0 only
     double stage;                                // us that a K block takes a workgroup on a full chip
 };
-constexpr Fp8Tile kFp8Tiles[] = {{256, 256, 2, false, 1.5}, {128, 256, 3, true, 0.85}, {128, 128, 4, false, 0.6},
-                                 {64, 128, 3, false, 0.43}, {32, 128, 3, false, 0.39}, {32, 64, 4, false, 0.2}};
+constexpr Fp8Tile kFp8Tiles[] = {{256, 256, false, 1.63}, {128, 256, true, 1.02}, {64, 256, true, 0.8}, {128, 128, false, 0.72},
+                                 {64, 128, false, 0.57},  {32, 128, false, 0.41}, {32, 64, false, 0.28}};
 
 // Tiles of tile_rows x tile_cols, one of kFp8Tiles; K % 16 == 0.
 int launch_gemm_fp8(const Fp8Gemm& g, int tile_rows, int tile_cols, hipStream_t stream);

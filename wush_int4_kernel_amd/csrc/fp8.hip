@@ -67,24 +67,27 @@ struct Plan {
     int kernel, rows, cols, splits;
 };
 
-// Up to four rows take dot products, more the tile and the split of K with the least estimated time, in microseconds.
+// Up to four rows take dot products, more the tile and the split of K with the least estimated time, in microseconds: rounds
+// of workgroups with the time of their stages (3/4 of it on an empty chip), or the weights' way from HBM (slower where several
+// row tiles read them), whichever is longer, a part of the shorter, and for a split its launch and partial sums.  The
+// constants are fitted to 94 shapes from 5 x 8192 x 28672 to 4000 x 4096 x 4096, weights from HBM: 0.8% slower than the fastest
+// of all tiles and splits on average, 12% at worst.
 Plan plan_of(int64_t M, int64_t N, int64_t K, size_t room) {
     if (fp8_gemv_shape(M, K)) return {WUSH_FP8_DOT, (int)M, 1, 1};
     Plan best = {WUSH_FP8_TILES, 32, 64, 1};
     const int64_t stages = (K + 127) / 128;
     double least = 1e30;
     for (const auto& t : kFp8Tiles) {
-        if ((t.rows > 32 && t.rows >= 2 * M) || (t.runs && N % 8 != 0)) continue;
+        if ((t.rows > 64 && t.rows >= 2 * M) || (t.runs && N % 8 != 0)) continue;
         const int64_t tiles = ((M + t.rows - 1) / t.rows) * ((N + t.cols - 1) / t.cols);
         for (int s = 1; s <= 8 && (s == 1 || (stages / s >= 4 && t.cols < 256)); ++s) {
             if (s > 1 && (size_t)M * N * 4 * s > room) break;
             const double groups = (double)tiles * s, full = groups / 256 < 1 ? groups / 256 : 1;
             const double rounds = groups <= 1024 ? (double)(int64_t)((groups + 255) / 256) : groups / 256;
-            const double busy = t.stage * (0.6 + 0.4 * full), idle = 0.72 / (t.depth - 1);
-            const double work = rounds * (double)((stages + s - 1) / s) * (busy > idle ? busy : idle);
-            const double hbm = (double)N * K / 7e6;
-            double us = 4.0 + 1.0 * rounds + (work > hbm ? work : hbm);
-            if (s > 1) us += 3.3 + (double)M * N * (8.0 * s + 2) / 4.5e6;
+            const double work = rounds * (double)((stages + s - 1) / s) * t.stage * (0.75 + 0.25 * full);
+            const double hbm = (double)N * K / (M <= t.rows ? 6.3e6 : 4.4e6);
+            double us = 4.6 + rounds + (work > hbm ? work + 0.08 * hbm : hbm + 0.08 * work);
+            if (s > 1) us += 2.1 + (double)M * N * (8.0 * s + 2) / 4.4e6;
             if (us < least) {
                 least = us;
                 best = {WUSH_FP8_TILES, t.rows, t.cols, s};
@@ -158,6 +161,7 @@ int wush_gemm_fp8(const uint8_t* xq, const float* xs, const uint8_t* wq, const f
     g.N = (int)N;
     g.K = (int)K;
     g.splits = p.splits;
+    g.once = M <= p.rows;
     if (p.rows < 256 && p.cols == 256) return wush::launch_gemm_fp8_runs(g, p.rows, stream);
     return wush::launch_gemm_fp8(g, p.rows, p.cols, stream);
 }

@@ -49,7 +49,8 @@ __device__ __forceinline__ void wait_all_but(int stages) {
 // kPlain: one matrix.  kRows: each expert's, over its rows.
 enum { kPlain, kRows };
 
-template <int RB, int CB, int WR, int WC, int NB, int BR, int OCC, int MODE, int OUT, bool F16>
+// NT: one row tile, whose weights are read once.
+template <int RB, int CB, int WR, int WC, int NB, int BR, int OCC, int MODE, int OUT, bool F16, bool NT>
 __global__ __launch_bounds__(64 * WR * WC) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
 void gemm_fp8_kernel(const Fp8Gemm g) {
     constexpr int NW = WR * WC, TR = 16 * RB * WR, TC = 16 * CB * WC;
@@ -162,6 +163,7 @@ void gemm_fp8_kernel(const Fp8Gemm g) {
         const size_t o = (size_t)at * 128;
         const uint32_t v = voff[k] - (tail && at == KB - 1 ? past[k >= DA][(k < DA ? k : k - DA) & 1] : 0u);
         if (k < DA) dma16_uniform(abase + o, v, dst + (wave * DA + k) * 1024);
+        else if constexpr (NT) dma16_uniform_nt(bbase + o, v, dst + kA + (wave * DB + k - DA) * 1024);
         else dma16_uniform(bbase + o, v, dst + kA + (wave * DB + k - DA) * 1024);
     };
 
@@ -405,18 +407,24 @@ __global__ __launch_bounds__(256) void fp8_sum_kernel(const float* __restrict__ 
 template <int RB, int CB, int WR, int WC, int NB, int BR, int OCC>
 int launch_plain(const Fp8Gemm& g, unsigned grid, hipStream_t stream) {
     constexpr int T = 64 * WR * WC;
-    if (g.out == WUSH_DTYPE_BF16)
-        gemm_fp8_kernel<RB, CB, WR, WC, NB, BR, OCC, kPlain, WUSH_DTYPE_BF16, false><<<grid, T, 0, stream>>>(g);
-    else
-        gemm_fp8_kernel<RB, CB, WR, WC, NB, BR, OCC, kPlain, WUSH_DTYPE_F16, false><<<grid, T, 0, stream>>>(g);
+    constexpr int BF = WUSH_DTYPE_BF16, HF = WUSH_DTYPE_F16;
+    const bool bf = g.out == BF;
+    if (g.M <= 16 * RB * WR) {
+        if (bf) gemm_fp8_kernel<RB, CB, WR, WC, NB, BR, OCC, kPlain, BF, false, true><<<grid, T, 0, stream>>>(g);
+        else gemm_fp8_kernel<RB, CB, WR, WC, NB, BR, OCC, kPlain, HF, false, true><<<grid, T, 0, stream>>>(g);
+    } else {
+        if (bf) gemm_fp8_kernel<RB, CB, WR, WC, NB, BR, OCC, kPlain, BF, false, false><<<grid, T, 0, stream>>>(g);
+        else gemm_fp8_kernel<RB, CB, WR, WC, NB, BR, OCC, kPlain, HF, false, false><<<grid, T, 0, stream>>>(g);
+    }
     return (int)hipGetLastError();
 }
 
+// experts' tiles are for few rows each: mostly one tile an expert
 template <int RB, int CB, int WR, int WC, int NB, int BR>
 int launch_rows(const Fp8Gemm& g, unsigned grid, hipStream_t stream) {
     constexpr int T = 64 * WR * WC;
-    if (g.wide) gemm_fp8_kernel<RB, CB, WR, WC, NB, BR, 1, kRows, kOutF32, true><<<grid, T, 0, stream>>>(g);
-    else gemm_fp8_kernel<RB, CB, WR, WC, NB, BR, 1, kRows, kOutF32, false><<<grid, T, 0, stream>>>(g);
+    if (g.wide) gemm_fp8_kernel<RB, CB, WR, WC, NB, BR, 1, kRows, kOutF32, true, true><<<grid, T, 0, stream>>>(g);
+    else gemm_fp8_kernel<RB, CB, WR, WC, NB, BR, 1, kRows, kOutF32, false, true><<<grid, T, 0, stream>>>(g);
     return (int)hipGetLastError();
 }
 

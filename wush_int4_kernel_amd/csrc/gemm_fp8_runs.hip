@@ -47,7 +47,7 @@ __device__ __forceinline__ void rows_transpose(uint32_t (&v)[4]) {
     }
 }
 
-template <int RB, int WR, int WC, int NB, int MODE, bool BF16, bool F16>
+template <int RB, int WR, int WC, int NB, int MODE, bool BF16, bool F16, bool NT>
 __global__ __launch_bounds__(64 * WR * WC) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void gemm_fp8_runs_kernel(const Fp8Gemm g) {
     constexpr int NW = WR * WC, TR = 16 * RB * WR, TC = 256;
@@ -187,7 +187,8 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
         } else if constexpr (k < DA) {
             dma16_uniform(ia, voff[k] - (DA & 1 ? pastx : past[k & 1]), idst + (wave * DA + k) * 1024);
         } else {
-            dma16_uniform(ib, voff[k] - past[(k - DA) & 1], idst + kA + (wave * DB + k - DA) * 1024);
+            if constexpr (NT) dma16_uniform_nt(ib, voff[k] - past[(k - DA) & 1], idst + kA + (wave * DB + k - DA) * 1024);
+            else dma16_uniform(ib, voff[k] - past[(k - DA) & 1], idst + kA + (wave * DB + k - DA) * 1024);
         }
     };
     static_assert((DA == 1 || DA % 2 == 0) && DB % 2 == 0);
@@ -461,15 +462,15 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
     WUSH_WAIT_VMCNT(0);                          // no load may reach LDS that is another workgroup's by then
 }
 
-template <int RB>
+template <int RB, bool NT>
 int launch(const Fp8Gemm& g, unsigned grid, hipStream_t stream) {
     constexpr int WR = 2, WC = 4, NB = 3, T = 64 * WR * WC;
-    if (g.act && g.wide) gemm_fp8_runs_kernel<RB, WR, WC, NB, kAct, false, true><<<grid, T, 0, stream>>>(g);
-    else if (g.act) gemm_fp8_runs_kernel<RB, WR, WC, NB, kAct, false, false><<<grid, T, 0, stream>>>(g);
-    else if (g.tiles && g.shared) gemm_fp8_runs_kernel<RB, WR, WC, NB, kShared, false, false><<<grid, T, 0, stream>>>(g);
-    else if (g.tiles) gemm_fp8_runs_kernel<RB, WR, WC, NB, kWide, false, false><<<grid, T, 0, stream>>>(g);
-    else if (g.out == WUSH_DTYPE_BF16) gemm_fp8_runs_kernel<RB, WR, WC, NB, kPlain, true, false><<<grid, T, 0, stream>>>(g);
-    else gemm_fp8_runs_kernel<RB, WR, WC, NB, kPlain, false, false><<<grid, T, 0, stream>>>(g);
+    if (g.act && g.wide) gemm_fp8_runs_kernel<RB, WR, WC, NB, kAct, false, true, NT><<<grid, T, 0, stream>>>(g);
+    else if (g.act) gemm_fp8_runs_kernel<RB, WR, WC, NB, kAct, false, false, NT><<<grid, T, 0, stream>>>(g);
+    else if (g.tiles && g.shared) gemm_fp8_runs_kernel<RB, WR, WC, NB, kShared, false, false, NT><<<grid, T, 0, stream>>>(g);
+    else if (g.tiles) gemm_fp8_runs_kernel<RB, WR, WC, NB, kWide, false, false, NT><<<grid, T, 0, stream>>>(g);
+    else if (g.out == WUSH_DTYPE_BF16) gemm_fp8_runs_kernel<RB, WR, WC, NB, kPlain, true, false, NT><<<grid, T, 0, stream>>>(g);
+    else gemm_fp8_runs_kernel<RB, WR, WC, NB, kPlain, false, false, NT><<<grid, T, 0, stream>>>(g);
     return (int)hipGetLastError();
 }
 
@@ -483,7 +484,8 @@ int launch_gemm_fp8_runs(const Fp8Gemm& g, int tile_rows, hipStream_t stream) {
     const long long tiles = rows * (g.act ? g.N / 256 : (g.N + 255) / 256);
     WUSH_REQUIRE(tiles <= 0x7fffffffLL);
     const unsigned grid = (unsigned)(tiles < kFp8Workgroups ? tiles : kFp8Workgroups);
-    return tile_rows == 64 ? launch<2>(g, grid, stream) : launch<4>(g, grid, stream);
+    if (tile_rows == 64) return g.once ? launch<2, true>(g, grid, stream) : launch<2, false>(g, grid, stream);
+    return g.once ? launch<4, true>(g, grid, stream) : launch<4, false>(g, grid, stream);
 }
 
 }  // namespace wush

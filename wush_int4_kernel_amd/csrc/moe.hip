@@ -9,6 +9,7 @@
 // Experts: rows of x by expert; a = q(x) up_e^T, h = silu(a_gate) a_up, o = q(h) down_e^T, y = sum of w o over a
 // token's experts.  a, h and o are kept in fp32, h and x quantized as in fp8_device.h.
 #include <cmath>
+#include <type_traits>
 
 #include "fp8.h"
 #include "fp8_device.h"
@@ -20,25 +21,59 @@ namespace {
 // ------------------------------------------------------------------- the router
 typedef unsigned long long u64;
 
-// Order of doubles as that of unsigned integers; NaN below all, 0 left for "not there".
+// Order of floats (doubles) as that of unsigned integers; NaN below all, 0 left for "not there".
+__device__ __forceinline__ uint32_t order_key(float c) {
+    if (c != c) return 1;
+    const uint32_t b = __float_as_uint(c + 0.0f);                // -0 is 0
+    return b >> 31 ? ~b : b | 1u << 31;
+}
 __device__ __forceinline__ u64 order_key(double c) {
     if (c != c) return 1;
-    const u64 b = __builtin_bit_cast(u64, c + 0.0);              // -0 is 0
+    const u64 b = __builtin_bit_cast(u64, c + 0.0);
     return b >> 63 ? ~b : b | 1ull << 63;
 }
+__device__ __forceinline__ float order_value(uint32_t key) {
+    return key <= 1 ? __builtin_nanf("") : __uint_as_float(key >> 31 ? key & ~(1u << 31) : ~key);
+}
 __device__ __forceinline__ double order_value(u64 key) {
-    if (key <= 1) return __builtin_nan("");
-    return __builtin_bit_cast(double, key >> 63 ? key & ~(1ull << 63) : ~key);
+    return key <= 1 ? __builtin_nan("") : __builtin_bit_cast(double, key >> 63 ? key & ~(1ull << 63) : ~key);
 }
 __device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
-__device__ __forceinline__ double lane_value(double v, int lane) {
-    const u64 b = __builtin_bit_cast(u64, v);
-    return __builtin_bit_cast(double, (u64)lane_value((uint32_t)(b >> 32), lane) << 32 | lane_value((uint32_t)b, lane));
+__device__ __forceinline__ u64 lane_value(u64 v, int lane) {
+    return (u64)lane_value((uint32_t)(v >> 32), lane) << 32 | lane_value((uint32_t)v, lane);
+}
+
+// Maximum over the wavefront, in every lane: rows by DPP as in row16_max, row_bcast:15 and :31 fold them into the last
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ uint32_t dpp_max_rows(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROW_MASK, 0xf, false));
 }
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d));
-    return v;
+    v = dpp_max_rows<0x143, 0xc>(dpp_max_rows<0x142, 0xa>(row16_max(v)));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+// The first of the lanes with the largest key, equal ones by `least`
+__device__ __forceinline__ u64 first_of(bool me, int e) {
+    const uint32_t least = ~wave_max_u32(me ? ~(uint32_t)e : 0);
+    return __ballot(me && (uint32_t)e == least);
+}
+__device__ __forceinline__ int wave_first_largest(uint32_t key, int e) {
+    const uint32_t top = wave_max_u32(key);
+    u64 who = __ballot(key == top);
+    if (who & (who - 1)) who = first_of(key == top, e);
+    return (int)__builtin_ctzll(who);
+}
+__device__ __forceinline__ int wave_first_largest(u64 key, int e) {
+    const uint32_t hi = (uint32_t)(key >> 32), top = wave_max_u32(hi);
+    u64 who = __ballot(hi == top);
+    if (who & (who - 1)) {                       // several lanes: the low words, then the index
+        const bool me = hi == top;
+        const uint32_t lo = wave_max_u32(me ? (uint32_t)key : 0);
+        const bool still = me && (uint32_t)key == lo;
+        who = __ballot(still);
+        if (who & (who - 1)) who = first_of(still, e);
+    }
+    return (int)__builtin_ctzll(who);
 }
 
 struct RouteArgs {
@@ -53,79 +88,91 @@ struct RouteArgs {
     float scale;
 };
 
-// A wavefront per row.  Lane group * lanes + sub holds experts group * size + sub + lanes * i.
-template <int V, int DT>
+template <int DT>
+__device__ __forceinline__ float logit(const RouteArgs& p, int64_t row, int e) {
+    if constexpr (DT == WUSH_DTYPE_F32) return static_cast<const float*>(p.logits)[row * p.stride + e];
+    const uint32_t w = static_cast<const uint16_t*>(p.logits)[row * p.stride + e];
+    return DT == WUSH_DTYPE_BF16 ? bf16_to_f32(w) : f16_to_f32(w);
+}
+__device__ __forceinline__ double sigmoid64(float x) { return 1.0 / (1.0 + exp(-(double)x)); }
+
+// A wavefront per row.  Lane group * lanes + sub holds experts group * size + sub + lanes * i.  With a bias, keys are
+// those of the biased scores in 64 bits.  Without one (BIAS false) the logits order the experts as the scores do:
+// 32-bit keys of logits, and scores of the chosen ones only, and of all for softmax's sum.
+template <int V, int DT, bool BIAS>
 __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs p) {
+    typedef std::conditional_t<BIAS, u64, uint32_t> Key;
     const int lane = threadIdx.x & 63;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= p.rows) return;
-    const int group = lane / p.lanes, sub = lane % p.lanes;
+    const int group = lane / p.lanes, sub = lane & (p.lanes - 1), first = group * p.size + sub;
     float x[V];
     bool in[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int o = sub + p.lanes * i, e = group * p.size + o;
-        in[i] = group < p.groups && o < p.size;
-        x[i] = -__builtin_inff();
-        if (in[i]) {
-            if constexpr (DT == WUSH_DTYPE_F32) x[i] = static_cast<const float*>(p.logits)[row * p.stride + e];
-            else {
-                const uint32_t w = static_cast<const uint16_t*>(p.logits)[row * p.stride + e];
-                x[i] = DT == WUSH_DTYPE_BF16 ? bf16_to_f32(w) : f16_to_f32(w);
-            }
-        }
+        in[i] = group < p.groups && sub + p.lanes * i < p.size;
+        x[i] = in[i] ? logit<DT>(p, row, first + p.lanes * i) : -__builtin_inff();
     }
-    double s[V], total = 1.0;
-    if (p.sigmoid) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) s[i] = 1.0 / (1.0 + exp(-(double)x[i]));
-    } else {
-        float mx = x[0];
-        bool nan = x[0] != x[0];
-#pragma unroll
-        for (int i = 1; i < V; ++i) {
-            mx = fmaxf(mx, x[i]);
-            nan |= x[i] != x[i];
-        }
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
-        nan = __any(nan) || mx == __builtin_inff();              // inf - inf
-        const bool none = mx == -__builtin_inff();               // nothing but -inf: every score 0
-        total = 0.0;
+    // softmax: the largest logit, whether the scores are NaN (inf - inf among them), and their sum where it is needed
+    float mx = 0.0f;
+    bool bad = false;
+    double total = 1.0;
+    if (!p.sigmoid) {
+        uint32_t top = 0;
+        bool nan = false;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            s[i] = nan ? __builtin_nan("") : none ? 0.0 : exp((double)x[i] - (double)mx);
-            total += in[i] ? s[i] : 0.0;
+            top = max(top, order_key(x[i]));
+            nan |= x[i] != x[i];
         }
+        mx = order_value(wave_max_u32(top));
+        bad = __any(nan) || mx == __builtin_inff();
+        if (!bad && mx == -__builtin_inff()) mx = 0.0f;          // nothing but -inf: every score 0
+        if (BIAS || !p.renorm) {
+            total = 0.0;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
-        if (none && !nan) total = 1.0;
+            for (int i = 0; i < V; ++i) total += exp((double)x[i] - (double)mx);
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+            if (total == 0.0) total = 1.0;
+        }
     }
-    // without a bias the order of exp(x - max) is that of the scores
-    u64 key[V];
+    Key key[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int e = group * p.size + sub + p.lanes * i;
-        double c = s[i];
-        if (p.bias && in[i]) c = (p.sigmoid ? s[i] : s[i] / total) + (double)p.bias[e];
-        key[i] = in[i] ? order_key(c) : 0;
+        if constexpr (BIAS) {
+            double c = __builtin_nan("");
+            if (in[i] && !bad) c = (p.sigmoid ? sigmoid64(x[i]) : exp((double)x[i] - (double)mx) / total) + (double)p.bias[first + p.lanes * i];
+            key[i] = in[i] ? order_key(c) : 0;
+        } else {
+            key[i] = in[i] ? bad ? 1u : order_key(x[i]) : 0u;
+        }
     }
     if (p.groups > 1) {
-        u64 a = 0, b = 0;                        // the group's two largest
+        Key a = 0, b = 0;                        // the group's two largest
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             b = max(b, min(a, key[i]));
             a = max(a, key[i]);
         }
         for (int d = 1; d < p.lanes; d <<= 1) {
-            const u64 oa = __shfl_xor(a, d), ob = __shfl_xor(b, d);
+            const Key oa = __shfl_xor(a, d), ob = __shfl_xor(b, d);
             b = max(min(a, oa), max(b, ob));
             a = max(a, oa);
         }
-        const u64 score = p.best == 2 ? order_key(order_value(a) + order_value(b)) : a;
+        u64 score = a;
+        if (p.best == 2) {
+            if constexpr (BIAS) {
+                score = order_key(order_value(a) + order_value(b));
+            } else if (p.sigmoid) {
+                score = order_key(sigmoid64(order_value(a)) + sigmoid64(order_value(b)));
+            } else {
+                score = bad ? 1 : order_key(exp((double)order_value(a) - (double)mx) + exp((double)order_value(b) - (double)mx));
+            }
+        }
         int above = 0;
         for (int g = 0; g < p.groups; ++g) {
-            const u64 o = (u64)lane_value((uint32_t)(score >> 32), g * p.lanes) << 32 | lane_value((uint32_t)score, g * p.lanes);
+            const u64 o = lane_value(score, g * p.lanes);
             above += o > score || (o == score && g < group);
         }
         if (above >= p.keep) {
@@ -134,60 +181,57 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs p) {
         }
     }
     int id = 0;                                  // lane j: choice j
-    double w = 0.0, sum = 0.0;
     for (int j = 0; j < p.k; ++j) {
-        u64 top = key[0];
+        Key top = key[0];
         int at = 0;
-        double sc = s[0];
 #pragma unroll
         for (int i = 1; i < V; ++i)
             if (key[i] > top) {
                 top = key[i];
                 at = i;
-                sc = s[i];
             }
-        const uint32_t hi = wave_max_u32((uint32_t)(top >> 32));
-        u64 who = __ballot((uint32_t)(top >> 32) == hi);
-        int e = group * p.size + sub + p.lanes * at;
-        if (who & (who - 1)) {                   // several lanes: the low words, then the index
-            const bool me = (uint32_t)(top >> 32) == hi;
-            const uint32_t lo = wave_max_u32(me ? (uint32_t)top : 0);
-            const bool still = me && (uint32_t)top == lo;
-            const uint32_t least = ~wave_max_u32(still ? ~(uint32_t)e : 0);
-            who = __ballot(still && (uint32_t)e == least);
-        }
-        const int winner = (int)__builtin_ctzll(who);
+        const int e = first + p.lanes * at, winner = wave_first_largest(top, e);
         const int chosen = (int)lane_value((uint32_t)e, winner);
-        const double score = lane_value(sc, winner);
-        sum += score;
-        if (lane == j) {
-            id = chosen;
-            w = score;
-        }
+        if (lane == j) id = chosen;
         if (lane == winner) {
 #pragma unroll
             for (int i = 0; i < V; ++i)
                 if (i == at) key[i] = 0;
         }
     }
-    if (lane < p.k) {
-        if (p.renorm) w = sum > 0.0 || sum != sum ? w / sum : 0.0;
-        else if (!p.sigmoid) w = w / total;
+    // the chosen ones' scores
+    const bool mine = lane < p.k;
+    const float c = mine ? logit<DT>(p, row, id) : 0.0f;
+    double w = !mine ? 0.0 : p.sigmoid ? sigmoid64(c) : bad ? __builtin_nan("") : exp((double)c - (double)mx);
+    if (p.renorm) {
+        double sum = w;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+        w = sum > 0.0 || sum != sum ? w / sum : 0.0;
+    } else {
+        w /= total;
+    }
+    if (mine) {
         p.weights[row * p.k + lane] = (float)(w * (double)p.scale);
         p.ids[row * p.k + lane] = id;
     }
 }
 
+template <int V, int DT>
+void launch_route_v(const RouteArgs& a, hipStream_t stream) {
+    const unsigned grid = (unsigned)((a.rows + 3) / 4);
+    if (a.bias) moe_route_kernel<V, DT, true><<<grid, 256, 0, stream>>>(a);
+    else moe_route_kernel<V, DT, false><<<grid, 256, 0, stream>>>(a);
+}
 template <int DT>
 int launch_route(const RouteArgs& a, hipStream_t stream) {
     const int v = (a.size + a.lanes - 1) / a.lanes;
-    const unsigned grid = (unsigned)((a.rows + 3) / 4);
-    if (v <= 1) moe_route_kernel<1, DT><<<grid, 256, 0, stream>>>(a);
-    else if (v <= 2) moe_route_kernel<2, DT><<<grid, 256, 0, stream>>>(a);
-    else if (v <= 4) moe_route_kernel<4, DT><<<grid, 256, 0, stream>>>(a);
-    else if (v <= 8) moe_route_kernel<8, DT><<<grid, 256, 0, stream>>>(a);
-    else if (v <= 16) moe_route_kernel<16, DT><<<grid, 256, 0, stream>>>(a);
-    else moe_route_kernel<32, DT><<<grid, 256, 0, stream>>>(a);
+    if (v <= 1) launch_route_v<1, DT>(a, stream);
+    else if (v <= 2) launch_route_v<2, DT>(a, stream);
+    else if (v <= 4) launch_route_v<4, DT>(a, stream);
+    else if (v <= 8) launch_route_v<8, DT>(a, stream);
+    else if (v <= 16) launch_route_v<16, DT>(a, stream);
+    else launch_route_v<32, DT>(a, stream);
     return (int)hipGetLastError();
 }
 
@@ -341,7 +385,7 @@ constexpr int64_t kRunPairs = 65536;
 
 struct ExpertsPlan {
     int64_t tokens, pairs;                       // of a run
-    bool few, fused, shared;                     // see experts_plan
+    bool few, fused, shared, once;                    // see experts_plan
     int tile_rows, tile_cols, most_tiles;
     size_t xq, xs, row_of, pos, tiles, ntiles, a, hq, hs, o, os, bytes;
 };
@@ -379,6 +423,7 @@ ExpertsPlan experts_plan(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, 
     p.shared = p.fused && dtype == WUSH_DTYPE_BF16;
     p.tile_rows = !p.fused ? 32 : rows <= 80 ? 64 : 128;
     p.tile_cols = p.fused ? 256 : 64;
+    p.once = rows <= 30;                         // mostly one tile an expert
     p.most_tiles = (int)(p.pairs / p.tile_rows + (p.pairs < E ? p.pairs : E));
     auto take = [&](size_t n) {
         const size_t at = p.bytes;
@@ -502,6 +547,7 @@ int wush_moe_experts_fp8(const void* x, int dtype, int64_t row_stride, const flo
         g.ntiles = ntiles;
         g.row_of = row_of;
         g.most_tiles = p.most_tiles;
+        g.once = p.once;
         g.act = p.fused;
         g.wide = !p.shared;
         g.y = p.fused ? static_cast<void*>(ws + p.hq) : a;
