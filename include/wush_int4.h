@@ -428,10 +428,10 @@ typedef struct wush_moe_choice {
 } wush_moe_choice;
 
 /* The router's choice for each row of logits (rows, experts), bf16, fp16 or fp32, rows `row_stride`
- * elements apart: scores s, choices by c = s + bias (experts fp32, or NULL), all in 64 bits; ids (rows, k) the k experts of
- * the largest c in the groups that stay, in falling order, equal ones by rising index; weights (rows, k) =
- * s[ids], with renorm divided by their sum (a sum of 0 gives zeros), times scale, rounded once.  A NaN counts below
- * every number.  A row of nothing but -inf has scores of 0; with softmax a NaN or +inf makes all of the row's scores NaN.
+ * elements apart: scores s, choices by c = s + bias (experts fp32, all in 64 bits), or by x itself where bias is NULL (groups by
+ * s still); ids (rows, k) the k experts of the largest c in the groups that stay, in falling order, equal ones by rising
+ * index; weights (rows, k) = s[ids], with renorm divided by their sum (a sum of 0 gives zeros), times scale, in
+ * 64 bits and rounded once.  A NaN counts below every number.  A row of nothing but -inf has scores of 0; with softmax a NaN or +inf makes all of the row's scores NaN.
  * experts <= 1024, groups <= 64, k <= 64. */
 int wush_moe_route(const void *logits, int dtype, int64_t row_stride, const float *bias, int64_t rows, int64_t experts,
                    const wush_moe_choice *choice, float *weights, int32_t *ids, hipStream_t stream);
@@ -440,7 +440,8 @@ int wush_moe_route(const void *logits, int dtype, int64_t row_stride, const floa
  * (an id out of [0, E) adds nothing).  x (T, H), rows row_stride elements apart, and y (T, H) bf16 or fp16; weights fp32
  * and ids int32 (T, k).  w_up codes (E, 2 I, H), the gate's I rows before the up projection's, s_up
  * (E, 2 I / 128, H / 128); w_down (E, H, I), s_down (E, H / 128, I / 128).  Both inner inputs are quantized as by
- * wush_quant_fp8_block, all between in fp32, y rounded once.  H % 16 == 0, I % 128 == 0, E <= 1024, k <= 64.  The workspace is 16-byte
+ * wush_quant_fp8_block, all else in fp32, but for an expert's rows of a bf16 y, which may be held in
+ * fp16 with a power of two for each 64 columns; y rounded once.  H % 16 == 0, I % 128 == 0, E <= 1024, k <= 64.  The workspace is 16-byte
  * aligned, of at least wush_moe_experts_fp8_workspace_bytes. */
 size_t wush_moe_experts_fp8_workspace_bytes(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, int dtype);
 int wush_moe_experts_fp8(const void *x, int dtype, int64_t row_stride, const float *weights, const int32_t *ids,

@@ -3,8 +3,8 @@
 //
 // Route: s = softmax(x) or sigmoid(x), c = s + bias; of each group of experts the sum of its best one or
 // two c, the best groups stay; ids are the k largest c left, equal ones by the lowest
-// index; weights s[ids], divided by their sum or not, times a factor.  Scores and sums are in 64
-// bits: in 32, of 16384 x 256 choices some would hang on a rounding.
+// index; weights s[ids], divided by their sum or not, times a factor.  Without a bias x itself orders the
+// experts; with one the choice is that of 64-bit scores.  Weights and their sums are in 64 bits.
 //
 // Experts: rows of x by expert; a = q(x) up_e^T, h = silu(a_gate) a_up, o = q(h) down_e^T, y = sum of w o over a
 // token's experts.  a, h and o are kept in fp32, h and x quantized as in fp8_device.h.
@@ -48,32 +48,18 @@ template <int CTRL, int ROW_MASK>
 __device__ __forceinline__ uint32_t dpp_max_rows(uint32_t v) {
     return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROW_MASK, 0xf, false));
 }
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     v = dpp_max_rows<0x143, 0xc>(dpp_max_rows<0x142, 0xa>(row16_max(v)));
     return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
-// The first of the lanes with the largest key, equal ones by `least`
-__device__ __forceinline__ u64 first_of(bool me, int e) {
-    const uint32_t least = ~wave_max_u32(me ? ~(uint32_t)e : 0);
-    return __ballot(me && (uint32_t)e == least);
+__device__ __forceinline__ u64 wave_max(u64 v) {
+    const uint32_t hi = wave_max((uint32_t)(v >> 32));
+    return (u64)hi << 32 | wave_max((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
 }
-__device__ __forceinline__ int wave_first_largest(uint32_t key, int e) {
-    const uint32_t top = wave_max_u32(key);
-    u64 who = __ballot(key == top);
-    if (who & (who - 1)) who = first_of(key == top, e);
-    return (int)__builtin_ctzll(who);
-}
-__device__ __forceinline__ int wave_first_largest(u64 key, int e) {
-    const uint32_t hi = (uint32_t)(key >> 32), top = wave_max_u32(hi);
-    u64 who = __ballot(hi == top);
-    if (who & (who - 1)) {                       // several lanes: the low words, then the index
-        const bool me = hi == top;
-        const uint32_t lo = wave_max_u32(me ? (uint32_t)key : 0);
-        const bool still = me && (uint32_t)key == lo;
-        who = __ballot(still);
-        if (who & (who - 1)) who = first_of(still, e);
-    }
-    return (int)__builtin_ctzll(who);
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+    return v;
 }
 
 struct RouteArgs {
@@ -83,130 +69,240 @@ struct RouteArgs {
     float* weights;
     int32_t* ids;
     int64_t rows;
-    int E, k, groups, size, keep, best, lanes;   // size: experts of a group; lanes: of a group, a power of two
+    int dtype, E, k, groups, size, keep, best;   // size: experts of a group
+    int lanes, shift;                            // of a group: a power of two, and its logarithm
     int sigmoid, renorm;
     float scale;
 };
 
-template <int DT>
 __device__ __forceinline__ float logit(const RouteArgs& p, int64_t row, int e) {
-    if constexpr (DT == WUSH_DTYPE_F32) return static_cast<const float*>(p.logits)[row * p.stride + e];
-    const uint32_t w = static_cast<const uint16_t*>(p.logits)[row * p.stride + e];
-    return DT == WUSH_DTYPE_BF16 ? bf16_to_f32(w) : f16_to_f32(w);
+    const int64_t at = row * p.stride + e;
+    if (p.dtype == WUSH_DTYPE_F32) return static_cast<const float*>(p.logits)[at];
+    const uint32_t w = static_cast<const uint16_t*>(p.logits)[at];
+    return p.dtype == WUSH_DTYPE_BF16 ? bf16_to_f32(w) : f16_to_f32(w);
 }
 __device__ __forceinline__ double sigmoid64(float x) { return 1.0 / (1.0 + exp(-(double)x)); }
 
-// A wavefront per row.  Lane group * lanes + sub holds experts group * size + sub + lanes * i.  With a bias, keys are
-// those of the biased scores in 64 bits.  Without one (BIAS false) the logits order the experts as the scores do:
-// 32-bit keys of logits, and scores of the chosen ones only, and of all for softmax's sum.
-template <int V, int DT, bool BIAS>
+// The k experts of the largest keys, equal ones by index, choice j and its key in lane j; `key` keeps what is not chosen.
+// One lane holds a maximum but for equal keys: a ballot names it, and only for those the indexes are compared too.
+// (Halving towards a border that k keys reach instead: 16384 x 256 23.5 us for 22.5, but 4096 x 128 in bf16, where
+// equal keys are common and take every step, 8.6 for 5.5.)
+template <int V, typename Key>
+__device__ __forceinline__ void largest(Key (&key)[V], int first, int lanes, int lane, int k, int& id, Key& taken) {
+    id = 0;
+    taken = 0;
+    for (int j = 0; j < k; ++j) {
+        Key top = key[0];
+        int e = first;
+#pragma unroll
+        for (int i = 1; i < V; ++i)
+            if (key[i] > top) {
+                top = key[i];
+                e = first + lanes * i;
+            }
+        const Key most = wave_max(top);
+        const u64 at = __ballot(top == most);
+        int chosen;
+        if (at & (at - 1)) chosen = (int)~wave_max(top == most ? ~(uint32_t)e : 0u);
+        else chosen = __builtin_amdgcn_readlane(e, __builtin_ctzll(at));
+        if (lane == j) {
+            id = chosen;
+            taken = most;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (first + lanes * i == chosen && key[i] == most) key[i] = 0;
+    }
+}
+
+// A group's two largest keys, in all of its lanes
+template <int V, typename Key>
+__device__ __forceinline__ void two_largest(const Key (&key)[V], int lanes, Key& a, Key& b) {
+    a = b = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        b = max(b, min(a, key[i]));
+        a = max(a, key[i]);
+    }
+    for (int d = 1; d < lanes; d <<= 1) {
+        const Key oa = __shfl_xor(a, d), ob = __shfl_xor(b, d);
+        b = max(min(a, oa), max(b, ob));
+        a = max(a, oa);
+    }
+}
+// Groups whose score is above that of this lane's, equal ones by index
+template <typename Key>
+__device__ __forceinline__ int groups_above(Key score, const RouteArgs& p, int group) {
+    int above = 0;
+    for (int g = 0; g < p.groups; ++g) {
+        const Key o = lane_value(score, g << p.shift);
+        above += o > score || (o == score && g < group);
+    }
+    return above;
+}
+
+// A wavefront per row.  Lane group * lanes + sub holds experts group * size + sub + lanes * i.
+// Without a bias (BIAS false) the logits order the experts as the scores do: 32-bit keys of logits, and scores of the
+// chosen ones only, and of all for softmax's sum.  With one, scores in 32 bits decide wherever they are further apart than their
+// errors: s is off by less than 2^-20 (a few units of the last bit; softmax, with a sum of up to 38 roundings, 2^-17), s + b by
+// 2^-23 |s + b| more, and a sum of two by twice that.  A row in which two that matter are nearer, or that holds what is not finite,
+// is chosen again in 64 bits.
+// 4096 x 128 bf16, 8 of them: 5.5 us.  16384 x 256 fp32 with a bias, 8 groups: 22.5 us (64 bits throughout: 28), where
+// the choices' chain of maxima and the chosen scores' exponentials bound it, not the 17 MB (3.4 us).  A row on 16 lanes instead
+// of 64, which shares that chain among four rows, takes 30: one row that is chosen again holds up three.
+template <int V, bool BIAS>
 __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs p) {
-    typedef std::conditional_t<BIAS, u64, uint32_t> Key;
     const int lane = threadIdx.x & 63;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= p.rows) return;
-    const int group = lane / p.lanes, sub = lane & (p.lanes - 1), first = group * p.size + sub;
-    float x[V];
+    const int group = lane >> p.shift, sub = lane & (p.lanes - 1), first = group * p.size + sub;
+    const bool there = group < p.groups;
+    float x[V], b[V];
     bool in[V];
+    int at[V];                                   // every lane loads, at once: no branches between the loads
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        in[i] = group < p.groups && sub + p.lanes * i < p.size;
-        x[i] = in[i] ? logit<DT>(p, row, first + p.lanes * i) : -__builtin_inff();
+        in[i] = there && sub + p.lanes * i < p.size;
+        at[i] = in[i] ? first + p.lanes * i : 0;
+    }
+    if (p.dtype == WUSH_DTYPE_F32) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = static_cast<const float*>(p.logits)[row * p.stride + at[i]];
+    } else {
+        uint32_t u[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) u[i] = static_cast<const uint16_t*>(p.logits)[row * p.stride + at[i]];
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = p.dtype == WUSH_DTYPE_BF16 ? bf16_to_f32(u[i]) : f16_to_f32(u[i]);
+    }
+    if constexpr (BIAS) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) b[i] = p.bias[at[i]];
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        if (!in[i]) x[i] = -__builtin_inff();
+        if (!BIAS || !in[i]) b[i] = 0.0f;
     }
     // softmax: the largest logit, whether the scores are NaN (inf - inf among them), and their sum where it is needed
     float mx = 0.0f;
-    bool bad = false;
-    double total = 1.0;
-    if (!p.sigmoid) {
+    bool bad = false, nan = false;
+    if (BIAS || !p.sigmoid) {
         uint32_t top = 0;
-        bool nan = false;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             top = max(top, order_key(x[i]));
             nan |= x[i] != x[i];
         }
-        mx = order_value(wave_max_u32(top));
-        bad = __any(nan) || mx == __builtin_inff();
-        if (!bad && mx == -__builtin_inff()) mx = 0.0f;          // nothing but -inf: every score 0
-        if (BIAS || !p.renorm) {
-            total = 0.0;
-#pragma unroll
-            for (int i = 0; i < V; ++i) total += exp((double)x[i] - (double)mx);
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
-            if (total == 0.0) total = 1.0;
+        nan = __any(nan);
+        if (!p.sigmoid) {
+            mx = order_value(wave_max(top));
+            bad = nan || mx == __builtin_inff();
+            if (!bad && mx == -__builtin_inff()) mx = 0.0f;      // nothing but -inf: every score 0
         }
     }
-    Key key[V];
+    double total = 1.0;
+    auto sum64 = [&] {
+        total = 0.0;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        if constexpr (BIAS) {
-            double c = __builtin_nan("");
-            if (in[i] && !bad) c = (p.sigmoid ? sigmoid64(x[i]) : exp((double)x[i] - (double)mx) / total) + (double)p.bias[first + p.lanes * i];
-            key[i] = in[i] ? order_key(c) : 0;
-        } else {
-            key[i] = in[i] ? bad ? 1u : order_key(x[i]) : 0u;
+        for (int i = 0; i < V; ++i) total += exp((double)x[i] - (double)mx);
+        total = wave_sum(total);
+        if (total == 0.0) total = 1.0;
+    };
+    if (!p.sigmoid && !p.renorm) sum64();
+
+    int id;                                      // lane j: choice j
+    if constexpr (!BIAS) {
+        uint32_t key[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) key[i] = in[i] ? bad ? 1u : order_key(x[i]) : 0u;
+        if (p.groups > 1) {
+            uint32_t one, two;
+            two_largest<V>(key, p.lanes, one, two);
+            int above;
+            if (p.best == 1) above = groups_above(one, p, group);
+            else if (p.sigmoid) above = groups_above(order_key(sigmoid64(order_value(one)) + sigmoid64(order_value(two))), p, group);
+            else above = groups_above(bad ? (u64)1 : order_key(exp((double)order_value(one) - (double)mx) + exp((double)order_value(two) - (double)mx)), p, group);
+            if (above >= p.keep) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) key[i] = 0;
+            }
         }
-    }
-    if (p.groups > 1) {
-        Key a = 0, b = 0;                        // the group's two largest
+        uint32_t taken;
+        largest<V>(key, first, p.lanes, lane, p.k, id, taken);
+    } else {
+        const float kApart = p.sigmoid ? 0x1p-19f : 0x1p-16f;    // twice the errors
+        constexpr float kPart = 0x1p-22f;
+        uint32_t key[V];
+        float sum = 0.0f, c[V];
+        bool odd = bad || nan, wild = false;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            b = max(b, min(a, key[i]));
-            a = max(a, key[i]);
+            // 1 / (1 + exp(-x)), or exp(x - max)
+            const float e = __builtin_amdgcn_exp2f((p.sigmoid ? -x[i] : x[i] - mx) * 1.44269504f);
+            c[i] = p.sigmoid ? __builtin_amdgcn_rcpf(1.0f + e) : e;
+            sum += c[i];
         }
-        for (int d = 1; d < p.lanes; d <<= 1) {
-            const Key oa = __shfl_xor(a, d), ob = __shfl_xor(b, d);
-            b = max(min(a, oa), max(b, ob));
-            a = max(a, oa);
+        const float by = p.sigmoid ? 1.0f : __builtin_amdgcn_rcpf(wave_sum_dpp(sum));
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            c[i] = c[i] * by + b[i];
+            wild |= in[i] && !(__builtin_fabsf(c[i]) < 0x1p100f);
+            key[i] = in[i] ? order_key(c[i]) : 0u;
         }
-        u64 score = a;
-        if (p.best == 2) {
-            if constexpr (BIAS) {
-                score = order_key(order_value(a) + order_value(b));
-            } else if (p.sigmoid) {
-                score = order_key(sigmoid64(order_value(a)) + sigmoid64(order_value(b)));
-            } else {
-                score = bad ? 1 : order_key(exp((double)order_value(a) - (double)mx) + exp((double)order_value(b) - (double)mx));
+        odd |= __any(wild);
+        if (p.groups > 1) {
+            uint32_t one, two;
+            two_largest<V>(key, p.lanes, one, two);
+            const uint32_t score = p.best == 1 ? one : order_key(order_value(one) + order_value(two));
+            const bool keep = groups_above(score, p, group) < p.keep;
+            // the least of the groups that stay and the largest of the others
+            const float last = order_value(~wave_max(keep && there ? ~score : 0u));
+            const uint32_t out = wave_max(!keep && there ? score : 0u);
+            odd |= out != 0 && !(last - order_value(out) > 2.0f * (kApart + kPart * __builtin_fabsf(last)));
+            if (!keep) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) key[i] = 0;
             }
         }
-        int above = 0;
-        for (int g = 0; g < p.groups; ++g) {
-            const u64 o = lane_value(score, g * p.lanes);
-            above += o > score || (o == score && g < group);
-        }
-        if (above >= p.keep) {
+        uint32_t taken;
+        largest<V>(key, first, p.lanes, lane, p.k, id, taken);
+        // each choice against the next, the last against the largest left
+        uint32_t rest = 0;
 #pragma unroll
-            for (int i = 0; i < V; ++i) key[i] = 0;
-        }
-    }
-    int id = 0;                                  // lane j: choice j
-    for (int j = 0; j < p.k; ++j) {
-        Key top = key[0];
-        int at = 0;
+        for (int i = 0; i < V; ++i) rest = max(rest, key[i]);
+        rest = wave_max(rest);
+        uint32_t next = (uint32_t)__shfl((int)taken, lane + 1);
+        if (lane == p.k - 1) next = rest;
+        const float v = order_value(taken);
+        odd |= __any(lane < p.k && next != 0 && !(v - order_value(next) > kApart + kPart * __builtin_fabsf(v)));
+        if (odd) {
+            if (!p.sigmoid && p.renorm) sum64();
+            u64 key[V];
 #pragma unroll
-        for (int i = 1; i < V; ++i)
-            if (key[i] > top) {
-                top = key[i];
-                at = i;
+            for (int i = 0; i < V; ++i) {
+                double c = __builtin_nan("");
+                if (in[i] && !bad) c = (p.sigmoid ? sigmoid64(x[i]) : exp((double)x[i] - (double)mx) / total) + (double)b[i];
+                key[i] = in[i] ? order_key(c) : 0;
             }
-        const int e = first + p.lanes * at, winner = wave_first_largest(top, e);
-        const int chosen = (int)lane_value((uint32_t)e, winner);
-        if (lane == j) id = chosen;
-        if (lane == winner) {
+            if (p.groups > 1) {
+                u64 one, two;
+                two_largest<V>(key, p.lanes, one, two);
+                if (groups_above(p.best == 1 ? one : order_key(order_value(one) + order_value(two)), p, group) >= p.keep) {
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (i == at) key[i] = 0;
+                    for (int i = 0; i < V; ++i) key[i] = 0;
+                }
+            }
+            u64 taken;
+            largest<V>(key, first, p.lanes, lane, p.k, id, taken);
         }
     }
     // the chosen ones' scores
     const bool mine = lane < p.k;
-    const float c = mine ? logit<DT>(p, row, id) : 0.0f;
+    const float c = mine ? logit(p, row, id) : 0.0f;
     double w = !mine ? 0.0 : p.sigmoid ? sigmoid64(c) : bad ? __builtin_nan("") : exp((double)c - (double)mx);
     if (p.renorm) {
-        double sum = w;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+        const double sum = wave_sum(w);
         w = sum > 0.0 || sum != sum ? w / sum : 0.0;
     } else {
         w /= total;
@@ -217,21 +313,20 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs p) {
     }
 }
 
-template <int V, int DT>
+template <int V>
 void launch_route_v(const RouteArgs& a, hipStream_t stream) {
     const unsigned grid = (unsigned)((a.rows + 3) / 4);
-    if (a.bias) moe_route_kernel<V, DT, true><<<grid, 256, 0, stream>>>(a);
-    else moe_route_kernel<V, DT, false><<<grid, 256, 0, stream>>>(a);
+    if (a.bias) moe_route_kernel<V, true><<<grid, 256, 0, stream>>>(a);
+    else moe_route_kernel<V, false><<<grid, 256, 0, stream>>>(a);
 }
-template <int DT>
 int launch_route(const RouteArgs& a, hipStream_t stream) {
     const int v = (a.size + a.lanes - 1) / a.lanes;
-    if (v <= 1) launch_route_v<1, DT>(a, stream);
-    else if (v <= 2) launch_route_v<2, DT>(a, stream);
-    else if (v <= 4) launch_route_v<4, DT>(a, stream);
-    else if (v <= 8) launch_route_v<8, DT>(a, stream);
-    else if (v <= 16) launch_route_v<16, DT>(a, stream);
-    else launch_route_v<32, DT>(a, stream);
+    if (v <= 1) launch_route_v<1>(a, stream);
+    else if (v <= 2) launch_route_v<2>(a, stream);
+    else if (v <= 4) launch_route_v<4>(a, stream);
+    else if (v <= 8) launch_route_v<8>(a, stream);
+    else if (v <= 16) launch_route_v<16>(a, stream);
+    else launch_route_v<32>(a, stream);
     return (int)hipGetLastError();
 }
 
@@ -482,13 +577,16 @@ int wush_moe_route(const void* logits, int dtype, int64_t row_stride, const floa
     a.keep = c.keep_groups;
     a.best = c.group_best;
     a.lanes = 64;
-    while (a.lanes * c.groups > 64) a.lanes >>= 1;
+    a.shift = 6;
+    while (a.lanes * c.groups > 64) {
+        a.lanes >>= 1;
+        --a.shift;
+    }
+    a.dtype = dtype;
     a.sigmoid = c.sigmoid != 0;
     a.renorm = c.renorm != 0;
     a.scale = c.scale;
-    if (dtype == WUSH_DTYPE_BF16) return wush::launch_route<WUSH_DTYPE_BF16>(a, stream);
-    if (dtype == WUSH_DTYPE_F16) return wush::launch_route<WUSH_DTYPE_F16>(a, stream);
-    return wush::launch_route<WUSH_DTYPE_F32>(a, stream);
+    return wush::launch_route(a, stream);
 }
 
 size_t wush_moe_experts_fp8_workspace_bytes(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, int dtype) {
