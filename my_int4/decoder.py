@@ -9,6 +9,10 @@ The parts, in the order in which a step runs them:
   norm -> W4A4 step of my_int4.chain (WUSH transform, quantization, product)
        -> activation -> w8a8_linear (down projection) -> add
 
+or, in a layer of experts, for the second line:
+
+  norm -> router -> moe_route -> fp8_experts (beside fp8_linear for a shared expert) -> add
+
 The same call takes one new token per sequence (decode) or many (prefill, or a
 chunk of it): ``cu_q`` says where each sequence's tokens begin.  Nothing in it
 synchronizes, so a decode step can be captured with ``my_int4.chain.graphed``
@@ -30,6 +34,15 @@ def quant_weight_int8(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     wf = w.float()
     s = (wf.abs().amax(1) / 127).clamp_min(2.0 ** -126)
     return (wf / s[:, None]).round().clamp(-127, 127).to(torch.int8), s
+
+
+def quant_weight_fp8(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(..., N, K) weights -> e4m3 codes and an fp32 scale per block of 128 x 128, (..., N / 128, K / 128)."""
+    N, K = w.shape[-2:]
+    b = torch.nn.functional.pad(w.float(), (0, -K % 128, 0, -N % 128)).unflatten(-1, (-1, 128)).unflatten(-3, (-1, 128))
+    s = (b.abs().amax((-3, -1)) / 448).clamp_min(2.0 ** -126)                # b: (..., N / 128, 128, K / 128, 128)
+    q = (b / s[..., :, None, :, None]).flatten(-2).flatten(-3, -2)[..., :N, :K]
+    return q.contiguous().to(torch.float8_e4m3fn), s
 
 
 def rotation_table(positions: int, channels: int, theta: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -86,19 +99,53 @@ def _norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5) -> torch.Ten
 
 
 @dataclass
+class ExpertLayer:
+    """A router and its gated experts, weights as (codes, scales) of quant_weight_fp8: ``up`` (experts, 2 I, K), each
+    gate's rows before its up projection's, ``down`` (experts, K, I); ``shared`` the same two of an expert that
+    every token takes.  A process that holds some of the experts only (expert parallelism) has their
+    weights here, all experts' router, and the first one's number in ``first``: the others' choices add nothing."""
+    router: torch.Tensor                                       # (all experts, K) fp32
+    k: int
+    up: Tuple[torch.Tensor, torch.Tensor]
+    down: Tuple[torch.Tensor, torch.Tensor]
+    bias: Optional[torch.Tensor] = None
+    sigmoid: bool = False
+    groups: int = 1
+    keep_groups: int = 1
+    group_best: int = 1
+    renorm: bool = True
+    scale: float = 1.0
+    shared: Optional[Tuple[Tuple[torch.Tensor, torch.Tensor], Tuple[torch.Tensor, torch.Tensor]]] = None
+    first: int = 0
+
+    def __call__(self, x: torch.Tensor) -> torch.Tensor:
+        """x (tokens, K) bf16 or fp16 -> the weighted sum of its experts."""
+        logits = torch.nn.functional.linear(x.float(), self.router)
+        weights, ids = _C.moe_route(logits, self.k, bias=self.bias, sigmoid=self.sigmoid, groups=self.groups,
+                                    keep_groups=self.keep_groups, group_best=self.group_best, renorm=self.renorm, scale=self.scale)
+        y = _C.fp8_experts(x, weights, ids - self.first if self.first else ids, *self.up, *self.down)
+        if self.shared is not None:
+            gate, up = _C.fp8_linear(x, *self.shared[0]).float().chunk(2, -1)
+            y = y + _C.fp8_linear((torch.nn.functional.silu(gate) * up).to(x.dtype), *self.shared[1])
+        return y
+
+
+@dataclass
 class DecoderLayer:
     """Weights of a layer: W8A8 projections as (codes, scales) of
-    quant_weight_int8, the up projection as W4A4 codes, scales and transform."""
+    quant_weight_int8, the up projection as W4A4 codes, scales and transform; with ``experts``, those instead of
+    ``up`` and ``down``."""
     q_heads: int
     kv_heads: int
     qkv: Tuple[torch.Tensor, torch.Tensor]
     out: Tuple[torch.Tensor, torch.Tensor]
-    up: Tuple[torch.Tensor, torch.Tensor, torch.Tensor]        # (transform, wq, ws)
-    down: Tuple[torch.Tensor, torch.Tensor]
+    up: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]]        # (transform, wq, ws)
+    down: Optional[Tuple[torch.Tensor, torch.Tensor]]
     norm1: torch.Tensor
     norm2: torch.Tensor
     window: int = 0
     softcap: float = 0.0
+    experts: Optional[ExpertLayer] = None
 
     def attention(self, x, cache: KV8Cache, cos_sin, block_table, seq_lens, cu_q: Optional[torch.Tensor] = None,
                   max_len: int = 0) -> torch.Tensor:
@@ -116,6 +163,8 @@ class DecoderLayer:
         """x (tokens, K) bf16 -> the layer's output, the new tokens' keys and
         values in the cache.  seq_lens counts them."""
         x = self.attention(x, cache, cos_sin, block_table, seq_lens, cu_q, max_len)
+        if self.experts is not None:
+            return x + self.experts(_norm(x, self.norm2))
         h = make_chain(_norm(x, self.norm2), *self.up)().view(x.shape[0], -1)     # fp16
         h = torch.nn.functional.gelu(h.float()).to(x.dtype)
         return x + _C.w8a8_linear(h, *self.down)
