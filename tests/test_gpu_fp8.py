@@ -185,6 +185,28 @@ def test_nan_code_stays_in_its_column(dev):
         assert torch.equal(y[:, keep], clean[:, keep])
 
 
+@pytest.mark.parametrize("M,N,K", [(640, 32768, 256), (300, 65536, 144), (60, 131072, 128)])
+def test_non_finite_rows_and_scales_stay_alone_from_tile_to_tile(dev, M, N, K):
+    # more tiles than workgroups, one after another
+    from my_int4 import _C
+    g = gen(31)
+    x = acts(g, M, K).to(dev)
+    w, ws = plain.weights(g, N, K, dev=dev)
+    clean = _C.fp8_linear(x, w, ws)
+    bad = x.clone()
+    bad[::7, 3] = math.inf
+    y = _C.fp8_linear(bad, w, ws)
+    keep = torch.ones(M, dtype=torch.bool, device=dev)
+    keep[::7] = False
+    assert torch.isnan(y[~keep]).all()
+    assert torch.equal(y[keep], clean[keep])
+    ws[::5, 0] = math.nan
+    y = _C.fp8_linear(x, w, ws)
+    cols = (torch.arange(N, device=dev) // 128) % 5 == 0
+    assert torch.isnan(y[:, cols]).all()
+    assert torch.equal(y[:, ~cols], clean[:, ~cols])
+
+
 def test_graph_and_stream(dev):
     from my_int4 import _C
     g = gen(8)

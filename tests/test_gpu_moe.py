@@ -216,6 +216,20 @@ def test_experts_non_finite_tokens_stay_alone(dev):
         assert torch.equal(y[keep], clean[keep])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,E", [(1300, 64), (2700, 8)])
+def test_experts_non_finite_tokens_stay_alone_from_tile_to_tile(dev, T, E, dtype):
+    # more tiles than workgroups, one after another
+    from my_int4 import _C
+    args = case(10, T, E, 2, 2048, 1024, dev, dtype=dtype)
+    clean = _C.fp8_experts(*args)
+    args[0][::9, 200] = math.inf
+    y = _C.fp8_experts(*args)
+    bad = torch.arange(T, device=dev) % 9 == 0
+    assert torch.isnan(y[bad]).all()
+    assert torch.equal(y[~bad], clean[~bad])
+
+
 def test_route_and_experts_in_a_graph(dev):
     from my_int4 import _C
     for T in (1, 24, 300):

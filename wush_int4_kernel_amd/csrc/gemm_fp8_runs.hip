@@ -241,10 +241,10 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
             for (int j = 0; j < CB; ++j) acc[i][j] = (v4f){0, 0, 0, 0};
 #pragma unroll
         for (int t = 0; t < (F16 ? 2 * RB : kTmp); ++t) tmp[t] = (v4f){0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < RB; ++i) sc[NSW - 1][i] = 0.0f;      // the last tile's may be NaN, which no zero product undoes
     };
     clear();
-#pragma unroll
-    for (int i = 0; i < RB; ++i) sc[NSW - 1][i] = 0.0f;
     WUSH_WAIT_VMCNT(0);
     WUSH_LDS_BARRIER();
     __builtin_amdgcn_sched_barrier(0);
