@@ -263,6 +263,13 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
         for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(t[r], s[i], acc[i][j][r]);
         asm volatile("" : "+v"(acc[i][j]));      // here, and not where the compiler finds its next use
     };
+    // the next stage has landed in all wavefronts' view, and all have read this one's columns
+    auto next_landed = [&](auto first) {
+        WUSH_WAIT_VMCNT((NB - 2) * ND + (first.value ? kStores : 0));
+        WUSH_LDS_BARRIER();
+        aim(buf);
+        __builtin_amdgcn_sched_barrier(0);
+    };
     // One stage, whose buffer takes the next one to be issued.  Operands read past the last stage are not used.
     // FIRST: one of a tile's first NB - 1, the loads of whose successors were issued before the last tile's
     // kStores stores (loads and stores complete, for the counter, in the order of their issue).
@@ -283,13 +290,7 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
                 a[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
             }
         }
-        // the next stage has landed in all wavefronts' view, and all have read this one's columns
-        auto landed = [&] {
-            WUSH_WAIT_VMCNT((NB - 2) * ND + (first.value ? kStores : 0));
-            WUSH_LDS_BARRIER();
-            aim(buf);
-            __builtin_amdgcn_sched_barrier(0);
-        };
+        auto landed = [&] { next_landed(first); };
         auto refill_part = [&](auto qc, auto nc) {               // share q of n
             constexpr int q = qc.value, n = nc.value;
             static_for<(q + 1) * ND / n - q * ND / n>([&](auto dc) { issue(std::integral_constant<int, q * ND / n + dc.value>{}); });
@@ -345,6 +346,28 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
         asm volatile("" ::: "memory");           // the reads above stay above
         buf = nbuf;
         advance();
+    };
+    // One stage of a wavefront whose rows are all past the tile's last: its part of the loads only
+    auto idle_stage = [&](auto first) {
+        next_landed(first);
+        static_for<ND>(issue);
+        buf = buf + 1 == NB ? 0 : buf + 1;
+        advance();
+    };
+    auto idle_tile = [&] {
+        for (st = 0; st < min(NB - 1, KB); ++st) idle_stage(std::true_type{});
+        for (; st < KB; ++st) idle_stage(std::false_type{});
+        read_s(buf);
+#pragma unroll
+        for (int i = 0; i < RB; ++i) read_a(buf, i);
+#pragma unroll
+        for (int j = 0; j < BR - 1; ++j) read_b(buf, j);
+        if constexpr (MODE == kAct) {
+            WUSH_LDS_BARRIER();
+            WUSH_LDS_BARRIER();
+        }
+        WUSH_WAIT_VMCNT(0);                      // no stores: as below
+        __builtin_amdgcn_sched_barrier(0);
     };
     // The tile's outputs.  Rows past M hold what row M - 1 does, and are stored there.
     auto finish = [&] {
@@ -450,9 +473,13 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
     };
 
     for (;;) {
-        for (st = 0; st < min(NB - 1, KB); ++st) stage(std::true_type{});
-        for (; st < KB; ++st) stage(std::false_type{});
-        finish();
+        if (m0 + wr * RB * 16 < M) {
+            for (st = 0; st < min(NB - 1, KB); ++st) stage(std::true_type{});
+            for (; st < KB; ++st) stage(std::false_type{});
+            finish();
+        } else {
+            idle_tile();
+        }
         cur += step;
         if (cur >= run_end) break;
         place(cur, tm, tn);
