@@ -448,20 +448,48 @@ __global__ __launch_bounds__(256) void moe_sum_kernel(const void* __restrict__ o
     if (t >= T) return;
     const int c = (int)(at - t * units) * 8;
     float v[8] = {};
-    for (int j = 0; j < k; ++j) {
-        const int r = pos[t * k + j];
-        if (r < 0) continue;
-        float w = weights[t * k + j], f[8];
-        if constexpr (SHARED) {
-            w *= os[(int64_t)r * ((H + 63) >> 6) + (c >> 6)];
-            fp8_unpack8<WUSH_DTYPE_F16>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(o) + (int64_t)r * H + c), f);
-        } else {
-            const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(o) + (int64_t)r * H + c);
-            const float4 a = p[0], b = p[1];
-            f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-        }
+    constexpr int kAhead = 4;                    // rows in flight
+    for (int j0 = 0; j0 < k; j0 += kAhead) {
+        int r[kAhead];
+        float w[kAhead];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(w, f[i], v[i]);
+        for (int u = 0; u < kAhead; ++u) {
+            const int64_t j = t * k + min(j0 + u, k - 1);
+            r[u] = j0 + u < k ? pos[j] : -1;
+            w[u] = weights[j];
+        }
+        if constexpr (SHARED) {
+            uint4 h[kAhead];
+            float by[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int64_t row = max(r[u], 0);
+                by[u] = os[row * ((H + 63) >> 6) + (c >> 6)];
+                h[u] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(o) + row * H + c);
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                if (r[u] < 0) continue;
+                float f[8];
+                fp8_unpack8<WUSH_DTYPE_F16>(h[u], f);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(w[u] * by[u], f[i], v[i]);
+            }
+        } else {
+            float4 f[kAhead][2];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(o) + (int64_t)max(r[u], 0) * H + c);
+                f[u][0] = p[0], f[u][1] = p[1];
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                if (r[u] < 0) continue;
+                const float g[8] = {f[u][0].x, f[u][0].y, f[u][0].z, f[u][0].w, f[u][1].x, f[u][1].y, f[u][1].z, f[u][1].w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(w[u], g[i], v[i]);
+            }
+        }
     }
     uint32_t out[4];
 #pragma unroll
