@@ -1,6 +1,5 @@
-// fp8.h -- what the e4m3 sources share: fp8.hip (quantization, the choice between
-// the kernels), gemm_fp8.hip and
-// gemm_fp8_runs.hip (tiles), fp8_gemv.hip (few rows) and moe.hip (experts).
+// fp8.h -- what the e4m3 sources share: fp8.hip (quantization, the choice between the kernels),
+// gemm_fp8.hip and gemm_fp8_runs.hip (tiles), fp8_gemv.hip (few rows) and moe.hip (experts).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -10,9 +9,8 @@ namespace wush {
 
 constexpr int kFp8Block = 128;                   // channels (and weight rows) that share a scale
 
-// Types of y beside WUSH_DTYPE_BF16 and WUSH_DTYPE_F16; kOutShared: fp16 with a power of two for each
-// row's 64 columns.
-constexpr int kOutF32 = 2, kOutShared = 3;
+// Type of y beside WUSH_DTYPE_BF16 and WUSH_DTYPE_F16
+constexpr int kOutF32 = 2;
 
 // y = x w^T of one matrix, or of one for each expert.
 struct Fp8Gemm {
@@ -51,8 +49,9 @@ constexpr Fp8Tile kFp8Tiles[] = {{256, 256, false, 1.63}, {128, 256, true, 1.02}
 // Tiles of tile_rows x tile_cols, one of kFp8Tiles; K % 16 == 0.
 int launch_gemm_fp8(const Fp8Gemm& g, int tile_rows, int tile_cols, hipStream_t stream);
 
-// The same over experts, fp32 out: tiles of 32 x 64, 64 x 128, 128 x 128.
-int launch_gemm_fp8_rows(const Fp8Gemm& g, int tile_rows, int tile_cols, hipStream_t stream);
+// The same over experts, fp32 out, tiles of kFp8RowsTile x kFp8RowsTile * 2.
+constexpr int kFp8RowsTile = 32;
+int launch_gemm_fp8_rows(const Fp8Gemm& g, hipStream_t stream);
 
 // Tiles of tile_rows (64 or 128) x 256 by workgroups that take one after another: one matrix with N % 8 == 0 and
 // 16-byte aligned y, or experts with act or shared.

