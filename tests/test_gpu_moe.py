@@ -116,6 +116,19 @@ def test_route_layouts(dev):
     assert _C.moe_route(x[:0], 6)[0].shape == (0, 6)
 
 
+def test_route_more_rows_than_a_launch(dev):
+    # 2^26 + 5 rows: three launches of 2^25 rows at most, the last of a few
+    from my_int4 import _C
+    T = (1 << 26) + 5
+    x = torch.zeros(T, 2, dtype=torch.bfloat16, device=dev)
+    x[:, 1] = torch.arange(T, device=dev) % 7 - 3
+    w, ids = _C.moe_route(x, 1, sigmoid=True, renorm=False)
+    assert torch.equal(ids[:, 0], (x[:, 1] > 0).int())
+    few = torch.cat((torch.arange(9), torch.arange((1 << 25) - 3, (1 << 25) + 3), torch.arange(T - 9, T))).to(dev)
+    check_route(_C, x[few], 1, None, True, 1, 1, 1, False)
+    assert torch.equal(w[few], _C.moe_route(x[few], 1, sigmoid=True, renorm=False)[0])
+
+
 def case(seed, T, E, k, H, I, dev, dtype=torch.bfloat16, away=0.0):
     g = gen(seed)
     x = torch.randn(T, H, generator=g).to(dtype)

@@ -319,15 +319,26 @@ void launch_route_v(const RouteArgs& a, hipStream_t stream) {
     if (a.bias) moe_route_kernel<V, true><<<grid, 256, 0, stream>>>(a);
     else moe_route_kernel<V, false><<<grid, 256, 0, stream>>>(a);
 }
-int launch_route(const RouteArgs& a, hipStream_t stream) {
+// a launch has fewer than 2^32 threads: kRouteRows rows each
+constexpr int64_t kRouteRows = 1 << 25;
+
+int launch_route(RouteArgs a, hipStream_t stream) {
     const int v = (a.size + a.lanes - 1) / a.lanes;
-    if (v <= 1) launch_route_v<1>(a, stream);
-    else if (v <= 2) launch_route_v<2>(a, stream);
-    else if (v <= 4) launch_route_v<4>(a, stream);
-    else if (v <= 8) launch_route_v<8>(a, stream);
-    else if (v <= 16) launch_route_v<16>(a, stream);
-    else launch_route_v<32>(a, stream);
-    return (int)hipGetLastError();
+    for (int64_t left = a.rows; left > 0; left -= kRouteRows) {
+        a.rows = left < kRouteRows ? left : kRouteRows;
+        if (v <= 1) launch_route_v<1>(a, stream);
+        else if (v <= 2) launch_route_v<2>(a, stream);
+        else if (v <= 4) launch_route_v<4>(a, stream);
+        else if (v <= 8) launch_route_v<8>(a, stream);
+        else if (v <= 16) launch_route_v<16>(a, stream);
+        else launch_route_v<32>(a, stream);
+        const int st = (int)hipGetLastError();
+        if (st) return st;
+        a.logits = static_cast<const uint8_t*>(a.logits) + kRouteRows * a.stride * (a.dtype == WUSH_DTYPE_F32 ? 4 : 2);
+        a.weights += kRouteRows * a.k;
+        a.ids += kRouteRows * a.k;
+    }
+    return (int)hipSuccess;
 }
 
 // ------------------------------------------------------------------- the experts
