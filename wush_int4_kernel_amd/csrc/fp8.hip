@@ -13,53 +13,19 @@
 namespace wush {
 namespace {
 
-// A workgroup takes ROWS rows and 16 / ROWS blocks of each, a row of 16 lanes a block, and
-// kQuantSteps times that along K.  Sixteen rows together write a block's scales as 64 bytes.
-// 4096 x 4096 bf16: 15 us, 3.4 TB/s; 51 x 4096 4.2 us, which is a launch and one way to memory.
-constexpr int kQuantSteps = 4;
-
 template <int DT, int ROWS>
 __global__ __launch_bounds__(256) void quant_fp8_block_kernel(const uint16_t* __restrict__ x, uint8_t* __restrict__ q,
                                                               float* __restrict__ s, int64_t rows, int K, int64_t stride) {
-    constexpr int BLOCKS = 16 / ROWS;
-    const int group = threadIdx.x >> 4, l16 = threadIdx.x & 15;
-    const int64_t row = (int64_t)blockIdx.x * ROWS + group % ROWS;
-    const int KB = (K + 127) >> 7;
-    const int64_t at = row < rows ? row : rows - 1;
-    const uint16_t* px = x + at * stride;
-    uint4 w[kQuantSteps];
-    const int b0 = (int)blockIdx.y * BLOCKS * kQuantSteps + group / ROWS;
-#pragma unroll
-    for (int u = 0; u < kQuantSteps; ++u) {
-        const int k = (b0 + u * BLOCKS) * 128 + 8 * l16;
-        w[u] = k < K ? *reinterpret_cast<const uint4*>(px + k) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int u = 0; u < kQuantSteps; ++u) {
-        const int b = b0 + u * BLOCKS, k = b * 128 + 8 * l16;
-        float v[8];
-        fp8_unpack8<DT>(w[u], v);
-        const float amax = fp8_amax(row16_max(fp8_largest8(v)));
-        if (row >= rows || b >= KB) continue;
-        if (l16 == 0) s[(size_t)b * rows + row] = fp8_scale(amax);
-        const Fp8Divisor by = fp8_divisor(amax);
-        if (k < K)
-            *reinterpret_cast<uint2*>(q + row * K + k) = make_uint2(fp8_codes4(v[0], v[1], v[2], v[3], by, amax != amax),
-                                                                    fp8_codes4(v[4], v[5], v[6], v[7], by, amax != amax));
-    }
+    fp8_quant<DT, ROWS>(x, q, s, rows, K, stride, (int)blockIdx.x, (int)blockIdx.y, (int)threadIdx.x);
 }
 
 template <int DT>
 int launch_quant(const void* x, uint8_t* q, float* s, int64_t rows, int64_t K, int64_t stride, hipStream_t stream) {
     const uint16_t* p = static_cast<const uint16_t*>(x);
-    const int64_t KB = (K + 127) / 128;
-    if (rows < 16) {
-        const dim3 grid((unsigned)rows, (unsigned)((KB + 16 * kQuantSteps - 1) / (16 * kQuantSteps)));
-        quant_fp8_block_kernel<DT, 1><<<grid, 256, 0, stream>>>(p, q, s, rows, (int)K, stride);
-    } else {
-        const dim3 grid((unsigned)((rows + 15) / 16), (unsigned)((KB + kQuantSteps - 1) / kQuantSteps));
-        quant_fp8_block_kernel<DT, 16><<<grid, 256, 0, stream>>>(p, q, s, rows, (int)K, stride);
-    }
+    const Fp8QuantGrid g = fp8_quant_grid(rows, K);
+    const dim3 grid((unsigned)g.x, (unsigned)g.y);
+    if (g.rows == 1) quant_fp8_block_kernel<DT, 1><<<grid, 256, 0, stream>>>(p, q, s, rows, (int)K, stride);
+    else quant_fp8_block_kernel<DT, 16><<<grid, 256, 0, stream>>>(p, q, s, rows, (int)K, stride);
     return (int)hipGetLastError();
 }
 

@@ -127,5 +127,51 @@ __device__ __forceinline__ uint32_t fp8_largest8(const float (&v)[8]) {
     return mx;
 }
 
+// Codes and scales of x: 256 threads take ROWS rows and 16 / ROWS blocks of each, a row of 16 lanes a block, and
+// kFp8QuantSteps times that along K.  Sixteen rows together write a block's scales as 64 bytes.
+// 4096 x 4096 bf16: 15 us, 3.4 TB/s; 51 x 4096 4.2 us, which is a launch and one way to memory.
+constexpr int kFp8QuantSteps = 4;
+
+struct Fp8QuantGrid {
+    int rows;                                    // ROWS
+    int64_t x, y;                                // groups of rows, of blocks
+};
+inline Fp8QuantGrid fp8_quant_grid(int64_t rows, int64_t K) {
+    const int64_t KB = (K + 127) / 128;
+    if (rows < 16) return {1, rows, (KB + 16 * kFp8QuantSteps - 1) / (16 * kFp8QuantSteps)};
+    return {16, (rows + 15) / 16, (KB + kFp8QuantSteps - 1) / kFp8QuantSteps};
+}
+
+template <int DT, int ROWS>
+__device__ __forceinline__ void fp8_quant(const uint16_t* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ s,
+                                          int64_t rows, int K, int64_t stride, int gx, int gy, int tid) {
+    constexpr int BLOCKS = 16 / ROWS;
+    const int group = tid >> 4, l16 = tid & 15;
+    const int64_t row = (int64_t)gx * ROWS + group % ROWS;
+    const int KB = (K + 127) >> 7;
+    const int64_t at = row < rows ? row : rows - 1;
+    const uint16_t* px = x + at * stride;
+    uint4 w[kFp8QuantSteps];
+    const int b0 = gy * BLOCKS * kFp8QuantSteps + group / ROWS;
+#pragma unroll
+    for (int u = 0; u < kFp8QuantSteps; ++u) {
+        const int k = (b0 + u * BLOCKS) * 128 + 8 * l16;
+        w[u] = k < K ? *reinterpret_cast<const uint4*>(px + k) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < kFp8QuantSteps; ++u) {
+        const int b = b0 + u * BLOCKS, k = b * 128 + 8 * l16;
+        float v[8];
+        fp8_unpack8<DT>(w[u], v);
+        const float amax = fp8_amax(row16_max(fp8_largest8(v)));
+        if (row >= rows || b >= KB) continue;
+        if (l16 == 0) s[(size_t)b * rows + row] = fp8_scale(amax);
+        const Fp8Divisor by = fp8_divisor(amax);
+        if (k < K)
+            *reinterpret_cast<uint2*>(q + row * K + k) = make_uint2(fp8_codes4(v[0], v[1], v[2], v[3], by, amax != amax),
+                                                                    fp8_codes4(v[4], v[5], v[6], v[7], by, amax != amax));
+    }
+}
+
 }  // namespace
 }  // namespace wush

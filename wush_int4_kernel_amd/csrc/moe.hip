@@ -347,13 +347,35 @@ int launch_route(RouteArgs a, hipStream_t stream) {
 // expert's first + its pairs in earlier workgroups + the rank among this one's.  The last two come
 // from an LDS counter: which of an expert's rows a pair gets may differ from call to call, what
 // is computed in that row does not depend on it.
-// 408 pairs of 128 experts 3.8 us, 32768 10 us (their counts, 32 loads deep in each workgroup): latency.
+// Alone, 408 pairs of 128 experts 3.8 us, 32768 10 us (their counts, 32 loads deep in each workgroup): latency.
 constexpr int kSortThreads = 1024, kSortPairs = 1024, kMostExperts = 1024;
 
-__global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(const int32_t* __restrict__ ids, int P, int k, int E,
-                                                                int tile_rows, int* __restrict__ row_of,
-                                                                int* __restrict__ pos, int4* __restrict__ tiles,
-                                                                int* __restrict__ ntiles) {
+// The workgroups behind those `sorts` quantize x meanwhile, in four parts of 256 threads: 51 tokens 5 us, 4096 tokens 18
+// (a launch for each: 4.8 and 4.8, 11 and 15).
+struct BeginArgs {
+    const int32_t* ids;
+    int P, k, E, tile_rows;
+    int *row_of, *pos, *ntiles;
+    int4* tiles;
+    const uint16_t* x;
+    uint8_t* q;
+    float* s;
+    int64_t rows, stride;
+    int K, sorts, gx, gy;
+};
+template <int DT, int ROWS>
+__global__ __launch_bounds__(kSortThreads) void moe_begin_kernel(const BeginArgs a) {
+    if ((int)blockIdx.x >= a.sorts) {
+        const int part = ((int)blockIdx.x - a.sorts) * (kSortThreads / 256) + ((int)threadIdx.x >> 8);
+        if (part < a.gx * a.gy) fp8_quant<DT, ROWS>(a.x, a.q, a.s, a.rows, a.K, a.stride, part % a.gx, part / a.gx, (int)threadIdx.x & 255);
+        return;
+    }
+    const int32_t* __restrict__ ids = a.ids;
+    const int P = a.P, k = a.k, E = a.E, tile_rows = a.tile_rows;
+    int* __restrict__ row_of = a.row_of;
+    int* __restrict__ pos = a.pos;
+    int4* __restrict__ tiles = a.tiles;
+    int* __restrict__ ntiles = a.ntiles;
     __shared__ int all[kMostExperts], before[kMostExperts], start[kMostExperts], tile0[kMostExperts];
     __shared__ int wave_rows[kSortThreads / 64], wave_tiles[kSortThreads / 64];
     const int tid = threadIdx.x, first = blockIdx.x * kSortPairs;
@@ -417,6 +439,19 @@ __global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(const int32_t* _
             for (int i = 0; i < t; ++i) tiles[tile0[tid] + i] = make_int4(tid, start[tid] + i * tile_rows, start[tid] + n, 0);
         if (tid == kSortThreads - 1) *ntiles = ot + stl;
     }
+}
+
+int launch_begin(const BeginArgs& a, int dtype, int rows, hipStream_t stream) {
+    constexpr int parts = kSortThreads / 256;
+    const unsigned grid = (unsigned)(a.sorts + (a.gx * a.gy + parts - 1) / parts);
+    if (dtype == WUSH_DTYPE_BF16) {
+        if (rows == 1) moe_begin_kernel<WUSH_DTYPE_BF16, 1><<<grid, kSortThreads, 0, stream>>>(a);
+        else moe_begin_kernel<WUSH_DTYPE_BF16, 16><<<grid, kSortThreads, 0, stream>>>(a);
+    } else {
+        if (rows == 1) moe_begin_kernel<WUSH_DTYPE_F16, 1><<<grid, kSortThreads, 0, stream>>>(a);
+        else moe_begin_kernel<WUSH_DTYPE_F16, 16><<<grid, kSortThreads, 0, stream>>>(a);
+    }
+    return (int)hipGetLastError();
 }
 
 // h = silu(gate) * up of a row's 128 channels, quantized: 16 lanes a block
@@ -666,12 +701,13 @@ int wush_moe_experts_fp8(const void* x, int dtype, int64_t row_stride, const flo
     float* os = reinterpret_cast<float*>(ws + p.os);
     for (int64_t t = 0; t < T; t += p.tokens) {
         const int64_t n = T - t < p.tokens ? T - t : p.tokens;
-        int st = wush_quant_fp8_block(px + t * row_stride, dtype, ws + p.xq, reinterpret_cast<float*>(ws + p.xs), n, H, row_stride, stream);
-        if (st) return st;
         const int P = (int)(n * k);
-        wush::moe_sort_kernel<<<(unsigned)((P + wush::kSortPairs - 1) / wush::kSortPairs), wush::kSortThreads, 0, stream>>>(
-            ids + t * k, P, (int)k, (int)E, p.tile_rows, row_of, pos, tiles, ntiles);
-        if ((st = (int)hipGetLastError())) return st;
+        const wush::Fp8QuantGrid qg = wush::fp8_quant_grid(n, H);
+        const wush::BeginArgs b = {ids + t * k, P, (int)k, (int)E, p.tile_rows, row_of, pos, ntiles, tiles, px + t * row_stride,
+                                   ws + p.xq, reinterpret_cast<float*>(ws + p.xs), n, row_stride, (int)H,
+                                   (P + wush::kSortPairs - 1) / wush::kSortPairs, (int)qg.x, (int)qg.y};
+        int st = wush::launch_begin(b, dtype, qg.rows, stream);
+        if (st) return st;
         wush::Fp8Gemm g = {};
         g.x = ws + p.xq;
         g.xs = reinterpret_cast<float*>(ws + p.xs);
