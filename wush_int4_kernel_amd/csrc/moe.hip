@@ -144,9 +144,9 @@ __device__ __forceinline__ int groups_above(Key score, const RouteArgs& p, int g
 // A wavefront per row.  Lane group * lanes + sub holds experts group * size + sub + lanes * i.
 // Without a bias (BIAS false) the logits order the experts as the scores do: 32-bit keys of logits, and scores of the
 // chosen ones only, and of all for softmax's sum.  With one, scores in 32 bits decide wherever they are further apart than their
-// errors: s is off by less than 2^-20 (a few units of the last bit; softmax, with a sum of up to 38 roundings, 2^-17), s + b by
-// 2^-23 |s + b| more, and a sum of two by twice that.  A row in which two that matter are nearer, or that holds what is not finite,
-// is chosen again in 64 bits.
+// errors: s is off by less than 2^-20 (a few units of the last bit; softmax, with a sum of up to 38 roundings, 2^-17), c = s + b by
+// 2^-24 |c| more, and a sum of two by both of theirs and 2^-24 of itself: by magnitudes, since biases of opposite signs leave
+// a small sum of large c.  A row in which two that matter are nearer, or that holds what is not finite, is chosen again in 64 bits.
 // 4096 x 128 bf16, 8 of them: 5.5 us.  16384 x 256 fp32 with a bias, 8 groups: 22.5 us (64 bits throughout: 28), where
 // the choices' chain of maxima and the chosen scores' exponentials bound it, not the 17 MB (3.4 us).  A row on 16 lanes instead
 // of 64, which shares that chain among four rows, takes 30: one row that is chosen again holds up three.
@@ -259,7 +259,12 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs p) {
             // the least of the groups that stay and the largest of the others
             const float last = order_value(~wave_max(keep && there ? ~score : 0u));
             const uint32_t out = wave_max(!keep && there ? score : 0u);
-            odd |= out != 0 && !(last - order_value(out) > 2.0f * (kApart + kPart * __builtin_fabsf(last)));
+            float size = __builtin_fabsf(last);
+            if (p.best == 2) {                   // the largest |c| + |c| of any group: the two at the border may have others
+                const float both = __builtin_fabsf(order_value(one)) + __builtin_fabsf(order_value(two));
+                size = __uint_as_float(wave_max(there ? __float_as_uint(both) : 0u));
+            }
+            odd |= out != 0 && !(last - order_value(out) > 2.0f * (kApart + kPart * size));
             if (!keep) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) key[i] = 0;
