@@ -259,12 +259,9 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs p) {
             // the least of the groups that stay and the largest of the others
             const float last = order_value(~wave_max(keep && there ? ~score : 0u));
             const uint32_t out = wave_max(!keep && there ? score : 0u);
-            float size = __builtin_fabsf(last);
-            if (p.best == 2) {                   // the largest |c| + |c| of any group: the two at the border may have others
-                const float both = __builtin_fabsf(order_value(one)) + __builtin_fabsf(order_value(two));
-                size = __uint_as_float(wave_max(there ? __float_as_uint(both) : 0u));
-            }
-            odd |= out != 0 && !(last - order_value(out) > 2.0f * (kApart + kPart * size));
+            // the errors' size, of any group: the two at the border may not have the largest
+            const float size = p.best == 1 ? __builtin_fabsf(last) : __builtin_fabsf(order_value(one)) + __builtin_fabsf(order_value(two));
+            odd |= out != 0 && __any(there && !(last - order_value(out) > 2.0f * (kApart + kPart * size)));
             if (!keep) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) key[i] = 0;
