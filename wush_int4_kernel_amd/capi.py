@@ -71,6 +71,7 @@ SIGNATURES = {
     "wush_linear_fp8": ([_P, _I64, _P, _P, _P, _I, _I64, _I64, _I64, _P, _SZ, _P], _I),
     "wush_moe_route": ([_P, _I, _I64, _P, _I64, _I64, ctypes.POINTER(MoeChoice), _P, _P, _P], _I),
     "wush_moe_experts_fp8_workspace_bytes": ([_I64, _I64, _I64, _I64, _I64, _I], _SZ),
+    "wush_moe_experts_fp8_plan": ([_I64, _I64, _I64, _I64, _I64, _I, ctypes.POINTER(ctypes.c_int32)], _I),
     "wush_moe_experts_fp8": ([_P, _I, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _SZ, _P], _I),
 }
 
@@ -218,4 +219,15 @@ def gemm_fp8_plan(M, N, K, workspace_bytes=None) -> tuple:
         workspace_bytes = load().wush_gemm_fp8_workspace_bytes(M, N, K)
     plan = (ctypes.c_int32 * 4)()
     _check(load().wush_gemm_fp8_plan(M, N, K, workspace_bytes, plan), "wush_gemm_fp8_plan")
+    return tuple(plan)
+
+
+# ways of moe_experts_fp8_plan
+MOE_DOT, MOE_ROWS, MOE_FUSED = range(3)
+
+
+def moe_experts_fp8_plan(T, k, E, H, I, dtype) -> tuple:
+    """(way, rows of a tile, whether most experts have one tile, tokens taken at once) of fp8_experts."""
+    plan = (ctypes.c_int32 * 4)()
+    _check(load().wush_moe_experts_fp8_plan(T, k, E, H, I, dtype, plan), "wush_moe_experts_fp8_plan")
     return tuple(plan)

@@ -673,6 +673,17 @@ size_t wush_moe_experts_fp8_workspace_bytes(int64_t T, int64_t k, int64_t E, int
     return wush::experts_plan(T, k, E, H, I, dtype).bytes;
 }
 
+int wush_moe_experts_fp8_plan(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, int dtype, int32_t plan[4]) {
+    WUSH_REQUIRE(plan && T > 0 && wush::experts_sizes(T, k, E, H, I));
+    WUSH_REQUIRE(dtype == WUSH_DTYPE_BF16 || dtype == WUSH_DTYPE_F16);
+    const wush::ExpertsPlan p = wush::experts_plan(T, k, E, H, I, dtype);
+    plan[0] = p.few ? WUSH_MOE_DOT : p.fused ? WUSH_MOE_FUSED : WUSH_MOE_ROWS;
+    plan[1] = p.tile_rows;
+    plan[2] = p.once;
+    plan[3] = (int32_t)p.tokens;
+    return (int)hipSuccess;
+}
+
 int wush_moe_experts_fp8(const void* x, int dtype, int64_t row_stride, const float* weights, const int32_t* ids,
                          const uint8_t* w_up, const float* s_up, const uint8_t* w_down, const float* s_down, void* y,
                          int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, void* workspace, size_t workspace_bytes,
