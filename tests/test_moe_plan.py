@@ -48,3 +48,16 @@ def test_runs(capi):
         for T in (1000, 5000, 40000, 1 << 20):
             assert capi.moe_experts_fp8_plan(T, k, 4, H, I, BF16)[3] == min(T, most)
         assert size(70000, k, 4, H, I, BF16) == size(1 << 20, k, 4, H, I, BF16)
+
+
+def test_another_way_s_products_are_told_apart():
+    """The GPU tests' check refuses an fp16 output that is what the bf16 way computes."""
+    import torch
+
+    import _fp8 as plain
+    from test_gpu_moe import case
+    from test_gpu_moe_ways import ALL, DOWN, check_way
+    args = case(3, 64, 4, 2, 512, 512, "cpu", torch.float16)
+    y = plain.experts(*args, *ALL)[0].to(torch.float16)
+    with pytest.raises(AssertionError):
+        check_way(y, args, DOWN)
