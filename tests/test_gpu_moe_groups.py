@@ -46,3 +46,21 @@ def test_near_equal_groups(dev, size, groups, keep, big, sigmoid):
     step = big * 2.0 ** -24 * (4.0 if sigmoid else groups * size)          # of the logits, in scores about 2^-24 big
     x = 2.0 * step * torch.randn(400, groups * size, generator=g)
     same_choice(_C, x.to(dev), bias, min(4, keep), groups, keep, sigmoid, 2.5)
+
+
+def test_scores_that_64_bits_do_not_tell_apart(dev):
+    """Sigmoids of 40 and 50 are both 1 in 64 bits.  Without a bias logits order experts and, by their best one, groups; sums of two
+    scores and scores with a bias are equal there, and go by index."""
+    from my_int4 import _C
+    x = torch.tensor([[40.0, 39.0, 50.0, 45.0, 3.0, 2.0, 60.0, 1.0]], device=dev)
+
+    def choice(k=1, **kw):
+        return _C.moe_route(x, k, sigmoid=True, **kw)[1][0].tolist()
+
+    zeros = torch.zeros(8, device=dev)
+    assert choice(4) == [6, 2, 3, 0] and choice(4, bias=zeros) == [0, 1, 2, 3]
+    assert choice(2, groups=4, keep_groups=2) == [6, 2] and choice(2, groups=4, keep_groups=2, bias=zeros) == [0, 1]
+    assert choice(2, groups=4, keep_groups=1, group_best=2) == [0, 1] == choice(2, groups=4, keep_groups=1, group_best=2, bias=zeros)
+    y = torch.tensor([[-900.0, -800.0, 0.0, -2.0, -850.0, -700.0]], device=dev)      # softmax: 0 in 64 bits below -745
+    assert _C.moe_route(y, 6)[1][0].tolist() == [2, 3, 5, 1, 4, 0]
+    assert _C.moe_route(y, 6, bias=torch.zeros(6, device=dev))[1][0].tolist() == [2, 3, 5, 0, 1, 4]

@@ -3,11 +3,11 @@
 //
 // Route: s = softmax(x) or sigmoid(x), c = s + bias; of each group of experts the sum of its best one or
 // two c, the best groups stay; ids are the k largest c left, equal ones by the lowest
-// index; weights s[ids], divided by their sum or not, times a factor.  Without a bias x itself orders the
-// experts; with one the choice is that of 64-bit scores.  Weights and their sums are in 64 bits.
+// index; weights s[ids], divided by their sum or not, times a factor.  Without a bias x itself orders the experts, and groups by
+// their best one; with one, and for sums of two, the choice is that of 64-bit scores.  Weights and their sums are in 64 bits.
 //
 // Experts: rows of x by expert; a = q(x) up_e^T, h = silu(a_gate) a_up, o = q(h) down_e^T, y = sum of w o over a
-// token's experts.  a, h and o are kept in fp32, h and x quantized as in fp8_device.h.
+// token's experts.  a and h are kept in fp32, o too but for bf16's fused way (see experts_plan), h and x quantized as in fp8_device.h.
 #include <cmath>
 #include <type_traits>
 
