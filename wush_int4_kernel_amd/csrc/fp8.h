@@ -58,8 +58,8 @@ int launch_gemm_fp8_rows(const Fp8Gemm& g, hipStream_t stream);
 constexpr int kFp8Workgroups = 256;              // one for each of the chip's CUs
 int launch_gemm_fp8_runs(const Fp8Gemm& g, int tile_rows, hipStream_t stream);
 
-// Up to four rows (see fp8_gemv_shape) on dot products: x as bf16 or fp16 rows of y's type (xs null), or as codes with
-// scales xs (K / 128, M).
+// Up to four rows (one with K up to 32768, two up to 16384, three and four up to 8192: fp8_gemv_shape) on dot products:
+// x as bf16 or fp16 rows of y's type (xs null), or as codes with scales xs (K / 128, M).
 bool fp8_gemv_shape(int64_t M, int64_t K);
 int launch_fp8_gemv(const void* x, int64_t row_stride, const float* xs, const uint8_t* w, const float* ws, uint16_t* y,
                     int dtype, int64_t M, int64_t N, int64_t K, hipStream_t stream);

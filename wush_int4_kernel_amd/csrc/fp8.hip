@@ -34,8 +34,8 @@ struct Plan {
     int kernel, rows, cols, splits;
 };
 
-// Up to four rows take dot products, more the tile and the split of K with the least estimated time, in microseconds: rounds
-// of workgroups with the time of their stages (3/4 of it on an empty chip), or the weights' way from HBM (slower where several
+// Up to four rows take dot products where they fit (fp8_gemv_shape), all else the tile and the split of K with the least
+// estimated time, in microseconds: rounds of workgroups with the time of their stages (3/4 of it on an empty chip), or the weights' way from HBM (slower where several
 // row tiles read them), whichever is longer, a part of the shorter, and for a split its launch and partial sums.  The
 // constants are fitted to 94 shapes from 5 x 8192 x 28672 to 4000 x 4096 x 4096, weights from HBM: 0.8% slower than the fastest
 // of all tiles and splits on average, 12% at worst.
