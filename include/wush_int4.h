@@ -456,7 +456,7 @@ int wush_moe_experts_fp8(const void *x, int dtype, int64_t row_stride, const flo
 enum wush_moe_experts_way {
     WUSH_MOE_DOT = 0,               /* dot products, an expert's weights read for each choice; none */
     WUSH_MOE_ROWS = 1,              /* rows sorted by expert, tiles of 32 x 64; the down projection's */
-    WUSH_MOE_FUSED = 2              /* tiles of 64 or 128 x 256; all in bf16, whose experts' rows are fp16, the down projection's in fp16 */
+    WUSH_MOE_FUSED = 2              /* tiles of 64 or 128 x 256; the down projection's, and a bf16 y's experts' rows are fp16 */
 };
 
 /* The plan wush_moe_experts_fp8 runs: plan = {way, rows of a tile (0: no tiles), whether most experts have one

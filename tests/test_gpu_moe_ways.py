@@ -14,7 +14,8 @@ pytestmark = pytest.mark.gpu
 DTYPES = [torch.bfloat16, torch.float16]
 
 # (gate and up products cut, down products cut, half a unit of the rows' type)
-EXACT, DOWN, ALL = (False, False, 0.0), (False, True, 0.0), (True, True, 2.0 ** -11)
+EXACT, DOWN, HALF = (False, False, 0.0), (False, True, 0.0), (False, True, 2.0 ** -11)
+ALL = (True, True, 2.0 ** -11)                                   # no way's: what the e4m3 instruction would make of the hidden codes
 
 
 def plan_of(T, k, E, H, I, dtype):
@@ -26,7 +27,7 @@ def model_of(plan, dtype):
     from wush_int4_kernel_amd import capi
     if plan[0] == capi.MOE_DOT:
         return EXACT
-    return ALL if plan[0] == capi.MOE_FUSED and dtype == torch.bfloat16 else DOWN
+    return HALF if plan[0] == capi.MOE_FUSED and dtype == torch.bfloat16 else DOWN
 
 
 def spread_of(dtype, model, codes):
@@ -52,9 +53,11 @@ def check_way(y, args, model):
     # What the model leaves over (roundings, for the most part) has nothing to do with what sets the other models apart: on
     # the line from this model to another the outputs lie at 0, those of the other at 1, give or take |rest| / (sqrt n |line|).
     for other in (EXACT, DOWN, ALL):
+        if other[:2] == model[:2]:
+            continue
         line = plain.experts(*args, *other)[0] - ref
         far = float(line.norm())
-        if other != model and 8 * limit * norm / y.numel() ** 0.5 < far:
+        if 8 * limit * norm / y.numel() ** 0.5 < far:
             assert abs(float(((got - ref) * line).sum())) < 0.5 * far ** 2, other
     # and all of it: the roundings, and what this model is from the exact products
     exact = plain.experts(*args, *EXACT)[0]
@@ -133,7 +136,7 @@ def test_few_rows_of_many_columns(dev, shape):
     # 512 workgroups for the gate and up projections: bf16 is fused, fp16 is not
     from wush_int4_kernel_amd import capi
     T, E, k, H, I = shape
-    for dtype, way, model in ((torch.bfloat16, capi.MOE_FUSED, ALL), (torch.float16, capi.MOE_ROWS, DOWN)):
+    for dtype, way, model in ((torch.bfloat16, capi.MOE_FUSED, HALF), (torch.float16, capi.MOE_ROWS, DOWN)):
         plan = plan_of(T, k, E, H, I, dtype)
         assert plan[0] == way and plan[2] == 1
         check_way(*run(dev, dtype, shape), model)
@@ -160,11 +163,19 @@ def test_non_finite_tokens_stay_alone(dev, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_documented_accuracy(dev, dtype):
-    """Against 64 bits: what the cut of the gate and up products turns of the hidden codes is at most 1.8e-3 of a bf16 layer's
-    output; an fp16 one has the down projection's cut, of 7 of 8 products by 2^-13 of the largest at most: 2^-13 sqrt(7 / 3)."""
-    shape = (700, 16, 3, 1040, 1280)
+@pytest.mark.parametrize("shape", [(300, 60, 8, 2048, 1408), (700, 16, 3, 1040, 1280), (100, 64, 6, 400, 384), (51, 128, 8, 2048, 512)])
+def test_outlier_channels(dev, shape, dtype):
+    """Activations with some channels twenty times the others, next to whose products the matrix instruction cuts the others': the
+    hidden codes are those of exact sums all the same.  Against 64 bits: the roundings, and the down projection's cut, 7 of 8
+    products by 2^-13 of the largest at most, sqrt(7 / 3) 2^-13 of their root sum of squares."""
+    from my_int4 import _C
     T, E, k, H, I = shape
+    args = case(T + H, T, E, k, H, I, dev, torch.float32)
+    args[0][:, torch.randperm(H, generator=gen(5))[:H // 100].to(dev)] *= 20
+    args[0] = args[0].to(dtype)
+    y = _C.fp8_experts(*args)
     model = model_of(plan_of(T, k, E, H, I, dtype), dtype)
-    apart = check_way(*run(dev, dtype, shape), model)
-    assert apart <= (1.8e-3 if dtype == torch.bfloat16 else 2.0 ** -13 * (7 / 3) ** 0.5)
+    check_way(y, args, model)
+    exact = plain.experts(*args, *EXACT)[0]
+    limit = math.hypot(spread_of(dtype, model, T * k * I), 2.0 ** -13 * (7 / 3) ** 0.5)
+    assert float((y.double() - exact).norm() / exact.norm()) <= limit

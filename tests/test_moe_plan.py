@@ -51,7 +51,7 @@ def test_runs(capi):
 
 
 def test_another_way_s_products_are_told_apart():
-    """The GPU tests' check refuses an fp16 output that is what the bf16 way computes."""
+    """The GPU tests' check refuses outputs whose gate and up products were cut."""
     import torch
 
     import _fp8 as plain

@@ -34,7 +34,7 @@ struct Fp8Gemm {
     int act, shared;
     float* hs;
     int64_t ldh;
-    int wide;                                    // products in fp16 matrix instructions, which cut none
+    int wide;                                    // products in fp16 matrix instructions, which cut none (with act: always)
     int once;                                    // weights are mostly read for one tile of rows only
 };
 

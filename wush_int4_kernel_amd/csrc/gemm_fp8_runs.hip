@@ -496,8 +496,7 @@ void gemm_fp8_runs_kernel(const Fp8Gemm g) {
 template <int RB, bool NT>
 int launch(const Fp8Gemm& g, unsigned grid, hipStream_t stream) {
     constexpr int WR = 2, WC = 4, NB = 3, T = 64 * WR * WC;
-    if (g.act && g.wide) gemm_fp8_runs_kernel<RB, WR, WC, NB, kAct, false, true, NT><<<grid, T, 0, stream>>>(g);
-    else if (g.act) gemm_fp8_runs_kernel<RB, WR, WC, NB, kAct, false, false, NT><<<grid, T, 0, stream>>>(g);
+    if (g.act) gemm_fp8_runs_kernel<RB, WR, WC, NB, kAct, false, true, NT><<<grid, T, 0, stream>>>(g);
     else if (g.tiles && g.shared) gemm_fp8_runs_kernel<RB, WR, WC, NB, kShared, false, false, NT><<<grid, T, 0, stream>>>(g);
     else if (g.tiles) gemm_fp8_runs_kernel<RB, WR, WC, NB, kWide, false, false, NT><<<grid, T, 0, stream>>>(g);
     else if (g.out == WUSH_DTYPE_BF16) gemm_fp8_runs_kernel<RB, WR, WC, NB, kPlain, true, false, NT><<<grid, T, 0, stream>>>(g);

@@ -565,15 +565,14 @@ struct ExpertsPlan {
 
 // Three ways.
 // A few tokens: dot products that read an expert's weights for each choice (fp8_gemv.hip).
-// Fused: tiles of 64 or 128 x 256, one after another (gemm_fp8_runs.hip), whose epilogue makes the hidden codes.  For bf16 all
-// products are on the e4m3 matrix instruction and experts' rows in fp16 with shared powers of two.
-// That instruction cuts small products next to large ones (at 2^-13 of the largest of 8), which turns
-// one in some thousand of the hidden codes to the other side of a half: 1.2e-3 of the output, below bf16's rounding (1.7e-3)
-// but above fp16's (2.1e-4).  For fp16 the gate and up projections therefore take the fp16 matrix
-// instruction, and experts' rows are fp32.
-// Otherwise (few rows an expert, and few workgroups of the other kind): tiles of 32 x 64, the gate
-// and up projections on the fp16 instruction, at half the rate where the weights' stream bounds the time anyway, and
-// intermediate rows in fp32.
+// Fused: tiles of 64 or 128 x 256, one after another (gemm_fp8_runs.hip), whose epilogue makes the hidden codes.  Experts'
+// rows are fp32 for fp16, and for bf16 fp16 with shared powers of two, 2^-12 of a value where y's own rounding is up to 2^-8 of it.
+// Otherwise (few rows an expert, and few workgroups of the other kind): tiles of 32 x 64, and intermediate rows in fp32.
+// Both take the gate and up products on the fp16 matrix instruction, which cuts none, at half the e4m3 one's rate and with the codes
+// widened first.  The e4m3 instruction cuts small products next to large ones, at 2^-13 of the largest of 8: where a
+// channel in a hundred is twenty times the others that turns 3 in 1000 of the hidden codes to the other side of a half, 1.1e-3 to
+// 2.1e-3 of the output, as much as all of bf16's rounding (1.7e-3) and ten times fp16's (4096 tokens, 8 of 128 experts of
+// 4096 x 1024, bf16: 764 us for 1015; 51 tokens 184 for 187).  The down products are cut: 4e-5 of the output.
 // us, bf16, by tokens, three ways (dots, 32, 64 rows): 64 experts of 2048 x 1408, 6 choices: 4: 46, 53, 51;
 // 8: 77, 66, 69; 64: -, 108, 110; 256: -, 150, 124; 1024: -, 333, 185.  8 of 4096 x
 // 1792, 2 choices: 4: 33, 43, 49; 8: 55, 44, 50; 48: -, 57, 58; 256: -, 108, 59; 512: -, 150, 93.
@@ -738,7 +737,7 @@ int wush_moe_experts_fp8(const void* x, int dtype, int64_t row_stride, const flo
         g.most_tiles = p.most_tiles;
         g.once = p.once;
         g.act = p.fused;
-        g.wide = !p.shared;
+        g.wide = 1;
         g.y = p.fused ? static_cast<void*>(ws + p.hq) : a;
         g.hs = hs;
         g.ldh = p.pairs;
