@@ -133,13 +133,13 @@ def test_fused(dev, rows, shape, many, dtype):
 
 @pytest.mark.parametrize("shape", [(52, 64, 8, 400, 1408), (8, 8, 2, 256, 14336)])
 def test_few_rows_of_many_columns(dev, shape):
-    # 512 workgroups for the gate and up projections: bf16 is fused, fp16 is not
+    # few rows an expert, but workgroups enough for the gate and up projections
     from wush_int4_kernel_amd import capi
     T, E, k, H, I = shape
-    for dtype, way, model in ((torch.bfloat16, capi.MOE_FUSED, HALF), (torch.float16, capi.MOE_ROWS, DOWN)):
+    for dtype in DTYPES:
         plan = plan_of(T, k, E, H, I, dtype)
-        assert plan[0] == way and plan[2] == 1
-        check_way(*run(dev, dtype, shape), model)
+        assert plan[:3] == (capi.MOE_FUSED, 64, 1)
+        check_way(*run(dev, dtype, shape), model_of(plan, dtype))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

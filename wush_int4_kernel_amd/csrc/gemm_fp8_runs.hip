@@ -7,8 +7,9 @@
 // lanes of a row: LDS belongs to the next tile by then.
 //
 // 27 x 57344 x 8192, tiles of 64 x 256: 71 us, 6.6 TB/s of weights (one tile a workgroup: 82).  The experts' layer of 4096 tokens,
-// 8 of 128 experts of 4096 x 1024: 420 to 520 us for the gate and up projections (1.3 PFLOP/s at most; 350 where every
-// expert has 256 rows), 290 to 320 for the down projections; LDS reads take as long as the MFMAs there.
+// 8 of 128 experts of 4096 x 1024: 265 to 290 us for the down projections, where LDS reads take as long as the MFMAs, and 745 to
+// 790 for the gate and up projections, in fp16 instructions (0.7 PFLOP/s), where the issue of vector instructions takes longest: 250
+// and 64 MFMAs of 9 cycles each for a block of K in a wavefront, half of them to widen codes.
 #include "fp8.h"
 #include "fp8_device.h"
 #include "../../include/wush_int4.h"

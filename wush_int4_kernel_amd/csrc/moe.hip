@@ -147,7 +147,7 @@ __device__ __forceinline__ int groups_above(Key score, const RouteArgs& p, int g
 // errors: s is off by less than 2^-20 (a few units of the last bit; softmax, with a sum of up to 38 roundings, 2^-17), c = s + b by
 // 2^-24 |c| more, and a sum of two by both of theirs and 2^-24 of itself: by magnitudes, since biases of opposite signs leave
 // a small sum of large c.  A row in which two that matter are nearer, or that holds what is not finite, is chosen again in 64 bits.
-// 4096 x 128 bf16, 8 of them: 5.5 us.  16384 x 256 fp32 with a bias, 8 groups: 22.5 us (64 bits throughout: 28), where
+// 4096 x 128 bf16, 8 of them: 5.5 us.  16384 x 256 fp32 with a bias, 8 groups: 23 us (64 bits throughout: 28), where
 // the choices' chain of maxima and the chosen scores' exponentials bound it, not the 17 MB (3.4 us).  A row on 16 lanes instead
 // of 64, which shares that chain among four rows, takes 30: one row that is chosen again holds up three.
 template <int V, bool BIAS>
@@ -572,12 +572,18 @@ struct ExpertsPlan {
 // widened first.  The e4m3 instruction cuts small products next to large ones, at 2^-13 of the largest of 8: where a
 // channel in a hundred is twenty times the others that turns 3 in 1000 of the hidden codes to the other side of a half, 1.1e-3 to
 // 2.1e-3 of the output, as much as all of bf16's rounding (1.7e-3) and ten times fp16's (4096 tokens, 8 of 128 experts of
-// 4096 x 1024, bf16: 764 us for 1015; 51 tokens 184 for 187).  The down products are cut: 4e-5 of the output.
-// us, bf16, by tokens, three ways (dots, 32, 64 rows): 64 experts of 2048 x 1408, 6 choices: 4: 46, 53, 51;
-// 8: 77, 66, 69; 64: -, 108, 110; 256: -, 150, 124; 1024: -, 333, 185.  8 of 4096 x
-// 1792, 2 choices: 4: 33, 43, 49; 8: 55, 44, 50; 48: -, 57, 58; 256: -, 108, 59; 512: -, 150, 93.
-// 64 or 128 rows, weights from HBM, by rows an expert: 28: 115, 115; 50: 406, 379; 66: 193, 171; 73: 193, 174; but where
-// half of the choices lie elsewhere, which the host does not see, at 73: 144, 158.  Hence 80, between the two.
+// 4096 x 1024, bf16: 764 us for 1015; 51 tokens 184 for 190).  The down products are cut: 4e-5 of the output.
+// us, bf16, by tokens, three ways (dots, 32, 64 rows): 64 experts of 2048 x 1408, 6 choices: 4: 43, 49, 45;
+// 8: 62, 60, 67; 64: -, 92, 100; 256: -, 167, 124; 1024: -, 430, 203.  8 of 4096 x
+// 1792, 2 choices: 4: 30, 40, 56; 8: 43, 43, 58; 48: -, 53, 60; 256: -, 111, 70; 512: -, 173, 93.
+// Fused from 12 rows an expert on, or where the gate and up projections have 640 workgroups' columns, two and a half for each CU:
+// over nine layers (8 experts of 4096 x 14336 to 256 of 2048 x 512) and 1/4 to 16 rows an expert, both types, 1.6% behind
+// the faster on average; by rows alone 2.5%.  4 and 8 rows, 64 rows' time over 32's: 256 of 2048 x 512 0.92, 0.84; 128 of
+// 4096 x 1024 1.00, 0.98; 8 of 4096 x 1792 1.29, 1.33.
+// 64 or 128 rows: over eight layers of those and 24 to 128 rows an expert, both types, a border of 80 is 0.7% behind the faster
+// on average with all choices here (56: 1.7%; 72 and 96: 0.9%; 112: 1.5%), and with half of them here as well, which the host
+// does not see, 1.4% (96: 1.2%).  64 rows' time over 128's at 56, 80 and 96: bf16 0.91, 1.00, 1.03, fp16 0.94, 0.96, 1.02; at 80
+// with half of the choices here 0.92, 0.93.
 ExpertsPlan experts_plan(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, int dtype) {
     ExpertsPlan p = {};
     // us: every choice reads its expert's weights; tiles read each expert once that some choice meets, after some launches
@@ -593,7 +599,7 @@ ExpertsPlan experts_plan(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, 
     p.tokens = T < most ? T : most;
     p.pairs = p.tokens * k;
     const double rows = (double)p.pairs / (double)E;
-    p.fused = rows > 12 || (dtype == WUSH_DTYPE_BF16 && met * (double)(I / 128) >= 512);
+    p.fused = rows > 12 || met * (double)(I / 128) >= 640;
     p.shared = p.fused && dtype == WUSH_DTYPE_BF16;
     p.tile_rows = !p.fused ? kFp8RowsTile : rows <= 80 ? 64 : 128;
     p.once = rows <= 30;                         // mostly one tile an expert
