@@ -429,12 +429,13 @@ typedef struct wush_moe_choice {
 } wush_moe_choice;
 
 /* The router's choice for each row of logits (rows, experts), bf16, fp16 or fp32, rows `row_stride`
- * elements apart: scores s, choices by c = s + bias (experts fp32, all in 64 bits).  Where bias is NULL x itself orders
- * the experts, and the groups too with a group_best of 1, as exact scores would: logits whose scores are equal in 64 bits (sigmoids above
- * some 37) still differ.  Sums of two scores are in 64 bits, with a bias or without.  ids (rows, k) the k experts of the largest c in the groups that stay, in falling order, equal ones by rising
+ * elements apart: scores s, choices by c = s + bias (experts fp32, all in 64 bits).  Where bias is NULL x itself
+ * orders the experts, and the groups too with a group_best of 1, as exact scores would: logits whose scores are equal in
+ * 64 bits (sigmoids above some 37) still differ.  Sums of two scores are in 64 bits, with a bias or without.
+ * ids (rows, k) the k experts of the largest c in the groups that stay, in falling order, equal ones by rising
  * index; weights (rows, k) = s[ids], with renorm divided by their sum (a sum of 0 gives zeros), times scale, in
- * 64 bits and rounded once.  A NaN counts below every number.  A row of nothing but -inf has scores of 0; with softmax a NaN or +inf makes all of the row's scores NaN.
- * experts <= 1024, groups <= 64, k <= 64. */
+ * 64 bits and rounded once.  A NaN counts below every number.  A row of nothing but -inf has scores of 0; with softmax
+ * a NaN or +inf makes all of the row's scores NaN.  experts <= 1024, groups <= 64, k <= 64. */
 int wush_moe_route(const void *logits, int dtype, int64_t row_stride, const float *bias, int64_t rows, int64_t experts,
                    const wush_moe_choice *choice, float *weights, int32_t *ids, hipStream_t stream);
 

@@ -126,10 +126,10 @@ class ExpertLayer:
                                     keep_groups=self.keep_groups, group_best=self.group_best, renorm=self.renorm, scale=self.scale)
         y = _C.fp8_experts(x, weights, ids - self.first if self.first else ids, *self.up, *self.down)
         if self.shared is not None:
-            # gate, up and h are rounded to x's type between the two products: 1.5e-2 of this expert's exact output in bf16 and
-            # 5e-3 in fp16, where e4m3 weights and activations themselves are 6e-2 from unquantized ones (6.39e-2 with, 6.39e-2
-            # without).  fp8_experts with one expert keeps them in fp32 (1.8e-3, 2e-4), but does not split K: 4096 x 4096, bf16, 16 tokens
-            # 70 us for 43, 128 tokens 85 for 53, 4096 tokens 288 for 319.
+            # gate, up and h are rounded to x's type between the two products, as between any two layers: 1.5e-2 of this expert's
+            # exact output in bf16 and 5e-3 in fp16, where e4m3 weights and activations themselves are 6.39e-2 from unquantized ones
+            # (6.39e-2 with these roundings too).  fp8_experts with one expert keeps them in fp32 (1.7e-3, 2e-4), but has tiles for
+            # few CUs and does not split K: 4096 x 4096, bf16, 16 tokens 77 us for 42, 128 tokens 111 for 53, 4096 tokens 356 for 309.
             gate, up = _C.fp8_linear(x, *self.shared[0]).float().chunk(2, -1)
             y = y + _C.fp8_linear((torch.nn.functional.silu(gate) * up).to(x.dtype), *self.shared[1])
         return y

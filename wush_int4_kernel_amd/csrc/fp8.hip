@@ -35,10 +35,10 @@ struct Plan {
 };
 
 // Up to four rows take dot products where they fit (fp8_gemv_shape), all else the tile and the split of K with the least
-// estimated time, in microseconds: rounds of workgroups with the time of their stages (3/4 of it on an empty chip), or the weights' way from HBM (slower where several
-// row tiles read them), whichever is longer, a part of the shorter, and for a split its launch and partial sums.  The
-// constants are fitted to 94 shapes from 5 x 8192 x 28672 to 4000 x 4096 x 4096, weights from HBM: 0.8% slower than the fastest
-// of all tiles and splits on average, 12% at worst.
+// estimated time, in microseconds: rounds of workgroups with the time of their stages (3/4 of it on an empty chip), or the
+// weights' way from HBM (slower where several row tiles read them), whichever is longer, a part of the shorter, and for a
+// split its launch and partial sums.  The constants are fitted to 94 shapes from 5 x 8192 x 28672 to 4000 x 4096 x 4096,
+// weights from HBM: 0.8% slower than the fastest of all tiles and splits on average, 12% at worst.
 Plan plan_of(int64_t M, int64_t N, int64_t K, size_t room) {
     if (fp8_gemv_shape(M, K)) return {WUSH_FP8_DOT, (int)M, 1, 1};
     Plan best = {WUSH_FP8_TILES, 32, 64, 1};
